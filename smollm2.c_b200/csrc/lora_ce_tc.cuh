@@ -588,8 +588,12 @@ __global__ void __launch_bounds__(kThreadsT, 1)
         xb[half * kBM + row] = cm;
         named_bar_sync(1 + quarter, 64);
         cm = fmaxf(cm, xb[(half ^ 1) * kBM + row]);
-        if (cm > m + kLazyT) {
-          const float f = ex2f((m - cm) * kLog2e);  // 0 when m = -inf
+        // The TMEM rescale below is warp-wide (tcgen05.ld / st are .aligned):
+        // all lanes take it when any row of the warp moves, rows that do not
+        // move with the factor 1.
+        const bool move = cm > m + kLazyT;
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = move ? ex2f((m - cm) * kLog2e) : 1.0f;  // 0 when m = -inf
           s2 = __fmul2_rn(s2, make_float2(f, f));
           if (!first_tile) {
             // rescale this half's columns of the rank accumulator once the
@@ -609,8 +613,10 @@ __global__ void __launch_bounds__(kThreadsT, 1)
               }
             }
           }
-          m = cm;
-          mL = cm * kLog2e;
+          if (move) {
+            m = cm;
+            mL = cm * kLog2e;
+          }
         }
         // (b) P = 2^4 e^(z - m) as f16 hi/lo, the sum, the target logit
         const float2 nmL2 = make_float2(kP1Exp - mL, kP1Exp - mL);
@@ -641,6 +647,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
                     : "f"(z[i]), "r"(k), "r"(i));
               g.z_tgt[rr] = zt;
             }
+            __syncwarp();  // the target's lanes rejoin before the warp-wide TMEM stores
             if (c == 0) wait_p_free();
             tmem_st<8>(pb + (uint32_t)(16 * c), hi);
             tmem_st<8>(pb + (uint32_t)(16 * c + 8), lo);
