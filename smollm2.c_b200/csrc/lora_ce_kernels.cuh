@@ -143,6 +143,18 @@ struct GemmArgs {
   // tensor-core rank sums (lce_gemm_tc)
   int stages;         // streamed-operand ring stages
   const float* nml;   // pass 2: per position -M*log2(e) + log2(1/S) + 14
+  // kTemp epilogues: softmax of z * lg / log2(e) (lg: log2(e) / temperature,
+  // times the accumulator correction), and the lazy-max thresholds in units of z
+  float lg, lazy, redo;
+  float drain_gain;   // 1 + the relative loss of one accumulation of rank sums (lce_gemm_tc)
+  // EpiScore (lora_head.cuh): entropy sums, and the records of a row's logits
+  float* p_ent;       // [seg][Tcap]
+  float* sub_max;     // [record][sub_ld]
+  float* sub_second;
+  float* sub_rest;
+  uint8_t* sub_arg;
+  uint8_t* sub_arg2;
+  long long sub_ld;
 };
 
 // Dynamic shared memory: [resident K-blocks | streamed ring (ring bytes) | staged
@@ -225,9 +237,24 @@ __device__ __forceinline__ void mbar_drain_wait(uint64_t* bar, uint32_t parity, 
 
 __device__ __forceinline__ float2 f2(float x, float y) { return make_float2(x, y); }
 
+// hi + lo += part.x + part.y with the rounding of hi kept in lo; part = 0.
+__device__ __forceinline__ void fold_sum(float2& part, float& hi, float& lo) {
+  const float x = part.x + part.y;
+  const float t = __fadd_rn(hi, x);
+  const float b = __fsub_rn(t, hi);
+  lo += __fadd_rn(__fsub_rn(hi, __fsub_rn(t, b)), __fsub_rn(x, b));
+  hi = t;
+  part = f2(0.f, 0.f);
+}
+
 // Pass 1: the thread owns position t; columns are vocab ids; the records of
 // a column pair are B[:, v], B[:, v+1] interleaved (2R floats).
-template <int R, bool kAug_ = (R >= LCE_AUG_MIN_RANK), bool kChunk = false>
+// kTemp: softmax at a temperature (GemmArgs::lg), no target logit, and sums
+// in two levels: 64 columns at a time are added up by themselves and then
+// folded into the row's sums (S with the rounding carried along).  Where one
+// logit holds most of a row, thousands of small terms added to it one by one
+// would each be rounded away, a background of 1e-5 of the sum with them.
+template <int R, bool kAug_ = (R >= LCE_AUG_MIN_RANK), bool kChunk = false, bool kTemp = false>
 struct EpiLse {
   static constexpr bool kAug = kAug_;  // rank term in the accumulator
   static constexpr int kRec = R;  // floats per column
@@ -248,6 +275,17 @@ struct EpiLse {
   float m, mL;    // reference max, m*log2(e)
   float2 s2;      // sum of e^(z-m) over even / odd columns
   float2 q2[R];   // sum of e^(z-m) * B[j][v] over even / odd columns
+  float S, Slo;   // kTemp: folded sums
+  float Q[kTemp ? R : 1];
+
+  __device__ __forceinline__ void fold() {
+    fold_sum(s2, S, Slo);
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      Q[j] += q2[j].x + q2[j].y;
+      q2[j] = f2(0.f, 0.f);
+    }
+  }
 
   __device__ static const float* global_recs(const GemmArgs& g, int b) {
     return g.Bt + (long long)b * kBN * R;
@@ -265,12 +303,18 @@ struct EpiLse {
         sU2[j] = f2(u, u);
       }
     }
-    tgt = valid ? __float_as_int(g.tok[tidx(tt, g.rank_total + 2, g.rank_total)]) : -1;
+    if constexpr (!kTemp)
+      tgt = valid ? __float_as_int(g.tok[tidx(tt, g.rank_total + 2, g.rank_total)]) : -1;
     m = -INFINITY;
     mL = -INFINITY;
     s2 = f2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < R; ++j) q2[j] = f2(0.f, 0.f);
+    if constexpr (kTemp) {
+      S = Slo = 0.f;
+#pragma unroll
+      for (int j = 0; j < R; ++j) Q[j] = 0.f;
+    }
   }
 
   // Per column: z = acc + sU.B[:,v], e = e^(z - m), s += e, q += e*B[:,v],
@@ -287,7 +331,9 @@ struct EpiLse {
     float2 q_old[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) q_old[j] = q2[j];
-    const float2 L2 = f2(kLog2e, kLog2e);
+    const float L = kTemp ? g.lg : kLog2e;
+    const float lazy = kTemp ? g.lazy : kLazy, redo = kTemp ? g.redo : kRedo;
+    const float2 L2 = f2(L, L);
     const float2 nmL2 = f2(-mL, -mL);
     float cm = -INFINITY;
 #pragma unroll
@@ -312,10 +358,16 @@ struct EpiLse {
 #pragma unroll
       for (int j = 0; j < R; ++j) q2[j] = __ffma2_rn(e2, f2(b[2 * j], b[2 * j + 1]), q2[j]);
     }
-    if (cm > m + kLazy) {
-      const float f = ex2f((m - cm) * kLog2e);  // 0 when m = -inf
+    if (cm > m + lazy) {
+      const float f = ex2f((m - cm) * L);  // 0 when m = -inf
       const float2 ff = f2(f, f);
-      if (cm - m <= kRedo) {
+      if constexpr (kTemp) {
+        S *= f;
+        Slo *= f;
+#pragma unroll
+        for (int j = 0; j < R; ++j) Q[j] *= f;
+      }
+      if (cm - m <= redo) {
         s2 = __fmul2_rn(s2, ff);
 #pragma unroll
         for (int j = 0; j < R; ++j) q2[j] = __fmul2_rn(q2[j], ff);
@@ -323,7 +375,7 @@ struct EpiLse {
         s2 = __fmul2_rn(s_old, ff);
 #pragma unroll
         for (int j = 0; j < R; ++j) q2[j] = __fmul2_rn(q_old[j], ff);
-        const float2 ncmL2 = f2(-cm * kLog2e, -cm * kLog2e);
+        const float2 ncmL2 = f2(-cm * L, -cm * L);
         const volatile float* vr = recs;  // fresh loads: keeps the first loop's rows dead
 #pragma unroll
         for (int p = 0; p < kCW / 2; ++p) {
@@ -336,9 +388,12 @@ struct EpiLse {
         }
       }
       m = cm;
-      mL = cm * kLog2e;
+      mL = cm * L;
     }
-    if (valid && (unsigned)(tgt - v0) < (unsigned)kCW) {
+    if constexpr (kTemp) {
+      if (((v0 + kCW) & 63) == 0) fold();
+    }
+    if (!kTemp && valid && (unsigned)(tgt - v0) < (unsigned)kCW) {
       // Opaque selects keep acc[] in registers (a plain acc[tgt - v0] would
       // move the whole array to local memory).
       float zt = 0.f;
@@ -356,6 +411,13 @@ struct EpiLse {
     if (!valid) return;
     const long long o = (long long)slot * g.Tcap + t;
     g.p_max[o] = m;
+    if constexpr (kTemp) {
+      fold();
+      g.p_sum[o] = S + Slo;
+#pragma unroll
+      for (int j = 0; j < R; ++j) g.p_q[o * g.rank_total + g.rank_off + j] = Q[j];
+      return;
+    }
     g.p_sum[o] = s2.x + s2.y;
 #pragma unroll
     for (int j = 0; j < R; ++j) g.p_q[o * g.rank_total + g.rank_off + j] = q2[j].x + q2[j].y;
@@ -366,7 +428,7 @@ struct EpiLse {
 // of a position pair are tok[] fields interleaved (2(R+4) floats).  This
 // pass accumulates the p part of dl = p - onehot; lce_onehot adds the
 // onehot part.
-template <int R, bool kAug_ = (R >= LCE_AUG_MIN_RANK), bool kChunk = false>
+template <int R, bool kAug_ = (R >= LCE_AUG_MIN_RANK), bool kChunk = false, bool kTemp = false>
 struct EpiGrad {
   static constexpr bool kAug = kAug_;  // rank term in the accumulator
   // rank chunks read their own records {sU[0..16), -M log2 e, 1/S}
@@ -409,7 +471,8 @@ struct EpiGrad {
   __device__ __forceinline__ void chunk(const GemmArgs& g, int t0, float (&acc)[kCW],
                                         const float* recs) {
     if (kTail && t0 >= g.T) return;  // fully padded chunk (zero records) adds nothing
-    const float2 L2 = f2(kLog2e, kLog2e);
+    const float L = kTemp ? g.lg : kLog2e;
+    const float2 L2 = f2(L, L);
 #pragma unroll
     for (int p = 0; p < kCW / 2; ++p) {
       const float* rp = recs + p * 2 * kRec;

@@ -165,7 +165,15 @@ __device__ __forceinline__ void read_rank_acc(uint32_t q_addr, int j0, float (&q
 // pass 1 writes per (segment, column half) max / sum / q with q's ranks
 // split between the halves (zeros elsewhere); pass 2 writes one dB slot per
 // segment, the halves taking half of the ranks each.
-template <int kPass, int R>
+// kTemp: softmax at a temperature (GemmArgs::lg), no target logit, and sums in
+// two levels.  S as EpiLse.  The rank accumulator is truncated towards zero at
+// every MMA, a relative loss of about 1.7e-8 a step where it grows evenly
+// (acc_short, lora_head.cu), 1.5e-5 over a CTA's 1,000 steps at 8,000
+// positions.  So it is read and added to f32 registers every tc_drain tiles
+// (48 or 64 steps), whose known loss of 1e-6 is made good; the read waits until
+// the epilogue is done with the following tile, so that no one waits for it.
+__host__ __device__ constexpr int tc_drain(int R) { return R <= 32 ? 2 : 4; }
+template <int kPass, int R, bool kTemp = false>
 __global__ void __launch_bounds__(kThreadsT, 1)
     lce_gemm_tc(const __grid_constant__ CUtensorMap map_res,
                 const __grid_constant__ CUtensorMap map_str,
@@ -182,6 +190,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
   constexpr int kStBytesT = TcLayout::stage_bytes(R);
   constexpr int kXBlocksT = kBNT / kBK;
   constexpr int kResRows = 2 * kBM;
+  constexpr int kDrain = tc_drain(R);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int kSt = g.stages;
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
@@ -320,7 +329,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
       uint32_t phase = 0;
       int cur_a = -1;
       uint32_t a_uses = 0;
-      int blk = -1;
+      int blk = -1, in_blk = 0;
       long long li = 0;
       bool ok = true;
       bool have_prev = false, prev_first = false, prev_last = false;
@@ -353,13 +362,20 @@ __global__ void __launch_bounds__(kThreadsT, 1)
       };
       for (long long x = x_begin; x < x_end && ok; ++x, ++li) {
         const int a = (int)(x / g.n_b);
-        const bool first = a != cur_a;
+        bool first = a != cur_a;  // of an accumulation: a block's, or a period's
         if (first) {
           if (!mbar_wait(&bars[kTAFull], a_uses & 1, g.err, kErrWaitMma)) break;
           ++a_uses;
           cur_a = a;
-          ++blk;
+          in_blk = 0;
         }
+        bool last = false;
+        if constexpr (kTemp) {
+          first = in_blk % kDrain == 0;
+          last = in_blk % kDrain == kDrain - 1;
+          ++in_blk;
+        }
+        if (first) ++blk;
         const int buf = (int)(li & 1);
         // in place, tile li-2's probabilities sit in this buffer until its
         // rank MMAs are done
@@ -423,7 +439,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
         }
         have_prev = true;
         prev_first = first;
-        prev_last = last_of_a;
+        prev_last = last_of_a || last;
         prev_li = li;
         prev_blk = blk;
       }
@@ -444,7 +460,9 @@ __global__ void __launch_bounds__(kThreadsT, 1)
     constexpr int kHalfCols = kBNT / 2;
     constexpr int NCH = kHalfCols / 16;
     constexpr int kQW = R < 16 ? R : 16;
-    const float2 L2 = make_float2(kLog2e, kLog2e);
+    const float L = kTemp ? g.lg : kLog2e;
+    const float lazy = kTemp ? g.lazy : kLazyT;
+    const float2 L2 = make_float2(L, L);
     int cur_a = -1, blk = -1;
     long long li = 0;
     bool failed = false, first_tile = false;
@@ -454,11 +472,67 @@ __global__ void __launch_bounds__(kThreadsT, 1)
     int tgt = -1;                         // pass 1
     float m = -INFINITY, mL = -INFINITY;  // pass 1 lazy max
     float2 s2 = make_float2(0.f, 0.f);    // pass 1 sum of 16 e^(z - m), even / odd columns
+    // kTemp: folded sums of the row (Q: this half's ranks)
+    constexpr int kHR = R / 2, kDW = kHR < 16 ? kHR : 16;
+    float S = 0.f, Slo = 0.f;
+    float Q[kTemp ? kHR : 1];
+    int in_blk = 0, pending = -1;
+    if constexpr (kTemp) {
+#pragma unroll
+      for (int i = 0; i < kHR; ++i) Q[i] = 0.f;
+    }
+    // Reads accumulation `which` (complete) into Q and gives the accumulator back.
+    auto drain = [&](int which) {
+      if (!failed && !mbar_wait(&bars[kTQFull], (uint32_t)(which & 1), g.err, kErrWaitEpilogue))
+        failed = true;
+      __syncwarp();
+      tc_fence_after();
+      if constexpr (kTemp) {
+#pragma unroll
+        for (int i0 = 0; i0 < kHR; i0 += kDW) {
+          float u[kDW], w[kDW];
+          tmem_ld<kDW>(q_addr + (uint32_t)(half * kHR + i0), u);
+          tmem_ld<kDW>(q_addr + (uint32_t)(R + half * kHR + i0), w);
+          tmem_ld_wait<kDW>(u);
+          tmem_ld_wait<kDW>(w);
+#pragma unroll
+          for (int i = 0; i < kDW; ++i) Q[i0 + i] = fmaf(u[i] + w[i], g.drain_gain, Q[i0 + i]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&bars[kTQEmpty]), 0));
+    };
 
     // The rank accumulator of the finished block: pass 1 q (this half's
     // ranks, zeros for the other half's), pass 2 dB (this half's ranks).
     auto flush_block = [&](int a_done, int blk_done) {
       const int seg = unit - tile_owner((long long)a_done * g.n_b, total, G);
+      if constexpr (kTemp) {
+        drain(pending);
+        pending = -1;
+        if (valid && !failed) {
+          if constexpr (kPass == 1) {
+            const long long o = (long long)(2 * seg + half) * g.Tcap + rr;
+            g.p_max[o] = m;
+            g.p_sum[o] = (S + Slo) * (1.0f / 16.0f);
+#pragma unroll
+            for (int i = 0; i < kHR; ++i) {
+              g.p_q[o * R + half * kHR + i] = Q[i] * (1.0f / 16.0f);
+              g.p_q[o * R + (half ^ 1) * kHR + i] = 0.f;
+            }
+          } else {
+            float* o = g.gBp + (long long)seg * g.Vpad * R;
+#pragma unroll
+            for (int i = 0; i < kHR; ++i)
+              o[bidx(rr, half * kHR + i, R)] = Q[i] * (1.0f / 16384.0f);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kHR; ++i) Q[i] = 0.f;
+        S = Slo = 0.f;
+        return;
+      }
       if (!failed && !mbar_wait(&bars[kTQFull], (uint32_t)(blk_done & 1), g.err, kErrWaitEpilogue))
         failed = true;
       tc_fence_after();
@@ -510,7 +584,8 @@ __global__ void __launch_bounds__(kThreadsT, 1)
         rr = (g.a0 + a) * kResRows + (int)rank * kBM + row;
         if constexpr (kPass == 1) {
           valid = rr < g.T;
-          tgt = valid ? __float_as_int(g.tok[tidx(rr, g.rank_total + 2, g.rank_total)]) : -1;
+          if constexpr (!kTemp)
+            tgt = valid ? __float_as_int(g.tok[tidx(rr, g.rank_total + 2, g.rank_total)]) : -1;
           m = -INFINITY;
           mL = -INFINITY;
           s2 = make_float2(0.f, 0.f);
@@ -518,8 +593,12 @@ __global__ void __launch_bounds__(kThreadsT, 1)
           valid = rr < g.V;
         }
         cur_a = a;
-        ++blk;
+        if constexpr (!kTemp) ++blk;
+        in_blk = 0;
         first_tile = true;
+      }
+      if constexpr (kTemp) {
+        if (in_blk % kDrain == 0) ++blk;
       }
       const int buf = (int)(li & 1);
       if (!failed && !mbar_wait(&bars[kTZFull + buf], (uint32_t)((li >> 1) & 1), g.err,
@@ -591,10 +670,16 @@ __global__ void __launch_bounds__(kThreadsT, 1)
         // The TMEM rescale below is warp-wide (tcgen05.ld / st are .aligned):
         // all lanes take it when any row of the warp moves, rows that do not
         // move with the factor 1.
-        const bool move = cm > m + kLazyT;
+        const bool move = cm > m + lazy;
         if (__any_sync(0xffffffffu, move)) {
-          const float f = move ? ex2f((m - cm) * kLog2e) : 1.0f;  // 0 when m = -inf
+          const float f = move ? ex2f((m - cm) * L) : 1.0f;  // 0 when m = -inf
           s2 = __fmul2_rn(s2, make_float2(f, f));
+          if constexpr (kTemp) {
+            S *= f;
+            Slo *= f;
+#pragma unroll
+            for (int i = 0; i < kHR; ++i) Q[i] *= f;
+          }
           if (!first_tile) {
             // rescale this half's columns of the rank accumulator once the
             // previous tile's rank MMAs have landed
@@ -615,7 +700,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
           }
           if (move) {
             m = cm;
-            mL = cm * kLog2e;
+            mL = cm * L;
           }
         }
         // (b) P = 2^4 e^(z - m) as f16 hi/lo, the sum, the target logit
@@ -637,7 +722,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
               s2 = __fadd2_rn(s2, e2);
               split_f16x2(e2, hi[p], lo[p]);
             }
-            if (valid && (unsigned)(tgt - v0) < 16u) {
+            if (!kTemp && valid && (unsigned)(tgt - v0) < 16u) {
               float zt = 0.f;
               const int k = tgt - v0;
 #pragma unroll
@@ -711,6 +796,18 @@ __global__ void __launch_bounds__(kThreadsT, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&bars[kTPFull]), 0));
       first_tile = false;
+      if constexpr (kTemp) {
+        if constexpr (kPass == 1) fold_sum(s2, S, Slo);
+        if (pending >= 0) {
+          // both halves of the rows have done their rescale of this tile
+          if constexpr (kPass == 1) named_bar_sync(1 + quarter, 64);
+          drain(pending);
+          pending = -1;
+        }
+        const bool last_of_a = x + 1 == x_end || (int)((x + 1) / g.n_b) != a;
+        if (in_blk % kDrain == kDrain - 1 || last_of_a) pending = blk;
+        ++in_blk;
+      }
     }
     if (cur_a >= 0) flush_block(cur_a, blk);
   } else if (warp == kXWarpT) {

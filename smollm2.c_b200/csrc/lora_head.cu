@@ -1,0 +1,935 @@
+// lora_head.cu — host side of the operators declared in include/lora_head.h:
+// argument checks, workspace layout and the launch sequences.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <map>
+#include <mutex>
+#include <string>
+#include <tuple>
+
+#include "lora_ce_kernels.cuh"
+#include "lora_ce_plan.cuh"
+#include "lora_ce_tc.cuh"
+#include "lora_head.cuh"
+#include "lora_head.h"
+#include "lora_head_core.h"
+
+using namespace lce;
+
+namespace {
+
+thread_local std::string g_head_error;
+
+int hfail(int code, const char* msg) {
+  g_head_error = msg;
+  return code;
+}
+
+// How the rank term joins the MMA: one K-block up to rank 16, 2R columns above.
+// Its operands are only as wide as they are used (a multiple of 16 bytes); the
+// loads fill the rest of a 64-column block with zeros.
+struct Aug {
+  int R = 0, layout = 0, width = 0;
+};
+Aug aug_of(int r) {
+  Aug a;
+  if (r == 0) return a;
+  a.R = kernel_rank(r);
+  a.layout = a.R <= 16 ? 1 : 2;
+  a.width = a.R <= 16 ? (3 * a.R + 7) / 8 * 8 : 2 * a.R;
+  return a;
+}
+void aug_schedule(GemmArgs& g, const Aug& a) {
+  switch (a.R) {
+    case 8: RankPlan<8>::schedule(g); break;
+    case 16: RankPlan<16>::schedule(g); break;
+    case 32: RankPlan<32>::schedule(g); break;
+    case 64: RankPlan<64>::schedule(g); break;
+    default:
+      g.n_aug = a.R ? 1 : 0;  // rank 4: 12 of 64 columns, one K-step
+      g.aug_a[0] = g.aug_b[0] = 0;
+  }
+}
+
+// The share by which the accumulator of a large logit falls short
+// (lora_head.cuh): partial sums at 1/n, 2/n .. 1 of it over the n K-steps of
+// h . W, then at all of it over the rank term's.
+double acc_short(int n, int n_aug) {
+  return 0.79 * (0.5 * (n + 1) + n_aug) * std::ldexp(1.0, -25) / std::log(2.0);
+}
+
+// Co-resident owners (CTA pairs) of a kernel on the current device, found once
+// per device, kernel and shared-memory size; also lets the kernel use that
+// much shared memory.
+int resident_pairs(const void* kern, int threads, int smem) {
+  static std::mutex mu;
+  static std::map<std::tuple<int, const void*, int>, int> known;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  const auto key = std::make_tuple(dev, kern, smem);
+  const auto it = known.find(key);
+  if (it != known.end()) return it->second;
+  // the attribute keeps the largest size that any call has asked for
+  cudaFuncAttributes fa;
+  if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) return 0;
+  if (fa.maxDynamicSharedSizeBytes < smem &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return 0;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)(sms / 2 * 2));
+  lc.blockDim = dim3((unsigned)threads);
+  lc.dynamicSmemBytes = (size_t)smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &lc) != cudaSuccess || n < 1) return 0;
+  known[key] = n;
+  return n;
+}
+
+// Same for kernels without clusters: only the shared-memory attribute.
+bool allow_smem(const void* kern, size_t smem) {
+  if (smem <= 48 * 1024) return true;
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, size_t> known;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  std::lock_guard<std::mutex> lock(mu);
+  size_t& have = known[std::make_pair(dev, kern)];
+  if (have >= smem) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+      cudaSuccess)
+    return false;
+  have = smem;
+  return true;
+}
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess)
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+// An upper bound on the owners, the same on every call, for sizing partials.
+constexpr int kMaxPairs = 80;
+
+// Most slots per row of a pass whose owners are at most kMaxPairs.
+int most_segments(int n_a, int n_b) {
+  const long long total = (long long)n_a * n_b;
+  // an owner's run is at least floor(total / G) tiles, so a row of n_b tiles
+  // meets at most n_b / run + 2 owners
+  const int G = (int)std::min<long long>(kMaxPairs, total);
+  const long long run = total / G;
+  return (int)std::min<long long>(G, n_b / run + 2);
+}
+
+struct Carve {
+  uint8_t* base;
+  size_t off = 0;
+  template <class T>
+  T* take(size_t count) {
+    const size_t at = off;
+    off = (off + count * sizeof(T) + 255) / 256 * 256;
+    return base ? reinterpret_cast<T*>(base + at) : nullptr;
+  }
+};
+
+template <class K, class... Args>
+bool launch_pairs(K kern, int pairs, int threads, int smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)(2 * pairs));
+  lc.blockDim = dim3((unsigned)threads);
+  lc.dynamicSmemBytes = (size_t)smem;
+  lc.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  return cudaLaunchKernelEx(&lc, kern, args...) == cudaSuccess;
+}
+
+using PassKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap,
+                            const CUtensorMap, const GemmArgs);
+
+struct PassPlan {
+  PassKernel kern = nullptr;
+  int threads = 0, smem = 0;
+};
+
+// EpiScore with the largest ring that fits beside the resident K-blocks.
+template <int kSub>
+PassPlan score_plan(int kblocks) {
+  PassPlan p;
+  p.threads = block_threads(EpiScore<65536, kSub>::kWarps);
+  if (kblocks <= 10) {
+    p.kern = lce_gemm_kernel<EpiScore<65536, kSub>, false, 2>;
+    p.smem = SmemLayout::bytes(kblocks, 0, 65536);
+  } else if (kblocks == 11) {
+    p.kern = lce_gemm_kernel<EpiScore<49152, kSub>, false, 2>;
+    p.smem = SmemLayout::bytes(kblocks, 0, 49152);
+  } else {
+    p.kern = lce_gemm_kernel<EpiScore<32768, kSub>, false, 2>;
+    p.smem = SmemLayout::bytes(kblocks, 0, 32768);
+  }
+  return p;
+}
+
+// Columns per record: the widest that leaves four records per alternative.
+int record_columns(int V, int top_k) {
+  const int want = 4 * std::max(top_k, kMinPick);
+  return (V + 63) / 64 >= want ? 64 : (V + 7) / 8 >= want ? 8 : 1;
+}
+
+// The passes of ranks 4 and 8 (rank sums in the epilogue): records staged in
+// shared memory where they fit.
+template <class Epi>
+PassPlan sums_plan(int kblocks) {
+  PassPlan p;
+  p.threads = block_threads(Epi::kWarps);
+  p.smem = SmemLayout::bytes(kblocks, Epi::kRec * Epi::kRecBufs, Epi::kRing);
+  if (p.smem <= kMaxDynSmem) {
+    p.kern = lce_gemm_kernel<Epi, true, 2>;
+  } else {
+    p.smem = SmemLayout::bytes(kblocks, 0, Epi::kRing);
+    p.kern = lce_gemm_kernel<Epi, false, 2>;
+  }
+  return p;
+}
+
+// Tiles, partials and temperature factors of a pass whose resident rows are
+// positions.
+void fill_pass1(GemmArgs& g, const HeadCore& hd, const Aug& aug, int T, float tau) {
+  g.kmain = hd.d / kBK;
+  g.kblocks = g.kstr = g.kmain + (aug.width + kBK - 1) / kBK;
+  aug_schedule(g, aug);
+  g.rank_total = g.R = aug.R;
+  g.T = T;
+  g.V = hd.V;
+  g.Vpad = round_up(hd.V, kBN);
+  g.n_a = (T + 2 * kBM - 1) / (2 * kBM);
+  g.Tcap = (long long)g.n_a * 2 * kBM;
+  const double shortfall = acc_short(4 * g.kmain, g.kblocks > g.kmain ? g.n_aug : 0);
+  g.lg = (float)((1.0 + shortfall) / (std::log(2.0) * tau));
+  g.lazy = 8.0f * tau;
+  g.redo = 80.0f * tau;
+}
+
+constexpr int kPrepRows = 4;  // positions per warp of lh_prep at large T
+
+// lh_prep over positions and vocab rows.  A warp takes 4 positions, whose A
+// loads it shares, where that still fills the SMs twice; else 1.
+int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_blocks, bool pack,
+                int sms, cudaStream_t st) {
+  const bool wide = pa.Tpad >= 2 * sms * kRowWarps * kPrepRows;
+  const int per = kRowWarps * (wide ? kPrepRows : 1);
+  const int prep_blocks = rows ? (pa.Tpad + per - 1) / per : 0;
+  const int pack_blocks = pack ? (int)(pk.Vpad / kPackRows) : 0;
+  const size_t smem = std::max(rows ? (size_t)per * pa.d * 4 : 0,
+                               pack ? (size_t)pk.R * (kPackRows + 1) * 4 : 0);
+  auto kern = wide ? lh_prep<kPrepRows> : lh_prep<1>;
+  if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return LORA_CE_ECUDA;
+  kern<<<prep_blocks + max_blocks + pack_blocks, 32 * kRowWarps, smem, st>>>(pa, pk, prep_blocks,
+                                                                            max_blocks);
+  return 0;
+}
+
+struct ScoreWs {
+  int* stats;
+  __half *h16, *haug, *waug;
+  double* sU;
+  float *p_max, *p_sum, *p_ent, *sub_max, *sub_second, *sub_rest;
+  uint8_t *sub_arg, *sub_arg2;
+  long long sub_ld;
+  int sub, n_sub;
+  size_t bytes;
+};
+
+ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
+  const Aug aug = aug_of(hd.r);
+  ScoreWs w{};
+  Carve c{static_cast<uint8_t*>(ws)};
+  const long long Vpad = round_up(hd.V, kBN);
+  const int n_a = (T + 2 * kBM - 1) / (2 * kBM), n_b = (int)(Vpad / kBN);
+  const size_t part = (size_t)4 * most_segments(n_a, n_b) * n_a * 2 * kBM;
+  w.sub = record_columns(hd.V, top_k);
+  w.n_sub = (hd.V + w.sub - 1) / w.sub;
+  w.sub_ld = round_up(T, 32);
+  w.stats = c.take<int>(kStatWords);
+  w.h16 = c.take<__half>((size_t)T * hd.d);
+  w.sU = c.take<double>((size_t)T * aug.R);
+  w.haug = c.take<__half>((size_t)T * aug.width);
+  w.waug = c.take<__half>((size_t)Vpad * aug.width);
+  w.p_max = c.take<float>(part);
+  w.p_sum = c.take<float>(part);
+  w.p_ent = c.take<float>(part);
+  const size_t recs = (size_t)w.n_sub * w.sub_ld;
+  w.sub_max = c.take<float>(recs);
+  w.sub_second = c.take<float>(w.sub == 64 ? recs : 0);
+  w.sub_rest = c.take<float>(w.sub > 1 ? recs : 0);
+  w.sub_arg = c.take<uint8_t>(w.sub > 1 ? recs : 0);
+  w.sub_arg2 = c.take<uint8_t>(w.sub == 64 ? recs : 0);
+  w.bytes = c.off;
+  return w;
+}
+
+struct DistillWs {
+  int* stats;
+  __half *h16, *haug, *waug, *xv, *xt;
+  double* sU;
+  float *wt, *p_max, *p_sum, *p_q, *tok, *Bt, *nml, *dU, *gAp, *gBp, *Ap;
+  unsigned long long* corr;
+  size_t zero_bytes;  // stats and corr: cleared by every call
+  size_t bytes;
+};
+
+DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
+  const Aug aug = aug_of(hd.r);
+  const int R = aug.R;
+  const bool tc = R >= 16;
+  DistillWs w{};
+  Carve c{static_cast<uint8_t*>(ws)};
+  const long long Vpad = round_up(hd.V, kBN), Tpad = round_up(T, kBN);
+  const int bn = grads && tc ? tc_bn(R) : kBN;
+  const int n_a = (T + 2 * kBM - 1) / (2 * kBM), n_b = (hd.V + bn - 1) / bn;
+  const size_t part = (size_t)(grads && tc ? 2 : 4) * most_segments(n_a, n_b) * n_a * 2 * kBM;
+  w.stats = c.take<int>(kStatWords);
+  if (grads) w.corr = c.take<unsigned long long>((size_t)Vpad * R);
+  w.zero_bytes = c.off;
+  w.h16 = c.take<__half>((size_t)T * hd.d);
+  w.sU = c.take<double>((size_t)T * R);
+  w.wt = c.take<float>(T);
+  // rank 4 keeps the rank term in the epilogues of the gradient passes
+  const bool in_mma = !grads || R > 4;
+  w.haug = c.take<__half>(in_mma ? (size_t)T * aug.width : 0);
+  w.waug = c.take<__half>(in_mma ? (size_t)Vpad * aug.width : 0);
+  w.p_max = c.take<float>(part);
+  w.p_sum = c.take<float>(part);
+  if (grads) {
+    // chunks of four or eight epilogue columns a row: up to 4 slots per owner
+    const int n_a2 = (hd.V + 2 * kBM - 1) / (2 * kBM), n_b2 = (T + bn - 1) / bn;
+    const size_t segs = (size_t)(tc ? 1 : 4) * most_segments(n_a2, n_b2);
+    w.p_q = c.take<float>(part * R);
+    w.tok = c.take<float>(tc ? 0 : (size_t)Tpad * tok_stride(R));
+    w.Bt = c.take<float>(hd.layout ? 0 : (size_t)Vpad * R);
+    w.xv = c.take<__half>(tc ? (size_t)2 * R * Vpad : 0);
+    w.xt = c.take<__half>(tc ? (size_t)2 * R * Tpad : 0);
+    w.nml = c.take<float>(tc ? (size_t)Tpad + kMaxBNT : 0);
+    w.dU = c.take<float>((size_t)T * R);
+    w.gAp = c.take<float>((size_t)((T + kDAChunk - 1) / kDAChunk) * hd.d * R);
+    w.gBp = c.take<float>(segs * Vpad * R);
+  }
+  w.bytes = c.off;
+  return w;
+}
+
+LogitArgs logit_args(const HeadCore& hd, const Aug& aug, int T, const __half* h16,
+                     const double* sU) {
+  LogitArgs z{};
+  z.W = hd.W;
+  z.h16 = h16;
+  z.sU = sU;
+  z.B = BView{hd.B, hd.V, hd.r, aug.R, hd.layout};
+  z.T = T;
+  z.V = hd.V;
+  z.d = hd.d;
+  z.r = hd.r;
+  z.R = aug.R;
+  return z;
+}
+
+PrepArgs prep_args(const HeadCore& hd, const Aug& aug, const void* H, int dtype, int T) {
+  PrepArgs p{};
+  p.H = H;
+  p.dtype = dtype;
+  p.T = p.Tpad = T;
+  p.d = hd.d;
+  p.A = hd.A;
+  p.lda = hd.lda;
+  p.r = hd.r;
+  p.R = aug.R;
+  p.scale = hd.scale;
+  p.aug_layout = aug.layout;
+  p.aug_width = aug.width;
+  return p;
+}
+
+// The gradient passes of kernel rank R.
+struct Step {
+  const HeadCore& hd;
+  const DistillWs& w;
+  Aug aug;
+  int T, sms;
+  float tau;
+  cudaStream_t st;
+  GemmArgs g;      // pass 1's, filled
+  SlotPlan slots;  // out: pass 1's partials
+  int cparts2 = 0, n_b2 = 0, G2 = 0;
+  const float* Bt = nullptr;
+};
+
+constexpr const char* kNoMap = "cuTensorMapEncodeTiled failed";
+constexpr const char* kNoFit = "a GEMM pass cannot be made resident on this device";
+constexpr const char* kNoLaunch = "kernel launch failed";
+
+template <class Epi>
+int sums_pass1(Step& s, const char** why) {
+  const int d = s.hd.d;
+  CUtensorMap mh, mw, mha, mwa;
+  if (!make_map(&mh, s.w.h16, s.T, d, kBM) || !make_map(&mw, s.hd.W, s.hd.V, d, kBM))
+    return *why = kNoMap, LORA_CE_ECUDA;
+  mha = mh;
+  mwa = mw;
+  if (Epi::kAug && (!make_map(&mha, s.w.haug, s.T, s.aug.width, kBM) ||
+                    !make_map(&mwa, s.w.waug, s.hd.V, s.aug.width, kBM)))
+    return *why = kNoMap, LORA_CE_ECUDA;
+  const PassPlan p = sums_plan<Epi>(s.g.kblocks);
+  const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
+                                                       p.threads, p.smem));
+  if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
+  s.g.n_b = (int)(s.g.Vpad / kBN);
+  const int G = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
+  if (!launch_pairs(p.kern, G, p.threads, p.smem, s.st, mh, mw, mha, mwa, s.g))
+    return *why = kNoLaunch, LORA_CE_ECUDA;
+  s.slots = SlotPlan{col_parts(Epi::kWarps), s.g.n_a, s.g.n_b, units, s.g.Tcap,
+                     s.w.p_max, s.w.p_sum, nullptr, s.w.p_q};
+  return 0;
+}
+
+template <class Epi>
+int sums_pass2(Step& s, const char** why) {
+  const int d = s.hd.d;
+  CUtensorMap mh, mw, mha, mwa;
+  if (!make_map(&mh, s.w.h16, s.T, d, kBM) || !make_map(&mw, s.hd.W, s.hd.V, d, kBM))
+    return *why = kNoMap, LORA_CE_ECUDA;
+  mha = mh;
+  mwa = mw;
+  if (Epi::kAug && (!make_map(&mha, s.w.haug, s.T, s.aug.width, kBM) ||
+                    !make_map(&mwa, s.w.waug, s.hd.V, s.aug.width, kBM)))
+    return *why = kNoMap, LORA_CE_ECUDA;
+  const PassPlan p = sums_plan<Epi>(s.g.kblocks);
+  const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
+                                                       p.threads, p.smem));
+  if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
+  s.g.n_a = (s.hd.V + 2 * kBM - 1) / (2 * kBM);
+  s.g.n_b = s.n_b2 = (s.T + kBN - 1) / kBN;
+  s.G2 = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
+  s.cparts2 = col_parts(Epi::kWarps);
+  if (!launch_pairs(p.kern, s.G2, p.threads, p.smem, s.st, mw, mh, mwa, mha, s.g))
+    return *why = kNoLaunch, LORA_CE_ECUDA;
+  return 0;
+}
+
+template <int kPass, int R>
+int tc_pass(Step& s, const char** why) {
+  const int d = s.hd.d, V = s.hd.V, T = s.T, aw = s.aug.width;
+  const long long Tpad = round_up(T, kBN);
+  const int half = tc_bn(R) / 2;
+  CUtensorMap mres, mstr, mra, msa, mx;
+  const bool ok =
+      kPass == 1 ? make_map(&mres, s.w.h16, T, d, kBM) && make_map(&mstr, s.hd.W, V, d, half) &&
+                       make_map(&mra, s.w.haug, T, aw, kBM) &&
+                       make_map(&msa, s.w.waug, V, aw, half) &&
+                       make_map_ld(&mx, s.w.xv, 2 * R, V, s.g.Vpad, R)
+                 : make_map(&mres, s.hd.W, V, d, kBM) && make_map(&mstr, s.w.h16, T, d, half) &&
+                       make_map(&mra, s.w.waug, V, aw, kBM) &&
+                       make_map(&msa, s.w.haug, T, aw, half) &&
+                       make_map_ld(&mx, s.w.xt, 2 * R, T, Tpad, R);
+  if (!ok) return *why = kNoMap, LORA_CE_ECUDA;
+  s.g.stages = TcLayout::stages(s.g.kblocks, R);
+  s.g.drain_gain = (float)(1.0 + acc_short(2 * tc_drain(R) * tc_bn(R) / 16, 0));
+  const int smem = TcLayout::bytes(s.g.kblocks, s.g.stages, R);
+  auto kern = lce_gemm_tc<kPass, R, true>;
+  if (s.g.stages < 2 || smem > kMaxDynSmem) return *why = kNoFit, LORA_CE_ECUDA;
+  const int units =
+      std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(kern), kThreadsT, smem));
+  if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
+  s.g.n_a = ((kPass == 1 ? T : V) + 2 * kBM - 1) / (2 * kBM);
+  s.g.n_b = ((kPass == 1 ? V : T) + tc_bn(R) - 1) / tc_bn(R);
+  const int G = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
+  if (!launch_pairs(kern, G, kThreadsT, smem, s.st, mres, mstr, mra, msa, mx, s.g))
+    return *why = kNoLaunch, LORA_CE_ECUDA;
+  if (kPass == 1) {
+    s.slots = SlotPlan{2, s.g.n_a, s.g.n_b, units, s.g.Tcap, s.w.p_max, s.w.p_sum, nullptr,
+                       s.w.p_q};
+  } else {
+    s.n_b2 = s.g.n_b;
+    s.G2 = G;
+    s.cparts2 = 1;
+  }
+  return 0;
+}
+
+template <int kPass>
+int grad_pass(Step& s, int R, const char** why) {
+  switch (R) {
+    case 4:
+      if constexpr (kPass == 1) return sums_pass1<EpiLse<4, false, false, true>>(s, why);
+      else return sums_pass2<EpiGrad<4, false, false, true>>(s, why);
+    case 8:
+      if constexpr (kPass == 1) return sums_pass1<EpiLse<8, true, false, true>>(s, why);
+      else return sums_pass2<EpiGrad<8, true, false, true>>(s, why);
+    case 16: return tc_pass<kPass, 16>(s, why);
+    case 32: return tc_pass<kPass, 32>(s, why);
+    default: return tc_pass<kPass, 64>(s, why);
+  }
+}
+
+template <int RC>
+void launch_dA(const Step& s, int R, const DistillWs& w) {
+  const int n_chunks = (s.T + kDAChunk - 1) / kDAChunk;
+  for (int r0 = 0; r0 < R; r0 += RC)
+    lce_dA_partial<RC><<<dim3(n_chunks, s.hd.d / 64), dim3(32, da_rows(RC)), 0, s.st>>>(
+        s.T, s.hd.d, w.h16, w.dU, w.gAp, R, r0);
+}
+
+}  // namespace
+
+namespace lce {
+
+size_t head_score_bytes(const HeadCore& hd, int T, int top_k) {
+  return score_ws(hd, T, top_k, nullptr).bytes;
+}
+
+size_t head_distill_bytes(const HeadCore& hd, int T, int, bool grads) {
+  return distill_ws(hd, T, grads, nullptr).bytes;
+}
+
+int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const int32_t* tokens,
+                   int top_k, float* logprob, float* entropy, int32_t* top_ids,
+                   float* top_logprobs, void* ws, cudaStream_t st, const char** why) {
+  const Aug aug = aug_of(hd.r);
+  const ScoreWs w = score_ws(hd, T, top_k, ws);
+  const int sms = sm_count();
+  GemmArgs g{};
+  fill_pass1(g, hd, aug, T, 1.0f);
+  g.n_b = (int)(g.Vpad / kBN);
+  g.err = w.stats + kStErr;
+  g.p_max = w.p_max;
+  g.p_sum = w.p_sum;
+  g.p_ent = w.p_ent;
+  g.sub_max = w.sub_max;
+  g.sub_second = w.sub_second;
+  g.sub_rest = w.sub_rest;
+  g.sub_arg = w.sub_arg;
+  g.sub_arg2 = w.sub_arg2;
+  g.sub_ld = w.sub_ld;
+  const PassPlan p = w.sub == 64  ? score_plan<64>(g.kblocks)
+                     : w.sub == 8 ? score_plan<8>(g.kblocks) : score_plan<1>(g.kblocks);
+  const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
+                                                       p.threads, p.smem));
+  if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
+  CUtensorMap mh, mw, mha, mwa;
+  if (!make_map(&mh, w.h16, T, hd.d, kBM) || !make_map(&mw, hd.W, hd.V, hd.d, kBM))
+    return *why = kNoMap, LORA_CE_ECUDA;
+  mha = mh;
+  mwa = mw;
+  if (aug.R && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
+                !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
+    return *why = kNoMap, LORA_CE_ECUDA;
+  // per-row kernel: a warp per position, or the whole block where positions
+  // are too few to fill the SMs that way
+  ScoreArgs a{};
+  a.n_sub = w.n_sub;
+  a.sub = w.sub;
+  a.top_k = top_k;
+  a.n_pick = std::min(w.n_sub, std::max(top_k, kMinPick));
+  a.cap = 2 * score_picks(a.n_pick) + top_k + 64;
+  const size_t team = score_team_smem(a.n_pick, a.cap);
+  const bool warps = T >= sms * kRowWarps && w.n_sub <= 32 * 32;
+  void (*rows)(ScoreArgs) = warps ? lh_score_rows<1, 32>
+                            : w.n_sub <= 8 * 256 ? lh_score_rows<kRowWarps, 8>
+                                                 : lh_score_rows<kRowWarps, 32>;
+  const size_t rows_smem = warps ? team * kRowWarps : team;
+  if (!allow_smem(reinterpret_cast<const void*>(rows), rows_smem))
+    return *why = kNoFit, LORA_CE_ECUDA;
+
+  PrepArgs pa = prep_args(hd, aug, H, dtype, T);
+  pa.h16 = w.h16;
+  pa.sU = w.sU;
+  pa.haug = aug.R ? w.haug : nullptr;
+  pa.stats = w.stats;
+  PackArgs pk{};
+  pk.B = BView{hd.B, hd.V, hd.r, aug.R, hd.layout};
+  pk.V = hd.V;
+  pk.r = hd.r;
+  pk.R = aug.R;
+  pk.Vpad = g.Vpad;
+  pk.waug = w.waug;
+  pk.aug_layout = aug.layout;
+  pk.aug_width = aug.width;
+  if (launch_prep(pa, pk, true, 0, aug.R != 0, sms, st)) return *why = kNoFit, LORA_CE_ECUDA;
+  const int G = (int)std::min<long long>(units, (long long)g.n_a * g.n_b);
+  if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, g))
+    return *why = kNoLaunch, LORA_CE_ECUDA;
+  a.z = logit_args(hd, aug, T, w.h16, w.sU);
+  a.p = SlotPlan{col_parts(EpiScore<65536, 64>::kWarps), g.n_a, g.n_b, units, g.Tcap,
+                 w.p_max, w.p_sum, w.p_ent, nullptr};
+  a.lg = g.lg;
+  a.sub_ld = w.sub_ld;
+  a.sub_max = w.sub_max;
+  a.sub_second = w.sub_second;
+  a.sub_rest = w.sub_rest;
+  a.sub_arg = w.sub_arg;
+  a.sub_arg2 = w.sub_arg2;
+  a.tokens = tokens;
+  a.stats = w.stats;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.top_ids = top_ids;
+  a.top_logprobs = top_logprobs;
+  rows<<<warps ? (T + kRowWarps - 1) / kRowWarps : T, 32 * kRowWarps, rows_smem, st>>>(a);
+  if (cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
+  return 0;
+}
+
+int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
+                     const int32_t* ids, const float* teacher, float tau, const float* weight,
+                     float* loss, const GradOut& out, void* ws, cudaStream_t st,
+                     const char** why) {
+  const bool grads = out.gA != nullptr;
+  Aug aug = aug_of(hd.r);
+  const int R = aug.R;
+  const DistillWs w = distill_ws(hd, T, grads, ws);
+  const bool tc = grads && R >= 16;
+  if (grads && R == 4) aug.layout = aug.width = 0;
+  Step s{hd, w, aug, T, sm_count(), tau, st, GemmArgs{}, SlotPlan{}};
+  fill_pass1(s.g, hd, aug, T, tau);
+  s.Bt = hd.layout ? hd.B : w.Bt;
+  s.g.err = w.stats + kStErr;
+  s.g.p_max = w.p_max;
+  s.g.p_sum = w.p_sum;
+  s.g.p_q = w.p_q;
+  s.g.tok = w.tok;
+  s.g.Bt = s.Bt;
+  s.g.gBp = w.gBp;
+  s.g.nml = w.nml;
+
+  if (cudaMemsetAsync(w.stats, 0, w.zero_bytes, st) != cudaSuccess)
+    return *why = "cudaMemsetAsync failed", LORA_CE_ECUDA;
+  PrepArgs pa = prep_args(hd, aug, H, dtype, T);
+  pa.h16 = w.h16;
+  pa.sU = w.sU;
+  pa.haug = aug.width ? w.haug : nullptr;
+  pa.stats = w.stats;
+  pa.ids = ids;
+  pa.weight = weight;
+  pa.K = K;
+  pa.tau = tau;
+  pa.wt = w.wt;
+  if (grads && !tc) {
+    pa.tok = w.tok;
+    pa.Tpad = (int)round_up(T, kBN);
+  }
+  PackArgs pk{};
+  pk.B = BView{hd.B, hd.V, hd.r, R, hd.layout};
+  pk.V = hd.V;
+  pk.r = hd.r;
+  pk.R = R;
+  pk.Vpad = s.g.Vpad;
+  pk.Bt = grads && !hd.layout ? w.Bt : nullptr;
+  pk.waug = aug.width ? w.waug : nullptr;
+  pk.aug_layout = aug.layout;
+  pk.aug_width = aug.width;
+  pk.xv = tc ? w.xv : nullptr;
+  pk.stats = w.stats;
+  const bool pack = pk.Bt || pk.waug || pk.xv;
+  // the scale of xv needs the largest |B| first
+  if (launch_prep(pa, pk, true, tc ? 2 * s.sms : 0, pack && !tc, s.sms, st) ||
+      (tc && launch_prep(pa, pk, false, 0, true, s.sms, st)))
+    return *why = kNoFit, LORA_CE_ECUDA;
+
+  int rc = 0;
+  if (grads) {
+    rc = grad_pass<1>(s, R, why);
+  } else {
+    const PassPlan p = score_plan<0>(s.g.kblocks);
+    const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
+                                                         p.threads, p.smem));
+    if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
+    CUtensorMap mh, mw, mha, mwa;
+    if (!make_map(&mh, w.h16, T, hd.d, kBM) || !make_map(&mw, hd.W, hd.V, hd.d, kBM))
+      return *why = kNoMap, LORA_CE_ECUDA;
+    mha = mh;
+    mwa = mw;
+    if (R && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
+              !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
+      return *why = kNoMap, LORA_CE_ECUDA;
+    s.g.n_b = (int)(s.g.Vpad / kBN);
+    const int G = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
+    if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, s.g))
+      rc = (*why = kNoLaunch, LORA_CE_ECUDA);
+    s.slots = SlotPlan{col_parts(EpiScore<65536, 0>::kWarps), s.g.n_a, s.g.n_b, units,
+                       s.g.Tcap, w.p_max, w.p_sum, nullptr, nullptr};
+  }
+  if (rc) return rc;
+  DistillArgs a{};
+  a.z = logit_args(hd, aug, T, w.h16, w.sU);
+  a.z.R = R;
+  a.z.B.R = R;
+  a.p = s.slots;
+  a.lg = s.g.lg;
+  a.tau = tau;
+  a.scale = hd.scale;
+  a.K = K;
+  a.ids = ids;
+  a.teacher = teacher;
+  a.wt = w.wt;
+  a.Bt = s.Bt;
+  a.stats = w.stats;
+  a.loss = loss;
+  a.tok = grads && !tc ? w.tok : nullptr;
+  a.nml = tc ? w.nml : nullptr;
+  a.dU = w.dU;
+  a.corr = w.corr;
+  const bool warps = T >= s.sms * kRowWarps;
+  auto rows = grads ? (warps ? lh_distill_rows<true, 1> : lh_distill_rows<true, kRowWarps>)
+                    : (warps ? lh_distill_rows<false, 1> : lh_distill_rows<false, kRowWarps>);
+  rows<<<warps ? (T + kRowWarps - 1) / kRowWarps : T, 32 * kRowWarps, 0, st>>>(a);
+  if (!grads) {
+    if (cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
+    return 0;
+  }
+  if (tc) {
+    const long long n = (long long)T * R;
+    lh_xt<<<(int)std::min<long long>((n + 255) / 256, 8LL * s.sms), 256, 0, st>>>(
+        T, R, round_up(T, kBN), w.sU, w.wt, w.stats, w.xt);
+  }
+  if ((rc = grad_pass<2>(s, R, why))) return rc;
+  switch (R) {
+    case 4: launch_dA<4>(s, R, w); break;
+    case 8: launch_dA<8>(s, R, w); break;
+    default: launch_dA<16>(s, R, w); break;
+  }
+  GradArgs ga{};
+  ga.T = T;
+  ga.d = hd.d;
+  ga.V = hd.V;
+  ga.r = hd.r;
+  ga.R = R;
+  ga.n_chunks = (T + kDAChunk - 1) / kDAChunk;
+  ga.cparts = s.cparts2;
+  ga.res_rows = 2 * kBM;
+  ga.n_b2 = s.n_b2;
+  ga.G2 = s.G2;
+  ga.Vpad = s.g.Vpad;
+  ga.gAp = w.gAp;
+  ga.gBp = w.gBp;
+  ga.corr = w.corr;
+  ga.scaled = tc;
+  ga.stats = w.stats;
+  ga.gA = out.gA;
+  ga.gB = out.gB;
+  ga.layout = out.layout;
+  ga.loss = loss;
+  ga.wt = w.wt;
+  ga.tail = out.tail;
+  const int a_blocks = ((out.layout ? R : hd.r) * hd.d + 255) / 256;
+  lh_grads<<<(int)(s.g.Vpad / kPackRows) + a_blocks, 256, 0, st>>>(ga);
+  if (cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
+  return 0;
+}
+
+}  // namespace lce
+
+namespace {
+
+int check_head(const lora_head* h, int T) {
+  if (!h) return hfail(LORA_CE_EINVAL, "null head");
+  if (h->dim < 64 || h->dim % 64 != 0 || h->dim > 64 * kMaxHead64)
+    return hfail(LORA_CE_EINVAL, "dim must be a multiple of 64 in [64, 640]");
+  if (h->vocab < 1 || h->vocab > (1 << 19))
+    return hfail(LORA_CE_EINVAL, "vocab must be in [1, 2^19]");
+  if (h->rank < 0 || h->rank > kMaxFusedRank)
+    return hfail(LORA_CE_EINVAL, "rank must be in [0, 64]");
+  if (!std::isfinite(h->scale)) return hfail(LORA_CE_EINVAL, "scale must be finite");
+  if (T < 1 || T > LORA_HEAD_MAX_TOKENS) return hfail(LORA_CE_EINVAL, "T must be in [1, 2^20]");
+  return 0;
+}
+
+HeadCore core_of(const lora_head* h) {
+  return HeadCore{reinterpret_cast<const __half*>(h->W), h->A, h->rank, h->B, 0,
+                  h->dim, h->vocab, h->rank, h->scale};
+}
+
+// Every buffer is memory of the current device, with its alignment.
+struct Buffers {
+  int dev = -1;
+  int rc = 0;
+  void need(const void* p, uintptr_t align, const char* name) {
+    if (rc) return;
+    if (!p) {
+      rc = hfail(LORA_CE_EINVAL, "");
+      g_head_error = std::string(name) + " is null";
+      return;
+    }
+    if (reinterpret_cast<uintptr_t>(p) % align != 0) {
+      rc = hfail(LORA_CE_EINVAL, "");
+      g_head_error = std::string(name) + " must be " + std::to_string(align) + "-byte aligned";
+    }
+  }
+  // after every need(): where the memory is
+  void here(const void* p, const char* name) {
+    if (rc || !p) return;
+    if (dev < 0 && cudaGetDevice(&dev) != cudaSuccess) {
+      rc = hfail(LORA_CE_ECUDA, "no CUDA device");
+      cudaGetLastError();
+      return;
+    }
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+      cudaGetLastError();
+      at.type = cudaMemoryTypeUnregistered;
+    }
+    if ((at.type != cudaMemoryTypeDevice || at.device != dev) && at.type != cudaMemoryTypeManaged) {
+      rc = hfail(LORA_CE_EINVAL, "");
+      g_head_error = std::string(name) + " is not memory of the current device";
+    }
+  }
+};
+
+int check_arch() {
+  static std::mutex mu;
+  static std::map<int, int> major;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return hfail(LORA_CE_ECUDA, "no CUDA device");
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = major.find(dev);
+  if (it == major.end()) {
+    int m = 0;
+    if (cudaDeviceGetAttribute(&m, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
+      return hfail(LORA_CE_ECUDA, "cudaDeviceGetAttribute failed");
+    it = major.emplace(dev, m).first;
+  }
+  if (it->second != 10) return hfail(LORA_CE_ECUDA, "this library runs on sm_100 (B200) only");
+  if (!encode_fn()) return hfail(LORA_CE_ECUDA, "cuTensorMapEncodeTiled unavailable");
+  return 0;
+}
+
+int check_score(const lora_head* h, int T, int top_k) {
+  if (int rc = check_head(h, T)) return rc;
+  if (top_k < 0 || top_k > LORA_HEAD_MAX_TOP || top_k > h->vocab)
+    return hfail(LORA_CE_EINVAL, "top_k must be in [0, 128] and no more than vocab");
+  return 0;
+}
+
+int check_distill(const lora_head* h, int T, int K, bool grads) {
+  if (int rc = check_head(h, T)) return rc;
+  if (K < 1 || K > LORA_HEAD_MAX_TOP) return hfail(LORA_CE_EINVAL, "K must be in [1, 128]");
+  if (grads && h->rank < 1) return hfail(LORA_CE_EINVAL, "gradients need a rank of at least 1");
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* lora_head_last_error(void) { return g_head_error.c_str(); }
+
+size_t lora_head_score_workspace(const lora_head* h, int32_t T, int32_t top_k) {
+  return check_score(h, T, top_k) ? 0 : head_score_bytes(core_of(h), T, top_k);
+}
+
+size_t lora_head_distill_workspace(const lora_head* h, int32_t T, int32_t K, int32_t grads) {
+  return check_distill(h, T, K, grads != 0) ? 0 : head_distill_bytes(core_of(h), T, K, grads != 0);
+}
+
+int lora_head_score(const lora_head* h, const void* H, int32_t h_dtype, int32_t T,
+                    const int32_t* tokens, int32_t top_k, float* logprob, float* entropy,
+                    int32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes,
+                    void* stream) {
+  if (int rc = check_score(h, T, top_k)) return rc;
+  if (h_dtype < LORA_CE_BF16 || h_dtype > LORA_CE_F32)
+    return hfail(LORA_CE_EINVAL, "bad hidden-state dtype");
+  if ((tokens == nullptr) != (logprob == nullptr))
+    return hfail(LORA_CE_EINVAL, "tokens and logprob go together");
+  if (!logprob && !entropy && top_k == 0) return hfail(LORA_CE_EINVAL, "nothing is asked for");
+  Buffers b;
+  struct {
+    const void* p;
+    uintptr_t align;
+    const char* name;
+    bool used;
+  } all[] = {{h->W, 16, "W", true},
+             {h->A, 4, "A", h->rank > 0},
+             {h->B, 4, "B", h->rank > 0},
+             {H, 16, "H", true},
+             {tokens, 4, "tokens", tokens != nullptr},
+             {logprob, 4, "logprob", logprob != nullptr},
+             {entropy, 4, "entropy", entropy != nullptr},
+             {top_ids, 4, "top_ids", top_k > 0},
+             {top_logprobs, 4, "top_logprobs", top_k > 0},
+             {ws, 256, "workspace", true}};
+  for (const auto& x : all)
+    if (x.used) b.need(x.p, x.align, x.name);
+  if (!b.rc && ws_bytes < head_score_bytes(core_of(h), T, top_k))
+    return hfail(LORA_CE_EINVAL, "workspace too small");
+  for (const auto& x : all)
+    if (x.used) b.here(x.p, x.name);
+  if (b.rc) return b.rc;
+  if (int rc = check_arch()) return rc;
+  const char* why = "";
+  const int rc = head_score_run(core_of(h), H, h_dtype, T, tokens, top_k, logprob, entropy,
+                                top_ids, top_logprobs, ws, static_cast<cudaStream_t>(stream), &why);
+  return rc ? hfail(rc, why) : 0;
+}
+
+int lora_head_distill(const lora_head* h, const void* H, int32_t h_dtype, int32_t T, int32_t K,
+                      const int32_t* ids, const float* teacher, float temperature,
+                      const float* weight, float* loss, float* gA, float* gB, void* ws,
+                      size_t ws_bytes, void* stream) {
+  if ((gA == nullptr) != (gB == nullptr))
+    return hfail(LORA_CE_EINVAL, "gA and gB go together");
+  const bool grads = gA != nullptr;
+  if (int rc = check_distill(h, T, K, grads)) return rc;
+  if (h_dtype < LORA_CE_BF16 || h_dtype > LORA_CE_F32)
+    return hfail(LORA_CE_EINVAL, "bad hidden-state dtype");
+  if (!(temperature >= 0.01f && temperature <= 100.0f))
+    return hfail(LORA_CE_EINVAL, "temperature must be in [0.01, 100]");
+  Buffers b;
+  struct {
+    const void* p;
+    uintptr_t align;
+    const char* name;
+    bool used;
+  } all[] = {{h->W, 16, "W", true},
+             {h->A, 4, "A", h->rank > 0},
+             {h->B, 4, "B", h->rank > 0},
+             {H, 16, "H", true},
+             {ids, 4, "ids", true},
+             {teacher, 4, "teacher", true},
+             {weight, 4, "weight", weight != nullptr},
+             {loss, 4, "loss", true},
+             {gA, 4, "gA", grads},
+             {gB, 4, "gB", grads},
+             {ws, 256, "workspace", true}};
+  for (const auto& x : all)
+    if (x.used) b.need(x.p, x.align, x.name);
+  if (!b.rc && ws_bytes < head_distill_bytes(core_of(h), T, K, grads))
+    return hfail(LORA_CE_EINVAL, "workspace too small");
+  for (const auto& x : all)
+    if (x.used) b.here(x.p, x.name);
+  if (b.rc) return b.rc;
+  if (int rc = check_arch()) return rc;
+  const char* why = "";
+  const int rc = head_distill_run(core_of(h), H, h_dtype, T, K, ids, teacher, temperature, weight,
+                                  loss, GradOut{gA, gB, 0, nullptr}, ws,
+                                  static_cast<cudaStream_t>(stream), &why);
+  return rc ? hfail(rc, why) : 0;
+}
+
+}  // extern "C"

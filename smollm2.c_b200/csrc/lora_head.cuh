@@ -1,0 +1,1185 @@
+// lora_head.cuh — device code of the operators on the LoRA head: token log
+// probabilities with entropy and top alternatives (score), and distillation
+// from a teacher's top logits (distill).  Both form
+//   z[t][v] = h[t].W[v] + s (h[t].A).B[:,v],   h = f16(H)
+// in the GEMM passes of lora_ce_kernels.cuh and lora_ce_tc.cuh; this file has
+// the epilogue and the per-row kernels that are theirs alone.
+//
+// Accuracy.  tcgen05 truncates towards zero when it adds a K-step's 16
+// products to the f32 accumulator, half a unit in the last place on average.
+// Where a logit is large its partial sums grow about linearly over the n
+// K-steps, and the mean of ulp(x) / x over a binade is 2^-23 / (2 ln 2), which
+// makes the accumulator fall short by z (n + 1) 2^-26 / ln 2.  Measured against
+// 64-bit sums over logits from 3 to 15: 0.79 of that at hidden sizes 64, 128
+// and 576 alike (6.2e-7 z at 576, with a spread of 1.6e-7 z; an f32 product of
+// a library has no shortfall and a spread of 3e-7 z).  acc_short() gives the
+// measured share and the softmax's exponent factor makes it good
+// (GemmArgs::lg).  Sums of many terms go in two levels (EpiLse, lce_gemm_tc).
+// Gradients of 8192 positions against 64 bits, where a bias adds up and
+// rounding does not: rank 4 9e-6 with neither, 6e-6 with the factor, 4e-7 with
+// both; rank 64 2e-5, 1.5e-5, 4e-7 (a library's f32 products: 2e-6 to 3e-6).
+// Few logits decide more than a sum: those of given tokens, of a teacher's
+// entries and of the alternatives (whose order has to be that of the exact
+// logits) are computed again from the f16 operands with 64-bit sums.
+#pragma once
+#include "lora_ce_kernels.cuh"
+
+namespace lce {
+
+constexpr int kMaxTop = 128;      // largest top_k, largest teacher list
+constexpr int kMinPick = 8;       // logits of a row that are computed again at least
+constexpr int kPickSlack = 16;    // records picked beyond that, to end the search early
+constexpr int kRowWarps = 8;      // warps per block of the per-row kernels
+constexpr int kMaxHead64 = 10;    // hidden size in units of 64
+
+// Device words at the start of a workspace.
+enum : int { kStErr = 0, kStBMax = 1, kStUMax = 2, kStatWords = 64 };
+
+// B of the head: [r][V] (layout 0), or the pair-interleaved layout of a
+// trainer's handle at kernel rank R (layout 1, bidx).
+struct BView {
+  const float* p;
+  long long V;
+  int r, R, layout;
+  __device__ __forceinline__ float at(int j, long long v) const {
+    return layout ? p[bidx(v, j, R)] : p[(long long)j * V + v];
+  }
+};
+
+// ------------------------------------------------------------- pass over z
+// The thread owns position t; columns are vocab ids (as EpiLse, without the
+// rank sums).  Per column: the online max and sum(exp) in units of log2.
+// kSub 0 is that alone (a loss).  Otherwise also the entropy sum and records
+// from which lh_score_rows picks the alternatives:
+//   kSub 64: per 64 columns the largest logit, the second largest of its 8-column
+//            chunks' maxima, both with their columns, and the largest of the rest
+//   kSub 8:  per 8 columns the largest, its column, the largest of the rest
+//   kSub 1:  the logit
+// A row's k largest logits lie in the k records with the largest maxima: were
+// one outside, k records would each hold a logit that precedes it.  So 14
+// bytes stand for 64 logits, and the columns of a record are computed again
+// only where its rest reaches into the k largest: for random rows at k = 64,
+// V = 49152 about four records in ten rows (with one logit per record only,
+// and none for the second, it was 2.7 records a row).  Fewer columns per record
+// where the vocabulary gives less than 4 records per alternative.
+// Issue slots per logit: 2 for kSub 0, about 9 for kSub 64, beside the 18 that
+// one SM has while its tensor core forms a 128 x 256 x 576 tile: the pass stays
+// bound by the MMAs and the loads of W.
+template <int kRing_, int kSub>
+struct EpiScore {
+  static constexpr bool kAug = true;
+  static constexpr int kRec = 0;
+  static constexpr int kRing = kRing_;
+  static constexpr int kRecBufs = 1;
+  static constexpr int kWarps = 16;
+  static constexpr int kCW = 8;
+  static constexpr bool kTop = kSub != 0;
+  int t;
+  bool valid;
+  float m, mL;   // reference max, m * lg
+  float2 s2;     // sum of e over even / odd columns
+  float2 e2s;    // sum of e * x, x the exponent in log2 units
+  float S, Slo, E, Elo;  // the same over the row so far, folded every 64 columns (as EpiLse)
+  float r1, r2, rest;    // kSub 64: the record so far
+  int a1, a2;
+
+  __device__ static const float* global_recs(const GemmArgs& g, int) { return g.Bt; }
+  __device__ static int limit(const GemmArgs& g) { return g.V; }
+
+  __device__ void begin(const GemmArgs& g, int abs_row) {
+    t = abs_row;
+    valid = t < g.T;
+    m = mL = -INFINITY;
+    s2 = e2s = f2(0.f, 0.f);
+    S = Slo = E = Elo = 0.f;
+    r1 = r2 = rest = -INFINITY;
+    a1 = a2 = 0;
+  }
+
+  // Adds the chunk's terms at reference nm = -(reference max) * lg.
+  template <bool kTail>
+  __device__ __forceinline__ void sum(const float (&z)[kCW], float2 L2, float nm) {
+    const float2 nm2 = f2(nm, nm);
+#pragma unroll
+    for (int p = 0; p < kCW / 2; ++p) {
+      float2 x2 = __ffma2_rn(f2(z[2 * p], z[2 * p + 1]), L2, nm2);
+      if (kTail && kTop) {  // masked columns: e = 0 and e * x = 0, not 0 * inf
+        x2.x = fmaxf(x2.x, -1e30f);
+        x2.y = fmaxf(x2.y, -1e30f);
+      }
+      const float2 e2 = f2(ex2f(x2.x), ex2f(x2.y));
+      s2 = __fadd2_rn(s2, e2);
+      if constexpr (kTop) e2s = __ffma2_rn(e2, x2, e2s);
+    }
+  }
+
+  template <bool kTail>
+  __device__ __forceinline__ void chunk(const GemmArgs& g, int v0, float (&acc)[kCW],
+                                        const float*) {
+    if (kTail) {
+#pragma unroll
+      for (int i = 0; i < kCW; ++i)
+        if (v0 + i >= g.V) acc[i] = -INFINITY;
+    }
+    float cm = -INFINITY;
+    if constexpr (kSub > 1) {
+      float c2 = -INFINITY;
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < kCW; ++i) {
+        const float z = acc[i];
+        c2 = fmaxf(c2, fminf(cm, z));
+        at = z > cm ? i : at;  // the lowest column among equals
+        cm = fmaxf(cm, z);
+      }
+      if constexpr (kSub == 8) {
+        if (valid && v0 < g.V) {
+          const long long o = (long long)(v0 / 8) * g.sub_ld + t;
+          g.sub_max[o] = cm;
+          g.sub_rest[o] = c2;
+          g.sub_arg[o] = (uint8_t)at;
+        }
+      } else {
+        at += v0 & 63;
+        if ((v0 & 63) == 0) {
+          r1 = cm;
+          a1 = at;
+          r2 = -INFINITY;
+          a2 = 0;
+          rest = c2;
+        } else {
+          const bool gt = cm > r1;
+          const float lo = fminf(cm, r1);
+          const int lo_at = gt ? a1 : at;
+          a1 = gt ? at : a1;
+          r1 = fmaxf(cm, r1);
+          rest = fmaxf(fmaxf(rest, c2), fminf(r2, lo));
+          a2 = lo > r2 ? lo_at : a2;
+          r2 = fmaxf(r2, lo);
+        }
+        if ((v0 & 63) == 64 - kCW && valid && v0 - (64 - kCW) < g.V) {
+          const long long o = (long long)(v0 / 64) * g.sub_ld + t;
+          g.sub_max[o] = r1;
+          g.sub_second[o] = r2;
+          g.sub_rest[o] = rest;
+          g.sub_arg[o] = (uint8_t)a1;
+          g.sub_arg2[o] = (uint8_t)a2;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCW; ++i) {
+        cm = fmaxf(cm, acc[i]);
+        if (kSub == 1 && valid && v0 + i < g.V) g.sub_max[(long long)(v0 + i) * g.sub_ld + t] = acc[i];
+      }
+    }
+    if (kTail && v0 >= g.V) return;
+    const float2 L2 = f2(g.lg, g.lg);
+    if (cm > m + g.lazy) {  // the reference moves before the chunk is added
+      const float f = ex2f((m - cm) * g.lg);  // 0 when m = -inf
+      if constexpr (kTop) {
+        // x counts from the new reference: sum e (x - delta)
+        const float delta = m == -INFINITY ? 0.f : (cm - m) * g.lg;
+        e2s = f2(f * fmaf(-delta, s2.x, e2s.x), f * fmaf(-delta, s2.y, e2s.y));
+        E = f * (fmaf(-delta, S, E) + fmaf(-delta, Slo, Elo));
+        Elo = 0.f;
+      }
+      s2 = f2(s2.x * f, s2.y * f);
+      S *= f;
+      Slo *= f;
+      m = cm;
+      mL = cm * g.lg;
+    }
+    __syncwarp();  // rejoin before the next warp-wide TMEM load
+    sum<kTail>(acc, L2, -mL);
+    if (((v0 + kCW) & 63) == 0) fold();
+  }
+
+  __device__ __forceinline__ void fold() {
+    fold_sum(s2, S, Slo);
+    if constexpr (kTop) fold_sum(e2s, E, Elo);
+  }
+
+  __device__ void flush(const GemmArgs& g, int slot) {
+    if (!valid) return;
+    const long long o = (long long)slot * g.Tcap + t;
+    g.p_max[o] = m;
+    fold();
+    g.p_sum[o] = S + Slo;
+    if constexpr (kTop) g.p_ent[o] = E + Elo;
+  }
+};
+
+// ------------------------------------------------------------- preparation
+struct PrepArgs {
+  const void* H;
+  int dtype, T, Tpad, d;
+  const float* A;  // [d][lda], r columns used
+  int lda, r, R;   // R: r rounded up to a kernel rank; 0 without an adapter
+  float scale;
+  __half* h16;     // [T][d]
+  double* sU;      // [T][R] s * U
+  float* tok;      // records (tidx layout) or null
+  __half* haug;    // [T][aug_width] or null
+  int aug_layout, aug_width;
+  // distillation: teacher lists and weights; wt[t] = weight * temperature of a
+  // position that has at least one entry, else 0 (and its hidden state is read
+  // as zeros, whatever it holds)
+  const int32_t* ids;
+  const float* weight;
+  int K;
+  float tau;
+  float* wt;
+  int* stats;
+};
+
+// h16, U = h16.A with 64-bit sums, and what the passes read of them: one
+// warp per P positions.  Lane l sums ranks l % RL, (+ 32) over every
+// (32 / RL)-th hidden element, so the A loads are contiguous across lanes and
+// shared by the P positions.
+template <int P>
+__device__ __forceinline__ void prep_rows(const PrepArgs& a, int t0, float* sh) {
+  const int lane = threadIdx.x & 31;
+  const int R = a.R;
+  float wt[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int t = t0 + p;
+    wt[p] = 0.f;
+    if (t >= a.T) continue;
+    bool active = true;
+    if (a.ids) {
+      bool any = false;
+      for (int k = lane; k < a.K; k += 32) any |= a.ids[(long long)t * a.K + k] >= 0;
+      const float w = a.weight ? a.weight[t] : 1.0f;
+      active = __any_sync(0xffffffffu, any) && w != 0.f;
+      wt[p] = active ? w * a.tau : 0.f;
+      if (lane == 0) a.wt[t] = wt[p];
+    }
+    for (int i = 2 * lane; i < a.d; i += 64) {
+      const long long o = (long long)t * a.d + i;
+      float2 x = make_float2(0.f, 0.f);
+      if (active) {
+        if (a.dtype == 0) x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(
+                              reinterpret_cast<const __nv_bfloat16*>(a.H) + o));
+        else if (a.dtype == 1) x = __half22float2(*reinterpret_cast<const __half2*>(
+                                   reinterpret_cast<const __half*>(a.H) + o));
+        else x = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(a.H) + o);
+      }
+      const __half2 hv = __floats2half2_rn(x.x, x.y);
+      *reinterpret_cast<__half2*>(a.h16 + o) = hv;
+      *reinterpret_cast<float2*>(sh + p * a.d + i) = __half22float2(hv);
+    }
+  }
+  if (R == 0) return;
+  __syncwarp();
+  const int RL = R < 32 ? R : 32, jl = lane & (RL - 1), sl = lane / RL, ns = 32 / RL;
+  double u[P][2];
+#pragma unroll
+  for (int p = 0; p < P; ++p) u[p][0] = u[p][1] = 0.0;
+  const bool two = R > 32;
+#pragma unroll 4
+  for (int i = sl; i < a.d; i += ns) {
+    const double a0 = jl < a.r ? (double)a.A[(long long)i * a.lda + jl] : 0.0;
+    const double a1 = two && jl + 32 < a.r ? (double)a.A[(long long)i * a.lda + jl + 32] : 0.0;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const double h = t0 + p < a.T ? (double)sh[p * a.d + i] : 0.0;
+      u[p][0] = fma(h, a0, u[p][0]);
+      if (two) u[p][1] = fma(h, a1, u[p][1]);
+    }
+  }
+  float umax = 0.f;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int t = t0 + p;
+    for (int off = RL; off < 32; off <<= 1) u[p][0] += __shfl_xor_sync(0xffffffffu, u[p][0], off);
+    if (t < a.T) {
+      if (sl == 0) {
+        for (int q = 0; q < (two ? 2 : 1); ++q) {
+          const int j = jl + 32 * q;
+          const double su = (double)a.scale * u[p][q];
+          a.sU[(long long)t * R + j] = su;
+          const float f = (float)su;
+          if (a.tok) a.tok[tidx(t, j, R)] = f;
+          if (a.haug) {
+            const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
+            __half* row = a.haug + (long long)t * a.aug_width;
+            row[j] = hi;
+            if (a.aug_layout == 1) {  // [hi | hi | lo | 0]
+              row[R + j] = hi;
+              row[2 * R + j] = lo;
+              for (int c = 3 * R + j; c < a.aug_width; c += R) row[c] = __float2half_rn(0.f);
+            } else {  // [hi | lo]
+              row[R + j] = lo;
+            }
+          }
+          const float m = fabsf(wt[p] * f);
+          if (isfinite(m)) umax = fmaxf(umax, m);
+        }
+      }
+      if (a.tok && lane == 0)  // -M lg, weight / S: lh_distill_rows
+        for (int f = R; f < R + 4; ++f) a.tok[tidx(t, f, R)] = 0.f;
+    } else if (t < a.Tpad && a.tok) {
+      for (int f = lane; f < tok_stride(R); f += 32) a.tok[tidx(t, f, R)] = 0.f;
+    }
+  }
+  if (a.ids && a.stats) {
+    const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(umax));
+    if (lane == 0 && m) atomicMax(reinterpret_cast<unsigned*>(a.stats) + kStUMax, m);
+  }
+}
+
+struct PackArgs {
+  BView B;
+  int V, r, R;
+  long long Vpad;
+  float* Bt;      // [Vpad][R] bidx layout, or null
+  __half* waug;   // [Vpad][aug_width], or null
+  int aug_layout, aug_width;
+  __half* xv;     // [2R][Vpad] B^T hi / lo times 2^(exponent of stats), or null
+  const int* stats;
+};
+
+// Exponent e with max * 2^e in [2^to, 2^(to + 1)).
+__device__ __forceinline__ int scale_exp(int max_bits, int to) {
+  const float m = __int_as_float(max_bits);
+  if (!(m > 0.f) || !isfinite(m)) return 0;
+  return to - ilogbf(m);
+}
+__device__ __forceinline__ double exp2i(int e) {
+  return __hiloint2double((1023 + e) << 20, 0);  // |e| < 1023
+}
+
+// The vocabulary side of the rank term for rows [v0, v0 + 64), through a tile
+// [R][65] in shared memory so that both sides are read and written whole
+// sectors at a time (row by row, a thread per row, it took 56 us at rank 4 and
+// 370 us at rank 64 for V = 49152).
+constexpr int kPackRows = 64;
+__device__ __forceinline__ void pack_tile(const PackArgs& a, long long v0, float* tile) {
+  constexpr int ld = kPackRows + 1;
+  const int R = a.R, nt = blockDim.x;
+  for (int k = threadIdx.x; k < R * kPackRows; k += nt) {
+    int j, i;
+    if (a.B.layout) {
+      j = k % (2 * R) / 2;
+      i = 2 * (k / (2 * R)) + (k & 1);
+    } else {
+      j = k / kPackRows;
+      i = k % kPackRows;
+    }
+    tile[j * ld + i] = j < a.r && v0 + i < a.V ? a.B.at(j, v0 + i) : 0.f;
+  }
+  __syncthreads();
+  if (a.Bt)
+    for (int k = threadIdx.x; k < R * kPackRows; k += nt)
+      a.Bt[v0 * R + k] = tile[k % (2 * R) / 2 * ld + 2 * (k / (2 * R)) + (k & 1)];
+  if (a.waug) {
+    const int groups = a.aug_width / 8;
+    for (int k = threadIdx.x; k < kPackRows * groups; k += nt) {
+      const int i = k / groups, c0 = k % groups * 8;
+      __align__(16) __half o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = c0 + e, part = c / R, j = c - part * R;
+        const bool used = part < (a.aug_layout == 1 ? 3 : 2);
+        const float b = used ? tile[j * ld + i] : 0.f;
+        const __half hi = __float2half_rn(b);
+        o[e] = part == 1 ? __float2half_rn(b - __half2float(hi)) : hi;  // [hi | lo | hi], [hi | lo]
+      }
+      *reinterpret_cast<uint4*>(a.waug + (v0 + i) * a.aug_width + c0) =
+          *reinterpret_cast<const uint4*>(o);
+    }
+  }
+  if (a.xv) {
+    const int ex = scale_exp(a.stats[kStBMax], 13);
+    for (int k = threadIdx.x; k < R * (kPackRows / 2); k += nt) {
+      const int j = k / (kPackRows / 2), i = 2 * (k % (kPackRows / 2));
+      const float x = ldexpf(tile[j * ld + i], ex), y = ldexpf(tile[j * ld + i + 1], ex);
+      const __half2 hi = __floats2half2_rn(x, y);
+      const float2 hf = __half22float2(hi);
+      const long long o = (long long)j * a.Vpad + v0 + i;
+      *reinterpret_cast<__half2*>(a.xv + o) = hi;
+      *reinterpret_cast<__half2*>(a.xv + (long long)R * a.Vpad + o) =
+          __floats2half2_rn(x - hf.x, y - hf.y);
+    }
+  }
+  __syncthreads();
+}
+
+// Blocks [0, prep_blocks) take positions, the next max_blocks look for the
+// largest finite |B| (the scale of a later launch's xv), the others pack vocab
+// rows.
+template <int P>
+static __global__ void __launch_bounds__(32 * kRowWarps) lh_prep(PrepArgs a, PackArgs b,
+                                                          int prep_blocks, int max_blocks) {
+  extern __shared__ __align__(16) float sh[];
+  const int warp = threadIdx.x >> 5, blk = (int)blockIdx.x;
+  if (blk < prep_blocks) {
+    if (blk == 0 && threadIdx.x == 0 && !a.ids) a.stats[kStErr] = 0;
+    const int t0 = (blk * kRowWarps + warp) * P;
+    if (t0 < a.Tpad) prep_rows<P>(a, t0, sh + warp * P * a.d);
+  } else if (blk < prep_blocks + max_blocks) {
+    float m = 0.f;
+    const long long n = b.B.layout ? b.Vpad * b.R : (long long)b.r * b.V;  // (padding is 0)
+    const long long step = (long long)max_blocks * blockDim.x;
+#pragma unroll 4
+    for (long long k = (long long)(blk - prep_blocks) * blockDim.x + threadIdx.x; k < n; k += step) {
+      const float x = fabsf(b.B.p[k]);
+      m = isfinite(x) ? fmaxf(m, x) : m;
+    }
+    const unsigned w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    if ((threadIdx.x & 31) == 0 && w)
+      atomicMax(reinterpret_cast<unsigned*>(a.stats) + kStBMax, w);
+  } else {
+    pack_tile(b, (long long)(blk - prep_blocks - max_blocks) * kPackRows, sh);
+  }
+}
+
+// ------------------------------------------------------------- logits again
+struct LogitArgs {
+  const __half* W;
+  const __half* h16;
+  const double* sU;  // [T][R]
+  BView B;
+  int T, V, d, r, R;
+};
+
+// A row's hidden state over the lanes of a warp (lane l: elements 64 k + 2 l,
+// + 1), for dot products with rows of W whose terms are exact and whose sums
+// have 64 bits.  An f16's exponent and mantissa, put where a double has its
+// own, are the number times 2^-1008 (subnormal f16 become subnormal doubles, at
+// the same ratio): an integer shift and mask instead of the slow conversion.
+// h carries 2^1000 of that, the sum's last factor 2^8 the rest.
+struct RowH {
+  double h[2 * kMaxHead64];
+  __device__ __forceinline__ void load(const LogitArgs& a, int t, int lane) {
+    const __half* row = a.h16 + (long long)t * a.d;
+    const double up = exp2i(1000);
+#pragma unroll
+    for (int k = 0; k < kMaxHead64; ++k) {
+      float2 x = make_float2(0.f, 0.f);
+      if (64 * k < a.d)
+        x = __half22float2(*reinterpret_cast<const __half2*>(row + 64 * k + 2 * lane));
+      h[2 * k] = (double)x.x * up;
+      h[2 * k + 1] = (double)x.y * up;
+    }
+  }
+};
+__device__ __forceinline__ double f16_bits_double(unsigned top) {  // the f16 in the upper half
+  return __hiloint2double(((int)top >> 6) & (int)0x81FFFC00, 0);
+}
+
+// z of four vocab ids; lane 8 n gets the n-th (as do lanes 8 n + 1 .. + 7).
+__device__ __forceinline__ double logits64(const LogitArgs& a, const RowH& x, int t,
+                                           const int (&id)[4], int lane) {
+  double z[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+  for (int k = 0; k < kMaxHead64; ++k) {
+    if (64 * k < a.d) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const unsigned w = *reinterpret_cast<const unsigned*>(
+            a.W + (long long)id[n] * a.d + 64 * k + 2 * lane);
+        z[n] = fma(x.h[2 * k], f16_bits_double(w << 16), z[n]);
+        z[n] = fma(x.h[2 * k + 1], f16_bits_double(w), z[n]);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n) z[n] *= 256.0;
+  for (int j = lane; j < a.r; j += 32) {
+    const double su = a.sU[(long long)t * a.R + j];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) z[n] = fma(su, (double)a.B.at(j, id[n]), z[n]);
+  }
+  // four sums over the warp at once: halves, then quarters, of the lanes keep
+  // one half of the sums each
+  const bool up16 = lane & 16, up8 = lane & 8;
+  double p0 = (up16 ? z[2] : z[0]) + __shfl_xor_sync(0xffffffffu, up16 ? z[0] : z[2], 16);
+  double p1 = (up16 ? z[3] : z[1]) + __shfl_xor_sync(0xffffffffu, up16 ? z[1] : z[3], 16);
+  double s = (up8 ? p1 : p0) + __shfl_xor_sync(0xffffffffu, up8 ? p0 : p1, 8);
+#pragma unroll
+  for (int off = 4; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  return s;
+}
+
+// ------------------------------------------------------------- teams
+// The per-row kernels give a position to one warp, or, where positions are too
+// few to fill the SMs with warps, to a block of eight.
+template <int TW>
+struct Team {
+  static constexpr int kThreads = 32 * TW;
+  int tid, lane, w;
+  double* red;  // TW > 1: 2 x TW doubles of shared memory
+  int parity = 0;
+  __device__ __forceinline__ void sync() const {
+    if constexpr (TW == 1) __syncwarp();
+    else __syncthreads();
+  }
+  template <class T, class F>
+  __device__ __forceinline__ T reduce(T x, F f) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, off));
+    if constexpr (TW > 1) {
+      T* b = reinterpret_cast<T*>(red + TW * parity);
+      parity ^= 1;
+      if (lane == 0) b[w] = x;
+      __syncthreads();
+      x = b[0];
+#pragma unroll
+      for (int i = 1; i < TW; ++i) x = f(x, b[i]);
+    }
+    return x;
+  }
+  __device__ __forceinline__ double sum(double x) {
+    return reduce(x, [](double p, double q) { return p + q; });
+  }
+  __device__ __forceinline__ int count(int x) {
+    x = __reduce_add_sync(0xffffffffu, x);
+    if constexpr (TW > 1) {
+      int* b = reinterpret_cast<int*>(red + TW * parity);
+      parity ^= 1;
+      if (lane == 0) b[w] = x;
+      __syncthreads();
+      x = 0;
+#pragma unroll
+      for (int i = 0; i < TW; ++i) x += b[i];
+    }
+    return x;
+  }
+  __device__ __forceinline__ unsigned max_u(unsigned x) {
+    return reduce(x, [](unsigned p, unsigned q) { return p > q ? p : q; });
+  }
+  __device__ __forceinline__ unsigned min_u(unsigned x) {
+    return reduce(x, [](unsigned p, unsigned q) { return p < q ? p : q; });
+  }
+  __device__ __forceinline__ float max_f(float x) {
+    return reduce(x, [](float p, float q) { return fmaxf(p, q); });
+  }
+};
+
+// Where the partial sums of a position sit: pass 1 over n_b column tiles,
+// 256-position blocks, tiles split over at most `units` owners.
+struct SlotPlan {
+  int cparts, n_a, n_b, units;
+  long long ld;  // row stride of the partial arrays
+  const float* p_max;
+  const float* p_sum;
+  const float* p_ent;
+  const float* p_q;
+  __device__ __forceinline__ int slots(int t) const {
+    const int ab = t / (2 * kBM);
+    const long long total = (long long)n_a * n_b;
+    const int G = (int)(total < units ? total : units);
+    const int s0 = tile_owner((long long)ab * n_b, total, G);
+    const int s1 = tile_owner((long long)ab * n_b + n_b - 1, total, G);
+    return cparts * (s1 - s0 + 1);
+  }
+};
+
+struct RowSum {
+  float M;
+  double S, E;  // reference max, sum of 2^x, sum of 2^x * x (x from M, log2 units)
+};
+
+// A row's slots merged in a fixed order.
+template <bool kEnt, int TW>
+__device__ __forceinline__ RowSum merge_row(const SlotPlan& p, int t, int nslot, float lg,
+                                            Team<TW>& team) {
+  float M = -INFINITY;
+#pragma unroll 2
+  for (int k = team.tid; k < nslot; k += team.kThreads)
+    M = fmaxf(M, p.p_max[(long long)k * p.ld + t]);
+  M = team.max_f(M);
+  double S = 0.0, E = 0.0;
+#pragma unroll 2
+  for (int k = team.tid; k < nslot; k += team.kThreads) {
+    const long long o = (long long)k * p.ld + t;
+    const float pm = p.p_max[o], s = p.p_sum[o], e = kEnt ? p.p_ent[o] : 0.f;
+    if (pm == -INFINITY && s == 0.f) continue;  // a slice that saw no valid column
+    const float x = (pm - M) * lg, f = exp2f(x);
+    S += (double)(s * f);
+    if constexpr (kEnt) E += (double)(f * fmaf(x, s, e));
+  }
+  S = team.sum(S);
+  if constexpr (kEnt) E = team.sum(E);
+  return RowSum{M, S, E};
+}
+
+// ------------------------------------------------------------- score, per row
+struct ScoreArgs {
+  LogitArgs z;
+  SlotPlan p;
+  float lg;
+  int n_sub, sub, top_k;  // records, columns per record
+  int n_pick;             // max(top_k, kMinPick), at most n_sub
+  int cap;                // candidates that fit
+  long long sub_ld;
+  const float* sub_max;
+  const float* sub_second;
+  const float* sub_rest;
+  const uint8_t* sub_arg;
+  const uint8_t* sub_arg2;
+  const int32_t* tokens;
+  const int* stats;
+  float* logprob;
+  float* entropy;
+  int32_t* top_ids;
+  float* top_logprobs;
+};
+
+// Shared memory of one team: logits [cap], the given token's, reductions; ids
+// and approximate logits [cap]; per picked record its place as it came, in
+// order, its three values and its columns; 64 columns; counters.
+__host__ __device__ inline int score_picks(int n_pick) { return n_pick + kPickSlack; }
+__host__ __device__ inline size_t score_team_smem(int n_pick, int cap) {
+  return (size_t)(cap + 1 + 2 * kRowWarps) * 8 + (size_t)cap * 8 + (size_t)score_picks(n_pick) * 24 +
+         64 * 4 + 4 * 4 + 8;
+}
+
+// Order of floats as order of unsigned words (-inf lowest, above 0).
+__device__ __forceinline__ unsigned order_key(float x) {
+  const unsigned u = __float_as_uint(x);
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_float(unsigned k) {
+  return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
+}
+
+// One team per position, NK records per thread.  Merge the sums; bisect for a
+// threshold that n_pick to n_pick + kPickSlack records reach; the n_pick-th
+// largest of their maxima, less what rounding may have moved, bounds the
+// n_pick-th largest logit from below; compute every logit that reaches the
+// bound again in 64 bits, sort, write.  The softmax's sums get the difference.
+template <int TW, int NK>
+static __global__ void __launch_bounds__(32 * kRowWarps) lh_score_rows(ScoreArgs a) {
+  constexpr int kTeams = kRowWarps / TW;
+  constexpr int kThreads = 32 * TW;
+  extern __shared__ __align__(16) uint8_t smem_rows[];
+  Team<TW> team;
+  team.lane = threadIdx.x & 31;
+  team.tid = threadIdx.x % kThreads;
+  team.w = team.tid >> 5;
+  const int lane = team.lane, tid = team.tid, w = team.w;
+  const int no = threadIdx.x / kThreads;
+  const int t = (int)blockIdx.x * kTeams + no;
+  if (t >= a.z.T) return;  // whole teams: with TW = 8 the grid is T blocks
+  const int P = score_picks(a.n_pick);
+  double* z64 = reinterpret_cast<double*>(smem_rows + no * score_team_smem(a.n_pick, a.cap));
+  double* extra = z64 + a.cap;  // the given token's logit
+  team.red = extra + 1;
+  int* ids = reinterpret_cast<int*>(team.red + 2 * kRowWarps);
+  float* approx = reinterpret_cast<float*>(ids + a.cap);
+  int* came = reinterpret_cast<int*>(approx + a.cap);
+  int* picked = came + P;
+  float* pmax = reinterpret_cast<float*>(picked + P);
+  float* psecond = pmax + P;
+  float* prest = psecond + P;
+  int* pcol = reinterpret_cast<int*>(prest + P);
+  float* cols = reinterpret_cast<float*>(pcol + P);
+  int* words = reinterpret_cast<int*>(cols + 64);
+
+  unsigned key[NK];
+  unsigned kmax = 0;
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    const int k = tid + i * kThreads;
+    key[i] = k < a.n_sub ? order_key(a.sub_max[(long long)k * a.sub_ld + t]) : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < NK; ++i) kmax = max(kmax, key[i]);
+  const int tk = a.tokens ? a.tokens[t] : -1;
+  const bool have_tok = tk >= 0 && tk < a.z.V;
+  RowH x;
+  x.load(a.z, t, lane);
+  if (tid == 0) words[0] = words[1] = 0;
+  const RowSum rs = merge_row<true>(a.p, t, a.p.slots(t), a.lg, team);
+  const float nan = __int_as_float(0x7fc00000);
+  // NaN or infinite logits, or a pass that gave up
+  if (!isfinite(rs.M) || !isfinite(rs.S) ||
+      *reinterpret_cast<const volatile int*>(a.stats + kStErr) != 0) {
+    if (tid == 0) {
+      if (a.logprob) a.logprob[t] = nan;
+      if (a.entropy) a.entropy[t] = nan;
+    }
+    for (int k = tid; k < a.top_k; k += kThreads) {
+      a.top_ids[(long long)t * a.top_k + k] = -1;
+      a.top_logprobs[(long long)t * a.top_k + k] = nan;
+    }
+    return;
+  }
+
+  // threshold `lo`: at least C records reach it
+  const int C = a.n_pick;
+  unsigned hi = team.max_u(kmax), lo = 1u;
+  if (C <= min(kThreads, a.n_sub)) lo = team.min_u(tid < a.n_sub ? kmax : 0xffffffffu);
+  int n_lo = a.n_sub;
+  while (lo < hi && n_lo > P) {
+    const unsigned mid = lo + (hi - lo + 1) / 2;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) c += key[i] >= mid;
+    c = team.count(c);
+    if (c >= C) {
+      lo = mid;
+      n_lo = c;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  team.sync();
+  if (n_lo <= P) {
+#pragma unroll
+    for (int i = 0; i < NK; ++i)
+      if (key[i] >= lo) came[atomicAdd(&words[0], 1)] = tid + i * kThreads;
+  } else if (w == 0) {
+    // more than P equal maxima: those above, and of the equal ones the lowest
+    int n_above = 0;
+    for (int k0 = 0; k0 < a.n_sub; k0 += 32) {
+      const int k = k0 + lane;
+      const bool gt = k < a.n_sub && order_key(a.sub_max[(long long)k * a.sub_ld + t]) > lo;
+      n_above += __popc(__ballot_sync(0xffffffffu, gt));
+    }
+    int n = 0, n_eq = 0;
+    for (int k0 = 0; k0 < a.n_sub && n < C; k0 += 32) {
+      const int k = k0 + lane;
+      const unsigned kk = k < a.n_sub ? order_key(a.sub_max[(long long)k * a.sub_ld + t]) : 0u;
+      const unsigned beq = __ballot_sync(0xffffffffu, kk == lo), below = (1u << lane) - 1u;
+      const bool take = kk > lo || (kk == lo && n_eq + __popc(beq & below) < C - n_above);
+      n_eq += __popc(beq);
+      const unsigned bt = __ballot_sync(0xffffffffu, take);
+      if (take) came[n + __popc(bt & below)] = k;
+      n += __popc(bt);
+    }
+    if (lane == 0) words[0] = n;
+  }
+  team.sync();
+  const int n_p = words[0];
+  // in record order (the order in which they came is not determined)
+  for (int c = tid; c < n_p; c += kThreads) {
+    const int k = came[c];
+    int at = 0;
+    for (int q = 0; q < n_p; ++q) at += came[q] < k;
+    const long long o = (long long)k * a.sub_ld + t;
+    picked[at] = k;
+    pmax[at] = a.sub_max[o];
+    psecond[at] = a.sub == 64 ? a.sub_second[o] : -INFINITY;
+    prest[at] = a.sub > 1 ? a.sub_rest[o] : -INFINITY;
+    pcol[at] = (a.sub > 1 ? a.sub_arg[o] : 0) | (a.sub == 64 ? a.sub_arg2[o] << 8 : 0);
+  }
+  team.sync();
+  // the C-th largest maximum
+  for (int c = tid; c < n_p; c += kThreads) {
+    const float mc = pmax[c];
+    int rank = 0;
+    for (int q = 0; q < n_p; ++q) rank += pmax[q] > mc || (pmax[q] == mc && q < c);
+    if (rank == C - 1) cols[0] = mc;
+  }
+  team.sync();
+  const float L = cols[0];
+  const float bound = L - 1e-5f * (1.0f + fmaxf(fabsf(L), fabsf(rs.M)));
+  if (w == 0) {
+    int n = 0;
+    for (int c0 = 0; c0 < n_p; c0 += 32) {
+      const int c = c0 + lane;
+      const bool one = c < n_p && pmax[c] >= bound, two = c < n_p && psecond[c] >= bound;
+      const unsigned b1 = __ballot_sync(0xffffffffu, one), b2 = __ballot_sync(0xffffffffu, two);
+      const unsigned below = (1u << lane) - 1u;
+      if (one) {
+        const int at = n + __popc(b1 & below);
+        ids[at] = picked[c] * a.sub + (pcol[c] & 255);
+        approx[at] = pmax[c];
+      }
+      n += __popc(b1);
+      if (two) {
+        const int at = n + __popc(b2 & below);
+        ids[at] = picked[c] * 64 + (pcol[c] >> 8);
+        approx[at] = psecond[c];
+      }
+      n += __popc(b2);
+    }
+    if (lane == 0) words[1] = n;
+  }
+  team.sync();
+  int n_c = words[1];
+  // records whose rest reaches the bound: their other columns, in 64 bits as well
+  for (int c = 0; c < n_p; ++c) {
+    if (!(prest[c] >= bound)) continue;
+    const int v0 = picked[c] * a.sub, c1 = pcol[c] & 255;
+    const int c2 = psecond[c] >= bound ? pcol[c] >> 8 : -1;
+    for (int q = 4 * w; q < a.sub; q += 4 * TW) {
+      int id[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) id[i] = min(v0 + q + i, a.z.V - 1);
+      const double z = logits64(a.z, x, t, id, lane);
+      if ((lane & 7) == 0) cols[q + (lane >> 3)] = (float)z;
+    }
+    team.sync();
+    if (w == 0) {
+      int n = n_c;
+      for (int q0 = 0; q0 < a.sub; q0 += 32) {
+        const int q = q0 + lane;
+        const bool take = q < a.sub && v0 + q < a.z.V && q != c1 && q != c2 && cols[q] >= bound;
+        const unsigned bt = __ballot_sync(0xffffffffu, take);
+        const int n_at = n + __popc(bt & ((1u << lane) - 1u));
+        if (take && n_at < a.cap) {
+          ids[n_at] = v0 + q;
+          approx[n_at] = -INFINITY;  // not known: the sums keep it as it is
+        }
+        n = min(n + __popc(bt), a.cap);
+      }
+      if (lane == 0) words[1] = n;
+    }
+    team.sync();
+    n_c = words[1];
+    team.sync();
+  }
+  const int n_z = n_c + (have_tok ? 1 : 0);
+  for (int c = 4 * w; c < n_z; c += 4 * TW) {
+    int id[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) id[i] = c + i < n_c ? ids[c + i] : have_tok ? tk : ids[n_c - 1];
+    const double z = logits64(a.z, x, t, id, lane);
+    const int n = c + (lane >> 3);
+    if ((lane & 7) == 0) {
+      if (n < n_c) z64[n] = z;
+      else if (n == n_c) *extra = z;
+    }
+  }
+  team.sync();
+  // the sums with these logits at their exact values
+  const double Ml = (double)rs.M * (double)a.lg;
+  double dS = 0.0, dE = 0.0;
+  for (int c = lane; c < n_c; c += 32) {
+    if (!(approx[c] > -INFINITY)) continue;
+    const double xe = z64[c] * 1.4426950408889634 - Ml, xa = (double)approx[c] * (double)a.lg - Ml;
+    // 2^xe - 2^xa = 2^xa (2^(xe - xa) - 1), without the cancellation
+    const float ea = exp2f((float)xa);
+    const double diff = (double)(ea * expm1f(0.69314718f * (float)(xe - xa)));
+    dS += diff;
+    dE += diff * xe + (double)ea * (xe - xa);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    dS += __shfl_xor_sync(0xffffffffu, dS, off);
+    dE += __shfl_xor_sync(0xffffffffu, dE, off);
+  }
+  const double S = rs.S + dS, E = rs.E + dE;
+  const double ln2 = 0.69314718055994531;
+  const double lnS = log(S), lse = Ml * ln2 + lnS;
+  if (tid == 0) {
+    if (a.logprob) a.logprob[t] = have_tok ? (float)(*extra - lse) : nan;
+    if (a.entropy) a.entropy[t] = (float)fmax(0.0, lnS - ln2 * E / S);
+  }
+  for (int c = tid; c < n_c; c += kThreads) {
+    int rank = 0;
+    for (int q = 0; q < n_c; ++q)
+      rank += z64[q] > z64[c] || (z64[q] == z64[c] && ids[q] < ids[c]);
+    if (rank < a.top_k) {
+      a.top_ids[(long long)t * a.top_k + rank] = ids[c];
+      a.top_logprobs[(long long)t * a.top_k + rank] = (float)(z64[c] - lse);
+    }
+  }
+}
+
+// ------------------------------------------------------------- distill, per row
+struct DistillArgs {
+  LogitArgs z;
+  SlotPlan p;
+  float lg, tau, scale;
+  int K;
+  const int32_t* ids;
+  const float* teacher;
+  float* wt;      // in: weight * tau of rows with entries; out: 0 where none counts
+  const float* Bt;  // bidx layout (gradients)
+  const int* stats;
+  float* loss;
+  // gradients
+  float* tok;     // records of ranks 4, 8
+  float* nml;     // exponent offsets of the tensor-core rank sums
+  float* dU;      // [T][R]
+  unsigned long long* corr;  // [Vpad][R] fixed point
+};
+
+// One team per position.  q = softmax(teacher / tau) over the entries with an
+// id; loss = w tau^2 (sum q (log q - z / tau) + log sum e^(z / tau)); then,
+// with kGrads, dU = s w tau (Q / S - sum q B[:, id]) and the sparse part of
+// dB, sum over t of w tau q s U[t], in fixed point: 2^38 times its largest
+// possible term, summed with integer atomics, so that the order in which
+// positions meet an id does not change the result.
+template <bool kGrads, int TW>
+static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(DistillArgs a) {
+  constexpr int kTeams = kRowWarps / TW, kThreads = 32 * TW;
+  constexpr int kPer = (kMaxTop + kThreads - 1) / kThreads;
+  __shared__ double s_red[kTeams][2 * kRowWarps];
+  __shared__ int s_n[kTeams];
+  __shared__ int s_id[kTeams][kMaxTop];
+  __shared__ float s_q[kTeams][kMaxTop];
+  __shared__ double s_lq[kTeams][kMaxTop];
+  __shared__ double s_Q[kTeams][kThreads > 64 ? kThreads : 64];
+  Team<TW> team;
+  team.lane = threadIdx.x & 31;
+  team.tid = threadIdx.x % kThreads;
+  team.w = team.tid >> 5;
+  const int lane = team.lane, tid = team.tid, no = threadIdx.x / kThreads;
+  team.red = s_red[no];
+  const int t = (int)blockIdx.x * kTeams + no;
+  if (t >= a.z.T) return;
+  const int R = a.z.R;
+  const int nslot = a.p.slots(t);
+  const float nan = __int_as_float(0x7fc00000);
+  float wt = a.wt[t];
+  // the teacher's distribution
+  int id[kPer];
+  double lq[kPer];
+  double top = -INFINITY;
+  int wrong = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int k = tid + i * kThreads;
+    id[i] = -1;
+    lq[i] = 0.0;
+    if (wt != 0.f && k < a.K) {
+      const int v = a.ids[(long long)t * a.K + k];
+      const float x = a.teacher[(long long)t * a.K + k];
+      if (v >= a.z.V || (v >= 0 && !(x < INFINITY))) wrong = 1;
+      else if (v >= 0 && x > -INFINITY) {
+        id[i] = v;
+        lq[i] = (double)x / (double)a.tau;
+        top = fmax(top, lq[i]);
+      }
+    }
+  }
+  if (tid == 0) s_n[no] = 0;
+  const RowSum rs = merge_row<false>(a.p, t, nslot, a.lg, team);
+  wrong = team.count(wrong);
+  top = team.reduce(top, [](double p, double q) { return fmax(p, q); });
+  if (top == -INFINITY && !wrong) wt = 0.f;  // no entry left
+  double total = 0.0;
+  double e[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    e[i] = id[i] >= 0 ? exp(lq[i] - top) : 0.0;
+    total += e[i];
+  }
+  total = team.sum(total);
+  const double ltotal = wt != 0.f && !wrong ? log(total) : 0.0;
+  if (wrong) wt = nan;
+  const double Ml = (double)rs.M * (double)a.lg;
+  const double lse = (Ml + log2(rs.S)) * 0.69314718055994531;
+  const bool counts = wt != 0.f && !wrong;
+  // the entries that weigh anything, in the order of the list
+  int base = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool have = counts && e[i] > 0.0;
+    const unsigned b = __ballot_sync(0xffffffffu, have);
+    if constexpr (TW == 1) {
+      if (have) {
+        const int n = base + __popc(b & ((1u << lane) - 1u));
+        s_id[no][n] = id[i];
+        s_lq[no][n] = lq[i] - top - ltotal;
+        s_q[no][n] = (float)(e[i] / total);
+      }
+      base += __popc(b);
+    } else {  // kPer 1: warps 0..3 hold the list
+      if (lane == 0) reinterpret_cast<int*>(s_Q[no])[team.w] = __popc(b);
+      __syncthreads();
+      int before = 0, n_all = 0;
+      for (int q = 0; q < TW; ++q) {
+        const int n = reinterpret_cast<int*>(s_Q[no])[q];
+        before += q < team.w ? n : 0;
+        n_all += n;
+      }
+      if (have) {
+        const int n = before + __popc(b & ((1u << lane) - 1u));
+        s_id[no][n] = id[i];
+        s_lq[no][n] = lq[i] - top - ltotal;
+        s_q[no][n] = (float)(e[i] / total);
+      }
+      base = n_all;
+    }
+  }
+  team.sync();
+  const int n = base;
+  double loss = 0.0;
+  if (n > 0) {
+    RowH x;
+    x.load(a.z, t, lane);
+    for (int c = 4 * team.w; c < n; c += 4 * TW) {
+      int v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = s_id[no][min(c + i, n - 1)];
+      const double z = logits64(a.z, x, t, v, lane);
+      const int k = c + (lane >> 3);
+      if ((lane & 7) == 0 && k < n) {
+        const double l = s_lq[no][k];
+        loss += exp(l) * (l - z / (double)a.tau);
+      }
+    }
+  }
+  loss = team.sum(loss);
+  const bool gave_up = *reinterpret_cast<const volatile int*>(a.stats + kStErr) != 0;
+  if (tid == 0)
+    a.loss[t] = wrong || gave_up ? nan
+                : counts         ? (float)((double)wt * (double)a.tau * (loss + lse)) : 0.f;
+  if constexpr (kGrads) {
+    const float inv = (float)(1.0 / rs.S);
+    if (tid == 0) {
+      a.wt[t] = wt;
+      if (a.tok) {
+        a.tok[tidx(t, R, R)] = -(rs.M * a.lg);
+        a.tok[tidx(t, R + 1, R)] = wt == 0.f ? 0.f : wt * inv;
+      }
+      if (a.nml) a.nml[t] = -(rs.M * a.lg) + log2f(inv) + 14.0f;
+    }
+    const double xb = (a.nml ? exp2i(-scale_exp(a.stats[kStBMax], 13)) : 1.0) / rs.S;
+    const int fe = scale_exp(a.stats[kStUMax], 37);
+    const double fx = fe > 1000 || fe < -1000 ? 0.0 : exp2i(fe);
+    // threads over (rank, slice of the slots or entries)
+    const int RL = R < kThreads ? R : kThreads, ns = kThreads / RL;
+    const int sl = tid / RL;
+    for (int j = tid % RL; j < R; j += RL) {
+      double Q = 0.0;
+#pragma unroll 2
+      for (int k = sl; k < nslot; k += ns) {
+        const long long o = (long long)k * a.p.ld + t;
+        const float pm = a.p.p_max[o], pq = a.p.p_q[o * R + j];
+        if (pm != -INFINITY) Q += (double)(pq * exp2f((pm - rs.M) * a.lg));
+      }
+      Q *= xb;
+      const double su = a.z.sU[(long long)t * R + j] * (double)wt * fx;
+      const bool scatter = j < a.z.r && wt != 0.f && isfinite(su);
+      for (int k = sl; k < n; k += ns) {
+        const int v = s_id[no][k];
+        const float qk = s_q[no][k];
+        const long long o = bidx(v, j, R);
+        Q -= (double)(qk * a.Bt[o]);
+        if (scatter) atomicAdd(&a.corr[o], (unsigned long long)__double2ll_rn(su * (double)qk));
+      }
+      if constexpr (TW == 1) {
+        for (int off = RL; off < 32; off <<= 1) Q += __shfl_xor_sync(0xffffffffu, Q, off);
+      } else {  // ns slices of R (<= 64) ranks
+        team.sync();
+        s_Q[no][sl * R + j] = Q;
+        team.sync();
+        if (sl == 0)
+          for (int q = 1; q < ns; ++q) Q += s_Q[no][q * R + j];
+      }
+      if (sl == 0)
+        a.dU[(long long)t * R + j] = wt == 0.f ? 0.f : (float)((double)a.scale * (double)wt * Q);
+    }
+  }
+}
+
+// Pass 2's rank operand on the tensor cores: xt[j][t] = wt s U[t][j] 2^e as
+// f16 hi / lo, e so that the largest entry is just below 2^14.
+static __global__ void lh_xt(int T, int R, long long ld, const double* __restrict__ sU,
+                             const float* __restrict__ wt, const int* __restrict__ stats,
+                             __half* __restrict__ xt) {
+  const double up = exp2i(scale_exp(stats[kStUMax], 13));
+  const long long n = (long long)T * R, stride = (long long)gridDim.x * blockDim.x;
+  for (long long k = (long long)blockIdx.x * blockDim.x + threadIdx.x; k < n; k += stride) {
+    const int j = (int)(k / T), t = (int)(k % T);
+    const float w = wt[t];
+    const float x = w == 0.f ? 0.f : (float)(sU[(long long)t * R + j] * (double)w * up);
+    const __half hi = __float2half_rn(x);
+    xt[(long long)j * ld + t] = hi;
+    xt[(long long)(R + j) * ld + t] = __float2half_rn(x - __half2float(hi));
+  }
+}
+
+struct GradArgs {
+  int T, d, V, r, R, n_chunks, cparts, res_rows, n_b2, G2;
+  long long Vpad;
+  const float* gAp;                // [chunk][d][R]
+  const float* gBp;                // [seg][Vpad][R] bidx
+  const unsigned long long* corr;  // [Vpad][R] bidx
+  int scaled;                      // gBp carries xt's 2^e
+  const int* stats;
+  float* gA;       // layout 0: [d][r] and [r][V]; layout 1: [d][R] and [Vpad][R] bidx
+  float* gB;
+  int layout;
+  // layout 1: [sum of losses, counted positions] behind the gradients
+  const float* loss;
+  const float* wt;
+  float* tail;
+};
+
+// The gradient sums in the caller's layout, every element in a fixed order.
+// Blocks [0, Vpad / 64) take 64 vocab rows each, through shared memory where
+// the caller's rows are ranks; the others gA; block 0 the tail too.
+static __global__ void __launch_bounds__(256) lh_grads(GradArgs a) {
+  __shared__ float tile[64 * (kPackRows + 1)];
+  const bool bad = *reinterpret_cast<const volatile int*>(a.stats + kStErr) != 0;
+  const float nan = __int_as_float(0x7fc00000);
+  const int blk = (int)blockIdx.x, tid = (int)threadIdx.x;
+  const int v_blocks = (int)(a.Vpad / kPackRows);
+  if (blk >= v_blocks) {
+    const int ra = a.layout ? a.R : a.r;
+    const long long k = (long long)(blk - v_blocks) * 256 + tid;
+    if (k >= (long long)a.d * ra) return;
+    const long long nA = (long long)a.d * a.R, o = k / ra * a.R + k % ra;
+    double s = 0.0;
+#pragma unroll 8
+    for (int c = 0; c < a.n_chunks; ++c) s += (double)a.gAp[c * nA + o];
+    a.gA[k] = bad ? nan : (float)s;
+    return;
+  }
+  const double ex = a.scaled ? exp2i(-scale_exp(a.stats[kStUMax], 13)) : 1.0;
+  const double fx = exp2i(-scale_exp(a.stats[kStUMax], 37));
+  const long long v0 = (long long)blk * kPackRows, stride = a.Vpad * a.R;
+  int slots = 0;
+  if (v0 < a.V) {
+    const long long total2 = (long long)((a.V + a.res_rows - 1) / a.res_rows) * a.n_b2;
+    const long long at = v0 / a.res_rows * a.n_b2;
+    slots = a.cparts * (tile_owner(at + a.n_b2 - 1, total2, a.G2) - tile_owner(at, total2, a.G2) + 1);
+  }
+  for (int k = tid; k < kPackRows * a.R; k += 256) {
+    const long long o = v0 * a.R + k;
+    const int i = 2 * (k / (2 * a.R)) + (k & 1), j = k % (2 * a.R) / 2;
+    double s = 0.0;
+    if (v0 + i < a.V) {
+#pragma unroll 4
+      for (int q = 0; q < slots; ++q) s += (double)a.gBp[q * stride + o];
+      s = s * ex - (double)(long long)a.corr[o] * fx;
+    }
+    const float g = bad ? nan : (float)s;
+    if (a.layout) a.gB[o] = g;
+    else tile[j * (kPackRows + 1) + i] = g;
+  }
+  if (!a.layout) {
+    __syncthreads();
+    for (int k = tid; k < a.r * kPackRows; k += 256) {
+      const int j = k / kPackRows, i = k % kPackRows;
+      if (v0 + i < a.V) a.gB[(long long)j * a.V + v0 + i] = tile[j * (kPackRows + 1) + i];
+    }
+  }
+  if (a.tail && blk == 0) {
+    __shared__ double red[256];
+    __shared__ int cnt[256];
+    double s = 0.0;
+    int c = 0;
+    for (int t = tid; t < a.T; t += 256) {
+      s += (double)a.loss[t];
+      c += a.wt[t] != 0.f;
+    }
+    red[tid] = s;
+    cnt[tid] = c;
+    __syncthreads();
+    for (int w = 128; w > 0; w >>= 1) {
+      if (tid < w) {
+        red[tid] += red[tid + w];
+        cnt[tid] += cnt[tid + w];
+      }
+      __syncthreads();
+    }
+    if (tid == 0) {
+      a.tail[0] = (float)red[0];
+      a.tail[1] = (float)cnt[0];
+    }
+  }
+}
+
+}  // namespace lce

@@ -58,6 +58,12 @@ BODY_EXPORTS = [
     "lora_body_stream", "lora_body_last_error", "lora_body_train_step",
 ]
 
+# Symbols declared in include/lora_head.h.
+HEAD_EXPORTS = [
+    "lora_head_score_workspace", "lora_head_distill_workspace", "lora_head_score",
+    "lora_head_distill", "lora_head_last_error",
+]
+
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared"]
 
@@ -65,8 +71,8 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", 
 def build(verbose: bool = False) -> str:
     """Compile csrc/ into liblora_ce.so (sm_100a) next to this file."""
     srcs = [os.path.join(HERE, "csrc", f) for f in ("lora_ce_api.cu", "lora_ce_noalloc.cu", "lora_ce_merge.cu",
-                                                         "lora_ce_q4k.cu", "lora_body.cu")]
-    cmd = ["nvcc", *NVCC_FLAGS, "-I" + os.path.join(REPO, "include"), "-o", LIB_PATH, *srcs,
+                                                         "lora_ce_q4k.cu", "lora_body.cu", "lora_head.cu")]
+    cmd = ["nvcc", *NVCC_FLAGS, "--threads", "0", "-I" + os.path.join(REPO, "include"), "-o", LIB_PATH, *srcs,
            "-ldl"]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
@@ -88,6 +94,13 @@ class BodyConfig(C.Structure):
                 ("n_kv_heads", C.c_int32), ("ffn_hidden", C.c_int32), ("vocab", C.c_int32),
                 ("rms_eps", C.c_float), ("rope_theta", C.c_float), ("max_seq", C.c_int32),
                 ("max_tokens", C.c_int32), ("device", C.c_int32)]
+
+
+class Head(C.Structure):
+    """The head of include/lora_head.h: device addresses of W [vocab][dim] f16,
+    A [dim][rank] and B [rank][vocab] f32 (0 with rank 0, the base model)."""
+    _fields_ = [("W", C.c_void_p), ("A", C.c_void_p), ("B", C.c_void_p), ("dim", C.c_int32),
+                ("vocab", C.c_int32), ("rank", C.c_int32), ("scale", C.c_float)]
 
 
 class LoraCEError(RuntimeError):
@@ -167,6 +180,19 @@ def load_library() -> C.CDLL:
     lib.lora_ce_merge_weight_device.restype = C.c_int
     lib.lora_ce_merge_last_error.argtypes = []
     lib.lora_ce_merge_last_error.restype = C.c_char_p
+    ph = C.POINTER(Head)
+    lib.lora_head_score_workspace.argtypes = [ph, C.c_int32, C.c_int32]
+    lib.lora_head_score_workspace.restype = C.c_size_t
+    lib.lora_head_distill_workspace.argtypes = [ph, C.c_int32, C.c_int32, C.c_int32]
+    lib.lora_head_distill_workspace.restype = C.c_size_t
+    lib.lora_head_score.argtypes = [ph, vp, C.c_int32, C.c_int32, vp, C.c_int32, vp, vp, vp, vp, vp,
+                                    C.c_size_t, vp]
+    lib.lora_head_score.restype = C.c_int
+    lib.lora_head_distill.argtypes = [ph, vp, C.c_int32, C.c_int32, C.c_int32, vp, vp, C.c_float, vp,
+                                      vp, vp, vp, vp, C.c_size_t, vp]
+    lib.lora_head_distill.restype = C.c_int
+    lib.lora_head_last_error.argtypes = []
+    lib.lora_head_last_error.restype = C.c_char_p
     lib.lora_ce_last_error.argtypes = []
     lib.lora_ce_last_error.restype = C.c_char_p
     for name in ["lora_ce_create", "lora_ce_destroy", "lora_ce_set_weight_f16",
@@ -236,6 +262,52 @@ def token_loss_noalloc(d_W: int, vocab: int, dim: int, d_A: int, d_B: int, scale
     if rc != 0:
         msg = lib.lora_ce_noalloc_last_error().decode(errors="replace")
         raise LoraCEError(f"lora_ce_token_loss_noalloc failed: {ERRORS.get(rc, rc)}: {msg}")
+
+
+def _hcheck(rc: int, what: str) -> None:
+    if rc != 0:
+        msg = load_library().lora_head_last_error().decode(errors="replace")
+        raise LoraCEError(f"{what} failed: {ERRORS.get(rc, rc)}: {msg}")
+
+
+def head_score_workspace(head: Head, T: int, top_k: int) -> int:
+    """Bytes of device workspace that head_score of these sizes needs."""
+    n = load_library().lora_head_score_workspace(C.byref(head), T, top_k)
+    if n == 0:
+        _hcheck(-1, "lora_head_score_workspace")
+    return n
+
+
+def head_score(head: Head, d_H: int, h_dtype: int, T: int, d_tokens: int, top_k: int,
+               d_logprob: int, d_entropy: int, d_top_ids: int, d_top_logprobs: int,
+               d_workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """lora_head_score on device addresses (see include/lora_head.h): log
+    probability of given tokens, entropy and the top_k alternatives of every
+    position.  0 stands for NULL."""
+    _hcheck(load_library().lora_head_score(
+        C.byref(head), d_H or None, h_dtype, T, d_tokens or None, top_k, d_logprob or None,
+        d_entropy or None, d_top_ids or None, d_top_logprobs or None, d_workspace or None,
+        workspace_bytes, stream or None), "lora_head_score")
+
+
+def head_distill_workspace(head: Head, T: int, K: int, grads: bool = True) -> int:
+    """Bytes of device workspace that head_distill of these sizes needs."""
+    n = load_library().lora_head_distill_workspace(C.byref(head), T, K, int(grads))
+    if n == 0:
+        _hcheck(-1, "lora_head_distill_workspace")
+    return n
+
+
+def head_distill(head: Head, d_H: int, h_dtype: int, T: int, K: int, d_ids: int, d_teacher: int,
+                 temperature: float, d_weight: int, d_loss: int, d_gA: int, d_gB: int,
+                 d_workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """lora_head_distill on device addresses (see include/lora_head.h): loss
+    per position against the teacher's top logits, and the gradient sums in A
+    and B (both 0: the loss alone).  0 stands for NULL."""
+    _hcheck(load_library().lora_head_distill(
+        C.byref(head), d_H or None, h_dtype, T, K, d_ids or None, d_teacher or None,
+        float(temperature), d_weight or None, d_loss or None, d_gA or None, d_gB or None,
+        d_workspace or None, workspace_bytes, stream or None), "lora_head_distill")
 
 
 def default_config(dim, vocab, rank, max_tokens, **kw) -> Config:
