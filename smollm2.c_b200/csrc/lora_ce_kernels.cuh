@@ -359,7 +359,8 @@ struct EpiLse {
       for (int j = 0; j < R; ++j) q2[j] = __ffma2_rn(e2, f2(b[2 * j], b[2 * j + 1]), q2[j]);
     }
     if (cm > m + lazy) {
-      const float f = ex2f((m - cm) * L);  // 0 when m = -inf
+      // 0 when m = -inf; kTemp: between the references as they are rounded
+      const float f = ex2f(kTemp ? mL - cm * L : (m - cm) * L);
       const float2 ff = f2(f, f);
       if constexpr (kTemp) {
         S *= f;
@@ -410,7 +411,7 @@ struct EpiLse {
   __device__ void flush(const GemmArgs& g, int slot) {
     if (!valid) return;
     const long long o = (long long)slot * g.Tcap + t;
-    g.p_max[o] = m;
+    g.p_max[o] = kTemp ? mL : m;  // kTemp: in log2 units, as the sums have it
     if constexpr (kTemp) {
       fold();
       g.p_sum[o] = S + Slo;

@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
         if (valid && !failed) {
           if constexpr (kPass == 1) {
             const long long o = (long long)(2 * seg + half) * g.Tcap + rr;
-            g.p_max[o] = m;
+            g.p_max[o] = mL;  // in log2 units, as the sums have it
             g.p_sum[o] = (S + Slo) * (1.0f / 16.0f);
 #pragma unroll
             for (int i = 0; i < kHR; ++i) {
@@ -672,7 +672,8 @@ __global__ void __launch_bounds__(kThreadsT, 1)
         // move with the factor 1.
         const bool move = cm > m + lazy;
         if (__any_sync(0xffffffffu, move)) {
-          const float f = move ? ex2f((m - cm) * L) : 1.0f;  // 0 when m = -inf
+          // 0 when m = -inf; kTemp: between the references as they are rounded
+          const float f = move ? ex2f(kTemp ? mL - cm * L : (m - cm) * L) : 1.0f;
           s2 = __fmul2_rn(s2, make_float2(f, f));
           if constexpr (kTemp) {
             S *= f;

@@ -229,22 +229,29 @@ void fill_pass1(GemmArgs& g, const HeadCore& hd, const Aug& aug, int T, float ta
   g.redo = 80.0f * tau;
 }
 
-constexpr int kPrepRows = 4;  // positions per warp of lh_prep at large T
-
-// lh_prep over positions and vocab rows.  A warp takes 4 positions, whose A
-// loads it shares, where that still fills the SMs twice; else 1.
+// lh_prep over positions and vocab rows: a block per position where that is at
+// most two waves of 8 blocks an SM, else 32 positions per block.
 int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_blocks, bool pack,
                 int sms, cudaStream_t st) {
-  const bool wide = pa.Tpad >= 2 * sms * kRowWarps * kPrepRows;
-  const int per = kRowWarps * (wide ? kPrepRows : 1);
-  const int prep_blocks = rows ? (pa.Tpad + per - 1) / per : 0;
+  const bool tiles = pa.Tpad > 16 * sms;
+  void (*kern)(PrepArgs, PackArgs, int, int) = lh_prep<-1>;
+  if (tiles) {
+    switch (pa.R) {
+      case 0: kern = lh_prep<0>; break;
+      case 4: kern = lh_prep<4>; break;
+      case 8: kern = lh_prep<8>; break;
+      case 16: kern = lh_prep<16>; break;
+      case 32: kern = lh_prep<32>; break;
+      default: kern = lh_prep<64>; break;
+    }
+  }
+  const int prep_blocks = !rows ? 0 : tiles ? (pa.Tpad + kTileRows - 1) / kTileRows : pa.Tpad;
   const int pack_blocks = pack ? (int)(pk.Vpad / kPackRows) : 0;
-  const size_t smem = std::max(rows ? (size_t)per * pa.d * 4 : 0,
-                               pack ? (size_t)pk.R * (kPackRows + 1) * 4 : 0);
-  auto kern = wide ? lh_prep<kPrepRows> : lh_prep<1>;
+  const size_t smem =
+      std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R) : (size_t)pa.d * 4 + 256 * 8,
+               pack ? (size_t)pk.R * (kPackRows + 1) * 4 : 0);
   if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return LORA_CE_ECUDA;
-  kern<<<prep_blocks + max_blocks + pack_blocks, 32 * kRowWarps, smem, st>>>(pa, pk, prep_blocks,
-                                                                            max_blocks);
+  kern<<<prep_blocks + max_blocks + pack_blocks, 256, smem, st>>>(pa, pk, prep_blocks, max_blocks);
   return 0;
 }
 
@@ -291,7 +298,7 @@ struct DistillWs {
   int* stats;
   __half *h16, *haug, *waug, *xv, *xt;
   double* sU;
-  float *wt, *p_max, *p_sum, *p_q, *tok, *Bt, *nml, *dU, *gAp, *gBp, *Ap;
+  float *wt, *p_max, *p_sum, *p_q, *tok, *Bt, *nml, *xs, *dU, *gAp, *gBp, *Ap;
   unsigned long long* corr;
   size_t zero_bytes;  // stats and corr: cleared by every call
   size_t bytes;
@@ -329,6 +336,7 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
     w.xv = c.take<__half>(tc ? (size_t)2 * R * Vpad : 0);
     w.xt = c.take<__half>(tc ? (size_t)2 * R * Tpad : 0);
     w.nml = c.take<float>(tc ? (size_t)Tpad + kMaxBNT : 0);
+    w.xs = c.take<float>(tc ? T : 0);
     w.dU = c.take<float>((size_t)T * R);
     w.gAp = c.take<float>((size_t)((T + kDAChunk - 1) / kDAChunk) * hd.d * R);
     w.gBp = c.take<float>(segs * Vpad * R);
@@ -694,6 +702,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   a.loss = loss;
   a.tok = grads && !tc ? w.tok : nullptr;
   a.nml = tc ? w.nml : nullptr;
+  a.xs = w.xs;
   a.dU = w.dU;
   a.corr = w.corr;
   const bool warps = T >= s.sms * kRowWarps;
@@ -707,7 +716,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   if (tc) {
     const long long n = (long long)T * R;
     lh_xt<<<(int)std::min<long long>((n + 255) / 256, 8LL * s.sms), 256, 0, st>>>(
-        T, R, round_up(T, kBN), w.sU, w.wt, w.stats, w.xt);
+        T, R, round_up(T, kBN), w.sU, w.wt, w.xs, w.stats, w.xt);
   }
   if ((rc = grad_pass<2>(s, R, why))) return rc;
   switch (R) {

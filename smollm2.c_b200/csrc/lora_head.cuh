@@ -176,10 +176,11 @@ struct EpiScore {
     if (kTail && v0 >= g.V) return;
     const float2 L2 = f2(g.lg, g.lg);
     if (cm > m + g.lazy) {  // the reference moves before the chunk is added
-      const float f = ex2f((m - cm) * g.lg);  // 0 when m = -inf
+      // between the references as they are rounded; 0 when m = -inf
+      const float to = cm * g.lg, f = ex2f(mL - to);
       if constexpr (kTop) {
         // x counts from the new reference: sum e (x - delta)
-        const float delta = m == -INFINITY ? 0.f : (cm - m) * g.lg;
+        const float delta = m == -INFINITY ? 0.f : to - mL;
         e2s = f2(f * fmaf(-delta, s2.x, e2s.x), f * fmaf(-delta, s2.y, e2s.y));
         E = f * (fmaf(-delta, S, E) + fmaf(-delta, Slo, Elo));
         Elo = 0.f;
@@ -188,7 +189,7 @@ struct EpiScore {
       S *= f;
       Slo *= f;
       m = cm;
-      mL = cm * g.lg;
+      mL = to;
     }
     __syncwarp();  // rejoin before the next warp-wide TMEM load
     sum<kTail>(acc, L2, -mL);
@@ -203,7 +204,7 @@ struct EpiScore {
   __device__ void flush(const GemmArgs& g, int slot) {
     if (!valid) return;
     const long long o = (long long)slot * g.Tcap + t;
-    g.p_max[o] = m;
+    g.p_max[o] = mL;
     fold();
     g.p_sum[o] = S + Slo;
     if constexpr (kTop) g.p_ent[o] = E + Elo;
@@ -233,101 +234,223 @@ struct PrepArgs {
   int* stats;
 };
 
-// h16, U = h16.A with 64-bit sums, and what the passes read of them: one
-// warp per P positions.  Lane l sums ranks l % RL, (+ 32) over every
-// (32 / RL)-th hidden element, so the A loads are contiguous across lanes and
-// shared by the P positions.
-template <int P>
-__device__ __forceinline__ void prep_rows(const PrepArgs& a, int t0, float* sh) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ float2 load_pair(const PrepArgs& a, int t, int i) {
+  const long long o = (long long)t * a.d + i;
+  if (a.dtype == 0) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(
+                        reinterpret_cast<const __nv_bfloat16*>(a.H) + o));
+  if (a.dtype == 1) return __half22float2(*reinterpret_cast<const __half2*>(
+                        reinterpret_cast<const __half*>(a.H) + o));
+  return *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(a.H) + o);
+}
+
+// weight * tau of a position that counts, else 0
+__device__ __forceinline__ float row_weight(const PrepArgs& a, int t, bool any) {
+  const float w = a.weight ? a.weight[t] : 1.0f;
+  return any && w != 0.f ? w * a.tau : 0.f;
+}
+
+// U[t][j] goes to what the passes read of it.
+__device__ __forceinline__ void put_u(const PrepArgs& a, int t, int j, double u, float& umax,
+                                      float wt) {
   const int R = a.R;
-  float wt[P];
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int t = t0 + p;
-    wt[p] = 0.f;
-    if (t >= a.T) continue;
-    bool active = true;
-    if (a.ids) {
-      bool any = false;
-      for (int k = lane; k < a.K; k += 32) any |= a.ids[(long long)t * a.K + k] >= 0;
-      const float w = a.weight ? a.weight[t] : 1.0f;
-      active = __any_sync(0xffffffffu, any) && w != 0.f;
-      wt[p] = active ? w * a.tau : 0.f;
-      if (lane == 0) a.wt[t] = wt[p];
+  const double su = (double)a.scale * u;
+  a.sU[(long long)t * R + j] = su;
+  const float f = (float)su;
+  if (a.tok) a.tok[tidx(t, j, R)] = f;
+  if (a.haug) {
+    const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
+    __half* row = a.haug + (long long)t * a.aug_width;
+    row[j] = hi;
+    if (a.aug_layout == 1) {  // [hi | hi | lo | 0]
+      row[R + j] = hi;
+      row[2 * R + j] = lo;
+      for (int c = 3 * R + j; c < a.aug_width; c += R) row[c] = __float2half_rn(0.f);
+    } else {  // [hi | lo]
+      row[R + j] = lo;
     }
-    for (int i = 2 * lane; i < a.d; i += 64) {
-      const long long o = (long long)t * a.d + i;
-      float2 x = make_float2(0.f, 0.f);
-      if (active) {
-        if (a.dtype == 0) x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(
-                              reinterpret_cast<const __nv_bfloat16*>(a.H) + o));
-        else if (a.dtype == 1) x = __half22float2(*reinterpret_cast<const __half2*>(
-                                   reinterpret_cast<const __half*>(a.H) + o));
-        else x = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(a.H) + o);
-      }
-      const __half2 hv = __floats2half2_rn(x.x, x.y);
-      *reinterpret_cast<__half2*>(a.h16 + o) = hv;
-      *reinterpret_cast<float2*>(sh + p * a.d + i) = __half22float2(hv);
-    }
+  }
+  const float m = fabsf(wt * f);
+  if (isfinite(m)) umax = fmaxf(umax, m);
+}
+
+// The other fields of a record; all of a padding position's.
+__device__ __forceinline__ void put_fields(const PrepArgs& a, int t, int from, int lane, int n) {
+  for (int f = from + lane; f < tok_stride(a.R); f += n) a.tok[tidx(t, f, a.R)] = 0.f;
+}
+
+__device__ __forceinline__ void put_max(const PrepArgs& a, float umax) {
+  const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(umax));
+  if ((threadIdx.x & 31) == 0 && m)
+    atomicMax(reinterpret_cast<unsigned*>(a.stats) + kStUMax, m);
+}
+
+// h16, U = h16.A with 64-bit sums, one block per position: thread (j, slice)
+// sums rank j over its slice of h.  Few positions: every A load of a thread is
+// in flight at once (one warp per position, 4 loads at a time, took 40 us at
+// rank 4 and 140 us at rank 16).
+__device__ __forceinline__ void prep_row(const PrepArgs& a, int t, uint8_t* smem) {
+  float* sh = reinterpret_cast<float*>(smem);                  // [d]
+  double* red = reinterpret_cast<double*>(smem + a.d * 4);     // [256] (d * 4 is a multiple of 8)
+  const int tid = threadIdx.x, R = a.R;
+  if (t >= a.T) {
+    if (a.tok) put_fields(a, t, 0, tid, 256);
+    return;
+  }
+  float wt = 0.f;
+  bool active = true;
+  if (a.ids) {
+    const bool mine = tid < a.K && a.ids[(long long)t * a.K + tid] >= 0;
+    wt = row_weight(a, t, __syncthreads_or(mine));
+    active = wt != 0.f;
+    if (tid == 0) a.wt[t] = wt;
+  }
+  for (int i = 2 * tid; i < a.d; i += 512) {
+    const float2 x = active ? load_pair(a, t, i) : make_float2(0.f, 0.f);
+    const __half2 hv = __floats2half2_rn(x.x, x.y);
+    *reinterpret_cast<__half2*>(a.h16 + (long long)t * a.d + i) = hv;
+    *reinterpret_cast<float2*>(sh + i) = __half22float2(hv);
   }
   if (R == 0) return;
-  __syncwarp();
-  const int RL = R < 32 ? R : 32, jl = lane & (RL - 1), sl = lane / RL, ns = 32 / RL;
-  double u[P][2];
+  const int j = tid % R, sl = tid / R, ns = 256 / R;
+  double u = 0.0;
+  __syncthreads();
+  if (j < a.r) {
+    float av[16];
+    for (int i0 = sl; i0 < a.d; i0 += 16 * ns) {
 #pragma unroll
-  for (int p = 0; p < P; ++p) u[p][0] = u[p][1] = 0.0;
-  const bool two = R > 32;
-#pragma unroll 4
-  for (int i = sl; i < a.d; i += ns) {
-    const double a0 = jl < a.r ? (double)a.A[(long long)i * a.lda + jl] : 0.0;
-    const double a1 = two && jl + 32 < a.r ? (double)a.A[(long long)i * a.lda + jl + 32] : 0.0;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const double h = t0 + p < a.T ? (double)sh[p * a.d + i] : 0.0;
-      u[p][0] = fma(h, a0, u[p][0]);
-      if (two) u[p][1] = fma(h, a1, u[p][1]);
-    }
-  }
-  float umax = 0.f;
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int t = t0 + p;
-    for (int off = RL; off < 32; off <<= 1) u[p][0] += __shfl_xor_sync(0xffffffffu, u[p][0], off);
-    if (t < a.T) {
-      if (sl == 0) {
-        for (int q = 0; q < (two ? 2 : 1); ++q) {
-          const int j = jl + 32 * q;
-          const double su = (double)a.scale * u[p][q];
-          a.sU[(long long)t * R + j] = su;
-          const float f = (float)su;
-          if (a.tok) a.tok[tidx(t, j, R)] = f;
-          if (a.haug) {
-            const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
-            __half* row = a.haug + (long long)t * a.aug_width;
-            row[j] = hi;
-            if (a.aug_layout == 1) {  // [hi | hi | lo | 0]
-              row[R + j] = hi;
-              row[2 * R + j] = lo;
-              for (int c = 3 * R + j; c < a.aug_width; c += R) row[c] = __float2half_rn(0.f);
-            } else {  // [hi | lo]
-              row[R + j] = lo;
-            }
-          }
-          const float m = fabsf(wt[p] * f);
-          if (isfinite(m)) umax = fmaxf(umax, m);
-        }
+      for (int q = 0; q < 16; ++q) {
+        const int i = i0 + q * ns;
+        av[q] = i < a.d ? a.A[(long long)i * a.lda + j] : 0.f;
       }
-      if (a.tok && lane == 0)  // -M lg, weight / S: lh_distill_rows
-        for (int f = R; f < R + 4; ++f) a.tok[tidx(t, f, R)] = 0.f;
-    } else if (t < a.Tpad && a.tok) {
-      for (int f = lane; f < tok_stride(R); f += 32) a.tok[tidx(t, f, R)] = 0.f;
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int i = i0 + q * ns;
+        if (i < a.d) u = fma((double)sh[i], (double)av[q], u);
+      }
     }
   }
-  if (a.ids && a.stats) {
-    const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(umax));
-    if (lane == 0 && m) atomicMax(reinterpret_cast<unsigned*>(a.stats) + kStUMax, m);
+  red[tid] = u;
+  __syncthreads();
+  float umax = 0.f;
+  if (tid < R) {
+    u = 0.0;
+    for (int q = 0; q < ns; ++q) u += red[q * R + tid];
+    put_u(a, t, tid, u, umax, wt);
   }
+  if (a.tok && tid < 4) put_fields(a, t, R, tid, 4);
+  if (a.ids && tid < 64) put_max(a, umax);
+}
+
+// The same for kTileRows positions per block: a product of tiles in 64 bits,
+// 64 of h at a time in shared memory (already converted: conversions to 64
+// bits are four times slower than the multiply-adds), the next 64 on the way.
+constexpr int kTileRows = 32;
+template <int R>
+__device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, uint8_t* smem) {
+  constexpr int ldh = 65;
+  constexpr int RT = R >= 64 ? 4 : R == 32 ? 2 : 1;      // ranks per thread
+  constexpr int PT = R >= 16 ? 2 : 1;                    // positions per thread
+  constexpr int TX = R > 0 ? R / RT : 1;                 // threads over ranks
+  constexpr int PG = kTileRows / PT;                     // position groups
+  constexpr int NS = R > 0 ? 256 / (TX * PG) : 1;        // slices of the 64
+  double* hD = reinterpret_cast<double*>(smem);          // [32][65]
+  double* aD = hD + kTileRows * ldh + (kTileRows & 1);   // [64][R]
+  float* swt = reinterpret_cast<float*>(aD + 64 * (R > 0 ? R : 1));  // [32]
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  if (a.ids) {  // a warp per 4 positions
+    for (int q = w; q < kTileRows; q += 8) {
+      const int t = t0 + q;
+      float wt = 0.f;
+      if (t < a.T) {
+        bool any = false;
+        for (int k = lane; k < a.K; k += 32) any |= a.ids[(long long)t * a.K + k] >= 0;
+        wt = row_weight(a, t, __any_sync(0xffffffffu, any));
+        if (lane == 0) a.wt[t] = wt;
+      }
+      if (lane == 0) swt[q] = wt;
+    }
+    __syncthreads();
+  }
+  float2 next[4];
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int t = t0 + w + 8 * q;
+      const bool in = t < a.T && (!a.ids || swt[w + 8 * q] != 0.f);
+      next[q] = in ? load_pair(a, t, 64 * c + 2 * lane) : make_float2(0.f, 0.f);
+    }
+  };
+  const int tx = tid % TX, py = tid / TX % PG, sl = tid / (TX * PG);
+  double u[PT][RT];
+#pragma unroll
+  for (int p = 0; p < PT; ++p)
+#pragma unroll
+    for (int q = 0; q < RT; ++q) u[p][q] = 0.0;
+  fetch(0);
+  const int chunks = a.d / 64;
+  for (int c = 0; c < chunks; ++c) {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int row = w + 8 * q, t = t0 + row;
+      const __half2 hv = __floats2half2_rn(next[q].x, next[q].y);
+      if (t < a.T)
+        *reinterpret_cast<__half2*>(a.h16 + (long long)t * a.d + 64 * c + 2 * lane) = hv;
+      if constexpr (R > 0) {
+        const float2 x = __half22float2(hv);
+        hD[row * ldh + 2 * lane] = (double)x.x;
+        hD[row * ldh + 2 * lane + 1] = (double)x.y;
+      }
+    }
+    if (c + 1 < chunks) fetch(c + 1);
+    if constexpr (R > 0) {
+#pragma unroll 4
+      for (int k = tid; k < 64 * R; k += 256) {
+        const int i = k / R, j = k % R;
+        aD[k] = j < a.r ? (double)a.A[(long long)(64 * c + i) * a.lda + j] : 0.0;
+      }
+      __syncthreads();
+#pragma unroll 8
+      for (int i = sl; i < 64; i += NS) {
+        double x[PT], y[RT];
+#pragma unroll
+        for (int p = 0; p < PT; ++p) x[p] = hD[(py + p * PG) * ldh + i];
+#pragma unroll
+        for (int q = 0; q < RT; ++q) y[q] = aD[i * R + tx * RT + q];
+#pragma unroll
+        for (int p = 0; p < PT; ++p)
+#pragma unroll
+          for (int q = 0; q < RT; ++q) u[p][q] = fma(x[p], y[q], u[p][q]);
+      }
+    }
+  }
+  if constexpr (R > 0) {
+    if constexpr (NS > 1) {  // rank 4: the two slices meet in shared memory
+      __syncthreads();
+      hD[tid] = u[0][0];
+      __syncthreads();
+      if (sl == 0)
+        for (int q = 1; q < NS; ++q) u[0][0] += hD[tid + q * TX * PG];
+    }
+    float umax = 0.f;
+    if (sl == 0) {
+#pragma unroll
+      for (int p = 0; p < PT; ++p) {
+        const int row = py + p * PG, t = t0 + row;
+        if (t >= a.T) continue;
+        const float wt = a.ids ? swt[row] : 0.f;
+#pragma unroll
+        for (int q = 0; q < RT; ++q) put_u(a, t, tx * RT + q, u[p][q], umax, wt);
+      }
+    }
+    if (a.tok)
+      for (int q = w; q < kTileRows; q += 8)
+        if (t0 + q < a.Tpad) put_fields(a, t0 + q, t0 + q < a.T ? R : 0, lane, 32);
+    if (a.ids) put_max(a, umax);
+  }
+}
+__host__ __device__ inline size_t prep_tile_smem(int R) {
+  return (size_t)(kTileRows * 65 + 64 * (R > 0 ? R : 1)) * 8 + kTileRows * 4;
 }
 
 struct PackArgs {
@@ -338,7 +461,7 @@ struct PackArgs {
   __half* waug;   // [Vpad][aug_width], or null
   int aug_layout, aug_width;
   __half* xv;     // [2R][Vpad] B^T hi / lo times 2^(exponent of stats), or null
-  const int* stats;
+  int* stats;
 };
 
 // Exponent e with max * 2^e in [2^to, 2^(to + 1)).
@@ -407,32 +530,33 @@ __device__ __forceinline__ void pack_tile(const PackArgs& a, long long v0, float
   __syncthreads();
 }
 
-// Blocks [0, prep_blocks) take positions, the next max_blocks look for the
-// largest finite |B| (the scale of a later launch's xv), the others pack vocab
-// rows.
-template <int P>
-static __global__ void __launch_bounds__(32 * kRowWarps) lh_prep(PrepArgs a, PackArgs b,
-                                                          int prep_blocks, int max_blocks) {
-  extern __shared__ __align__(16) float sh[];
-  const int warp = threadIdx.x >> 5, blk = (int)blockIdx.x;
+// Blocks [0, prep_blocks) take positions (kRank < 0: one each; else kTileRows at
+// kernel rank kRank), the next max_blocks look for the largest finite |B| (the
+// scale of a later launch's xv), the others pack vocab rows.
+template <int kRank>
+static __global__ void __launch_bounds__(256) lh_prep(PrepArgs a, PackArgs b, int prep_blocks,
+                                                      int max_blocks) {
+  extern __shared__ __align__(16) uint8_t smem_prep[];
+  const int blk = (int)blockIdx.x;
   if (blk < prep_blocks) {
     if (blk == 0 && threadIdx.x == 0 && !a.ids) a.stats[kStErr] = 0;
-    const int t0 = (blk * kRowWarps + warp) * P;
-    if (t0 < a.Tpad) prep_rows<P>(a, t0, sh + warp * P * a.d);
+    if constexpr (kRank < 0) prep_row(a, blk, smem_prep);
+    else prep_tile<kRank>(a, blk * kTileRows, smem_prep);
   } else if (blk < prep_blocks + max_blocks) {
     float m = 0.f;
     const long long n = b.B.layout ? b.Vpad * b.R : (long long)b.r * b.V;  // (padding is 0)
-    const long long step = (long long)max_blocks * blockDim.x;
-#pragma unroll 4
-    for (long long k = (long long)(blk - prep_blocks) * blockDim.x + threadIdx.x; k < n; k += step) {
+    const long long step = (long long)max_blocks * 256;
+#pragma unroll 8
+    for (long long k = (long long)(blk - prep_blocks) * 256 + threadIdx.x; k < n; k += step) {
       const float x = fabsf(b.B.p[k]);
       m = isfinite(x) ? fmaxf(m, x) : m;
     }
     const unsigned w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
     if ((threadIdx.x & 31) == 0 && w)
-      atomicMax(reinterpret_cast<unsigned*>(a.stats) + kStBMax, w);
+      atomicMax(reinterpret_cast<unsigned*>(b.stats) + kStBMax, w);
   } else {
-    pack_tile(b, (long long)(blk - prep_blocks - max_blocks) * kPackRows, sh);
+    pack_tile(b, (long long)(blk - prep_blocks - max_blocks) * kPackRows,
+              reinterpret_cast<float*>(smem_prep));
   }
 }
 
@@ -502,6 +626,41 @@ __device__ __forceinline__ double logits64(const LogitArgs& a, const RowH& x, in
 #pragma unroll
   for (int off = 4; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
   return s;
+}
+
+// About the logits (without the rank term) of 16 vocab ids v0 .. v0 + 15 of a
+// row: the warp's mma with the rows of W as A and h as the first column of B.
+// Lane c = lane % 4 takes 8 consecutive elements of each 32 as its share of two
+// K-steps (any order of K will do, as long as both operands have it), so W is
+// read 16 bytes at a time.
+__device__ __forceinline__ void logits_mma(const LogitArgs& a, int t, int v0, int lane,
+                                           float* out) {
+  const int c = lane & 3, g = lane >> 2;
+  const __half* w0 = a.W + (long long)min(v0 + g, a.V - 1) * a.d + 8 * c;
+  const __half* w1 = a.W + (long long)min(v0 + g + 8, a.V - 1) * a.d + 8 * c;
+  const __half* h = a.h16 + (long long)t * a.d + 8 * c;
+  float acc[2][4] = {};
+#pragma unroll 6
+  for (int k = 0; k < a.d; k += 32) {
+    const uint4 p = *reinterpret_cast<const uint4*>(w0 + k);
+    const uint4 q = *reinterpret_cast<const uint4*>(w1 + k);
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (g == 0) x = *reinterpret_cast<const uint4*>(h + k);
+    auto mma = [](float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                  unsigned b1) {
+      asm volatile(
+          "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+          "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+          : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    };
+    mma(acc[0], p.x, q.x, p.y, q.y, x.x, x.y);
+    mma(acc[1], p.z, q.z, p.w, q.w, x.z, x.w);
+  }
+  if (c == 0) {
+    out[g] = acc[0][0] + acc[1][0];
+    out[g + 8] = acc[0][2] + acc[1][2];
+  }
 }
 
 // ------------------------------------------------------------- teams
@@ -579,14 +738,13 @@ struct SlotPlan {
 };
 
 struct RowSum {
-  float M;
-  double S, E;  // reference max, sum of 2^x, sum of 2^x * x (x from M, log2 units)
+  float M;      // reference max, log2 units (as rounded in the sums' exponents)
+  double S, E;  // sum of 2^x, sum of 2^x * x, x from M
 };
 
 // A row's slots merged in a fixed order.
 template <bool kEnt, int TW>
-__device__ __forceinline__ RowSum merge_row(const SlotPlan& p, int t, int nslot, float lg,
-                                            Team<TW>& team) {
+__device__ __forceinline__ RowSum merge_row(const SlotPlan& p, int t, int nslot, Team<TW>& team) {
   float M = -INFINITY;
 #pragma unroll 2
   for (int k = team.tid; k < nslot; k += team.kThreads)
@@ -598,7 +756,7 @@ __device__ __forceinline__ RowSum merge_row(const SlotPlan& p, int t, int nslot,
     const long long o = (long long)k * p.ld + t;
     const float pm = p.p_max[o], s = p.p_sum[o], e = kEnt ? p.p_ent[o] : 0.f;
     if (pm == -INFINITY && s == 0.f) continue;  // a slice that saw no valid column
-    const float x = (pm - M) * lg, f = exp2f(x);
+    const float x = pm - M, f = exp2f(x);
     S += (double)(s * f);
     if constexpr (kEnt) E += (double)(f * fmaf(x, s, e));
   }
@@ -694,7 +852,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_score_rows(ScoreArgs
   RowH x;
   x.load(a.z, t, lane);
   if (tid == 0) words[0] = words[1] = 0;
-  const RowSum rs = merge_row<true>(a.p, t, a.p.slots(t), a.lg, team);
+  const RowSum rs = merge_row<true>(a.p, t, a.p.slots(t), team);
   const float nan = __int_as_float(0x7fc00000);
   // NaN or infinite logits, or a pass that gave up
   if (!isfinite(rs.M) || !isfinite(rs.S) ||
@@ -803,18 +961,21 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_score_rows(ScoreArgs
   }
   team.sync();
   int n_c = words[1];
-  // records whose rest reaches the bound: their other columns, in 64 bits as well
+  // records whose rest reaches the bound: their other columns that do
   for (int c = 0; c < n_p; ++c) {
     if (!(prest[c] >= bound)) continue;
     const int v0 = picked[c] * a.sub, c1 = pcol[c] & 255;
     const int c2 = psecond[c] >= bound ? pcol[c] >> 8 : -1;
-    for (int q = 4 * w; q < a.sub; q += 4 * TW) {
-      int id[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) id[i] = min(v0 + q + i, a.z.V - 1);
-      const double z = logits64(a.z, x, t, id, lane);
-      if ((lane & 7) == 0) cols[q + (lane >> 3)] = (float)z;
-    }
+    for (int q = 16 * w; q < a.sub; q += 16 * TW) logits_mma(a.z, t, v0 + q, lane, cols + q);
+    team.sync();
+    if (a.z.r > 0)
+      for (int q = tid; q < a.sub; q += kThreads) {
+        const int v = min(v0 + q, a.z.V - 1);
+        float z = cols[q];
+        for (int j = 0; j < a.z.r; ++j)
+          z = fmaf((float)a.z.sU[(long long)t * a.z.R + j], a.z.B.at(j, v), z);
+        cols[q] = z;
+      }
     team.sync();
     if (w == 0) {
       int n = n_c;
@@ -849,7 +1010,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_score_rows(ScoreArgs
   }
   team.sync();
   // the sums with these logits at their exact values
-  const double Ml = (double)rs.M * (double)a.lg;
+  const double Ml = (double)rs.M;
   double dS = 0.0, dE = 0.0;
   for (int c = lane; c < n_c; c += 32) {
     if (!(approx[c] > -INFINITY)) continue;
@@ -897,7 +1058,8 @@ struct DistillArgs {
   float* loss;
   // gradients
   float* tok;     // records of ranks 4, 8
-  float* nml;     // exponent offsets of the tensor-core rank sums
+  float* nml;     // tensor-core rank sums: exponent offsets, factors of the rank operand
+  float* xs;
   float* dU;      // [T][R]
   unsigned long long* corr;  // [Vpad][R] fixed point
 };
@@ -952,7 +1114,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(Distill
     }
   }
   if (tid == 0) s_n[no] = 0;
-  const RowSum rs = merge_row<false>(a.p, t, nslot, a.lg, team);
+  const RowSum rs = merge_row<false>(a.p, t, nslot, team);
   wrong = team.count(wrong);
   top = team.reduce(top, [](double p, double q) { return fmax(p, q); });
   if (top == -INFINITY && !wrong) wt = 0.f;  // no entry left
@@ -966,7 +1128,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(Distill
   total = team.sum(total);
   const double ltotal = wt != 0.f && !wrong ? log(total) : 0.0;
   if (wrong) wt = nan;
-  const double Ml = (double)rs.M * (double)a.lg;
+  const double Ml = (double)rs.M;
   const double lse = (Ml + log2(rs.S)) * 0.69314718055994531;
   const bool counts = wt != 0.f && !wrong;
   // the entries that weigh anything, in the order of the list
@@ -1029,10 +1191,19 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(Distill
     if (tid == 0) {
       a.wt[t] = wt;
       if (a.tok) {
-        a.tok[tidx(t, R, R)] = -(rs.M * a.lg);
+        a.tok[tidx(t, R, R)] = -rs.M;
         a.tok[tidx(t, R + 1, R)] = wt == 0.f ? 0.f : wt * inv;
       }
-      if (a.nml) a.nml[t] = -(rs.M * a.lg) + log2f(inv) + 14.0f;
+      if (a.nml) {
+        // p = 2^(z lg + nml - 14) xs: the exponent's share of 1 / S is a whole
+        // power of two and what rounding takes from nml goes into xs, so that a
+        // row's p is not off by the rounding of an offset of 10 or 20
+        const int ks = ilogb(rs.S);
+        const double off = 14.0 - (double)ks - Ml;
+        const float nml = (float)off;
+        a.nml[t] = nml;
+        a.xs[t] = (float)(exp2(off - (double)nml) * ldexp(1.0 / rs.S, ks));
+      }
     }
     const double xb = (a.nml ? exp2i(-scale_exp(a.stats[kStBMax], 13)) : 1.0) / rs.S;
     const int fe = scale_exp(a.stats[kStUMax], 37);
@@ -1046,7 +1217,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(Distill
       for (int k = sl; k < nslot; k += ns) {
         const long long o = (long long)k * a.p.ld + t;
         const float pm = a.p.p_max[o], pq = a.p.p_q[o * R + j];
-        if (pm != -INFINITY) Q += (double)(pq * exp2f((pm - rs.M) * a.lg));
+        if (pm != -INFINITY) Q += (double)(pq * exp2f(pm - rs.M));
       }
       Q *= xb;
       const double su = a.z.sU[(long long)t * R + j] * (double)wt * fx;
@@ -1073,17 +1244,18 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(Distill
   }
 }
 
-// Pass 2's rank operand on the tensor cores: xt[j][t] = wt s U[t][j] 2^e as
+// Pass 2's rank operand on the tensor cores: xt[j][t] = wt xs s U[t][j] 2^e as
 // f16 hi / lo, e so that the largest entry is just below 2^14.
 static __global__ void lh_xt(int T, int R, long long ld, const double* __restrict__ sU,
-                             const float* __restrict__ wt, const int* __restrict__ stats,
+                             const float* __restrict__ wt, const float* __restrict__ xs,
+                             const int* __restrict__ stats,
                              __half* __restrict__ xt) {
   const double up = exp2i(scale_exp(stats[kStUMax], 13));
   const long long n = (long long)T * R, stride = (long long)gridDim.x * blockDim.x;
   for (long long k = (long long)blockIdx.x * blockDim.x + threadIdx.x; k < n; k += stride) {
     const int j = (int)(k / T), t = (int)(k % T);
     const float w = wt[t];
-    const float x = w == 0.f ? 0.f : (float)(sU[(long long)t * R + j] * (double)w * up);
+    const float x = w == 0.f ? 0.f : (float)(sU[(long long)t * R + j] * (double)w * (double)xs[t] * up);
     const __half hi = __float2half_rn(x);
     xt[(long long)j * ld + t] = hi;
     xt[(long long)(R + j) * ld + t] = __float2half_rn(x - __half2float(hi));
