@@ -64,7 +64,9 @@ size_t lora_head_distill_workspace(const lora_head* head, int32_t T, int32_t K, 
  *   top_ids[t][k], top_logprobs[t][k]   the top_k (0..128, <= vocab) largest
  *                       logits in descending order, equal ones by ascending id
  *                       (ordered by logits computed with 64-bit sums); not
- *                       read with top_k 0
+ *                       read with top_k 0.  Where more than 24 further tokens
+ *                       come within 1e-5 (1 + |z|) of the last one, those of
+ *                       them with the lowest ids are ordered.
  * A position whose logits hold a NaN or an infinity gets NaN, and ids -1. */
 int lora_head_score(const lora_head* head, const void* H, int32_t h_dtype, int32_t T,
                     const int32_t* tokens, int32_t top_k, float* logprob, float* entropy,

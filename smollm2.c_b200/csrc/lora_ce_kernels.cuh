@@ -149,12 +149,12 @@ struct GemmArgs {
   float drain_gain;   // 1 + the relative loss of one accumulation of rank sums (lce_gemm_tc)
   // EpiScore (lora_head.cuh): entropy sums, and the records of a row's logits
   float* p_ent;       // [seg][Tcap]
-  float* sub_max;     // [record][sub_ld]
+  float* sub_max;     // [T / 8][n_sub][8]: eight rows' records side by side
   float* sub_second;
   float* sub_rest;
   uint8_t* sub_arg;
   uint8_t* sub_arg2;
-  long long sub_ld;
+  int n_sub;
 };
 
 // Dynamic shared memory: [resident K-blocks | streamed ring (ring bytes) | staged

@@ -229,11 +229,11 @@ void fill_pass1(GemmArgs& g, const HeadCore& hd, const Aug& aug, int T, float ta
   g.redo = 80.0f * tau;
 }
 
-// lh_prep over positions and vocab rows: a block per position where that is at
-// most two waves of 8 blocks an SM, else 32 positions per block.
+// lh_prep over positions and vocab rows: a block per position up to two an SM,
+// else 32 positions per block.
 int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_blocks, bool pack,
                 int sms, cudaStream_t st) {
-  const bool tiles = pa.Tpad > 16 * sms;
+  const bool tiles = pa.Tpad > 2 * sms;
   void (*kern)(PrepArgs, PackArgs, int, int) = lh_prep<-1>;
   if (tiles) {
     switch (pa.R) {
@@ -248,7 +248,7 @@ int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_block
   const int prep_blocks = !rows ? 0 : tiles ? (pa.Tpad + kTileRows - 1) / kTileRows : pa.Tpad;
   const int pack_blocks = pack ? (int)(pk.Vpad / kPackRows) : 0;
   const size_t smem =
-      std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R) : (size_t)pa.d * 4 + 256 * 8,
+      std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R) : (size_t)(pa.d + 256) * 4,
                pack ? (size_t)pk.R * (kPackRows + 1) * 4 : 0);
   if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return LORA_CE_ECUDA;
   kern<<<prep_blocks + max_blocks + pack_blocks, 256, smem, st>>>(pa, pk, prep_blocks, max_blocks);
@@ -258,10 +258,8 @@ int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_block
 struct ScoreWs {
   int* stats;
   __half *h16, *haug, *waug;
-  double* sU;
-  float *p_max, *p_sum, *p_ent, *sub_max, *sub_second, *sub_rest;
+  float *sU, *p_max, *p_sum, *p_ent, *sub_max, *sub_second, *sub_rest;
   uint8_t *sub_arg, *sub_arg2;
-  long long sub_ld;
   int sub, n_sub;
   size_t bytes;
 };
@@ -275,16 +273,15 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
   const size_t part = (size_t)4 * most_segments(n_a, n_b) * n_a * 2 * kBM;
   w.sub = record_columns(hd.V, top_k);
   w.n_sub = (hd.V + w.sub - 1) / w.sub;
-  w.sub_ld = round_up(T, 32);
   w.stats = c.take<int>(kStatWords);
   w.h16 = c.take<__half>((size_t)T * hd.d);
-  w.sU = c.take<double>((size_t)T * aug.R);
+  w.sU = c.take<float>((size_t)T * aug.R);
   w.haug = c.take<__half>((size_t)T * aug.width);
   w.waug = c.take<__half>((size_t)Vpad * aug.width);
   w.p_max = c.take<float>(part);
   w.p_sum = c.take<float>(part);
   w.p_ent = c.take<float>(part);
-  const size_t recs = (size_t)w.n_sub * w.sub_ld;
+  const size_t recs = (size_t)w.n_sub * round_up(T, 8);
   w.sub_max = c.take<float>(recs);
   w.sub_second = c.take<float>(w.sub == 64 ? recs : 0);
   w.sub_rest = c.take<float>(w.sub > 1 ? recs : 0);
@@ -297,8 +294,7 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
 struct DistillWs {
   int* stats;
   __half *h16, *haug, *waug, *xv, *xt;
-  double* sU;
-  float *wt, *p_max, *p_sum, *p_q, *tok, *Bt, *nml, *xs, *dU, *gAp, *gBp, *Ap;
+  float *sU, *wt, *p_max, *p_sum, *p_q, *tok, *Bt, *nml, *xs, *dU, *gAp, *gBp, *Ap;
   unsigned long long* corr;
   size_t zero_bytes;  // stats and corr: cleared by every call
   size_t bytes;
@@ -318,7 +314,7 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
   if (grads) w.corr = c.take<unsigned long long>((size_t)Vpad * R);
   w.zero_bytes = c.off;
   w.h16 = c.take<__half>((size_t)T * hd.d);
-  w.sU = c.take<double>((size_t)T * R);
+  w.sU = c.take<float>((size_t)T * R);
   w.wt = c.take<float>(T);
   // rank 4 keeps the rank term in the epilogues of the gradient passes
   const bool in_mma = !grads || R > 4;
@@ -346,11 +342,18 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
 }
 
 LogitArgs logit_args(const HeadCore& hd, const Aug& aug, int T, const __half* h16,
-                     const double* sU) {
+                     const float* sU, const __half* haug, const __half* waug) {
   LogitArgs z{};
   z.W = hd.W;
   z.h16 = h16;
   z.sU = sU;
+  z.haug = haug;
+  z.waug = aug.width ? waug : nullptr;
+  z.aug_layout = aug.layout;
+  z.aug_width = aug.width;
+  z.A = hd.A;
+  z.lda = hd.lda;
+  z.scale = hd.scale;
   z.B = BView{hd.B, hd.V, hd.r, aug.R, hd.layout};
   z.T = T;
   z.V = hd.V;
@@ -535,7 +538,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   g.sub_rest = w.sub_rest;
   g.sub_arg = w.sub_arg;
   g.sub_arg2 = w.sub_arg2;
-  g.sub_ld = w.sub_ld;
+  g.n_sub = w.n_sub;
   const PassPlan p = w.sub == 64  ? score_plan<64>(g.kblocks)
                      : w.sub == 8 ? score_plan<8>(g.kblocks) : score_plan<1>(g.kblocks);
   const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
@@ -556,13 +559,14 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   a.sub = w.sub;
   a.top_k = top_k;
   a.n_pick = std::min(w.n_sub, std::max(top_k, kMinPick));
-  a.cap = 2 * score_picks(a.n_pick) + top_k + 64;
+  a.cap = 2 * score_picks(a.n_pick) + top_k + 65;  // and the given token
   const size_t team = score_team_smem(a.n_pick, a.cap);
   const bool warps = T >= sms * kRowWarps && w.n_sub <= 32 * 32;
-  void (*rows)(ScoreArgs) = warps ? lh_score_rows<1, 32>
-                            : w.n_sub <= 8 * 256 ? lh_score_rows<kRowWarps, 8>
-                                                 : lh_score_rows<kRowWarps, 32>;
-  const size_t rows_smem = warps ? team * kRowWarps : team;
+  void (*rows)(ScoreArgs) = lh_score_rows<kRowWarps, 32>;
+  if (warps) rows = w.n_sub <= 24 * 32 ? lh_score_rows<1, 24> : lh_score_rows<1, 32>;
+  else if (w.n_sub <= 4 * 256) rows = lh_score_rows<kRowWarps, 4>;
+  const size_t rows_smem =
+      warps ? kScoreRows * (team + (size_t)(w.n_sub + 1) * 4) : team;
   if (!allow_smem(reinterpret_cast<const void*>(rows), rows_smem))
     return *why = kNoFit, LORA_CE_ECUDA;
 
@@ -584,11 +588,10 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   const int G = (int)std::min<long long>(units, (long long)g.n_a * g.n_b);
   if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, g))
     return *why = kNoLaunch, LORA_CE_ECUDA;
-  a.z = logit_args(hd, aug, T, w.h16, w.sU);
+  a.z = logit_args(hd, aug, T, w.h16, w.sU, w.haug, w.waug);
   a.p = SlotPlan{col_parts(EpiScore<65536, 64>::kWarps), g.n_a, g.n_b, units, g.Tcap,
                  w.p_max, w.p_sum, w.p_ent, nullptr};
   a.lg = g.lg;
-  a.sub_ld = w.sub_ld;
   a.sub_max = w.sub_max;
   a.sub_second = w.sub_second;
   a.sub_rest = w.sub_rest;
@@ -600,7 +603,8 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   a.entropy = entropy;
   a.top_ids = top_ids;
   a.top_logprobs = top_logprobs;
-  rows<<<warps ? (T + kRowWarps - 1) / kRowWarps : T, 32 * kRowWarps, rows_smem, st>>>(a);
+  rows<<<warps ? (T + kScoreRows - 1) / kScoreRows : T, warps ? 32 * kScoreRows : 32 * kRowWarps,
+         rows_smem, st>>>(a);
   if (cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
   return 0;
 }
@@ -650,6 +654,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pk.R = R;
   pk.Vpad = s.g.Vpad;
   pk.Bt = grads && !hd.layout ? w.Bt : nullptr;
+  pk.Bt_plain = tc;  // the rank sums' passes have xv instead
   pk.waug = aug.width ? w.waug : nullptr;
   pk.aug_layout = aug.layout;
   pk.aug_width = aug.width;
@@ -686,7 +691,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   }
   if (rc) return rc;
   DistillArgs a{};
-  a.z = logit_args(hd, aug, T, w.h16, w.sU);
+  a.z = logit_args(hd, aug, T, w.h16, w.sU, w.haug, w.waug);
   a.z.R = R;
   a.z.B.R = R;
   a.p = s.slots;
@@ -698,6 +703,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   a.teacher = teacher;
   a.wt = w.wt;
   a.Bt = s.Bt;
+  a.Bt_plain = pk.Bt && tc;
   a.stats = w.stats;
   a.loss = loss;
   a.tok = grads && !tc ? w.tok : nullptr;

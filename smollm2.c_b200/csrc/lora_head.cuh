@@ -28,7 +28,8 @@ namespace lce {
 
 constexpr int kMaxTop = 128;      // largest top_k, largest teacher list
 constexpr int kMinPick = 8;       // logits of a row that are computed again at least
-constexpr int kPickSlack = 16;    // records picked beyond that, to end the search early
+constexpr int kPickStop = 8;      // the search ends with up to so many records beyond that,
+constexpr int kPickSlack = 24;    // and takes near ties of the last up to so many
 constexpr int kRowWarps = 8;      // warps per block of the per-row kernels
 constexpr int kMaxHead64 = 10;    // hidden size in units of 64
 
@@ -47,6 +48,12 @@ struct BView {
 };
 
 // ------------------------------------------------------------- pass over z
+// Record k of position t: eight positions' side by side, so that an epilogue
+// warp's store fills sectors and a block of eight rows reads one run.
+__device__ __forceinline__ long long sub_idx(int t, int k, int n_sub) {
+  return ((long long)(t >> 3) * n_sub + k) * 8 + (t & 7);
+}
+
 // The thread owns position t; columns are vocab ids (as EpiLse, without the
 // rank sums).  Per column: the online max and sum(exp) in units of log2.
 // kSub 0 is that alone (a loss).  Otherwise also the entropy sum and records
@@ -134,7 +141,7 @@ struct EpiScore {
       }
       if constexpr (kSub == 8) {
         if (valid && v0 < g.V) {
-          const long long o = (long long)(v0 / 8) * g.sub_ld + t;
+          const long long o = sub_idx(t, v0 / 8, g.n_sub);
           g.sub_max[o] = cm;
           g.sub_rest[o] = c2;
           g.sub_arg[o] = (uint8_t)at;
@@ -158,7 +165,7 @@ struct EpiScore {
           r2 = fmaxf(r2, lo);
         }
         if ((v0 & 63) == 64 - kCW && valid && v0 - (64 - kCW) < g.V) {
-          const long long o = (long long)(v0 / 64) * g.sub_ld + t;
+          const long long o = sub_idx(t, v0 / 64, g.n_sub);
           g.sub_max[o] = r1;
           g.sub_second[o] = r2;
           g.sub_rest[o] = rest;
@@ -170,7 +177,7 @@ struct EpiScore {
 #pragma unroll
       for (int i = 0; i < kCW; ++i) {
         cm = fmaxf(cm, acc[i]);
-        if (kSub == 1 && valid && v0 + i < g.V) g.sub_max[(long long)(v0 + i) * g.sub_ld + t] = acc[i];
+        if (kSub == 1 && valid && v0 + i < g.V) g.sub_max[sub_idx(t, v0 + i, g.n_sub)] = acc[i];
       }
     }
     if (kTail && v0 >= g.V) return;
@@ -219,7 +226,7 @@ struct PrepArgs {
   int lda, r, R;   // R: r rounded up to a kernel rank; 0 without an adapter
   float scale;
   __half* h16;     // [T][d]
-  double* sU;      // [T][R] s * U
+  float* sU;       // [T][R] s * U
   float* tok;      // records (tidx layout) or null
   __half* haug;    // [T][aug_width] or null
   int aug_layout, aug_width;
@@ -250,12 +257,11 @@ __device__ __forceinline__ float row_weight(const PrepArgs& a, int t, bool any) 
 }
 
 // U[t][j] goes to what the passes read of it.
-__device__ __forceinline__ void put_u(const PrepArgs& a, int t, int j, double u, float& umax,
+__device__ __forceinline__ void put_u(const PrepArgs& a, int t, int j, float u, float& umax,
                                       float wt) {
   const int R = a.R;
-  const double su = (double)a.scale * u;
-  a.sU[(long long)t * R + j] = su;
-  const float f = (float)su;
+  const float f = a.scale * u;
+  a.sU[(long long)t * R + j] = f;
   if (a.tok) a.tok[tidx(t, j, R)] = f;
   if (a.haug) {
     const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
@@ -284,13 +290,12 @@ __device__ __forceinline__ void put_max(const PrepArgs& a, float umax) {
     atomicMax(reinterpret_cast<unsigned*>(a.stats) + kStUMax, m);
 }
 
-// h16, U = h16.A with 64-bit sums, one block per position: thread (j, slice)
-// sums rank j over its slice of h.  Few positions: every A load of a thread is
-// in flight at once (one warp per position, 4 loads at a time, took 40 us at
-// rank 4 and 140 us at rank 16).
-__device__ __forceinline__ void prep_row(const PrepArgs& a, int t, uint8_t* smem) {
-  float* sh = reinterpret_cast<float*>(smem);                  // [d]
-  double* red = reinterpret_cast<double*>(smem + a.d * 4);     // [256] (d * 4 is a multiple of 8)
+// h16 and U = h16.A, one block per position: thread (j, slice) sums rank j over
+// its slice of h.  Few positions: every A load of a thread is in flight at once
+// (one warp per position, 4 loads at a time, took 40 us at rank 4 and 140 us at
+// rank 16; this 6 and 9 us).
+__device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
+  float* red = sh + a.d;  // [256] behind h's [d]
   const int tid = threadIdx.x, R = a.R;
   if (t >= a.T) {
     if (a.tok) put_fields(a, t, 0, tid, 256);
@@ -312,7 +317,7 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, uint8_t* smem
   }
   if (R == 0) return;
   const int j = tid % R, sl = tid / R, ns = 256 / R;
-  double u = 0.0;
+  float u = 0.f;
   __syncthreads();
   if (j < a.r) {
     float av[16];
@@ -325,7 +330,7 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, uint8_t* smem
 #pragma unroll
       for (int q = 0; q < 16; ++q) {
         const int i = i0 + q * ns;
-        if (i < a.d) u = fma((double)sh[i], (double)av[q], u);
+        if (i < a.d) u = fmaf(sh[i], av[q], u);
       }
     }
   }
@@ -333,7 +338,7 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, uint8_t* smem
   __syncthreads();
   float umax = 0.f;
   if (tid < R) {
-    u = 0.0;
+    u = 0.f;
     for (int q = 0; q < ns; ++q) u += red[q * R + tid];
     put_u(a, t, tid, u, umax, wt);
   }
@@ -341,21 +346,20 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, uint8_t* smem
   if (a.ids && tid < 64) put_max(a, umax);
 }
 
-// The same for kTileRows positions per block: a product of tiles in 64 bits,
-// 64 of h at a time in shared memory (already converted: conversions to 64
-// bits are four times slower than the multiply-adds), the next 64 on the way.
+// The same for kTileRows positions per block: a product of tiles, 64 of h at a
+// time in shared memory, the next 64 on the way.
 constexpr int kTileRows = 32;
+constexpr int kTileLd = 68;  // floats per row of h's tile
 template <int R>
-__device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, uint8_t* smem) {
-  constexpr int ldh = 65;
+__device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem) {
   constexpr int RT = R >= 64 ? 4 : R == 32 ? 2 : 1;      // ranks per thread
   constexpr int PT = R >= 16 ? 2 : 1;                    // positions per thread
   constexpr int TX = R > 0 ? R / RT : 1;                 // threads over ranks
   constexpr int PG = kTileRows / PT;                     // position groups
   constexpr int NS = R > 0 ? 256 / (TX * PG) : 1;        // slices of the 64
-  double* hD = reinterpret_cast<double*>(smem);          // [32][65]
-  double* aD = hD + kTileRows * ldh + (kTileRows & 1);   // [64][R]
-  float* swt = reinterpret_cast<float*>(aD + 64 * (R > 0 ? R : 1));  // [32]
+  float* hT = smem;                                      // [32][kTileLd]
+  float* aT = hT + kTileRows * kTileLd;                  // [64][R]
+  float* swt = aT + 64 * R;                              // [32]
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   if (a.ids) {  // a warp per 4 positions
     for (int q = w; q < kTileRows; q += 8) {
@@ -381,12 +385,24 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, uint8_t* sm
     }
   };
   const int tx = tid % TX, py = tid / TX % PG, sl = tid / (TX * PG);
-  double u[PT][RT];
+  float u[PT][RT];
 #pragma unroll
   for (int p = 0; p < PT; ++p)
 #pragma unroll
-    for (int q = 0; q < RT; ++q) u[p][q] = 0.0;
+    for (int q = 0; q < RT; ++q) u[p][q] = 0.f;
+  constexpr int kAPer = R > 0 ? (64 * R + 255) / 256 : 1;
+  float an[kAPer];
+  auto fetch_a = [&](int c) {
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int q = 0; q < kAPer; ++q) {
+        const int k = tid + 256 * q, i = k / R, j = k % R;
+        an[q] = j < a.r ? a.A[(long long)(64 * c + i) * a.lda + j] : 0.f;
+      }
+    }
+  };
   fetch(0);
+  fetch_a(0);
   const int chunks = a.d / 64;
   for (int c = 0; c < chunks; ++c) {
     __syncthreads();
@@ -396,41 +412,40 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, uint8_t* sm
       const __half2 hv = __floats2half2_rn(next[q].x, next[q].y);
       if (t < a.T)
         *reinterpret_cast<__half2*>(a.h16 + (long long)t * a.d + 64 * c + 2 * lane) = hv;
-      if constexpr (R > 0) {
-        const float2 x = __half22float2(hv);
-        hD[row * ldh + 2 * lane] = (double)x.x;
-        hD[row * ldh + 2 * lane + 1] = (double)x.y;
-      }
+      if constexpr (R > 0)
+        *reinterpret_cast<float2*>(hT + row * kTileLd + 2 * lane) = __half22float2(hv);
     }
-    if (c + 1 < chunks) fetch(c + 1);
     if constexpr (R > 0) {
-#pragma unroll 4
-      for (int k = tid; k < 64 * R; k += 256) {
-        const int i = k / R, j = k % R;
-        aD[k] = j < a.r ? (double)a.A[(long long)(64 * c + i) * a.lda + j] : 0.0;
-      }
+#pragma unroll
+      for (int q = 0; q < kAPer; ++q) aT[tid + 256 * q] = an[q];
+    }
+    if (c + 1 < chunks) {
+      fetch(c + 1);
+      fetch_a(c + 1);
+    }
+    if constexpr (R > 0) {
       __syncthreads();
 #pragma unroll 8
       for (int i = sl; i < 64; i += NS) {
-        double x[PT], y[RT];
+        float x[PT], y[RT];
 #pragma unroll
-        for (int p = 0; p < PT; ++p) x[p] = hD[(py + p * PG) * ldh + i];
+        for (int p = 0; p < PT; ++p) x[p] = hT[(py + p * PG) * kTileLd + i];
 #pragma unroll
-        for (int q = 0; q < RT; ++q) y[q] = aD[i * R + tx * RT + q];
+        for (int q = 0; q < RT; ++q) y[q] = aT[i * R + tx * RT + q];
 #pragma unroll
         for (int p = 0; p < PT; ++p)
 #pragma unroll
-          for (int q = 0; q < RT; ++q) u[p][q] = fma(x[p], y[q], u[p][q]);
+          for (int q = 0; q < RT; ++q) u[p][q] = fmaf(x[p], y[q], u[p][q]);
       }
     }
   }
   if constexpr (R > 0) {
     if constexpr (NS > 1) {  // rank 4: the two slices meet in shared memory
       __syncthreads();
-      hD[tid] = u[0][0];
+      hT[tid] = u[0][0];
       __syncthreads();
       if (sl == 0)
-        for (int q = 1; q < NS; ++q) u[0][0] += hD[tid + q * TX * PG];
+        for (int q = 1; q < NS; ++q) u[0][0] += hT[tid + q * TX * PG];
     }
     float umax = 0.f;
     if (sl == 0) {
@@ -450,14 +465,15 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, uint8_t* sm
   }
 }
 __host__ __device__ inline size_t prep_tile_smem(int R) {
-  return (size_t)(kTileRows * 65 + 64 * (R > 0 ? R : 1)) * 8 + kTileRows * 4;
+  return (size_t)(kTileRows * kTileLd + 64 * R + kTileRows) * 4;
 }
 
 struct PackArgs {
   BView B;
   int V, r, R;
   long long Vpad;
-  float* Bt;      // [Vpad][R] bidx layout, or null
+  float* Bt;      // [Vpad][R], bidx layout or (Bt_plain) row by row; or null
+  int Bt_plain;
   __half* waug;   // [Vpad][aug_width], or null
   int aug_layout, aug_width;
   __half* xv;     // [2R][Vpad] B^T hi / lo times 2^(exponent of stats), or null
@@ -496,7 +512,8 @@ __device__ __forceinline__ void pack_tile(const PackArgs& a, long long v0, float
   __syncthreads();
   if (a.Bt)
     for (int k = threadIdx.x; k < R * kPackRows; k += nt)
-      a.Bt[v0 * R + k] = tile[k % (2 * R) / 2 * ld + 2 * (k / (2 * R)) + (k & 1)];
+      a.Bt[v0 * R + k] = a.Bt_plain ? tile[k % R * ld + k / R]
+                                    : tile[k % (2 * R) / 2 * ld + 2 * (k / (2 * R)) + (k & 1)];
   if (a.waug) {
     const int groups = a.aug_width / 8;
     for (int k = threadIdx.x; k < kPackRows * groups; k += nt) {
@@ -536,7 +553,7 @@ __device__ __forceinline__ void pack_tile(const PackArgs& a, long long v0, float
 template <int kRank>
 static __global__ void __launch_bounds__(256) lh_prep(PrepArgs a, PackArgs b, int prep_blocks,
                                                       int max_blocks) {
-  extern __shared__ __align__(16) uint8_t smem_prep[];
+  extern __shared__ __align__(16) float smem_prep[];
   const int blk = (int)blockIdx.x;
   if (blk < prep_blocks) {
     if (blk == 0 && threadIdx.x == 0 && !a.ids) a.stats[kStErr] = 0;
@@ -556,7 +573,7 @@ static __global__ void __launch_bounds__(256) lh_prep(PrepArgs a, PackArgs b, in
       atomicMax(reinterpret_cast<unsigned*>(b.stats) + kStBMax, w);
   } else {
     pack_tile(b, (long long)(blk - prep_blocks - max_blocks) * kPackRows,
-              reinterpret_cast<float*>(smem_prep));
+              smem_prep);
   }
 }
 
@@ -564,103 +581,125 @@ static __global__ void __launch_bounds__(256) lh_prep(PrepArgs a, PackArgs b, in
 struct LogitArgs {
   const __half* W;
   const __half* h16;
-  const double* sU;  // [T][R]
+  const float* sU;  // [T][R]
+  // the rank term as the passes' MMA has it (null: from sU and B)
+  const __half* haug;
+  const __half* waug;
+  int aug_layout, aug_width;
+  const float* A;   // for logit64
+  int lda;
+  float scale;
   BView B;
   int T, V, d, r, R;
 };
 
-// A row's hidden state over the lanes of a warp (lane l: elements 64 k + 2 l,
-// + 1), for dot products with rows of W whose terms are exact and whose sums
-// have 64 bits.  An f16's exponent and mantissa, put where a double has its
-// own, are the number times 2^-1008 (subnormal f16 become subnormal doubles, at
-// the same ratio): an integer shift and mask instead of the slow conversion.
-// h carries 2^1000 of that, the sum's last factor 2^8 the rest.
-struct RowH {
-  double h[2 * kMaxHead64];
-  __device__ __forceinline__ void load(const LogitArgs& a, int t, int lane) {
-    const __half* row = a.h16 + (long long)t * a.d;
-    const double up = exp2i(1000);
-#pragma unroll
-    for (int k = 0; k < kMaxHead64; ++k) {
-      float2 x = make_float2(0.f, 0.f);
-      if (64 * k < a.d)
-        x = __half22float2(*reinterpret_cast<const __half2*>(row + 64 * k + 2 * lane));
-      h[2 * k] = (double)x.x * up;
-      h[2 * k + 1] = (double)x.y * up;
+// Logits of 16 vocab ids (ids[min(i, n - 1)]) of position t, by one warp: mma
+// with the rows of W as A and h as the first column of B, the rank term's f16
+// halves (waug, haug) behind them.  Lane c = lane % 4 takes 8 consecutive elements
+// of each 32 as its share of two K-steps (any order of K will do, as long as both
+// operands have it), so W is read 16 bytes at a time.
+// kSum64: each 32 products are added up in a fresh accumulator, whose known loss
+// (kLoss32, as acc_short) is small and made good, and go to a 64-bit sum: off by
+// 4.3e-7 (1 + |z|) at most over 524,288 logits at hidden sizes 576 and 64, ranks
+// 0, 4 and 64.  About 250 instructions for 16 logits; with every product in 64
+// bits it is 1,600.  Else one f32 accumulator: to compare with a bound.
+constexpr double kLoss32 = 0.79 * 1.5 / 33554432.0 * 1.4426950408889634;
+template <bool kSum64, class Out>
+__device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* ids, int n, int lane,
+                                         Out* out) {
+  const int c = lane & 3, g = lane >> 2;
+  const long long v0 = ids[min(g, n - 1)], v1 = ids[min(g + 8, n - 1)];
+  double z0 = 0.0, z1 = 0.0;
+  float d[4] = {0.f, 0.f, 0.f, 0.f};
+  auto mma = [&](unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  };
+  auto step = [&](const __half* w0, const __half* w1, const __half* h, bool in) {
+    uint4 p = make_uint4(0u, 0u, 0u, 0u), q = p, x = p;
+    if (in) {
+      p = *reinterpret_cast<const uint4*>(w0);
+      q = *reinterpret_cast<const uint4*>(w1);
+      if (g == 0) x = *reinterpret_cast<const uint4*>(h);
     }
+    mma(p.x, q.x, p.y, q.y, x.x, x.y);
+    mma(p.z, q.z, p.w, q.w, x.z, x.w);
+    if constexpr (kSum64) {
+      z0 += (double)d[0];
+      z1 += (double)d[2];
+      d[0] = d[1] = d[2] = d[3] = 0.f;
+    }
+  };
+  {
+    const __half* w0 = a.W + v0 * a.d + 8 * c;
+    const __half* w1 = a.W + v1 * a.d + 8 * c;
+    const __half* h = a.h16 + (long long)t * a.d + 8 * c;
+#pragma unroll 6
+    for (int k = 0; k < a.d; k += 32) step(w0 + k, w1 + k, h + k, true);
   }
-};
-__device__ __forceinline__ double f16_bits_double(unsigned top) {  // the f16 in the upper half
-  return __hiloint2double(((int)top >> 6) & (int)0x81FFFC00, 0);
-}
-
-// z of four vocab ids; lane 8 n gets the n-th (as do lanes 8 n + 1 .. + 7).
-__device__ __forceinline__ double logits64(const LogitArgs& a, const RowH& x, int t,
-                                           const int (&id)[4], int lane) {
-  double z[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-  for (int k = 0; k < kMaxHead64; ++k) {
-    if (64 * k < a.d) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const unsigned w = *reinterpret_cast<const unsigned*>(
-            a.W + (long long)id[n] * a.d + 64 * k + 2 * lane);
-        z[n] = fma(x.h[2 * k], f16_bits_double(w << 16), z[n]);
-        z[n] = fma(x.h[2 * k + 1], f16_bits_double(w), z[n]);
+  if (a.waug) {
+    const __half* w0 = a.waug + v0 * a.aug_width + 8 * c;
+    const __half* w1 = a.waug + v1 * a.aug_width + 8 * c;
+    const __half* h = a.haug + (long long)t * a.aug_width + 8 * c;
+    if (a.aug_layout == 1) {
+      for (int k = 0; k < a.aug_width; k += 32)
+        step(w0 + k, w1 + k, h + k, k + 8 * c < a.aug_width);
+    } else {  // hi . hi, lo . hi, hi . lo
+      for (int k = 0; k < a.R; k += 32) {
+        step(w0 + k, w1 + k, h + k, true);
+        step(w0 + a.R + k, w1 + a.R + k, h + k, true);
+        step(w0 + k, w1 + k, h + a.R + k, true);
       }
     }
   }
-#pragma unroll
-  for (int n = 0; n < 4; ++n) z[n] *= 256.0;
-  for (int j = lane; j < a.r; j += 32) {
-    const double su = a.sU[(long long)t * a.R + j];
-#pragma unroll
-    for (int n = 0; n < 4; ++n) z[n] = fma(su, (double)a.B.at(j, id[n]), z[n]);
+  if constexpr (!kSum64) {
+    z0 = d[0];
+    z1 = d[2];
   }
-  // four sums over the warp at once: halves, then quarters, of the lanes keep
-  // one half of the sums each
-  const bool up16 = lane & 16, up8 = lane & 8;
-  double p0 = (up16 ? z[2] : z[0]) + __shfl_xor_sync(0xffffffffu, up16 ? z[0] : z[2], 16);
-  double p1 = (up16 ? z[3] : z[1]) + __shfl_xor_sync(0xffffffffu, up16 ? z[1] : z[3], 16);
-  double s = (up8 ? p1 : p0) + __shfl_xor_sync(0xffffffffu, up8 ? p0 : p1, 8);
-#pragma unroll
-  for (int off = 4; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-  return s;
+  // lane 4 g has rows g and g + 8
+  const double a0 = __shfl_sync(0xffffffffu, z0, 4 * (lane & 7));
+  const double a1 = __shfl_sync(0xffffffffu, z1, 4 * (lane & 7));
+  const int i = lane & 15;
+  double z = i < 8 ? a0 : a1;
+  if constexpr (kSum64) z = fma(z, kLoss32, z);
+  if (!a.waug && a.r > 0) {  // lane i % 16 takes row i, the halves of the warp every other rank
+    const int v = ids[min(i, n - 1)];
+    const float* su = a.sU + (long long)t * a.R;
+    float s = 0.f;
+    for (int j = lane >> 4; j < a.r; j += 2) s = fmaf(su[j], a.B.at(j, v), s);
+    s += __shfl_xor_sync(0xffffffffu, s, 16);
+    z += (double)s;
+  }
+  if (lane < 16 && i < n) out[i] = (Out)z;
 }
 
-// About the logits (without the rank term) of 16 vocab ids v0 .. v0 + 15 of a
-// row: the warp's mma with the rows of W as A and h as the first column of B.
-// Lane c = lane % 4 takes 8 consecutive elements of each 32 as its share of two
-// K-steps (any order of K will do, as long as both operands have it), so W is
-// read 16 bytes at a time.
-__device__ __forceinline__ void logits_mma(const LogitArgs& a, int t, int v0, int lane,
-                                           float* out) {
-  const int c = lane & 3, g = lane >> 2;
-  const __half* w0 = a.W + (long long)min(v0 + g, a.V - 1) * a.d + 8 * c;
-  const __half* w1 = a.W + (long long)min(v0 + g + 8, a.V - 1) * a.d + 8 * c;
-  const __half* h = a.h16 + (long long)t * a.d + 8 * c;
-  float acc[2][4] = {};
-#pragma unroll 6
-  for (int k = 0; k < a.d; k += 32) {
-    const uint4 p = *reinterpret_cast<const uint4*>(w0 + k);
-    const uint4 q = *reinterpret_cast<const uint4*>(w1 + k);
-    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-    if (g == 0) x = *reinterpret_cast<const uint4*>(h + k);
-    auto mma = [](float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
-                  unsigned b1) {
-      asm volatile(
-          "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
-          "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-          : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    };
-    mma(acc[0], p.x, q.x, p.y, q.y, x.x, x.y);
-    mma(acc[1], p.z, q.z, p.w, q.w, x.z, x.w);
+// How far apart two logits have to be for logits16 to tell their order: several
+// times the largest error seen.
+__device__ __forceinline__ float logit_gap(double z) { return 4e-6f * (1.0f + fabsf((float)z)); }
+
+// One logit by one warp with 64-bit sums throughout (products of f16 are exact
+// in f32; U is formed again): for those whose order logits16 does not tell.
+__device__ __forceinline__ double warp_sum(double s) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  return s;
+}
+__device__ __forceinline__ double logit64(const LogitArgs& a, int t, int v, int lane) {
+  const __half* h = a.h16 + (long long)t * a.d;
+  const __half* w = a.W + (long long)v * a.d;
+  double z = 0.0;
+  for (int i = lane; i < a.d; i += 32)
+    z += (double)(__half2float(h[i]) * __half2float(w[i]));
+  for (int j = 0; j < a.r; ++j) {
+    double u = 0.0;
+    for (int i = lane; i < a.d; i += 32)
+      u = fma((double)__half2float(h[i]), (double)a.A[(long long)i * a.lda + j], u);
+    z = fma(u, (double)a.scale * (double)a.B.at(j, v), z);  // the lanes' shares add up below
   }
-  if (c == 0) {
-    out[g] = acc[0][0] + acc[1][0];
-    out[g + 8] = acc[0][2] + acc[1][2];
-  }
+  return warp_sum(z);
 }
 
 // ------------------------------------------------------------- teams
@@ -773,7 +812,6 @@ struct ScoreArgs {
   int n_sub, sub, top_k;  // records, columns per record
   int n_pick;             // max(top_k, kMinPick), at most n_sub
   int cap;                // candidates that fit
-  long long sub_ld;
   const float* sub_max;
   const float* sub_second;
   const float* sub_rest;
@@ -787,71 +825,78 @@ struct ScoreArgs {
   float* top_logprobs;
 };
 
-// Shared memory of one team: logits [cap], the given token's, reductions; ids
-// and approximate logits [cap]; per picked record its place as it came, in
-// order, its three values and its columns; 64 columns; counters.
+// Shared memory of one team: reductions; logits computed again [cap, the given
+// token's last]; ids, logits as the pass had them, and ranks [cap]; per picked
+// record its number, its second and rest, its columns; 64 columns' ids and
+// logits; counters.  A multiple of 16 bytes.
 __host__ __device__ inline int score_picks(int n_pick) { return n_pick + kPickSlack; }
 __host__ __device__ inline size_t score_team_smem(int n_pick, int cap) {
-  return (size_t)(cap + 1 + 2 * kRowWarps) * 8 + (size_t)cap * 8 + (size_t)score_picks(n_pick) * 24 +
-         64 * 4 + 4 * 4 + 8;
+  return ((size_t)(2 * kRowWarps + cap) * 8 + (size_t)cap * 12 +
+          (size_t)score_picks(n_pick) * 16 + 128 * 4 + 16 * 4 + 15) / 16 * 16;
 }
-
-// Order of floats as order of unsigned words (-inf lowest, above 0).
-__device__ __forceinline__ unsigned order_key(float x) {
-  const unsigned u = __float_as_uint(x);
-  return (u >> 31) ? ~u : (u | 0x80000000u);
-}
-__device__ __forceinline__ float key_float(unsigned k) {
-  return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
-}
+constexpr int kScoreRows = 4;  // positions per block where each has a warp
 
 // One team per position, NK records per thread.  Merge the sums; bisect for a
-// threshold that n_pick to n_pick + kPickSlack records reach; the n_pick-th
-// largest of their maxima, less what rounding may have moved, bounds the
-// n_pick-th largest logit from below; compute every logit that reaches the
-// bound again in 64 bits, sort, write.  The softmax's sums get the difference.
+// threshold that n_pick to n_pick + kPickStop records reach: it is a lower
+// bound of the n_pick-th largest logit; compute every logit that reaches it,
+// less what rounding may have moved, again, with 64-bit sums where two are too
+// close to tell their order; sort, write.  The softmax's sums get the difference.
 template <int TW, int NK>
-static __global__ void __launch_bounds__(32 * kRowWarps) lh_score_rows(ScoreArgs a) {
-  constexpr int kTeams = kRowWarps / TW;
+static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW == 1 ? 6 : 2)
+    lh_score_rows(ScoreArgs a) {
+  constexpr int kTeams = TW == 1 ? kScoreRows : 1;
   constexpr int kThreads = 32 * TW;
+  constexpr unsigned kAll = 0xffffffffu;
   extern __shared__ __align__(16) uint8_t smem_rows[];
   Team<TW> team;
   team.lane = threadIdx.x & 31;
   team.tid = threadIdx.x % kThreads;
   team.w = team.tid >> 5;
   const int lane = team.lane, tid = team.tid, w = team.w;
+  const unsigned below = (1u << lane) - 1u;
   const int no = threadIdx.x / kThreads;
   const int t = (int)blockIdx.x * kTeams + no;
-  if (t >= a.z.T) return;  // whole teams: with TW = 8 the grid is T blocks
+  const size_t team_bytes = score_team_smem(a.n_pick, a.cap);
   const int P = score_picks(a.n_pick);
-  double* z64 = reinterpret_cast<double*>(smem_rows + no * score_team_smem(a.n_pick, a.cap));
-  double* extra = z64 + a.cap;  // the given token's logit
-  team.red = extra + 1;
-  int* ids = reinterpret_cast<int*>(team.red + 2 * kRowWarps);
+  team.red = reinterpret_cast<double*>(smem_rows + no * team_bytes);
+  double* z64 = team.red + 2 * kRowWarps;
+  int* ids = reinterpret_cast<int*>(z64 + a.cap);
   float* approx = reinterpret_cast<float*>(ids + a.cap);
-  int* came = reinterpret_cast<int*>(approx + a.cap);
-  int* picked = came + P;
-  float* pmax = reinterpret_cast<float*>(picked + P);
-  float* psecond = pmax + P;
+  int* ranks = reinterpret_cast<int*>(approx + a.cap);
+  int* picked = ranks + a.cap;
+  float* psecond = reinterpret_cast<float*>(picked + P);
   float* prest = psecond + P;
   int* pcol = reinterpret_cast<int*>(prest + P);
-  float* cols = reinterpret_cast<float*>(pcol + P);
-  int* words = reinterpret_cast<int*>(cols + 64);
+  int* col_id = pcol + P;
+  float* cols = reinterpret_cast<float*>(col_id + 64);
+  int* words = reinterpret_cast<int*>(cols + 64);  // [0..7] picks per warp, [8] picks
 
-  unsigned key[NK];
-  unsigned kmax = 0;
+  // this thread's records: (w NK + i) 32 + lane, so that record order is warp order
+  float key[NK];
+  if constexpr (TW == 1) {
+    // the block's rows' records are runs: through shared memory, [row][record]
+    float* stage = reinterpret_cast<float*>(smem_rows + kTeams * team_bytes);
+    const int ld = a.n_sub + 1, t0 = (int)blockIdx.x * kTeams;
+    const float* src = a.sub_max + (long long)(t0 >> 3) * a.n_sub * 8 + (t0 & 7);
+#pragma unroll 8
+    for (int k = threadIdx.x; k < a.n_sub * kTeams; k += 32 * kTeams)
+      stage[(k % kTeams) * ld + k / kTeams] = src[k / kTeams * 8 + k % kTeams];
+    __syncthreads();
+    if (t >= a.z.T) return;
 #pragma unroll
-  for (int i = 0; i < NK; ++i) {
-    const int k = tid + i * kThreads;
-    key[i] = k < a.n_sub ? order_key(a.sub_max[(long long)k * a.sub_ld + t]) : 0u;
+    for (int i = 0; i < NK; ++i) {
+      const int k = i * 32 + lane;
+      key[i] = k < a.n_sub ? stage[no * ld + k] : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int k = (w * NK + i) * 32 + lane;
+      key[i] = k < a.n_sub ? a.sub_max[sub_idx(t, k, a.n_sub)] : -INFINITY;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < NK; ++i) kmax = max(kmax, key[i]);
   const int tk = a.tokens ? a.tokens[t] : -1;
   const bool have_tok = tk >= 0 && tk < a.z.V;
-  RowH x;
-  x.load(a.z, t, lane);
-  if (tid == 0) words[0] = words[1] = 0;
   const RowSum rs = merge_row<true>(a.p, t, a.p.slots(t), team);
   const float nan = __int_as_float(0x7fc00000);
   // NaN or infinite logits, or a pass that gave up
@@ -868,13 +913,36 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_score_rows(ScoreArgs
     return;
   }
 
-  // threshold `lo`: at least C records reach it
+  // threshold `lo`: at least C records reach it, n_lo of them where that is known
+  // to be few enough
   const int C = a.n_pick;
-  unsigned hi = team.max_u(kmax), lo = 1u;
-  if (C <= min(kThreads, a.n_sub)) lo = team.min_u(tid < a.n_sub ? kmax : 0xffffffffu);
+  float kmax = -INFINITY, kmin = INFINITY;
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    kmax = fmaxf(kmax, key[i]);
+    if (key[i] > -INFINITY) kmin = fminf(kmin, key[i]);
+  }
+  float hi = team.max_f(kmax), lo;
   int n_lo = a.n_sub;
-  while (lo < hi && n_lo > P) {
-    const unsigned mid = lo + (hi - lo + 1) / 2;
+  if (TW == 1 && C <= min(32, a.n_sub)) {
+    // the C-th largest of the lanes' maxima: close to it from below
+    int rank = 0;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) {
+      const float x = __shfl_sync(kAll, kmax, q);
+      rank += x > kmax || (x == kmax && q < lane);
+    }
+    lo = __shfl_sync(kAll, kmax, __ffs(__ballot_sync(kAll, rank == C - 1)) - 1);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) c += key[i] >= lo;
+    n_lo = team.count(c);
+  } else {
+    lo = -team.max_f(-kmin);
+  }
+  while (n_lo > C + kPickStop && lo < hi) {
+    float mid = lo + 0.5f * (hi - lo);
+    if (!(mid > lo)) mid = hi;
     int c = 0;
 #pragma unroll
     for (int i = 0; i < NK; ++i) c += key[i] >= mid;
@@ -882,161 +950,184 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_score_rows(ScoreArgs
     if (c >= C) {
       lo = mid;
       n_lo = c;
+    } else if (mid == hi) {
+      break;
     } else {
-      hi = mid - 1;
+      hi = mid;
     }
   }
-  team.sync();
-  if (n_lo <= P) {
+  // records that reach the threshold but for rounding; where they are more than
+  // P (equal or nearly equal maxima, as of a padding row), those surely above it
+  // and of the others the lowest
+  const float eps = 1e-5f * (1.0f + fmaxf(fabsf(lo), fabsf(rs.M)));
+  const float bound = lo - eps, above = lo + eps;
+  int room = P;
+  bool crowded;
+  {
+    int c = 0;
 #pragma unroll
-    for (int i = 0; i < NK; ++i)
-      if (key[i] >= lo) came[atomicAdd(&words[0], 1)] = tid + i * kThreads;
-  } else if (w == 0) {
-    // more than P equal maxima: those above, and of the equal ones the lowest
-    int n_above = 0;
-    for (int k0 = 0; k0 < a.n_sub; k0 += 32) {
-      const int k = k0 + lane;
-      const bool gt = k < a.n_sub && order_key(a.sub_max[(long long)k * a.sub_ld + t]) > lo;
-      n_above += __popc(__ballot_sync(0xffffffffu, gt));
+    for (int i = 0; i < NK; ++i) c += key[i] >= bound;
+    crowded = team.count(c) > P;
+    if (crowded) {
+      c = 0;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) c += key[i] > above;
+      room = P - team.count(c);
     }
-    int n = 0, n_eq = 0;
-    for (int k0 = 0; k0 < a.n_sub && n < C; k0 += 32) {
-      const int k = k0 + lane;
-      const unsigned kk = k < a.n_sub ? order_key(a.sub_max[(long long)k * a.sub_ld + t]) : 0u;
-      const unsigned beq = __ballot_sync(0xffffffffu, kk == lo), below = (1u << lane) - 1u;
-      const bool take = kk > lo || (kk == lo && n_eq + __popc(beq & below) < C - n_above);
-      n_eq += __popc(beq);
-      const unsigned bt = __ballot_sync(0xffffffffu, take);
-      if (take) came[n + __popc(bt & below)] = k;
-      n += __popc(bt);
-    }
-    if (lane == 0) words[0] = n;
   }
-  team.sync();
-  const int n_p = words[0];
-  // in record order (the order in which they came is not determined)
-  for (int c = tid; c < n_p; c += kThreads) {
-    const int k = came[c];
-    int at = 0;
-    for (int q = 0; q < n_p; ++q) at += came[q] < k;
-    const long long o = (long long)k * a.sub_ld + t;
-    picked[at] = k;
-    pmax[at] = a.sub_max[o];
-    psecond[at] = a.sub == 64 ? a.sub_second[o] : -INFINITY;
-    prest[at] = a.sub > 1 ? a.sub_rest[o] : -INFINITY;
-    pcol[at] = (a.sub > 1 ? a.sub_arg[o] : 0) | (a.sub == 64 ? a.sub_arg2[o] << 8 : 0);
-  }
-  team.sync();
-  // the C-th largest maximum
-  for (int c = tid; c < n_p; c += kThreads) {
-    const float mc = pmax[c];
-    int rank = 0;
-    for (int q = 0; q < n_p; ++q) rank += pmax[q] > mc || (pmax[q] == mc && q < c);
-    if (rank == C - 1) cols[0] = mc;
-  }
-  team.sync();
-  const float L = cols[0];
-  const float bound = L - 1e-5f * (1.0f + fmaxf(fabsf(L), fabsf(rs.M)));
-  if (w == 0) {
-    int n = 0;
-    for (int c0 = 0; c0 < n_p; c0 += 32) {
-      const int c = c0 + lane;
-      const bool one = c < n_p && pmax[c] >= bound, two = c < n_p && psecond[c] >= bound;
-      const unsigned b1 = __ballot_sync(0xffffffffu, one), b2 = __ballot_sync(0xffffffffu, two);
-      const unsigned below = (1u << lane) - 1u;
-      if (one) {
-        const int at = n + __popc(b1 & below);
-        ids[at] = picked[c] * a.sub + (pcol[c] & 255);
-        approx[at] = pmax[c];
+  int n_p = 0;
+  {  // this warp's picks, in record order
+    int n_eq = 0;
+    if constexpr (TW > 1) {
+      int c = 0, e = 0;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        c += crowded ? key[i] > above : key[i] >= bound;
+        e += crowded && key[i] >= bound && !(key[i] > above);
       }
-      n += __popc(b1);
-      if (two) {
-        const int at = n + __popc(b2 & below);
+      c = __reduce_add_sync(kAll, c);
+      e = __reduce_add_sync(kAll, e);
+      if (lane == 0) words[w] = c << 16 | e;
+      team.sync();
+      for (int q = 0; q < w; ++q) {
+        const int eq = words[q] & 0xffff;
+        n_p += (words[q] >> 16) + min(eq, max(0, room - n_eq));
+        n_eq += eq;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      bool take = key[i] >= bound;
+      if (crowded) {
+        const bool eq = take && !(key[i] > above);
+        const unsigned beq = __ballot_sync(kAll, eq);
+        take = take && (!eq || n_eq + __popc(beq & below) < room);
+        n_eq += __popc(beq);
+      }
+      const unsigned bt = __ballot_sync(kAll, take);
+      if (take) picked[n_p + __popc(bt & below)] = (w * NK + i) * 32 + lane;
+      n_p += __popc(bt);
+    }
+    if constexpr (TW > 1) {
+      if (w == TW - 1 && lane == 0) words[8] = n_p;
+      team.sync();
+      n_p = words[8];
+    } else {
+      __syncwarp();
+    }
+  }
+  for (int c = tid; c < n_p; c += kThreads) {
+    const int k = picked[c];
+    const long long o = sub_idx(t, k, a.n_sub);
+    const int c1 = a.sub > 1 ? a.sub_arg[o] : 0, c2 = a.sub == 64 ? a.sub_arg2[o] : 0;
+    approx[c] = a.sub_max[o];
+    prest[c] = a.sub > 1 ? a.sub_rest[o] : -INFINITY;
+    psecond[c] = a.sub == 64 ? a.sub_second[o] : -INFINITY;
+    ids[c] = k * a.sub + c1;
+    pcol[c] = c1 | c2 << 8;
+  }
+  team.sync();
+  // seconds that reach the bound, then the columns of records whose rest does
+  int n_c = n_p;
+  if (a.sub == 64)
+    for (int c0 = 0; c0 < n_p; c0 += 32) {  // (every warp finds the same)
+      const int c = c0 + lane;
+      const bool two = c < n_p && psecond[c] >= bound;
+      const unsigned b = __ballot_sync(kAll, two);
+      if (two && w == 0) {
+        const int at = n_c + __popc(b & below);
         ids[at] = picked[c] * 64 + (pcol[c] >> 8);
         approx[at] = psecond[c];
       }
-      n += __popc(b2);
+      n_c += __popc(b);
     }
-    if (lane == 0) words[1] = n;
-  }
-  team.sync();
-  int n_c = words[1];
-  // records whose rest reaches the bound: their other columns that do
-  for (int c = 0; c < n_p; ++c) {
-    if (!(prest[c] >= bound)) continue;
-    const int v0 = picked[c] * a.sub, c1 = pcol[c] & 255;
-    const int c2 = psecond[c] >= bound ? pcol[c] >> 8 : -1;
-    for (int q = 16 * w; q < a.sub; q += 16 * TW) logits_mma(a.z, t, v0 + q, lane, cols + q);
-    team.sync();
-    if (a.z.r > 0)
-      for (int q = tid; q < a.sub; q += kThreads) {
-        const int v = min(v0 + q, a.z.V - 1);
-        float z = cols[q];
-        for (int j = 0; j < a.z.r; ++j)
-          z = fmaf((float)a.z.sU[(long long)t * a.z.R + j], a.z.B.at(j, v), z);
-        cols[q] = z;
-      }
-    team.sync();
-    if (w == 0) {
-      int n = n_c;
-      for (int q0 = 0; q0 < a.sub; q0 += 32) {
+  for (int c0 = 0; c0 < n_p && a.sub > 1; c0 += 32) {
+    unsigned more = __ballot_sync(kAll, c0 + lane < n_p && prest[min(c0 + lane, n_p - 1)] >= bound);
+    for (; more && n_c < a.cap - 1; more &= more - 1) {
+      const int c = c0 + __ffs(more) - 1;
+      const int v0 = picked[c] * a.sub, c1 = pcol[c] & 255, nv = min(a.sub, a.z.V - v0);
+      const int c2 = a.sub == 64 && psecond[c] >= bound ? pcol[c] >> 8 : -1;
+      for (int q = tid; q < nv; q += kThreads) col_id[q] = v0 + q;
+      team.sync();
+      for (int q = 16 * w; q < nv; q += 16 * TW)
+        logits16<false>(a.z, t, col_id + q, min(16, nv - q), lane, cols + q);
+      team.sync();
+      for (int q0 = 0; q0 < nv; q0 += 32) {  // (every warp finds the same)
         const int q = q0 + lane;
-        const bool take = q < a.sub && v0 + q < a.z.V && q != c1 && q != c2 && cols[q] >= bound;
-        const unsigned bt = __ballot_sync(0xffffffffu, take);
-        const int n_at = n + __popc(bt & ((1u << lane) - 1u));
-        if (take && n_at < a.cap) {
-          ids[n_at] = v0 + q;
-          approx[n_at] = -INFINITY;  // not known: the sums keep it as it is
+        const bool take = q < nv && q != c1 && q != c2 && cols[q] >= bound;
+        const unsigned bt = __ballot_sync(kAll, take);
+        const int at = n_c + __popc(bt & below);
+        if (take && w == 0 && at < a.cap - 1) {
+          ids[at] = v0 + q;
+          approx[at] = -INFINITY;  // not known: the sums keep it as it is
         }
-        n = min(n + __popc(bt), a.cap);
+        n_c = min(n_c + __popc(bt), a.cap - 1);
       }
-      if (lane == 0) words[1] = n;
+      team.sync();
     }
-    team.sync();
-    n_c = words[1];
-    team.sync();
   }
+  if (have_tok && tid == 0) ids[n_c] = tk;
+  team.sync();
   const int n_z = n_c + (have_tok ? 1 : 0);
-  for (int c = 4 * w; c < n_z; c += 4 * TW) {
-    int id[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) id[i] = c + i < n_c ? ids[c + i] : have_tok ? tk : ids[n_c - 1];
-    const double z = logits64(a.z, x, t, id, lane);
-    const int n = c + (lane >> 3);
-    if ((lane & 7) == 0) {
-      if (n < n_c) z64[n] = z;
-      else if (n == n_c) *extra = z;
+  for (int c = 16 * w; c < n_z; c += 16 * TW)
+    logits16<true>(a.z, t, ids + c, min(16, n_z - c), lane, z64 + c);
+  team.sync();
+  // ranks; all in 64 bits for logits too close to another to tell their order
+  bool any_close = false;
+  for (int c0 = 32 * w; c0 < n_c && a.top_k > 0; c0 += kThreads) {
+    const int c = c0 + lane;
+    const double z = c < n_c ? z64[c] : INFINITY;
+    const float gap = logit_gap(z);
+    int rank = 0;
+    bool close = false;
+    for (int q = 0; q < n_c; ++q) {
+      const float dz = (float)(z64[q] - z);
+      rank += dz > 0.f;
+      close |= fabsf(dz) <= gap && q != c;
+    }
+    if (c < n_c) ranks[c] = close ? -1 : rank;
+    any_close |= close;
+  }
+  if (team.count(any_close && a.top_k > 0) > 0) {
+    for (int c0 = 32 * w; c0 < n_c; c0 += kThreads) {
+      const int c = c0 + lane;
+      unsigned near = __ballot_sync(kAll, c < n_c && ranks[min(c, n_c - 1)] < 0);
+      for (; near; near &= near - 1) {
+        const int q = __ffs(near) - 1;
+        const double zq = logit64(a.z, t, ids[c0 + q], lane);
+        if (lane == q) z64[c] = zq;
+      }
     }
   }
   team.sync();
-  // the sums with these logits at their exact values
+  // the sums with these logits as they are now
+  const double ln2 = 0.69314718055994531, log2e = 1.4426950408889634;
   const double Ml = (double)rs.M;
   double dS = 0.0, dE = 0.0;
   for (int c = lane; c < n_c; c += 32) {
     if (!(approx[c] > -INFINITY)) continue;
-    const double xe = z64[c] * 1.4426950408889634 - Ml, xa = (double)approx[c] * (double)a.lg - Ml;
+    const double xe = z64[c] * log2e - Ml, xa = (double)approx[c] * (double)a.lg - Ml;
     // 2^xe - 2^xa = 2^xa (2^(xe - xa) - 1), without the cancellation
     const float ea = exp2f((float)xa);
     const double diff = (double)(ea * expm1f(0.69314718f * (float)(xe - xa)));
     dS += diff;
     dE += diff * xe + (double)ea * (xe - xa);
   }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    dS += __shfl_xor_sync(0xffffffffu, dS, off);
-    dE += __shfl_xor_sync(0xffffffffu, dE, off);
-  }
+  dS = warp_sum(dS);
+  dE = warp_sum(dE);
   const double S = rs.S + dS, E = rs.E + dE;
-  const double ln2 = 0.69314718055994531;
   const double lnS = log(S), lse = Ml * ln2 + lnS;
   if (tid == 0) {
-    if (a.logprob) a.logprob[t] = have_tok ? (float)(*extra - lse) : nan;
+    if (a.logprob) a.logprob[t] = have_tok ? (float)(z64[n_c] - lse) : nan;
     if (a.entropy) a.entropy[t] = (float)fmax(0.0, lnS - ln2 * E / S);
   }
-  for (int c = tid; c < n_c; c += kThreads) {
-    int rank = 0;
-    for (int q = 0; q < n_c; ++q)
-      rank += z64[q] > z64[c] || (z64[q] == z64[c] && ids[q] < ids[c]);
+  for (int c = tid; c < n_c && a.top_k > 0; c += kThreads) {
+    int rank = ranks[c];
+    if (rank < 0) {
+      rank = 0;
+      for (int q = 0; q < n_c; ++q)
+        rank += z64[q] > z64[c] || (z64[q] == z64[c] && ids[q] < ids[c]);
+    }
     if (rank < a.top_k) {
       a.top_ids[(long long)t * a.top_k + rank] = ids[c];
       a.top_logprobs[(long long)t * a.top_k + rank] = (float)(z64[c] - lse);
@@ -1053,7 +1144,8 @@ struct DistillArgs {
   const int32_t* ids;
   const float* teacher;
   float* wt;      // in: weight * tau of rows with entries; out: 0 where none counts
-  const float* Bt;  // bidx layout (gradients)
+  const float* Bt;  // [Vpad][R] (gradients): bidx layout, or row by row
+  int Bt_plain;
   const int* stats;
   float* loss;
   // gradients
@@ -1061,7 +1153,7 @@ struct DistillArgs {
   float* nml;     // tensor-core rank sums: exponent offsets, factors of the rank operand
   float* xs;
   float* dU;      // [T][R]
-  unsigned long long* corr;  // [Vpad][R] fixed point
+  unsigned long long* corr;  // [Vpad][R] fixed point, row by row
 };
 
 // One team per position.  q = softmax(teacher / tau) over the entries with an
@@ -1071,7 +1163,7 @@ struct DistillArgs {
 // possible term, summed with integer atomics, so that the order in which
 // positions meet an id does not change the result.
 template <bool kGrads, int TW>
-static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(DistillArgs a) {
+static __global__ void __launch_bounds__(32 * kRowWarps, 3) lh_distill_rows(DistillArgs a) {
   constexpr int kTeams = kRowWarps / TW, kThreads = 32 * TW;
   constexpr int kPer = (kMaxTop + kThreads - 1) / kThreads;
   __shared__ double s_red[kTeams][2 * kRowWarps];
@@ -1079,6 +1171,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(Distill
   __shared__ int s_id[kTeams][kMaxTop];
   __shared__ float s_q[kTeams][kMaxTop];
   __shared__ double s_lq[kTeams][kMaxTop];
+  __shared__ double s_z[kTeams][kMaxTop];
   __shared__ double s_Q[kTeams][kThreads > 64 ? kThreads : 64];
   Team<TW> team;
   team.lane = threadIdx.x & 31;
@@ -1166,20 +1259,12 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(Distill
   team.sync();
   const int n = base;
   double loss = 0.0;
-  if (n > 0) {
-    RowH x;
-    x.load(a.z, t, lane);
-    for (int c = 4 * team.w; c < n; c += 4 * TW) {
-      int v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = s_id[no][min(c + i, n - 1)];
-      const double z = logits64(a.z, x, t, v, lane);
-      const int k = c + (lane >> 3);
-      if ((lane & 7) == 0 && k < n) {
-        const double l = s_lq[no][k];
-        loss += exp(l) * (l - z / (double)a.tau);
-      }
-    }
+  for (int c = 16 * team.w; c < n; c += 16 * TW)
+    logits16<true>(a.z, t, s_id[no] + c, min(16, n - c), lane, s_z[no] + c);
+  team.sync();
+  for (int k = tid; k < n; k += kThreads) {
+    const double l = s_lq[no][k];
+    loss += exp(l) * (l - s_z[no][k] / (double)a.tau);
   }
   loss = team.sum(loss);
   const bool gave_up = *reinterpret_cast<const volatile int*>(a.stats + kStErr) != 0;
@@ -1220,13 +1305,13 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(Distill
         if (pm != -INFINITY) Q += (double)(pq * exp2f(pm - rs.M));
       }
       Q *= xb;
-      const double su = a.z.sU[(long long)t * R + j] * (double)wt * fx;
+      const double su = (double)a.z.sU[(long long)t * R + j] * (double)wt * fx;
       const bool scatter = j < a.z.r && wt != 0.f && isfinite(su);
       for (int k = sl; k < n; k += ns) {
         const int v = s_id[no][k];
         const float qk = s_q[no][k];
-        const long long o = bidx(v, j, R);
-        Q -= (double)(qk * a.Bt[o]);
+        const long long o = (long long)v * R + j;
+        Q -= (double)(qk * a.Bt[a.Bt_plain ? o : bidx(v, j, R)]);
         if (scatter) atomicAdd(&a.corr[o], (unsigned long long)__double2ll_rn(su * (double)qk));
       }
       if constexpr (TW == 1) {
@@ -1246,7 +1331,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps) lh_distill_rows(Distill
 
 // Pass 2's rank operand on the tensor cores: xt[j][t] = wt xs s U[t][j] 2^e as
 // f16 hi / lo, e so that the largest entry is just below 2^14.
-static __global__ void lh_xt(int T, int R, long long ld, const double* __restrict__ sU,
+static __global__ void lh_xt(int T, int R, long long ld, const float* __restrict__ sU,
                              const float* __restrict__ wt, const float* __restrict__ xs,
                              const int* __restrict__ stats,
                              __half* __restrict__ xt) {
@@ -1255,7 +1340,7 @@ static __global__ void lh_xt(int T, int R, long long ld, const double* __restric
   for (long long k = (long long)blockIdx.x * blockDim.x + threadIdx.x; k < n; k += stride) {
     const int j = (int)(k / T), t = (int)(k % T);
     const float w = wt[t];
-    const float x = w == 0.f ? 0.f : (float)(sU[(long long)t * R + j] * (double)w * (double)xs[t] * up);
+    const float x = w == 0.f ? 0.f : (float)((double)sU[(long long)t * R + j] * (double)w * (double)xs[t] * up);
     const __half hi = __float2half_rn(x);
     xt[(long long)j * ld + t] = hi;
     xt[(long long)(R + j) * ld + t] = __float2half_rn(x - __half2float(hi));
@@ -1267,7 +1352,7 @@ struct GradArgs {
   long long Vpad;
   const float* gAp;                // [chunk][d][R]
   const float* gBp;                // [seg][Vpad][R] bidx
-  const unsigned long long* corr;  // [Vpad][R] bidx
+  const unsigned long long* corr;  // [Vpad][R], row by row
   int scaled;                      // gBp carries xt's 2^e
   const int* stats;
   float* gA;       // layout 0: [d][r] and [r][V]; layout 1: [d][R] and [Vpad][R] bidx
@@ -1308,24 +1393,38 @@ static __global__ void __launch_bounds__(256) lh_grads(GradArgs a) {
     const long long at = v0 / a.res_rows * a.n_b2;
     slots = a.cparts * (tile_owner(at + a.n_b2 - 1, total2, a.G2) - tile_owner(at, total2, a.G2) + 1);
   }
-  for (int k = tid; k < kPackRows * a.R; k += 256) {
-    const long long o = v0 * a.R + k;
-    const int i = 2 * (k / (2 * a.R)) + (k & 1), j = k % (2 * a.R) / 2;
-    double s = 0.0;
-    if (v0 + i < a.V) {
-#pragma unroll 4
-      for (int q = 0; q < slots; ++q) s += (double)a.gBp[q * stride + o];
-      s = s * ex - (double)(long long)a.corr[o] * fx;
+  constexpr int ld = kPackRows + 1;
+  const int n = kPackRows * a.R;  // 256 to 4096
+  const float* src = a.gBp + v0 * a.R;
+  for (int k0 = tid; k0 < n; k0 += 4 * 256) {
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int q = 0; q < slots; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (k0 + 256 * e < n) s[e] += (double)src[q * stride + k0 + 256 * e];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = k0 + 256 * e, i = 2 * (k / (2 * a.R)) + (k & 1), j = k % (2 * a.R) / 2;
+      if (k < n) tile[j * ld + i] = v0 + i < a.V ? (float)(s[e] * ex) : 0.f;
     }
-    const float g = bad ? nan : (float)s;
-    if (a.layout) a.gB[o] = g;
-    else tile[j * (kPackRows + 1) + i] = g;
   }
-  if (!a.layout) {
-    __syncthreads();
+  __syncthreads();
+#pragma unroll 4
+  for (int k = tid; k < n; k += 256) {
+    const long long c = (long long)a.corr[v0 * a.R + k];
+    if (c != 0) {
+      float& x = tile[k % a.R * ld + k / a.R];
+      x = (float)((double)x - (double)c * fx);
+    }
+  }
+  __syncthreads();
+  if (a.layout) {
+    for (int k = tid; k < n; k += 256)
+      a.gB[v0 * a.R + k] = bad ? nan : tile[k % (2 * a.R) / 2 * ld + 2 * (k / (2 * a.R)) + (k & 1)];
+  } else {
     for (int k = tid; k < a.r * kPackRows; k += 256) {
       const int j = k / kPackRows, i = k % kPackRows;
-      if (v0 + i < a.V) a.gB[(long long)j * a.V + v0 + i] = tile[j * (kPackRows + 1) + i];
+      if (v0 + i < a.V) a.gB[(long long)j * a.V + v0 + i] = bad ? nan : tile[j * ld + i];
     }
   }
   if (a.tail && blk == 0) {
