@@ -163,6 +163,24 @@ bool launch_pairs(K kern, int pairs, int threads, int smem, cudaStream_t st, con
   return cudaLaunchKernelEx(&lc, kern, args...) == cudaSuccess;
 }
 
+// Launch with a programmatic dependency on the kernel ahead (whose end the kernel
+// waits for by itself, grid_wait).
+template <class K, class... Args>
+bool launch_after(K kern, int blocks, int threads, size_t smem, cudaStream_t st,
+                  const Args&... args) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)blocks);
+  lc.blockDim = dim3((unsigned)threads);
+  lc.dynamicSmemBytes = smem;
+  lc.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  return cudaLaunchKernelEx(&lc, kern, args...) == cudaSuccess;
+}
+
 using PassKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap,
                             const CUtensorMap, const GemmArgs);
 
@@ -255,6 +273,12 @@ int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_block
   return 0;
 }
 
+// The pass for few positions, one slot per 128 vocab rows; where records have 64
+// columns and the positions fit.
+constexpr int kFewMax = 32;
+bool few_positions(int T, int sub) { return T <= kFewMax && sub == 64; }
+int few_blocks(int V) { return (V + kFewRows - 1) / kFewRows; }
+
 struct ScoreWs {
   int* stats;
   __half *h16, *haug, *waug;
@@ -270,8 +294,10 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
   Carve c{static_cast<uint8_t*>(ws)};
   const long long Vpad = round_up(hd.V, kBN);
   const int n_a = (T + 2 * kBM - 1) / (2 * kBM), n_b = (int)(Vpad / kBN);
-  const size_t part = (size_t)4 * most_segments(n_a, n_b) * n_a * 2 * kBM;
   w.sub = record_columns(hd.V, top_k);
+  const size_t part = few_positions(T, w.sub)
+                          ? (size_t)few_blocks(hd.V) * kFewMax
+                          : (size_t)4 * most_segments(n_a, n_b) * n_a * 2 * kBM;
   w.n_sub = (hd.V + w.sub - 1) / w.sub;
   w.stats = c.take<int>(kStatWords);
   w.h16 = c.take<__half>((size_t)T * hd.d);
@@ -523,8 +549,10 @@ size_t head_distill_bytes(const HeadCore& hd, int T, int, bool grads) {
 int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const int32_t* tokens,
                    int top_k, float* logprob, float* entropy, int32_t* top_ids,
                    float* top_logprobs, void* ws, cudaStream_t st, const char** why) {
-  const Aug aug = aug_of(hd.r);
+  Aug aug = aug_of(hd.r);
   const ScoreWs w = score_ws(hd, T, top_k, ws);
+  const bool few = few_positions(T, w.sub);
+  if (few) aug.layout = aug.width = 0;  // the rank term from B as it is
   const int sms = sm_count();
   GemmArgs g{};
   fill_pass1(g, hd, aug, T, 1.0f);
@@ -539,19 +567,6 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   g.sub_arg = w.sub_arg;
   g.sub_arg2 = w.sub_arg2;
   g.n_sub = w.n_sub;
-  const PassPlan p = w.sub == 64  ? score_plan<64>(g.kblocks)
-                     : w.sub == 8 ? score_plan<8>(g.kblocks) : score_plan<1>(g.kblocks);
-  const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
-                                                       p.threads, p.smem));
-  if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
-  CUtensorMap mh, mw, mha, mwa;
-  if (!make_map(&mh, w.h16, T, hd.d, kBM) || !make_map(&mw, hd.W, hd.V, hd.d, kBM))
-    return *why = kNoMap, LORA_CE_ECUDA;
-  mha = mh;
-  mwa = mw;
-  if (aug.R && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
-                !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
-    return *why = kNoMap, LORA_CE_ECUDA;
   // per-row kernel: a warp per position, or the whole block where positions
   // are too few to fill the SMs that way
   ScoreArgs a{};
@@ -565,15 +580,14 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   void (*rows)(ScoreArgs) = lh_score_rows<kRowWarps, 32>;
   if (warps) rows = w.n_sub <= 24 * 32 ? lh_score_rows<1, 24> : lh_score_rows<1, 32>;
   else if (w.n_sub <= 4 * 256) rows = lh_score_rows<kRowWarps, 4>;
-  const size_t rows_smem =
-      warps ? kScoreRows * (team + (size_t)(w.n_sub + 1) * 4) : team;
+  const size_t rows_smem = warps ? kScoreRows * (team + (size_t)(w.n_sub + 1) * 4) : team;
   if (!allow_smem(reinterpret_cast<const void*>(rows), rows_smem))
     return *why = kNoFit, LORA_CE_ECUDA;
 
   PrepArgs pa = prep_args(hd, aug, H, dtype, T);
   pa.h16 = w.h16;
   pa.sU = w.sU;
-  pa.haug = aug.R ? w.haug : nullptr;
+  pa.haug = aug.width ? w.haug : nullptr;
   pa.stats = w.stats;
   PackArgs pk{};
   pk.B = BView{hd.B, hd.V, hd.r, aug.R, hd.layout};
@@ -584,14 +598,44 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   pk.waug = w.waug;
   pk.aug_layout = aug.layout;
   pk.aug_width = aug.width;
-  if (launch_prep(pa, pk, true, 0, aug.R != 0, sms, st)) return *why = kNoFit, LORA_CE_ECUDA;
-  const int G = (int)std::min<long long>(units, (long long)g.n_a * g.n_b);
-  if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, g))
-    return *why = kNoLaunch, LORA_CE_ECUDA;
+
+  if (few) {
+    if (launch_prep(pa, pk, true, 0, false, sms, st)) return *why = kNoFit, LORA_CE_ECUDA;
+    const int nt = (T + 7) / 8, blocks = few_blocks(hd.V);
+    void (*kern)(FewArgs) = nt == 1 ? lh_score_few<1> : nt == 2 ? lh_score_few<2> : lh_score_few<4>;
+    const size_t smem = few_smem(nt <= 2 ? nt : 4, hd.d, aug.R);
+    if (!allow_smem(reinterpret_cast<const void*>(kern), smem))
+      return *why = kNoFit, LORA_CE_ECUDA;
+    const float lg = (float)((1.0 + kLoss32) / std::log(2.0));
+    const FewArgs f{hd.W, w.h16, w.sU, pk.B, T, hd.V, hd.d, hd.r, aug.R, lg, kFewMax,
+                    w.p_max, w.p_sum, w.p_ent, w.sub_max, w.sub_second, w.sub_rest,
+                    w.sub_arg, w.sub_arg2, w.n_sub};
+    if (!launch_after(kern, blocks, 256, smem, st, f)) return *why = kNoLaunch, LORA_CE_ECUDA;
+    a.p = SlotPlan{1, 1, blocks, blocks, kFewMax, w.p_max, w.p_sum, w.p_ent, nullptr};
+    a.lg = lg;
+  } else {
+    const PassPlan p = w.sub == 64  ? score_plan<64>(g.kblocks)
+                       : w.sub == 8 ? score_plan<8>(g.kblocks) : score_plan<1>(g.kblocks);
+    const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
+                                                         p.threads, p.smem));
+    if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
+    CUtensorMap mh, mw, mha, mwa;
+    if (!make_map(&mh, w.h16, T, hd.d, kBM) || !make_map(&mw, hd.W, hd.V, hd.d, kBM))
+      return *why = kNoMap, LORA_CE_ECUDA;
+    mha = mh;
+    mwa = mw;
+    if (aug.R && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
+                  !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
+      return *why = kNoMap, LORA_CE_ECUDA;
+    if (launch_prep(pa, pk, true, 0, aug.R != 0, sms, st)) return *why = kNoFit, LORA_CE_ECUDA;
+    const int G = (int)std::min<long long>(units, (long long)g.n_a * g.n_b);
+    if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, g))
+      return *why = kNoLaunch, LORA_CE_ECUDA;
+    a.p = SlotPlan{col_parts(EpiScore<65536, 64>::kWarps), g.n_a, g.n_b, units, g.Tcap,
+                   w.p_max, w.p_sum, w.p_ent, nullptr};
+    a.lg = g.lg;
+  }
   a.z = logit_args(hd, aug, T, w.h16, w.sU, w.haug, w.waug);
-  a.p = SlotPlan{col_parts(EpiScore<65536, 64>::kWarps), g.n_a, g.n_b, units, g.Tcap,
-                 w.p_max, w.p_sum, w.p_ent, nullptr};
-  a.lg = g.lg;
   a.sub_max = w.sub_max;
   a.sub_second = w.sub_second;
   a.sub_rest = w.sub_rest;
@@ -603,9 +647,11 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   a.entropy = entropy;
   a.top_ids = top_ids;
   a.top_logprobs = top_logprobs;
-  rows<<<warps ? (T + kScoreRows - 1) / kScoreRows : T, warps ? 32 * kScoreRows : 32 * kRowWarps,
-         rows_smem, st>>>(a);
-  if (cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
+  const int per = warps ? kScoreRows : 1;
+  const int threads = warps ? 32 * kScoreRows : 32 * kRowWarps;
+  if (!launch_after(rows, (T + per - 1) / per, threads, rows_smem, st, a) ||
+      cudaGetLastError() != cudaSuccess)
+    return *why = kNoLaunch, LORA_CE_ECUDA;
   return 0;
 }
 

@@ -218,6 +218,18 @@ struct EpiScore {
   }
 };
 
+// ------------------------------------------------------------- launches
+// Programmatic dependent launch: a kernel's blocks may start before the kernel
+// ahead of it in the stream has ended; they touch nothing of its before
+// grid_wait() (which also makes its writes visible), and let the next one start
+// with grid_launch().
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void grid_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ------------------------------------------------------------- preparation
 struct PrepArgs {
   const void* H;
@@ -555,6 +567,7 @@ static __global__ void __launch_bounds__(256) lh_prep(PrepArgs a, PackArgs b, in
                                                       int max_blocks) {
   extern __shared__ __align__(16) float smem_prep[];
   const int blk = (int)blockIdx.x;
+  grid_launch();  // (a kernel launched to depend waits for this one's end)
   if (blk < prep_blocks) {
     if (blk == 0 && threadIdx.x == 0 && !a.ids) a.stats[kStErr] = 0;
     if constexpr (kRank < 0) prep_row(a, blk, smem_prep);
@@ -575,6 +588,15 @@ static __global__ void __launch_bounds__(256) lh_prep(PrepArgs a, PackArgs b, in
     pack_tile(b, (long long)(blk - prep_blocks - max_blocks) * kPackRows,
               smem_prep);
   }
+}
+
+// Order of floats as order of unsigned words (-inf lowest, above 0).
+__device__ __forceinline__ unsigned order_key(float x) {
+  const unsigned u = __float_as_uint(x);
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_float(unsigned k) {
+  return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
 }
 
 // ------------------------------------------------------------- logits again
@@ -804,6 +826,181 @@ __device__ __forceinline__ RowSum merge_row(const SlotPlan& p, int t, int nslot,
   return RowSum{M, S, E};
 }
 
+// ------------------------------------------------------------- few positions
+struct FewArgs {
+  const __half* W;
+  const __half* h16;
+  const float* sU;  // [T][R]
+  BView B;
+  int T, V, d, r, R;
+  float lg;
+  long long ld;  // row stride of the partials
+  float* p_max;
+  float* p_sum;
+  float* p_ent;
+  float* sub_max;
+  float* sub_second;
+  float* sub_rest;
+  uint8_t* sub_arg;
+  uint8_t* sub_arg2;
+  int n_sub;
+};
+constexpr int kFewRows = 128;           // vocab rows per block, 16 per warp
+constexpr int kFewLdZ = kFewRows + 4;   // floats per position of the logit tile
+__host__ __device__ constexpr int few_ldh(int d) { return d + 32; }  // f16 per position
+__host__ __device__ inline size_t few_smem(int NT, int d, int R) {
+  const size_t h = (size_t)8 * NT * few_ldh(d) * 2, z = (size_t)8 * NT * kFewLdZ * 4;
+  return (h > z ? h : z) + (size_t)8 * NT * R * 4;
+}
+
+// The pass over z for up to 8 NT positions, bound by reading W once: a warp takes
+// 16 vocab rows as A of mma (16 bytes per lane and row at a time, as logits16)
+// and the positions as B, from shared memory; every 32 products have their own
+// accumulator (kLoss32).  The rank term from B as it is, so that nothing of the
+// vocabulary's side is packed.  Then the block's logits, in shared memory, give
+// the same partial sums and records as EpiScore<64>, one slot per block.
+template <int NT>
+static __global__ void __launch_bounds__(256, 3) lh_score_few(FewArgs a) {
+  constexpr int kUnroll = 6;
+  constexpr unsigned kAll = 0xffffffffu;
+  extern __shared__ __align__(16) uint8_t smem_few[];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, c = lane & 3, g = lane >> 2;
+  const int ldh = few_ldh(a.d);
+  __half* sh = reinterpret_cast<__half*>(smem_few);
+  float* sz = reinterpret_cast<float*>(smem_few);  // over h once that is used up
+  float* su = reinterpret_cast<float*>(smem_few + few_smem(NT, a.d, 0));
+  const int v0 = (int)blockIdx.x * kFewRows;
+  const __half* w0 = a.W + (long long)min(v0 + 16 * w + g, a.V - 1) * a.d + 8 * c;
+  const __half* w1 = a.W + (long long)min(v0 + 16 * w + g + 8, a.V - 1) * a.d + 8 * c;
+  uint4 p[kUnroll], q[kUnroll];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = k0 + 32 * i;
+      p[i] = q[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (k < a.d) {
+        p[i] = *reinterpret_cast<const uint4*>(w0 + k);
+        q[i] = *reinterpret_cast<const uint4*>(w1 + k);
+      }
+    }
+  };
+  fetch(0);  // W is the caller's: its reads need not wait for the kernel ahead
+  grid_wait();
+  grid_launch();
+  for (int k = tid; k < 8 * NT * (a.d / 8); k += 256) {
+    const int t = k / (a.d / 8), i = k % (a.d / 8) * 8;
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (t < a.T) x = *reinterpret_cast<const uint4*>(a.h16 + (long long)t * a.d + i);
+    *reinterpret_cast<uint4*>(sh + t * ldh + i) = x;
+  }
+  for (int k = tid; k < 8 * NT * a.R; k += 256) su[k] = k < a.T * a.R ? a.sU[k] : 0.f;
+  __syncthreads();
+  float z[NT][4] = {};
+  for (int k0 = 0; k0 < a.d; k0 += 32 * kUnroll) {
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = k0 + 32 * i;
+      if (k < a.d) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 x = *reinterpret_cast<const uint4*>(sh + (8 * n + g) * ldh + k + 8 * c);
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          auto mma = [&](unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                         unsigned b1) {
+            asm volatile(
+                "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+                "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+          };
+          mma(p[i].x, q[i].x, p[i].y, q[i].y, x.x, x.y);
+          mma(p[i].z, q[i].z, p[i].w, q[i].w, x.z, x.w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z[n][e] += d[e];
+        }
+      }
+    }
+    if (k0 + 32 * kUnroll < a.d) fetch(k0 + 32 * kUnroll);
+  }
+  __syncthreads();
+  // lane (g, c): rows g, g + 8 of positions 2 c, 2 c + 1
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      sz[(8 * n + 2 * c + (e & 1)) * kFewLdZ + 16 * w + g + 8 * (e >> 1)] = z[n][e];
+  __syncthreads();
+  if (a.r > 0) {  // thread: one vocab row, every other position
+    const int i = tid & (kFewRows - 1), t0 = tid / kFewRows, v = min(v0 + i, a.V - 1);
+    float s[4 * NT] = {};
+#pragma unroll 4
+    for (int j = 0; j < a.r; ++j) {
+      const float b = a.B.at(j, v);
+#pragma unroll
+      for (int n = 0; n < 4 * NT; ++n) s[n] = fmaf(su[(2 * n + t0) * a.R + j], b, s[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < 4 * NT; ++n) sz[(2 * n + t0) * kFewLdZ + i] += s[n];
+    __syncthreads();
+  }
+  // a warp per position: partial sums of the block's rows, two records
+  for (int t = w; t < a.T; t += 8) {
+    float x[4];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = v0 + lane + 32 * i < a.V ? sz[t * kFewLdZ + lane + 32 * i] : -INFINITY;
+      m = fmaxf(m, x[i]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, off));
+    const float mL = m * a.lg;
+    float S = 0.f, E = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y = fmaxf(fmaf(x[i], a.lg, -mL), -1e30f), e = ex2f(y);
+      S += e;
+      E = fmaf(e, y, E);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      S += __shfl_xor_sync(kAll, S, off);
+      E += __shfl_xor_sync(kAll, E, off);
+    }
+    if (lane == 0) {
+      const long long o = (long long)blockIdx.x * a.ld + t;
+      a.p_max[o] = mL;
+      a.p_sum[o] = S;
+      a.p_ent[o] = E;
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int rec = v0 / 64 + half;
+      if (rec >= a.n_sub) break;
+      // the three largest, equal ones by column: columns lane and lane + 32
+      unsigned k0 = order_key(x[2 * half]), k1 = order_key(x[2 * half + 1]);
+      unsigned top[3];
+      int at[3];
+#pragma unroll
+      for (int q3 = 0; q3 < 3; ++q3) {
+        top[q3] = __reduce_max_sync(kAll, max(k0, k1));
+        at[q3] = (int)__reduce_min_sync(kAll, k0 == top[q3]   ? (unsigned)lane
+                                              : k1 == top[q3] ? (unsigned)lane + 32u : 64u);
+        if (at[q3] == lane) k0 = 0u;
+        if (at[q3] == lane + 32) k1 = 0u;
+      }
+      if (lane == 0) {
+        const long long o = sub_idx(t, rec, a.n_sub);
+        a.sub_max[o] = key_float(top[0]);
+        a.sub_second[o] = key_float(top[1]);
+        a.sub_rest[o] = key_float(top[2]);
+        a.sub_arg[o] = (uint8_t)at[0];
+        a.sub_arg2[o] = (uint8_t)at[1];
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------- score, per row
 struct ScoreArgs {
   LogitArgs z;
@@ -871,6 +1068,7 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   float* cols = reinterpret_cast<float*>(col_id + 64);
   int* words = reinterpret_cast<int*>(cols + 64);  // [0..7] picks per warp, [8] picks
 
+  grid_wait();
   // this thread's records: (w NK + i) 32 + lane, so that record order is warp order
   float key[NK];
   if constexpr (TW == 1) {

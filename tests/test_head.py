@@ -280,6 +280,12 @@ def check_score(p, k, out, rows=slice(None)):
     (100, 2048, 640, 13, 10, "f16"),   # 11 resident K-blocks
     (64, 49152, 576, 64, 20, "f32"),
     (1200, 4099, 128, 4, 8, "bf16"),   # a warp per position
+    (8, 49152, 576, 16, 20, "bf16"),   # few positions: one, two and four groups of eight
+    (9, 49000, 576, 4, 0, "f16"),
+    (32, 20001, 128, 33, 50, "f32"),
+    (33, 20001, 128, 33, 50, "f32"),   # and one more
+    (5, 20035, 640, 64, 8, "bf16"),    # the last block and record cut short
+    (3, 100000, 64, 0, 128, "bf16"),
     (1300, 257, 64, 33, 0, "bf16"),    # no alternatives
     (40, 140000, 64, 4, 9, "bf16"),    # a vocabulary larger than the model's
 ])
@@ -300,7 +306,7 @@ def test_score_parts_can_be_left_out():
 
 
 @gpu
-@pytest.mark.parametrize("T", [9, 1200])
+@pytest.mark.parametrize("T", [9, 1200, 40])
 def test_ties_go_to_the_lowest_id(T):
     """Hidden states of zeros (padding): every logit is 0.  And rows of W that
     repeat: their logits are equal to the last bit."""
