@@ -580,7 +580,8 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   void (*rows)(ScoreArgs) = lh_score_rows<kRowWarps, 32>;
   if (warps) rows = w.n_sub <= 24 * 32 ? lh_score_rows<1, 24> : lh_score_rows<1, 32>;
   else if (w.n_sub <= 4 * 256) rows = lh_score_rows<kRowWarps, 4>;
-  const size_t rows_smem = warps ? kScoreRows * (team + (size_t)(w.n_sub + 1) * 4) : team;
+  const size_t rows_smem =
+      warps ? kScoreRows * std::max(team, (size_t)(w.n_sub + 1) * 4) : team;
   if (!allow_smem(reinterpret_cast<const void*>(rows), rows_smem))
     return *why = kNoFit, LORA_CE_ECUDA;
 

@@ -629,6 +629,7 @@ constexpr double kLoss32 = 0.79 * 1.5 / 33554432.0 * 1.4426950408889634;
 template <bool kSum64, class Out>
 __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* ids, int n, int lane,
                                          Out* out) {
+  constexpr int kBatch = 6;
   const int c = lane & 3, g = lane >> 2;
   const long long v0 = ids[min(g, n - 1)], v1 = ids[min(g + 8, n - 1)];
   double z0 = 0.0, z1 = 0.0;
@@ -640,13 +641,8 @@ __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* i
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   };
-  auto step = [&](const __half* w0, const __half* w1, const __half* h, bool in) {
-    uint4 p = make_uint4(0u, 0u, 0u, 0u), q = p, x = p;
-    if (in) {
-      p = *reinterpret_cast<const uint4*>(w0);
-      q = *reinterpret_cast<const uint4*>(w1);
-      if (g == 0) x = *reinterpret_cast<const uint4*>(h);
-    }
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  auto add = [&](uint4 p, uint4 q, uint4 x) {
     mma(p.x, q.x, p.y, q.y, x.x, x.y);
     mma(p.z, q.z, p.w, q.w, x.z, x.w);
     if constexpr (kSum64) {
@@ -656,12 +652,35 @@ __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* i
     }
   };
   {
+    // six steps' rows at a time in flight: one after another, each would wait
+    // for the L2
     const __half* w0 = a.W + v0 * a.d + 8 * c;
     const __half* w1 = a.W + v1 * a.d + 8 * c;
     const __half* h = a.h16 + (long long)t * a.d + 8 * c;
-#pragma unroll 6
-    for (int k = 0; k < a.d; k += 32) step(w0 + k, w1 + k, h + k, true);
+    for (int k0 = 0; k0 < a.d; k0 += 32 * kBatch) {
+      uint4 p[kBatch], q[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        p[i] = q[i] = zero;
+        if (k0 + 32 * i < a.d) {
+          p[i] = *reinterpret_cast<const uint4*>(w0 + k0 + 32 * i);
+          q[i] = *reinterpret_cast<const uint4*>(w1 + k0 + 32 * i);
+        }
+      }
+      asm volatile("" ::: "memory");  // all of them issued before the first is used
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        uint4 x = zero;
+        if (g == 0 && k0 + 32 * i < a.d) x = *reinterpret_cast<const uint4*>(h + k0 + 32 * i);
+        add(p[i], q[i], x);
+      }
+    }
   }
+  auto step = [&](const __half* w0, const __half* w1, const __half* h, bool in) {
+    add(in ? *reinterpret_cast<const uint4*>(w0) : zero,
+        in ? *reinterpret_cast<const uint4*>(w1) : zero,
+        in && g == 0 ? *reinterpret_cast<const uint4*>(h) : zero);
+  };
   if (a.waug) {
     const __half* w0 = a.waug + v0 * a.aug_width + 8 * c;
     const __half* w1 = a.waug + v1 * a.aug_width + 8 * c;
@@ -700,7 +719,7 @@ __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* i
 
 // How far apart two logits have to be for logits16 to tell their order: several
 // times the largest error seen.
-__device__ __forceinline__ float logit_gap(double z) { return 4e-6f * (1.0f + fabsf((float)z)); }
+__device__ __forceinline__ float logit_gap(float z) { return 4e-6f * (1.0f + fabsf(z)); }
 
 // One logit by one warp with 64-bit sums throughout (products of f16 are exact
 // in f32; U is formed again): for those whose order logits16 does not tell.
@@ -713,10 +732,16 @@ __device__ __forceinline__ double logit64(const LogitArgs& a, int t, int v, int 
   const __half* h = a.h16 + (long long)t * a.d;
   const __half* w = a.W + (long long)v * a.d;
   double z = 0.0;
-  for (int i = lane; i < a.d; i += 32)
-    z += (double)(__half2float(h[i]) * __half2float(w[i]));
+#pragma unroll
+  for (int k = 0; k < kMaxHead64; ++k)
+    if (64 * k < a.d) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(h + 64 * k + 2 * lane));
+      const float2 y = __half22float2(*reinterpret_cast<const __half2*>(w + 64 * k + 2 * lane));
+      z += (double)(x.x * y.x) + (double)(x.y * y.y);
+    }
   for (int j = 0; j < a.r; ++j) {
     double u = 0.0;
+#pragma unroll 6
     for (int i = lane; i < a.d; i += 32)
       u = fma((double)__half2float(h[i]), (double)a.A[(long long)i * a.lda + j], u);
     z = fma(u, (double)a.scale * (double)a.B.at(j, v), z);  // the lanes' shares add up below
@@ -1028,7 +1053,7 @@ struct ScoreArgs {
 // logits; counters.  A multiple of 16 bytes.
 __host__ __device__ inline int score_picks(int n_pick) { return n_pick + kPickSlack; }
 __host__ __device__ inline size_t score_team_smem(int n_pick, int cap) {
-  return ((size_t)(2 * kRowWarps + cap) * 8 + (size_t)cap * 12 +
+  return ((size_t)(2 * kRowWarps + cap) * 8 + (size_t)cap * 16 +
           (size_t)score_picks(n_pick) * 16 + 128 * 4 + 16 * 4 + 15) / 16 * 16;
 }
 constexpr int kScoreRows = 4;  // positions per block where each has a warp
@@ -1039,7 +1064,7 @@ constexpr int kScoreRows = 4;  // positions per block where each has a warp
 // less what rounding may have moved, again, with 64-bit sums where two are too
 // close to tell their order; sort, write.  The softmax's sums get the difference.
 template <int TW, int NK>
-static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW == 1 ? 6 : 2)
+static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW == 1 ? 5 : 2)
     lh_score_rows(ScoreArgs a) {
   constexpr int kTeams = TW == 1 ? kScoreRows : 1;
   constexpr int kThreads = 32 * TW;
@@ -1059,7 +1084,8 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   double* z64 = team.red + 2 * kRowWarps;
   int* ids = reinterpret_cast<int*>(z64 + a.cap);
   float* approx = reinterpret_cast<float*>(ids + a.cap);
-  int* ranks = reinterpret_cast<int*>(approx + a.cap);
+  float* approx32 = approx + a.cap;  // again, rounded
+  int* ranks = reinterpret_cast<int*>(approx32 + a.cap);
   int* picked = ranks + a.cap;
   float* psecond = reinterpret_cast<float*>(picked + P);
   float* prest = psecond + P;
@@ -1072,20 +1098,22 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   // this thread's records: (w NK + i) 32 + lane, so that record order is warp order
   float key[NK];
   if constexpr (TW == 1) {
-    // the block's rows' records are runs: through shared memory, [row][record]
-    float* stage = reinterpret_cast<float*>(smem_rows + kTeams * team_bytes);
+    // the block's rows' records are runs: through shared memory, [row][record],
+    // which is the teams' after that
+    float* stage = reinterpret_cast<float*>(smem_rows);
     const int ld = a.n_sub + 1, t0 = (int)blockIdx.x * kTeams;
     const float* src = a.sub_max + (long long)(t0 >> 3) * a.n_sub * 8 + (t0 & 7);
 #pragma unroll 8
     for (int k = threadIdx.x; k < a.n_sub * kTeams; k += 32 * kTeams)
       stage[(k % kTeams) * ld + k / kTeams] = src[k / kTeams * 8 + k % kTeams];
     __syncthreads();
-    if (t >= a.z.T) return;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const int k = i * 32 + lane;
       key[i] = k < a.n_sub ? stage[no * ld + k] : -INFINITY;
     }
+    __syncthreads();
+    if (t >= a.z.T) return;
   } else {
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
@@ -1271,21 +1299,39 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
     logits16<true>(a.z, t, ids + c, min(16, n_z - c), lane, z64 + c);
   team.sync();
   // ranks; all in 64 bits for logits too close to another to tell their order
+  // (the difference of f32 values tells that as well)
+  constexpr int kItems = TW == 1 ? 3 : 1;
   bool any_close = false;
-  for (int c0 = 32 * w; c0 < n_c && a.top_k > 0; c0 += kThreads) {
-    const int c = c0 + lane;
-    const double z = c < n_c ? z64[c] : INFINITY;
-    const float gap = logit_gap(z);
-    int rank = 0;
-    bool close = false;
-    for (int q = 0; q < n_c; ++q) {
-      const float dz = (float)(z64[q] - z);
-      rank += dz > 0.f;
-      close |= fabsf(dz) <= gap && q != c;
+  for (int c = lane + 32 * w; c < n_c; c += kThreads) approx32[c] = (float)z64[c];
+  team.sync();
+  for (int c0 = 32 * kItems * w; c0 < n_c && a.top_k > 0; c0 += kItems * kThreads) {
+    float z[kItems], gap[kItems];
+    int rank[kItems], close[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int c = c0 + 32 * i + lane;
+      z[i] = c < n_c ? approx32[c] : INFINITY;
+      gap[i] = c < n_c ? logit_gap(z[i]) : -1.f;
+      rank[i] = close[i] = 0;
     }
-    if (c < n_c) ranks[c] = close ? -1 : rank;
-    any_close |= close;
+    for (int q = 0; q < n_c; ++q) {
+      const float zq = approx32[q];
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        rank[i] += zq > z[i];
+        close[i] += fabsf(zq - z[i]) <= gap[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int c = c0 + 32 * i + lane;
+      if (c < n_c) {
+        ranks[c] = close[i] > 1 ? -1 : rank[i];  // (it is close to itself)
+        any_close |= close[i] > 1;
+      }
+    }
   }
+  team.sync();
   if (team.count(any_close && a.top_k > 0) > 0) {
     for (int c0 = 32 * w; c0 < n_c; c0 += kThreads) {
       const int c = c0 + lane;
