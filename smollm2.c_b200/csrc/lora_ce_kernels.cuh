@@ -53,7 +53,7 @@ constexpr int kBM = 128;               // resident rows per tile (TMEM lanes)
 constexpr int kBN = 256;               // streamed rows per tile (TMEM columns)
 constexpr int kBK = 64;                // K elements per 128-byte swizzle row
 constexpr int kRingBytes = 65536;      // streamed-operand ring (2 x 32 KB, or 4 x 16 KB per CTA in pairs)
-constexpr int kMaxStages = 4;
+constexpr int kMaxStages = 5;
 constexpr int kAKBytes = kBM * kBK * 2;   // 16 KB per resident K-block
 // Per-CTA streamed rows per tile and stage geometry for 1-CTA (kPair 1) and
 // CTA-pair (kPair 2, cta_group::2) tiles.
@@ -257,6 +257,7 @@ __device__ __forceinline__ void fold_sum(float2& part, float& hi, float& lo) {
 template <int R, bool kAug_ = (R >= LCE_AUG_MIN_RANK), bool kChunk = false, bool kTemp = false>
 struct EpiLse {
   static constexpr bool kAug = kAug_;  // rank term in the accumulator
+  static constexpr bool kDepend = kTemp;  // launched to depend on the kernel ahead
   static constexpr int kRec = R;  // floats per column
   // ring (CTA pairs): 3 stages beside 10 resident K-blocks at rank 8, 2 at
   // rank 16 and in rank chunks (up to 11 resident K-blocks)
@@ -432,6 +433,7 @@ struct EpiLse {
 template <int R, bool kAug_ = (R >= LCE_AUG_MIN_RANK), bool kChunk = false, bool kTemp = false>
 struct EpiGrad {
   static constexpr bool kAug = kAug_;  // rank term in the accumulator
+  static constexpr bool kDepend = kTemp;  // launched to depend on the kernel ahead
   // rank chunks read their own records {sU[0..16), -M log2 e, 1/S}
   // (crec_idx), the others the position records tok[] (tidx)
   static constexpr int kRec = kChunk ? R + 2 : R + 4;
@@ -610,6 +612,10 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
   if constexpr (kPair == 2) cluster_sync();  // peer barriers initialised before any signal
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if constexpr (Epi::kDepend) {  // set up beside the end of the kernel ahead
+    grid_wait();
+    grid_launch();
+  }
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)

@@ -258,6 +258,10 @@ __global__ void __launch_bounds__(kThreadsT, 1)
   cluster_sync();  // peer barriers initialised before any signal
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if constexpr (kTemp) {  // launched to depend on the kernel ahead
+    grid_wait();
+    grid_launch();
+  }
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)

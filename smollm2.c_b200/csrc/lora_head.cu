@@ -146,6 +146,8 @@ struct Carve {
   }
 };
 
+// Launch of a GEMM pass on CTA pairs, with a programmatic dependency on the kernel
+// ahead (whose end the kernel waits for by itself, grid_wait).
 template <class K, class... Args>
 bool launch_pairs(K kern, int pairs, int threads, int smem, cudaStream_t st, const Args&... args) {
   cudaLaunchConfig_t lc = {};
@@ -153,18 +155,19 @@ bool launch_pairs(K kern, int pairs, int threads, int smem, cudaStream_t st, con
   lc.blockDim = dim3((unsigned)threads);
   lc.dynamicSmemBytes = (size_t)smem;
   lc.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   lc.attrs = attr;
-  lc.numAttrs = 1;
+  lc.numAttrs = 2;
   return cudaLaunchKernelEx(&lc, kern, args...) == cudaSuccess;
 }
 
-// Launch with a programmatic dependency on the kernel ahead (whose end the kernel
-// waits for by itself, grid_wait).
+// The same for any other kernel that waits.
 template <class K, class... Args>
 bool launch_after(K kern, int blocks, int threads, size_t smem, cudaStream_t st,
                   const Args&... args) {
@@ -189,22 +192,30 @@ struct PassPlan {
   int threads = 0, smem = 0;
 };
 
-// EpiScore with the largest ring that fits beside the resident K-blocks.
-template <int kSub>
-PassPlan score_plan(int kblocks) {
+// EpiScore with the largest ring that fits beside the resident K-blocks; at rank
+// 4 the rank term in the epilogue, from staged records.
+template <class Epi, bool kStage>
+PassPlan plan_of(int kblocks) {
   PassPlan p;
-  p.threads = block_threads(EpiScore<65536, kSub>::kWarps);
-  if (kblocks <= 10) {
-    p.kern = lce_gemm_kernel<EpiScore<65536, kSub>, false, 2>;
-    p.smem = SmemLayout::bytes(kblocks, 0, 65536);
-  } else if (kblocks == 11) {
-    p.kern = lce_gemm_kernel<EpiScore<49152, kSub>, false, 2>;
-    p.smem = SmemLayout::bytes(kblocks, 0, 49152);
-  } else {
-    p.kern = lce_gemm_kernel<EpiScore<32768, kSub>, false, 2>;
-    p.smem = SmemLayout::bytes(kblocks, 0, 32768);
-  }
+  p.kern = lce_gemm_kernel<Epi, kStage, 2>;
+  p.threads = block_threads(Epi::kWarps);
+  p.smem = SmemLayout::bytes(kblocks, kStage ? Epi::kRec * Epi::kRecBufs : 0, Epi::kRing);
   return p;
+}
+template <int kSub>
+PassPlan score_plan(int kblocks, bool r4) {
+  if (r4)
+    return kblocks <= 9 ? plan_of<EpiScore<65536, kSub, true>, true>(kblocks)
+                        : plan_of<EpiScore<49152, kSub, true>, true>(kblocks);
+  return kblocks <= 9    ? plan_of<EpiScore<81920, kSub>, false>(kblocks)
+         : kblocks == 10 ? plan_of<EpiScore<65536, kSub>, false>(kblocks)
+         : kblocks == 11 ? plan_of<EpiScore<49152, kSub>, false>(kblocks)
+                         : plan_of<EpiScore<32768, kSub>, false>(kblocks);
+}
+PassPlan score_plan(int kblocks, int sub, bool r4) {
+  return sub == 64  ? score_plan<64>(kblocks, r4)
+         : sub == 8 ? score_plan<8>(kblocks, r4)
+         : sub == 1 ? score_plan<1>(kblocks, r4) : score_plan<0>(kblocks, r4);
 }
 
 // Columns per record: the widest that leaves four records per alternative.
@@ -248,7 +259,7 @@ void fill_pass1(GemmArgs& g, const HeadCore& hd, const Aug& aug, int T, float ta
 }
 
 // lh_prep over positions and vocab rows: a block per position up to two an SM,
-// else 32 positions per block.
+// else kTileRows positions per block.
 int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_blocks, bool pack,
                 int sms, cudaStream_t st) {
   const bool tiles = pa.Tpad > 2 * sms;
@@ -266,7 +277,7 @@ int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_block
   const int prep_blocks = !rows ? 0 : tiles ? (pa.Tpad + kTileRows - 1) / kTileRows : pa.Tpad;
   const int pack_blocks = pack ? (int)(pk.Vpad / kPackRows) : 0;
   const size_t smem =
-      std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R) : (size_t)(pa.d + 256) * 4,
+      std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R, pa.d) : (size_t)(pa.d + 256) * 4,
                pack ? (size_t)pk.R * (kPackRows + 1) * 4 : 0);
   if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return LORA_CE_ECUDA;
   kern<<<prep_blocks + max_blocks + pack_blocks, 256, smem, st>>>(pa, pk, prep_blocks, max_blocks);
@@ -282,6 +293,7 @@ int few_blocks(int V) { return (V + kFewRows - 1) / kFewRows; }
 struct ScoreWs {
   int* stats;
   __half *h16, *haug, *waug;
+  float *tok, *Bt;
   float *sU, *p_max, *p_sum, *p_ent, *sub_max, *sub_second, *sub_rest;
   uint8_t *sub_arg, *sub_arg2;
   int sub, n_sub;
@@ -302,8 +314,11 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
   w.stats = c.take<int>(kStatWords);
   w.h16 = c.take<__half>((size_t)T * hd.d);
   w.sU = c.take<float>((size_t)T * aug.R);
-  w.haug = c.take<__half>((size_t)T * aug.width);
-  w.waug = c.take<__half>((size_t)Vpad * aug.width);
+  const bool r4 = aug.R == 4;  // the rank term in the epilogue
+  w.tok = c.take<float>(r4 ? (size_t)(T + 1) * tok_stride(4) : 0);
+  w.Bt = c.take<float>(r4 && !hd.layout ? (size_t)Vpad * 4 : 0);
+  w.haug = c.take<__half>(r4 ? 0 : (size_t)T * aug.width);
+  w.waug = c.take<__half>(r4 ? 0 : (size_t)Vpad * aug.width);
   w.p_max = c.take<float>(part);
   w.p_sum = c.take<float>(part);
   w.p_ent = c.take<float>(part);
@@ -342,19 +357,18 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
   w.h16 = c.take<__half>((size_t)T * hd.d);
   w.sU = c.take<float>((size_t)T * R);
   w.wt = c.take<float>(T);
-  // rank 4 keeps the rank term in the epilogues of the gradient passes
-  const bool in_mma = !grads || R > 4;
+  const bool in_mma = R > 4;  // rank 4 keeps the rank term in the epilogues
   w.haug = c.take<__half>(in_mma ? (size_t)T * aug.width : 0);
   w.waug = c.take<__half>(in_mma ? (size_t)Vpad * aug.width : 0);
   w.p_max = c.take<float>(part);
   w.p_sum = c.take<float>(part);
+  w.tok = c.take<float>(grads && tc ? 0 : R == 0 || (!grads && R > 4) ? 0 : (size_t)Tpad * tok_stride(R));
+  w.Bt = c.take<float>(hd.layout || (!grads && R != 4) ? 0 : (size_t)Vpad * R);
   if (grads) {
     // chunks of four or eight epilogue columns a row: up to 4 slots per owner
     const int n_a2 = (hd.V + 2 * kBM - 1) / (2 * kBM), n_b2 = (T + bn - 1) / bn;
     const size_t segs = (size_t)(tc ? 1 : 4) * most_segments(n_a2, n_b2);
     w.p_q = c.take<float>(part * R);
-    w.tok = c.take<float>(tc ? 0 : (size_t)Tpad * tok_stride(R));
-    w.Bt = c.take<float>(hd.layout ? 0 : (size_t)Vpad * R);
     w.xv = c.take<__half>(tc ? (size_t)2 * R * Vpad : 0);
     w.xt = c.take<__half>(tc ? (size_t)2 * R * Tpad : 0);
     w.nml = c.take<float>(tc ? (size_t)Tpad + kMaxBNT : 0);
@@ -526,12 +540,19 @@ int grad_pass(Step& s, int R, const char** why) {
   }
 }
 
-template <int RC>
-void launch_dA(const Step& s, int R, const DistillWs& w) {
-  const int n_chunks = (s.T + kDAChunk - 1) / kDAChunk;
-  for (int r0 = 0; r0 < R; r0 += RC)
-    lce_dA_partial<RC><<<dim3(n_chunks, s.hd.d / 64), dim3(32, da_rows(RC)), 0, s.st>>>(
-        s.T, s.hd.d, w.h16, w.dU, w.gAp, R, r0);
+template <int R>
+bool launch_dA(const Step& s, const DistillWs& w) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)((s.T + kDAChunk - 1) / kDAChunk), (unsigned)(s.hd.d / 64));
+  lc.blockDim = dim3(256);
+  lc.stream = s.st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  return cudaLaunchKernelEx(&lc, lh_dA<R>, s.T, s.hd.d, (const __half*)w.h16,
+                            (const float*)w.dU, w.gAp) == cudaSuccess;
 }
 
 }  // namespace
@@ -552,7 +573,8 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   Aug aug = aug_of(hd.r);
   const ScoreWs w = score_ws(hd, T, top_k, ws);
   const bool few = few_positions(T, w.sub);
-  if (few) aug.layout = aug.width = 0;  // the rank term from B as it is
+  const bool r4 = aug.R == 4;
+  if (few || r4) aug.layout = aug.width = 0;  // the rank term from B as it is
   const int sms = sm_count();
   GemmArgs g{};
   fill_pass1(g, hd, aug, T, 1.0f);
@@ -589,6 +611,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   pa.h16 = w.h16;
   pa.sU = w.sU;
   pa.haug = aug.width ? w.haug : nullptr;
+  pa.tok = r4 && !few ? w.tok : nullptr;
   pa.stats = w.stats;
   PackArgs pk{};
   pk.B = BView{hd.B, hd.V, hd.r, aug.R, hd.layout};
@@ -596,7 +619,8 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   pk.r = hd.r;
   pk.R = aug.R;
   pk.Vpad = g.Vpad;
-  pk.waug = w.waug;
+  pk.Bt = r4 && !hd.layout ? w.Bt : nullptr;
+  pk.waug = aug.width ? w.waug : nullptr;
   pk.aug_layout = aug.layout;
   pk.aug_width = aug.width;
 
@@ -615,8 +639,9 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
     a.p = SlotPlan{1, 1, blocks, blocks, kFewMax, w.p_max, w.p_sum, w.p_ent, nullptr};
     a.lg = lg;
   } else {
-    const PassPlan p = w.sub == 64  ? score_plan<64>(g.kblocks)
-                       : w.sub == 8 ? score_plan<8>(g.kblocks) : score_plan<1>(g.kblocks);
+    const PassPlan p = score_plan(g.kblocks, w.sub, r4);
+    g.tok = w.tok;
+    g.Bt = hd.layout ? hd.B : w.Bt;
     const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
                                                          p.threads, p.smem));
     if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
@@ -625,10 +650,11 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
       return *why = kNoMap, LORA_CE_ECUDA;
     mha = mh;
     mwa = mw;
-    if (aug.R && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
-                  !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
+    if (aug.width && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
+                      !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
       return *why = kNoMap, LORA_CE_ECUDA;
-    if (launch_prep(pa, pk, true, 0, aug.R != 0, sms, st)) return *why = kNoFit, LORA_CE_ECUDA;
+    if (launch_prep(pa, pk, true, 0, pk.Bt || pk.waug, sms, st))
+      return *why = kNoFit, LORA_CE_ECUDA;
     const int G = (int)std::min<long long>(units, (long long)g.n_a * g.n_b);
     if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, g))
       return *why = kNoLaunch, LORA_CE_ECUDA;
@@ -665,7 +691,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   const int R = aug.R;
   const DistillWs w = distill_ws(hd, T, grads, ws);
   const bool tc = grads && R >= 16;
-  if (grads && R == 4) aug.layout = aug.width = 0;
+  const bool r4 = R == 4;
+  if (r4) aug.layout = aug.width = 0;  // the rank term in the epilogues
   Step s{hd, w, aug, T, sm_count(), tau, st, GemmArgs{}, SlotPlan{}};
   fill_pass1(s.g, hd, aug, T, tau);
   s.Bt = hd.layout ? hd.B : w.Bt;
@@ -690,7 +717,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pa.K = K;
   pa.tau = tau;
   pa.wt = w.wt;
-  if (grads && !tc) {
+  if (grads ? !tc : r4) {
     pa.tok = w.tok;
     pa.Tpad = (int)round_up(T, kBN);
   }
@@ -700,7 +727,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pk.r = hd.r;
   pk.R = R;
   pk.Vpad = s.g.Vpad;
-  pk.Bt = grads && !hd.layout ? w.Bt : nullptr;
+  pk.Bt = (grads || r4) && !hd.layout ? w.Bt : nullptr;
   pk.Bt_plain = tc;  // the rank sums' passes have xv instead
   pk.waug = aug.width ? w.waug : nullptr;
   pk.aug_layout = aug.layout;
@@ -717,7 +744,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   if (grads) {
     rc = grad_pass<1>(s, R, why);
   } else {
-    const PassPlan p = score_plan<0>(s.g.kblocks);
+    const PassPlan p = score_plan(s.g.kblocks, 0, r4);
     const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
                                                          p.threads, p.smem));
     if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
@@ -726,8 +753,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
       return *why = kNoMap, LORA_CE_ECUDA;
     mha = mh;
     mwa = mw;
-    if (R && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
-              !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
+    if (aug.width && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
+                      !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
       return *why = kNoMap, LORA_CE_ECUDA;
     s.g.n_b = (int)(s.g.Vpad / kBN);
     const int G = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
@@ -761,22 +788,25 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   const bool warps = T >= s.sms * kRowWarps;
   auto rows = grads ? (warps ? lh_distill_rows<true, 1> : lh_distill_rows<true, kRowWarps>)
                     : (warps ? lh_distill_rows<false, 1> : lh_distill_rows<false, kRowWarps>);
-  rows<<<warps ? (T + kRowWarps - 1) / kRowWarps : T, 32 * kRowWarps, 0, st>>>(a);
+  if (!launch_after(rows, warps ? (T + kRowWarps - 1) / kRowWarps : T, 32 * kRowWarps, 0, st, a))
+    return *why = kNoLaunch, LORA_CE_ECUDA;
   if (!grads) {
     if (cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
     return 0;
   }
   if (tc) {
     const long long n = (long long)T * R;
-    lh_xt<<<(int)std::min<long long>((n + 255) / 256, 8LL * s.sms), 256, 0, st>>>(
-        T, R, round_up(T, kBN), w.sU, w.wt, w.xs, w.stats, w.xt);
+    if (!launch_after(lh_xt, (int)std::min<long long>((n + 255) / 256, 8LL * s.sms), 256, 0, st, T,
+                      R, (long long)round_up(T, kBN), (const float*)w.sU, (const float*)w.wt,
+                      (const float*)w.xs, (const int*)w.stats, w.xt))
+      return *why = kNoLaunch, LORA_CE_ECUDA;
   }
   if ((rc = grad_pass<2>(s, R, why))) return rc;
-  switch (R) {
-    case 4: launch_dA<4>(s, R, w); break;
-    case 8: launch_dA<8>(s, R, w); break;
-    default: launch_dA<16>(s, R, w); break;
-  }
+  const bool dA_ok = R == 4    ? launch_dA<4>(s, w)
+                     : R == 8  ? launch_dA<8>(s, w)
+                     : R == 16 ? launch_dA<16>(s, w)
+                     : R == 32 ? launch_dA<32>(s, w) : launch_dA<64>(s, w);
+  if (!dA_ok) return *why = kNoLaunch, LORA_CE_ECUDA;
   GradArgs ga{};
   ga.T = T;
   ga.d = hd.d;
@@ -801,8 +831,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   ga.wt = w.wt;
   ga.tail = out.tail;
   const int a_blocks = ((out.layout ? R : hd.r) * hd.d + 255) / 256;
-  lh_grads<<<(int)(s.g.Vpad / kPackRows) + a_blocks, 256, 0, st>>>(ga);
-  if (cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
+  if (!launch_after(lh_grads, (int)(s.g.Vpad / kPackRows) + a_blocks, 256, 0, st, ga) ||
+      cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
   return 0;
 }
 

@@ -72,12 +72,16 @@ __device__ __forceinline__ long long sub_idx(int t, int k, int n_sub) {
 // Issue slots per logit: 2 for kSub 0, about 9 for kSub 64, beside the 18 that
 // one SM has while its tensor core forms a 128 x 256 x 576 tile: the pass stays
 // bound by the MMAs and the loads of W.
-template <int kRing_, int kSub>
+// kR4: the rank term of ranks up to 4 here, four multiply-adds per logit from
+// staged rows of B (as EpiLse), instead of a tenth K-block in shared memory and in
+// the ring, of which it would use a quarter at most.
+template <int kRing_, int kSub, bool kR4 = false>
 struct EpiScore {
-  static constexpr bool kAug = true;
-  static constexpr int kRec = 0;
+  static constexpr bool kAug = !kR4;
+  static constexpr bool kDepend = true;
+  static constexpr int kRec = kR4 ? 4 : 0;
   static constexpr int kRing = kRing_;
-  static constexpr int kRecBufs = 1;
+  static constexpr int kRecBufs = kR4 ? 2 : 1;
   static constexpr int kWarps = 16;
   static constexpr int kCW = 8;
   static constexpr bool kTop = kSub != 0;
@@ -89,8 +93,11 @@ struct EpiScore {
   float S, Slo, E, Elo;  // the same over the row so far, folded every 64 columns (as EpiLse)
   float r1, r2, rest;    // kSub 64: the record so far
   int a1, a2;
+  float2 sU2[kR4 ? 4 : 1];
 
-  __device__ static const float* global_recs(const GemmArgs& g, int) { return g.Bt; }
+  __device__ static const float* global_recs(const GemmArgs& g, int b) {
+    return g.Bt + (long long)b * kBN * kRec;
+  }
   __device__ static int limit(const GemmArgs& g) { return g.V; }
 
   __device__ void begin(const GemmArgs& g, int abs_row) {
@@ -101,6 +108,13 @@ struct EpiScore {
     S = Slo = E = Elo = 0.f;
     r1 = r2 = rest = -INFINITY;
     a1 = a2 = 0;
+    if constexpr (kR4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float u = g.tok[tidx(valid ? t : 0, j, 4)];
+        sU2[j] = f2(u, u);
+      }
+    }
   }
 
   // Adds the chunk's terms at reference nm = -(reference max) * lg.
@@ -122,7 +136,19 @@ struct EpiScore {
 
   template <bool kTail>
   __device__ __forceinline__ void chunk(const GemmArgs& g, int v0, float (&acc)[kCW],
-                                        const float*) {
+                                        const float* recs) {
+    if constexpr (kR4) {
+#pragma unroll
+      for (int p = 0; p < kCW / 2; ++p) {
+        float b[8];
+        ld_vec<8>(recs + p * 8, b);
+        float2 z2 = f2(acc[2 * p], acc[2 * p + 1]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z2 = __ffma2_rn(sU2[j], f2(b[2 * j], b[2 * j + 1]), z2);
+        acc[2 * p] = z2.x;
+        acc[2 * p + 1] = z2.y;
+      }
+    }
     if (kTail) {
 #pragma unroll
       for (int i = 0; i < kCW; ++i)
@@ -217,18 +243,6 @@ struct EpiScore {
     if constexpr (kTop) g.p_ent[o] = E + Elo;
   }
 };
-
-// ------------------------------------------------------------- launches
-// Programmatic dependent launch: a kernel's blocks may start before the kernel
-// ahead of it in the stream has ended; they touch nothing of its before
-// grid_wait() (which also makes its writes visible), and let the next one start
-// with grid_launch().
-__device__ __forceinline__ void grid_wait() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void grid_launch() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
 
 // ------------------------------------------------------------- preparation
 struct PrepArgs {
@@ -358,50 +372,39 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
   if (a.ids && tid < 64) put_max(a, umax);
 }
 
-// The same for kTileRows positions per block: a product of tiles, 64 of h at a
-// time in shared memory, the next 64 on the way.
-constexpr int kTileRows = 32;
-constexpr int kTileLd = 68;  // floats per row of h's tile
+// The same for kTileRows positions per block: all of their hidden states on the
+// way at once (64 elements at a time with the next 64 in flight took 35 us for
+// 2,047 positions, waiting), then a product of tiles, 64 rows of A at a time with
+// the next 64 in flight.
+constexpr int kTileRows = 16;
 template <int R>
 __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem) {
   constexpr int RT = R >= 64 ? 4 : R == 32 ? 2 : 1;      // ranks per thread
-  constexpr int PT = R >= 16 ? 2 : 1;                    // positions per thread
   constexpr int TX = R > 0 ? R / RT : 1;                 // threads over ranks
-  constexpr int PG = kTileRows / PT;                     // position groups
-  constexpr int NS = R > 0 ? 256 / (TX * PG) : 1;        // slices of the 64
-  float* hT = smem;                                      // [32][kTileLd]
-  float* aT = hT + kTileRows * kTileLd;                  // [64][R]
-  float* swt = aT + 64 * R;                              // [32]
+  constexpr int NS = R > 0 ? 256 / (TX * kTileRows) : 1; // slices of the 64
+  const int ldh = a.d + 4;
+  float* hT = smem;                                      // [16][d + 4]
+  float* aT = hT + kTileRows * ldh;                      // [64][R], then [256] sums
+  __shared__ float swt[kTileRows];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  if (a.ids) {  // a warp per 4 positions
-    for (int q = w; q < kTileRows; q += 8) {
-      const int t = t0 + q;
-      float wt = 0.f;
-      if (t < a.T) {
-        bool any = false;
-        for (int k = lane; k < a.K; k += 32) any |= a.ids[(long long)t * a.K + k] >= 0;
-        wt = row_weight(a, t, __any_sync(0xffffffffu, any));
-        if (lane == 0) a.wt[t] = wt;
+  if (a.ids) {  // sixteen threads per position, every 16th entry each
+    const int t = t0 + (tid >> 4);
+    bool any = false;
+    if (t < a.T) {
+#pragma unroll
+      for (int q = 0; q < kMaxTop / 16; ++q) {
+        const int k = (tid & 15) + 16 * q;
+        any |= k < a.K && a.ids[(long long)t * a.K + k] >= 0;
       }
-      if (lane == 0) swt[q] = wt;
+    }
+    const unsigned b = __ballot_sync(0xffffffffu, any) >> (lane & 16) & 0xffffu;
+    if ((tid & 15) == 0) {
+      const float wt = t < a.T ? row_weight(a, t, b != 0) : 0.f;
+      swt[tid >> 4] = wt;
+      if (t < a.T) a.wt[t] = wt;
     }
     __syncthreads();
   }
-  float2 next[4];
-  auto fetch = [&](int c) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int t = t0 + w + 8 * q;
-      const bool in = t < a.T && (!a.ids || swt[w + 8 * q] != 0.f);
-      next[q] = in ? load_pair(a, t, 64 * c + 2 * lane) : make_float2(0.f, 0.f);
-    }
-  };
-  const int tx = tid % TX, py = tid / TX % PG, sl = tid / (TX * PG);
-  float u[PT][RT];
-#pragma unroll
-  for (int p = 0; p < PT; ++p)
-#pragma unroll
-    for (int q = 0; q < RT; ++q) u[p][q] = 0.f;
   constexpr int kAPer = R > 0 ? (64 * R + 255) / 256 : 1;
   float an[kAPer];
   auto fetch_a = [&](int c) {
@@ -413,62 +416,59 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
       }
     }
   };
-  fetch(0);
   fetch_a(0);
-  const int chunks = a.d / 64;
-  for (int c = 0; c < chunks; ++c) {
-    __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int row = w + 8 * q, t = t0 + row;
-      const __half2 hv = __floats2half2_rn(next[q].x, next[q].y);
-      if (t < a.T)
-        *reinterpret_cast<__half2*>(a.h16 + (long long)t * a.d + 64 * c + 2 * lane) = hv;
-      if constexpr (R > 0)
-        *reinterpret_cast<float2*>(hT + row * kTileLd + 2 * lane) = __half22float2(hv);
-    }
-    if constexpr (R > 0) {
+  for (int p = 0; p < 2; ++p) {  // two rows per warp
+    const int row = w + 8 * p, t = t0 + row;
+    const bool in = t < a.T && (!a.ids || swt[row] != 0.f);
+    float2 x[kMaxHead64];
 #pragma unroll
-      for (int q = 0; q < kAPer; ++q) aT[tid + 256 * q] = an[q];
-    }
-    if (c + 1 < chunks) {
-      fetch(c + 1);
-      fetch_a(c + 1);
-    }
-    if constexpr (R > 0) {
-      __syncthreads();
-#pragma unroll 8
-      for (int i = sl; i < 64; i += NS) {
-        float x[PT], y[RT];
+    for (int k = 0; k < kMaxHead64; ++k)
+      x[k] = in && 64 * k < a.d ? load_pair(a, t, 64 * k + 2 * lane) : make_float2(0.f, 0.f);
 #pragma unroll
-        for (int p = 0; p < PT; ++p) x[p] = hT[(py + p * PG) * kTileLd + i];
-#pragma unroll
-        for (int q = 0; q < RT; ++q) y[q] = aT[i * R + tx * RT + q];
-#pragma unroll
-        for (int p = 0; p < PT; ++p)
-#pragma unroll
-          for (int q = 0; q < RT; ++q) u[p][q] = fmaf(x[p], y[q], u[p][q]);
+    for (int k = 0; k < kMaxHead64; ++k)
+      if (64 * k < a.d) {
+        const __half2 hv = __floats2half2_rn(x[k].x, x[k].y);
+        if (t < a.T)
+          *reinterpret_cast<__half2*>(a.h16 + (long long)t * a.d + 64 * k + 2 * lane) = hv;
+        if constexpr (R > 0)
+          *reinterpret_cast<float2*>(hT + row * ldh + 64 * k + 2 * lane) = __half22float2(hv);
       }
-    }
   }
   if constexpr (R > 0) {
-    if constexpr (NS > 1) {  // rank 4: the two slices meet in shared memory
+    const int tx = tid % TX, py = tid / TX % kTileRows, sl = tid / (TX * kTileRows);
+    float u[RT];
+#pragma unroll
+    for (int q = 0; q < RT; ++q) u[q] = 0.f;
+    const int chunks = a.d / 64;
+    for (int c = 0; c < chunks; ++c) {
       __syncthreads();
-      hT[tid] = u[0][0];
+#pragma unroll
+      for (int q = 0; q < kAPer; ++q) aT[tid + 256 * q] = an[q];
+      if (c + 1 < chunks) fetch_a(c + 1);
       __syncthreads();
-      if (sl == 0)
-        for (int q = 1; q < NS; ++q) u[0][0] += hT[tid + q * TX * PG];
+      const float* x = hT + py * ldh + 64 * c;
+#pragma unroll 8
+      for (int i = sl; i < 64; i += NS) {
+        const float h = x[i];
+#pragma unroll
+        for (int q = 0; q < RT; ++q) u[q] = fmaf(h, aT[i * R + tx * RT + q], u[q]);
+      }
+    }
+    if constexpr (NS > 1) {  // ranks 4 and 8: the slices meet in shared memory
+      __syncthreads();
+      aT[tid] = u[0];
+      __syncthreads();
+      if (sl == 0) {
+#pragma unroll
+        for (int q = 1; q < NS; ++q) u[0] += aT[tid + q * TX * kTileRows];
+      }
     }
     float umax = 0.f;
-    if (sl == 0) {
+    if (sl == 0 && t0 + py < a.T) {
+      const float wt = a.ids ? swt[py] : 0.f;
 #pragma unroll
-      for (int p = 0; p < PT; ++p) {
-        const int row = py + p * PG, t = t0 + row;
-        if (t >= a.T) continue;
-        const float wt = a.ids ? swt[row] : 0.f;
-#pragma unroll
-        for (int q = 0; q < RT; ++q) put_u(a, t, tx * RT + q, u[p][q], umax, wt);
-      }
+      for (int q = 0; q < RT; ++q) put_u(a, t0 + py, tx * RT + q, u[q], umax, wt);
     }
     if (a.tok)
       for (int q = w; q < kTileRows; q += 8)
@@ -476,8 +476,8 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
     if (a.ids) put_max(a, umax);
   }
 }
-__host__ __device__ inline size_t prep_tile_smem(int R) {
-  return (size_t)(kTileRows * kTileLd + 64 * R + kTileRows) * 4;
+__host__ __device__ inline size_t prep_tile_smem(int R, int d) {
+  return R == 0 ? 0 : (size_t)(kTileRows * (d + 4) + 64 * R) * 4;
 }
 
 struct PackArgs {
@@ -509,31 +509,43 @@ __device__ __forceinline__ double exp2i(int e) {
 constexpr int kPackRows = 64;
 __device__ __forceinline__ void pack_tile(const PackArgs& a, long long v0, float* tile) {
   constexpr int ld = kPackRows + 1;
-  const int R = a.R, nt = blockDim.x;
-  for (int k = threadIdx.x; k < R * kPackRows; k += nt) {
-    int j, i;
-    if (a.B.layout) {
-      j = k % (2 * R) / 2;
-      i = 2 * (k / (2 * R)) + (k & 1);
-    } else {
-      j = k / kPackRows;
-      i = k % kPackRows;
+  const int R = a.R, lr = __ffs(R) - 1, tid = threadIdx.x;  // R is a power of two, 4 to 64
+  const int n = R * kPackRows;                              // 256 to 4096
+  // element k of the tile as [v][R] pair-interleaved: row (k >> (lr + 1)) * 2 + (k & 1)
+  auto pair_row = [&](int k) { return (k >> (lr + 1) << 1) | (k & 1); };
+  auto pair_col = [&](int k) { return (k & (2 * R - 1)) >> 1; };
+  for (int k0 = tid; k0 < n; k0 += 8 * 256) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int k = k0 + 256 * e;
+      const int j = a.B.layout ? pair_col(k) : k / kPackRows;
+      const int i = a.B.layout ? pair_row(k) : k % kPackRows;
+      x[e] = k < n && j < a.r && v0 + i < a.V ? a.B.at(j, v0 + i) : 0.f;
     }
-    tile[j * ld + i] = j < a.r && v0 + i < a.V ? a.B.at(j, v0 + i) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int k = k0 + 256 * e;
+      const int j = a.B.layout ? pair_col(k) : k / kPackRows;
+      const int i = a.B.layout ? pair_row(k) : k % kPackRows;
+      if (k < n) tile[j * ld + i] = x[e];
+    }
   }
   __syncthreads();
-  if (a.Bt)
-    for (int k = threadIdx.x; k < R * kPackRows; k += nt)
-      a.Bt[v0 * R + k] = a.Bt_plain ? tile[k % R * ld + k / R]
-                                    : tile[k % (2 * R) / 2 * ld + 2 * (k / (2 * R)) + (k & 1)];
+  if (a.Bt) {
+#pragma unroll 4
+    for (int k = tid; k < n; k += 256)
+      a.Bt[v0 * R + k] = a.Bt_plain ? tile[(k & (R - 1)) * ld + (k >> lr)]
+                                    : tile[pair_col(k) * ld + pair_row(k)];
+  }
   if (a.waug) {
     const int groups = a.aug_width / 8;
-    for (int k = threadIdx.x; k < kPackRows * groups; k += nt) {
-      const int i = k / groups, c0 = k % groups * 8;
+    for (int k = tid; k < kPackRows * groups; k += 256) {
+      const int i = k / groups, c0 = (k - i * groups) * 8;
       __align__(16) __half o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int c = c0 + e, part = c / R, j = c - part * R;
+        const int part = (c0 + e) >> lr, j = (c0 + e) & (R - 1);
         const bool used = part < (a.aug_layout == 1 ? 3 : 2);
         const float b = used ? tile[j * ld + i] : 0.f;
         const __half hi = __float2half_rn(b);
@@ -544,10 +556,11 @@ __device__ __forceinline__ void pack_tile(const PackArgs& a, long long v0, float
     }
   }
   if (a.xv) {
-    const int ex = scale_exp(a.stats[kStBMax], 13);
-    for (int k = threadIdx.x; k < R * (kPackRows / 2); k += nt) {
+    const float up = (float)exp2i(scale_exp(a.stats[kStBMax], 13));
+#pragma unroll 2
+    for (int k = tid; k < R * (kPackRows / 2); k += 256) {
       const int j = k / (kPackRows / 2), i = 2 * (k % (kPackRows / 2));
-      const float x = ldexpf(tile[j * ld + i], ex), y = ldexpf(tile[j * ld + i + 1], ex);
+      const float x = tile[j * ld + i] * up, y = tile[j * ld + i + 1] * up;
       const __half2 hi = __floats2half2_rn(x, y);
       const float2 hf = __half22float2(hi);
       const long long o = (long long)j * a.Vpad + v0 + i;
@@ -556,7 +569,6 @@ __device__ __forceinline__ void pack_tile(const PackArgs& a, long long v0, float
           __floats2half2_rn(x - hf.x, y - hf.y);
     }
   }
-  __syncthreads();
 }
 
 // Blocks [0, prep_blocks) take positions (kRank < 0: one each; else kTileRows at
@@ -1424,6 +1436,8 @@ static __global__ void __launch_bounds__(32 * kRowWarps, 3) lh_distill_rows(Dist
   const int lane = team.lane, tid = team.tid, no = threadIdx.x / kThreads;
   team.red = s_red[no];
   const int t = (int)blockIdx.x * kTeams + no;
+  grid_wait();
+  grid_launch();
   if (t >= a.z.T) return;
   const int R = a.z.R;
   const int nslot = a.p.slots(t);
@@ -1579,6 +1593,8 @@ static __global__ void lh_xt(int T, int R, long long ld, const float* __restrict
                              const float* __restrict__ wt, const float* __restrict__ xs,
                              const int* __restrict__ stats,
                              __half* __restrict__ xt) {
+  grid_wait();
+  grid_launch();
   const double up = exp2i(scale_exp(stats[kStUMax], 13));
   const long long n = (long long)T * R, stride = (long long)gridDim.x * blockDim.x;
   for (long long k = (long long)blockIdx.x * blockDim.x + threadIdx.x; k < n; k += stride) {
@@ -1589,6 +1605,77 @@ static __global__ void lh_xt(int T, int R, long long ld, const float* __restrict
     xt[(long long)j * ld + t] = hi;
     xt[(long long)(R + j) * ld + t] = __float2half_rn(x - __half2float(hi));
   }
+}
+
+// gAp[c][i][j] = sum over the kDAChunk positions of chunk c of h16[t][i] dU[t][j]:
+// blocks of 64 hidden elements by all R ranks, 64 positions at a time through
+// shared memory with the next 64 in flight.  (lce_dA_partial takes 16 ranks per
+// launch: 50 us at rank 64 and 8,000 positions, this DA_US.)
+template <int R>
+static __global__ void __launch_bounds__(256) lh_dA(int T, int d, const __half* __restrict__ h16,
+                                                    const float* __restrict__ dU,
+                                                    float* __restrict__ gAp) {
+  constexpr int JT = R >= 64 ? 4 : R == 32 ? 2 : 1;  // ranks per thread
+  constexpr int TJ = R / JT;                         // threads over ranks
+  constexpr int TI = 256 / TJ;                       // threads over hidden elements
+  constexpr int IT = 64 / TI;                        // hidden elements per thread
+  constexpr int kU = (64 * R + 255) / 256;
+  __shared__ __align__(16) float sh[64][64];
+  __shared__ __align__(16) float su[64][R];
+  grid_wait();
+  grid_launch();
+  const int tid = threadIdx.x, tj = tid % TJ, ti = tid / TJ;
+  const int c = (int)blockIdx.x, i0 = (int)blockIdx.y * 64;
+  const int t_lo = c * kDAChunk, t_hi = min(T, t_lo + kDAChunk);
+  float acc[IT][JT] = {};
+  uint4 hn[2];
+  float un[kU];
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {  // 8 f16 of row (tid + 256 q) / 8
+      const int row = (tid + 256 * q) >> 3, t = t0 + row;
+      hn[q] = make_uint4(0u, 0u, 0u, 0u);
+      if (t < t_hi)
+        hn[q] = *reinterpret_cast<const uint4*>(h16 + (long long)t * d + i0 + 8 * (tid & 7));
+    }
+#pragma unroll
+    for (int q = 0; q < kU; ++q) {
+      const int k = tid + 256 * q, t = t0 + k / R;
+      un[q] = t < t_hi ? dU[(long long)t0 * R + k] : 0.f;
+    }
+  };
+  fetch(t_lo);
+  for (int t0 = t_lo; t0 < t_hi; t0 += 64) {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const __half2* p = reinterpret_cast<const __half2*>(&hn[q]);
+      float* o = &sh[(tid + 256 * q) >> 3][8 * (tid & 7)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(o + 2 * e) = __half22float2(p[e]);
+    }
+#pragma unroll
+    for (int q = 0; q < kU; ++q) (&su[0][0])[tid + 256 * q] = un[q];
+    __syncthreads();
+    if (t0 + 64 < t_hi) fetch(t0 + 64);
+#pragma unroll 8
+    for (int t = 0; t < 64; ++t) {
+      float x[IT], y[JT];
+#pragma unroll
+      for (int e = 0; e < IT; ++e) x[e] = sh[t][ti * IT + e];
+#pragma unroll
+      for (int e = 0; e < JT; ++e) y[e] = su[t][tj * JT + e];
+#pragma unroll
+      for (int p = 0; p < IT; ++p)
+#pragma unroll
+        for (int q = 0; q < JT; ++q) acc[p][q] = fmaf(x[p], y[q], acc[p][q]);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < IT; ++p)
+#pragma unroll
+    for (int q = 0; q < JT; ++q)
+      gAp[((long long)c * d + i0 + ti * IT + p) * R + tj * JT + q] = acc[p][q];
 }
 
 struct GradArgs {
@@ -1613,6 +1700,7 @@ struct GradArgs {
 // the caller's rows are ranks; the others gA; block 0 the tail too.
 static __global__ void __launch_bounds__(256) lh_grads(GradArgs a) {
   __shared__ float tile[64 * (kPackRows + 1)];
+  grid_wait();
   const bool bad = *reinterpret_cast<const volatile int*>(a.stats + kStErr) != 0;
   const float nan = __int_as_float(0x7fc00000);
   const int blk = (int)blockIdx.x, tid = (int)threadIdx.x;
@@ -1642,6 +1730,7 @@ static __global__ void __launch_bounds__(256) lh_grads(GradArgs a) {
   const float* src = a.gBp + v0 * a.R;
   for (int k0 = tid; k0 < n; k0 += 4 * 256) {
     double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
     for (int q = 0; q < slots; ++q)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
