@@ -150,6 +150,36 @@ int lora_ce_get_token_loss(lora_ce_handle* h, float* loss_t, int32_t T);
 int lora_ce_apply_grads(lora_ce_handle* h, const float* gA_dxr, const float* gB_rxv,
                         float n_pred);
 
+/* The operators of include/lora_head.h on the handle's weight and adapter, ranks up
+ * to 64 (ranks above return LORA_CE_EINVAL).  Their workspace belongs to the handle
+ * (allocated when first needed, kept, grown when a call needs more).  Host buffers;
+ * the _device variants take buffers of the handle's device (H 16-byte aligned),
+ * run on the handle's stream and do not wait.  T <= max_tokens.
+ *
+ * lora_ce_score: log probabilities of given tokens, entropy and top alternatives
+ * as lora_head_score; the optimizer state is not touched. */
+int lora_ce_score(lora_ce_handle* h, const void* H, int32_t h_dtype, int32_t T,
+                  const int32_t* tokens, int32_t top_k, float* logprob, float* entropy,
+                  int32_t* top_ids, float* top_logprobs);
+int lora_ce_score_device(lora_ce_handle* h, const void* d_H, int32_t h_dtype, int32_t T,
+                         const int32_t* d_tokens, int32_t top_k, float* d_logprob,
+                         float* d_entropy, int32_t* d_top_ids, float* d_top_logprobs);
+
+/* One training step on the distillation loss of lora_head_distill: its gradient
+ * sums over all ranks, divided by the number of counted positions (weight not 0 and
+ * at least one entry) over all ranks, then the clip and Adam as lora_ce_step.
+ * *loss_out: the sum of losses over that number.  A step that counts no position
+ * anywhere has loss 0 and applies a gradient of zero.  lora_ce_get_grads and
+ * lora_ce_get_token_loss read the step's gradients and losses.  The host variant
+ * refuses weights that are not finite and, in rows with a weight, ids >= vocab and
+ * logits of NaN or +inf; in device buffers those make loss and gradients NaN. */
+int lora_ce_distill_step(lora_ce_handle* h, const void* H, int32_t h_dtype, int32_t T, int32_t K,
+                         const int32_t* ids, const float* teacher, float temperature,
+                         const float* weight, float* loss_out);
+int lora_ce_distill_step_device(lora_ce_handle* h, const void* d_H, int32_t h_dtype, int32_t T,
+                                int32_t K, const int32_t* d_ids, const float* d_teacher,
+                                float temperature, const float* d_weight, float* d_loss);
+
 /* Data-parallel token sharding: every rank runs the same steps on its own
  * positions; one NCCL sum all-reduce of [dA | dB | loss | n_pred] runs
  * between the gradient and the Adam kernels.  lora_ce_nccl_unique_id fills

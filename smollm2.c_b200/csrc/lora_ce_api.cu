@@ -22,6 +22,7 @@
 #include "lora_ce_plan.cuh"
 #include "lora_ce_tc.cuh"
 #include "lora_ce_wide.cuh"
+#include "lora_head_core.h"
 
 using namespace lce;
 
@@ -233,6 +234,12 @@ struct lora_ce_handle {
   float* w_dAp = nullptr;    // [kWMaxSplit][d][R] split partials of dA
   ncclComm_t comm = nullptr;
   int nranks = 1, rank = 0;
+  // head operators (lora_ce_score, lora_ce_distill_step): workspace and staging of
+  // host buffers, allocated when first needed and grown when a call needs more
+  void* head_ws = nullptr;
+  size_t head_ws_bytes = 0;
+  void* head_io = nullptr;
+  size_t head_io_bytes = 0;
   double comm_timeout_ms = 60000.0;  // bound on any wait that involves a collective
   bool stuck = false;  // streams still busy after an aborted collective
   // optional per-phase timing (events on the handle's stream)
@@ -279,7 +286,7 @@ void free_all(lora_ce_handle* h) {
                   h->loss_tok, h->dU, h->gAp,      h->gBp,    h->norm_parts, h->err, h->corr_fx,
                   h->d_loss, h->in_H, h->in_tgt, h->w_aug, h->h_aug, h->Bc, h->tokc,
                   h->xv, h->xt, h->nml, h->w_sU, h->w_Z, h->w_Bp, h->w_dB, h->w_dUp,
-                  h->w_dAp};
+                  h->w_dAp, h->head_ws, h->head_io};
   for (void* p : ptrs)
     if (p) cudaFree(p);
 }
@@ -1103,6 +1110,108 @@ int run_or_replay(lora_ce_handle* h, bool host, const void* H, int dtype, int T,
 
 namespace {
 
+// The handle's head for the operators of include/lora_head.h.
+HeadCore head_of(const lora_ce_handle* h) {
+  return HeadCore{h->W, h->params, h->R, h->params + (size_t)h->d * h->R, 1,
+                  h->d, h->V, h->r, h->cfg.scale};
+}
+
+// At least `bytes` behind *p; the handle's work is waited for before it moves.
+int grow(lora_ce_handle* h, void** p, size_t* have, size_t bytes) {
+  if (*have >= bytes) return 0;
+  if (int rc = wait_stream(h)) return rc;
+  if (*p) cudaFree(*p);
+  *p = nullptr;
+  *have = 0;
+  if (cudaMalloc(p, bytes) != cudaSuccess) {
+    *p = nullptr;
+    cudaGetLastError();  // not sticky
+    return fail(LORA_CE_ENOMEM, "cudaMalloc failed");
+  }
+  *have = bytes;
+  return 0;
+}
+
+int check_head_args(lora_ce_handle* h, const void* H, int dtype, int T) {
+  if (!h) return fail(LORA_CE_EINVAL, "null handle");
+  if (h->poisoned) return fail(LORA_CE_ESTATE, "handle poisoned by an earlier error");
+  if (!h->have_weight) return fail(LORA_CE_ESTATE, "lora_ce_set_weight_f16 not called");
+  if (!H) return fail(LORA_CE_EINVAL, "null input");
+  if (dtype < 0 || dtype > 2) return fail(LORA_CE_EINVAL, "bad hidden-state dtype");
+  if (T < 1 || T > h->cfg.max_tokens) return fail(LORA_CE_EINVAL, "T out of range");
+  return 0;
+}
+
+int check_score_args(lora_ce_handle* h, const void* H, int dtype, int T, const int32_t* tokens,
+                     int top_k, const float* logprob, const float* entropy, const int32_t* top_ids,
+                     const float* top_logprobs) {
+  if (int rc = check_head_args(h, H, dtype, T)) return rc;
+  if (const char* why = head_score_refuses(head_of(h), T, top_k)) return fail(LORA_CE_EINVAL, why);
+  if ((tokens == nullptr) != (logprob == nullptr))
+    return fail(LORA_CE_EINVAL, "tokens and logprob go together");
+  if (top_k > 0 && (!top_ids || !top_logprobs)) return fail(LORA_CE_EINVAL, "null output");
+  if (!logprob && !entropy && top_k == 0) return fail(LORA_CE_EINVAL, "nothing is asked for");
+  return 0;
+}
+
+int check_distill_args(lora_ce_handle* h, const void* H, int dtype, int T, int K,
+                       const int32_t* ids, const float* teacher, float tau) {
+  if (int rc = check_head_args(h, H, dtype, T)) return rc;
+  if (!ids || !teacher) return fail(LORA_CE_EINVAL, "null input");
+  if (const char* why = head_distill_refuses(head_of(h), T, K, true, tau))
+    return fail(LORA_CE_EINVAL, why);
+  return 0;
+}
+
+int run_score(lora_ce_handle* h, const void* dH, int dtype, int T, const int32_t* d_tokens,
+              int top_k, float* d_logprob, float* d_entropy, int32_t* d_ids, float* d_top) {
+  const HeadCore hd = head_of(h);
+  if (int rc = grow(h, &h->head_ws, &h->head_ws_bytes, head_score_bytes(hd, T, top_k))) return rc;
+  const char* why = "";
+  const int rc = head_score_run(hd, dH, dtype, T, d_tokens, top_k, d_logprob, d_entropy, d_ids,
+                                d_top, h->head_ws, h->stream, &why);
+  return rc ? fail(rc, why) : 0;
+}
+
+// lora_head_distill's gradient sums into G, then what follows them in every step:
+// the sum over ranks, the clip's norm, Adam.
+int run_distill_step(lora_ce_handle* h, const void* dH, int dtype, int T, int K,
+                     const int32_t* d_ids, const float* d_teacher, float tau,
+                     const float* d_weight, float* d_loss) {
+  const HeadCore hd = head_of(h);
+  if (int rc = grow(h, &h->head_ws, &h->head_ws_bytes, head_distill_bytes(hd, T, K, true)))
+    return rc;
+  cudaStream_t st = h->stream;
+  const long long nA = (long long)h->d * h->R, nparam = nA + h->Vpad * h->R;
+  float* const tail = h->Gbuf + nparam;
+  const char* why = "";
+  int rc = head_distill_run(hd, dH, dtype, T, K, d_ids, d_teacher, tau, d_weight, h->loss_tok,
+                            GradOut{h->Gbuf, h->Gbuf + nA, 1, tail}, h->head_ws, st, &why);
+  if (rc) return fail(rc, why);
+  if (h->comm) {
+    ncclResult_t r = nccl().AllReduce(h->Gbuf, h->Gbuf, (size_t)(nparam + 2), ncclFloat, ncclSum,
+                                      h->comm, st);
+    if (r == ncclInProgress) r = nccl_settle(h->comm, h->comm_timeout_ms);
+    if (r != ncclSuccess)
+      return fail(LORA_CE_ENCCL, std::string("ncclAllReduce: ") + nccl_str(r));
+  }
+  if (head_step_tail(h->head_ws, tail, h->err, st))
+    return fail(LORA_CE_ECUDA, "kernel launch failed");
+  const int32_t next_step = h->step + 1;
+  const AdamArgs aa = adam_args(h, nparam, next_step);
+  if (aa.clip > 0.f) lce_sqnorm<<<256, 256, 0, st>>>(nparam, h->Gbuf, h->norm_parts);
+  lce_adam<<<(int)std::min<long long>((nparam + 255) / 256, 8LL * h->num_sms), 256, 0, st>>>(
+      aa, h->params, h->mom1, h->mom2, h->Gbuf, h->gmean, h->norm_parts, d_loss);
+  LCE_CUDA(cudaGetLastError());
+  h->step = next_step;
+  h->last_T = T;
+  return 0;
+}
+
+}  // namespace
+
+namespace {
+
 // Buffers and streams of a wide-rank handle (ranks 65..256).  The logit
 // rows of one position block take at most 512 MB.
 int create_wide(lora_ce_handle* h) {
@@ -1574,6 +1683,103 @@ int lora_ce_apply_grads(lora_ce_handle* h, const float* gA, const float* gB, flo
   LCE_CUDA(cudaGetLastError());
   LCE_CUDA(cudaStreamSynchronize(h->stream));
   h->step = next_step;
+  return 0;
+}
+
+int lora_ce_score_device(lora_ce_handle* h, const void* dH, int32_t dtype, int32_t T,
+                         const int32_t* d_tokens, int32_t top_k, float* d_logprob,
+                         float* d_entropy, int32_t* d_top_ids, float* d_top_logprobs) {
+  int rc = check_score_args(h, dH, dtype, T, d_tokens, top_k, d_logprob, d_entropy, d_top_ids,
+                            d_top_logprobs);
+  if (rc) return rc;
+  if ((reinterpret_cast<uintptr_t>(dH) & 15) != 0)
+    return fail(LORA_CE_EINVAL, "hidden states must be 16-byte aligned");
+  LCE_CUDA(cudaSetDevice(h->cfg.device));
+  return run_score(h, dH, dtype, T, d_tokens, top_k, d_logprob, d_entropy, d_top_ids,
+                   d_top_logprobs);
+}
+
+int lora_ce_score(lora_ce_handle* h, const void* H, int32_t dtype, int32_t T,
+                  const int32_t* tokens, int32_t top_k, float* logprob, float* entropy,
+                  int32_t* top_ids, float* top_logprobs) {
+  int rc = check_score_args(h, H, dtype, T, tokens, top_k, logprob, entropy, top_ids, top_logprobs);
+  if (rc) return rc;
+  LCE_CUDA(cudaSetDevice(h->cfg.device));
+  const size_t n = (size_t)T, nk = n * top_k;
+  // [logprob | entropy | top_ids | top_logprobs]
+  if ((rc = grow(h, &h->head_io, &h->head_io_bytes, (2 * n + 2 * nk) * 4))) return rc;
+  float* d_lp = static_cast<float*>(h->head_io);
+  float* d_ent = d_lp + n;
+  int32_t* d_ids = reinterpret_cast<int32_t*>(d_ent + n);
+  float* d_top = reinterpret_cast<float*>(d_ids + nk);
+  LCE_CUDA(cudaMemcpyAsync(h->in_H, H, n * h->d * elt_size(dtype), cudaMemcpyHostToDevice,
+                           h->stream));
+  if (tokens)
+    LCE_CUDA(cudaMemcpyAsync(h->in_tgt, tokens, n * 4, cudaMemcpyHostToDevice, h->stream));
+  if ((rc = run_score(h, h->in_H, dtype, T, tokens ? h->in_tgt : nullptr, top_k,
+                      logprob ? d_lp : nullptr, entropy ? d_ent : nullptr, d_ids, d_top)))
+    return rc;
+  struct {
+    void* to;
+    const void* from;
+    size_t count;
+  } out[] = {{logprob, d_lp, n}, {entropy, d_ent, n}, {top_ids, d_ids, nk}, {top_logprobs, d_top, nk}};
+  for (const auto& o : out)
+    if (o.to && o.count)
+      LCE_CUDA(cudaMemcpyAsync(o.to, o.from, o.count * 4, cudaMemcpyDeviceToHost, h->stream));
+  return wait_stream(h);
+}
+
+int lora_ce_distill_step_device(lora_ce_handle* h, const void* dH, int32_t dtype, int32_t T,
+                                int32_t K, const int32_t* d_ids, const float* d_teacher,
+                                float temperature, const float* d_weight, float* d_loss) {
+  int rc = check_distill_args(h, dH, dtype, T, K, d_ids, d_teacher, temperature);
+  if (rc) return rc;
+  if ((reinterpret_cast<uintptr_t>(dH) & 15) != 0)
+    return fail(LORA_CE_EINVAL, "hidden states must be 16-byte aligned");
+  LCE_CUDA(cudaSetDevice(h->cfg.device));
+  rc = run_distill_step(h, dH, dtype, T, K, d_ids, d_teacher, temperature, d_weight,
+                        d_loss ? d_loss : h->d_loss);
+  if (rc) h->poisoned = true;
+  return rc;
+}
+
+int lora_ce_distill_step(lora_ce_handle* h, const void* H, int32_t dtype, int32_t T, int32_t K,
+                         const int32_t* ids, const float* teacher, float temperature,
+                         const float* weight, float* loss_out) {
+  int rc = check_distill_args(h, H, dtype, T, K, ids, teacher, temperature);
+  if (rc) return rc;
+  // what would make the gradients, and with them the adapter, NaN
+  for (int32_t t = 0; t < T; ++t) {
+    if (weight && !std::isfinite(weight[t])) return fail(LORA_CE_EINVAL, "a weight is not finite");
+    if (weight && weight[t] == 0.f) continue;
+    for (int64_t k = (int64_t)t * K; k < (int64_t)(t + 1) * K; ++k) {
+      if (ids[k] >= h->V) return fail(LORA_CE_EINVAL, "a token id is out of range");
+      if (ids[k] >= 0 && !(teacher[k] < INFINITY))
+        return fail(LORA_CE_EINVAL, "a teacher logit is NaN or +inf");
+    }
+  }
+  LCE_CUDA(cudaSetDevice(h->cfg.device));
+  const size_t n = (size_t)T, nk = n * K;
+  if ((rc = grow(h, &h->head_io, &h->head_io_bytes, (2 * nk + n) * 4))) return rc;
+  int32_t* d_ids = static_cast<int32_t*>(h->head_io);
+  float* d_teacher = reinterpret_cast<float*>(d_ids + nk);
+  float* d_weight = d_teacher + nk;
+  LCE_CUDA(cudaMemcpyAsync(h->in_H, H, n * h->d * elt_size(dtype), cudaMemcpyHostToDevice,
+                           h->stream));
+  LCE_CUDA(cudaMemcpyAsync(d_ids, ids, nk * 4, cudaMemcpyHostToDevice, h->stream));
+  LCE_CUDA(cudaMemcpyAsync(d_teacher, teacher, nk * 4, cudaMemcpyHostToDevice, h->stream));
+  if (weight)
+    LCE_CUDA(cudaMemcpyAsync(d_weight, weight, n * 4, cudaMemcpyHostToDevice, h->stream));
+  rc = run_distill_step(h, h->in_H, dtype, T, K, d_ids, d_teacher, temperature,
+                        weight ? d_weight : nullptr, h->d_loss);
+  if (rc) {
+    h->poisoned = true;
+    return rc;
+  }
+  LCE_CUDA(cudaMemcpyAsync(h->res_host, h->d_loss, 4, cudaMemcpyDeviceToHost, h->stream));
+  if ((rc = check_device_error(h))) return rc;  // waits
+  if (loss_out) *loss_out = h->res_host[0];
   return 0;
 }
 

@@ -53,7 +53,7 @@ constexpr int kBM = 128;               // resident rows per tile (TMEM lanes)
 constexpr int kBN = 256;               // streamed rows per tile (TMEM columns)
 constexpr int kBK = 64;                // K elements per 128-byte swizzle row
 constexpr int kRingBytes = 65536;      // streamed-operand ring (2 x 32 KB, or 4 x 16 KB per CTA in pairs)
-constexpr int kMaxStages = 5;
+constexpr int kMaxStages = 4;
 constexpr int kAKBytes = kBM * kBK * 2;   // 16 KB per resident K-block
 // Per-CTA streamed rows per tile and stage geometry for 1-CTA (kPair 1) and
 // CTA-pair (kPair 2, cta_group::2) tiles.
@@ -614,7 +614,6 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
   const uint32_t tmem_base = *tmem_slot;
   if constexpr (Epi::kDepend) {  // set up beside the end of the kernel ahead
     grid_wait();
-    grid_launch();
   }
 
   if (warp == 0) {

@@ -260,7 +260,6 @@ __global__ void __launch_bounds__(kThreadsT, 1)
   const uint32_t tmem_base = *tmem_slot;
   if constexpr (kTemp) {  // launched to depend on the kernel ahead
     grid_wait();
-    grid_launch();
   }
 
   if (warp == 0) {

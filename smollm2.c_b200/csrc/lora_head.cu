@@ -192,30 +192,22 @@ struct PassPlan {
   int threads = 0, smem = 0;
 };
 
-// EpiScore with the largest ring that fits beside the resident K-blocks; at rank
-// 4 the rank term in the epilogue, from staged records.
-template <class Epi, bool kStage>
+// EpiScore with the largest ring that fits beside the resident K-blocks.
+template <class Epi>
 PassPlan plan_of(int kblocks) {
-  PassPlan p;
-  p.kern = lce_gemm_kernel<Epi, kStage, 2>;
-  p.threads = block_threads(Epi::kWarps);
-  p.smem = SmemLayout::bytes(kblocks, kStage ? Epi::kRec * Epi::kRecBufs : 0, Epi::kRing);
-  return p;
+  return PassPlan{lce_gemm_kernel<Epi, false, 2>, block_threads(Epi::kWarps),
+                  SmemLayout::bytes(kblocks, 0, Epi::kRing)};
 }
 template <int kSub>
-PassPlan score_plan(int kblocks, bool r4) {
-  if (r4)
-    return kblocks <= 9 ? plan_of<EpiScore<65536, kSub, true>, true>(kblocks)
-                        : plan_of<EpiScore<49152, kSub, true>, true>(kblocks);
-  return kblocks <= 9    ? plan_of<EpiScore<81920, kSub>, false>(kblocks)
-         : kblocks == 10 ? plan_of<EpiScore<65536, kSub>, false>(kblocks)
-         : kblocks == 11 ? plan_of<EpiScore<49152, kSub>, false>(kblocks)
-                         : plan_of<EpiScore<32768, kSub>, false>(kblocks);
+PassPlan score_plan(int kblocks) {
+  return kblocks <= 10   ? plan_of<EpiScore<65536, kSub>>(kblocks)
+         : kblocks == 11 ? plan_of<EpiScore<49152, kSub>>(kblocks)
+                         : plan_of<EpiScore<32768, kSub>>(kblocks);
 }
-PassPlan score_plan(int kblocks, int sub, bool r4) {
-  return sub == 64  ? score_plan<64>(kblocks, r4)
-         : sub == 8 ? score_plan<8>(kblocks, r4)
-         : sub == 1 ? score_plan<1>(kblocks, r4) : score_plan<0>(kblocks, r4);
+PassPlan score_plan(int kblocks, int sub) {
+  return sub == 64  ? score_plan<64>(kblocks)
+         : sub == 8 ? score_plan<8>(kblocks)
+         : sub == 1 ? score_plan<1>(kblocks) : score_plan<0>(kblocks);
 }
 
 // Columns per record: the widest that leaves four records per alternative.
@@ -293,7 +285,6 @@ int few_blocks(int V) { return (V + kFewRows - 1) / kFewRows; }
 struct ScoreWs {
   int* stats;
   __half *h16, *haug, *waug;
-  float *tok, *Bt;
   float *sU, *p_max, *p_sum, *p_ent, *sub_max, *sub_second, *sub_rest;
   uint8_t *sub_arg, *sub_arg2;
   int sub, n_sub;
@@ -314,11 +305,8 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
   w.stats = c.take<int>(kStatWords);
   w.h16 = c.take<__half>((size_t)T * hd.d);
   w.sU = c.take<float>((size_t)T * aug.R);
-  const bool r4 = aug.R == 4;  // the rank term in the epilogue
-  w.tok = c.take<float>(r4 ? (size_t)(T + 1) * tok_stride(4) : 0);
-  w.Bt = c.take<float>(r4 && !hd.layout ? (size_t)Vpad * 4 : 0);
-  w.haug = c.take<__half>(r4 ? 0 : (size_t)T * aug.width);
-  w.waug = c.take<__half>(r4 ? 0 : (size_t)Vpad * aug.width);
+  w.haug = c.take<__half>((size_t)T * aug.width);
+  w.waug = c.take<__half>((size_t)Vpad * aug.width);
   w.p_max = c.take<float>(part);
   w.p_sum = c.take<float>(part);
   w.p_ent = c.take<float>(part);
@@ -357,18 +345,19 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
   w.h16 = c.take<__half>((size_t)T * hd.d);
   w.sU = c.take<float>((size_t)T * R);
   w.wt = c.take<float>(T);
-  const bool in_mma = R > 4;  // rank 4 keeps the rank term in the epilogues
+  // rank 4 keeps the rank term in the epilogues of the gradient passes
+  const bool in_mma = !grads || R > 4;
   w.haug = c.take<__half>(in_mma ? (size_t)T * aug.width : 0);
   w.waug = c.take<__half>(in_mma ? (size_t)Vpad * aug.width : 0);
   w.p_max = c.take<float>(part);
   w.p_sum = c.take<float>(part);
-  w.tok = c.take<float>(grads && tc ? 0 : R == 0 || (!grads && R > 4) ? 0 : (size_t)Tpad * tok_stride(R));
-  w.Bt = c.take<float>(hd.layout || (!grads && R != 4) ? 0 : (size_t)Vpad * R);
   if (grads) {
     // chunks of four or eight epilogue columns a row: up to 4 slots per owner
     const int n_a2 = (hd.V + 2 * kBM - 1) / (2 * kBM), n_b2 = (T + bn - 1) / bn;
     const size_t segs = (size_t)(tc ? 1 : 4) * most_segments(n_a2, n_b2);
     w.p_q = c.take<float>(part * R);
+    w.tok = c.take<float>(tc ? 0 : (size_t)Tpad * tok_stride(R));
+    w.Bt = c.take<float>(hd.layout ? 0 : (size_t)Vpad * R);
     w.xv = c.take<__half>(tc ? (size_t)2 * R * Vpad : 0);
     w.xt = c.take<__half>(tc ? (size_t)2 * R * Tpad : 0);
     w.nml = c.take<float>(tc ? (size_t)Tpad + kMaxBNT : 0);
@@ -573,8 +562,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   Aug aug = aug_of(hd.r);
   const ScoreWs w = score_ws(hd, T, top_k, ws);
   const bool few = few_positions(T, w.sub);
-  const bool r4 = aug.R == 4;
-  if (few || r4) aug.layout = aug.width = 0;  // the rank term from B as it is
+  if (few) aug.layout = aug.width = 0;  // the rank term from B as it is
   const int sms = sm_count();
   GemmArgs g{};
   fill_pass1(g, hd, aug, T, 1.0f);
@@ -611,7 +599,6 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   pa.h16 = w.h16;
   pa.sU = w.sU;
   pa.haug = aug.width ? w.haug : nullptr;
-  pa.tok = r4 && !few ? w.tok : nullptr;
   pa.stats = w.stats;
   PackArgs pk{};
   pk.B = BView{hd.B, hd.V, hd.r, aug.R, hd.layout};
@@ -619,7 +606,6 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   pk.r = hd.r;
   pk.R = aug.R;
   pk.Vpad = g.Vpad;
-  pk.Bt = r4 && !hd.layout ? w.Bt : nullptr;
   pk.waug = aug.width ? w.waug : nullptr;
   pk.aug_layout = aug.layout;
   pk.aug_width = aug.width;
@@ -639,9 +625,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
     a.p = SlotPlan{1, 1, blocks, blocks, kFewMax, w.p_max, w.p_sum, w.p_ent, nullptr};
     a.lg = lg;
   } else {
-    const PassPlan p = score_plan(g.kblocks, w.sub, r4);
-    g.tok = w.tok;
-    g.Bt = hd.layout ? hd.B : w.Bt;
+    const PassPlan p = score_plan(g.kblocks, w.sub);
     const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
                                                          p.threads, p.smem));
     if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
@@ -653,7 +637,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
     if (aug.width && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
                       !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
       return *why = kNoMap, LORA_CE_ECUDA;
-    if (launch_prep(pa, pk, true, 0, pk.Bt || pk.waug, sms, st))
+    if (launch_prep(pa, pk, true, 0, pk.waug != nullptr, sms, st))
       return *why = kNoFit, LORA_CE_ECUDA;
     const int G = (int)std::min<long long>(units, (long long)g.n_a * g.n_b);
     if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, g))
@@ -691,8 +675,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   const int R = aug.R;
   const DistillWs w = distill_ws(hd, T, grads, ws);
   const bool tc = grads && R >= 16;
-  const bool r4 = R == 4;
-  if (r4) aug.layout = aug.width = 0;  // the rank term in the epilogues
+  if (grads && R == 4) aug.layout = aug.width = 0;  // the rank term in the epilogues
   Step s{hd, w, aug, T, sm_count(), tau, st, GemmArgs{}, SlotPlan{}};
   fill_pass1(s.g, hd, aug, T, tau);
   s.Bt = hd.layout ? hd.B : w.Bt;
@@ -717,7 +700,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pa.K = K;
   pa.tau = tau;
   pa.wt = w.wt;
-  if (grads ? !tc : r4) {
+  if (grads && !tc) {
     pa.tok = w.tok;
     pa.Tpad = (int)round_up(T, kBN);
   }
@@ -727,7 +710,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pk.r = hd.r;
   pk.R = R;
   pk.Vpad = s.g.Vpad;
-  pk.Bt = (grads || r4) && !hd.layout ? w.Bt : nullptr;
+  pk.Bt = grads && !hd.layout ? w.Bt : nullptr;
   pk.Bt_plain = tc;  // the rank sums' passes have xv instead
   pk.waug = aug.width ? w.waug : nullptr;
   pk.aug_layout = aug.layout;
@@ -744,7 +727,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   if (grads) {
     rc = grad_pass<1>(s, R, why);
   } else {
-    const PassPlan p = score_plan(s.g.kblocks, 0, r4);
+    const PassPlan p = score_plan(s.g.kblocks, 0);
     const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
                                                          p.threads, p.smem));
     if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
@@ -836,22 +819,41 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   return 0;
 }
 
+int head_step_tail(const void* ws, float* tail, int* err, cudaStream_t st) {
+  lh_tail<<<1, 1, 0, st>>>(static_cast<const int*>(ws), tail, err);
+  return cudaGetLastError() == cudaSuccess ? 0 : LORA_CE_ECUDA;
+}
+
+namespace {
+const char* head_refuses(const HeadCore& hd, int T) {
+  if (hd.d < 64 || hd.d % 64 != 0 || hd.d > 64 * kMaxHead64)
+    return "dim must be a multiple of 64 in [64, 640]";
+  if (hd.V < 1 || hd.V > (1 << 19)) return "vocab must be in [1, 2^19]";
+  if (hd.r < 0 || hd.r > kMaxFusedRank) return "rank must be in [0, 64]";
+  if (!std::isfinite(hd.scale)) return "scale must be finite";
+  if (T < 1 || T > LORA_HEAD_MAX_TOKENS) return "T must be in [1, 2^20]";
+  return nullptr;
+}
+}  // namespace
+
+const char* head_score_refuses(const HeadCore& hd, int T, int top_k) {
+  if (const char* why = head_refuses(hd, T)) return why;
+  if (top_k < 0 || top_k > LORA_HEAD_MAX_TOP || top_k > hd.V)
+    return "top_k must be in [0, 128] and no more than vocab";
+  return nullptr;
+}
+
+const char* head_distill_refuses(const HeadCore& hd, int T, int K, bool grads, float tau) {
+  if (const char* why = head_refuses(hd, T)) return why;
+  if (K < 1 || K > LORA_HEAD_MAX_TOP) return "K must be in [1, 128]";
+  if (grads && hd.r < 1) return "gradients need a rank of at least 1";
+  if (!(tau >= 0.01f && tau <= 100.0f)) return "temperature must be in [0.01, 100]";
+  return nullptr;
+}
+
 }  // namespace lce
 
 namespace {
-
-int check_head(const lora_head* h, int T) {
-  if (!h) return hfail(LORA_CE_EINVAL, "null head");
-  if (h->dim < 64 || h->dim % 64 != 0 || h->dim > 64 * kMaxHead64)
-    return hfail(LORA_CE_EINVAL, "dim must be a multiple of 64 in [64, 640]");
-  if (h->vocab < 1 || h->vocab > (1 << 19))
-    return hfail(LORA_CE_EINVAL, "vocab must be in [1, 2^19]");
-  if (h->rank < 0 || h->rank > kMaxFusedRank)
-    return hfail(LORA_CE_EINVAL, "rank must be in [0, 64]");
-  if (!std::isfinite(h->scale)) return hfail(LORA_CE_EINVAL, "scale must be finite");
-  if (T < 1 || T > LORA_HEAD_MAX_TOKENS) return hfail(LORA_CE_EINVAL, "T must be in [1, 2^20]");
-  return 0;
-}
 
 HeadCore core_of(const lora_head* h) {
   return HeadCore{reinterpret_cast<const __half*>(h->W), h->A, h->rank, h->B, 0,
@@ -913,17 +915,15 @@ int check_arch() {
 }
 
 int check_score(const lora_head* h, int T, int top_k) {
-  if (int rc = check_head(h, T)) return rc;
-  if (top_k < 0 || top_k > LORA_HEAD_MAX_TOP || top_k > h->vocab)
-    return hfail(LORA_CE_EINVAL, "top_k must be in [0, 128] and no more than vocab");
-  return 0;
+  if (!h) return hfail(LORA_CE_EINVAL, "null head");
+  const char* why = head_score_refuses(core_of(h), T, top_k);
+  return why ? hfail(LORA_CE_EINVAL, why) : 0;
 }
 
-int check_distill(const lora_head* h, int T, int K, bool grads) {
-  if (int rc = check_head(h, T)) return rc;
-  if (K < 1 || K > LORA_HEAD_MAX_TOP) return hfail(LORA_CE_EINVAL, "K must be in [1, 128]");
-  if (grads && h->rank < 1) return hfail(LORA_CE_EINVAL, "gradients need a rank of at least 1");
-  return 0;
+int check_distill(const lora_head* h, int T, int K, bool grads, float tau) {
+  if (!h) return hfail(LORA_CE_EINVAL, "null head");
+  const char* why = head_distill_refuses(core_of(h), T, K, grads, tau);
+  return why ? hfail(LORA_CE_EINVAL, why) : 0;
 }
 
 }  // namespace
@@ -937,7 +937,8 @@ size_t lora_head_score_workspace(const lora_head* h, int32_t T, int32_t top_k) {
 }
 
 size_t lora_head_distill_workspace(const lora_head* h, int32_t T, int32_t K, int32_t grads) {
-  return check_distill(h, T, K, grads != 0) ? 0 : head_distill_bytes(core_of(h), T, K, grads != 0);
+  if (check_distill(h, T, K, grads != 0, 1.0f)) return 0;
+  return head_distill_bytes(core_of(h), T, K, grads != 0);
 }
 
 int lora_head_score(const lora_head* h, const void* H, int32_t h_dtype, int32_t T,
@@ -987,11 +988,9 @@ int lora_head_distill(const lora_head* h, const void* H, int32_t h_dtype, int32_
   if ((gA == nullptr) != (gB == nullptr))
     return hfail(LORA_CE_EINVAL, "gA and gB go together");
   const bool grads = gA != nullptr;
-  if (int rc = check_distill(h, T, K, grads)) return rc;
+  if (int rc = check_distill(h, T, K, grads, temperature)) return rc;
   if (h_dtype < LORA_CE_BF16 || h_dtype > LORA_CE_F32)
     return hfail(LORA_CE_EINVAL, "bad hidden-state dtype");
-  if (!(temperature >= 0.01f && temperature <= 100.0f))
-    return hfail(LORA_CE_EINVAL, "temperature must be in [0.01, 100]");
   Buffers b;
   struct {
     const void* p;

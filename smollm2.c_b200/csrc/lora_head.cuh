@@ -69,19 +69,18 @@ __device__ __forceinline__ long long sub_idx(int t, int k, int n_sub) {
 // V = 49152 about four records in ten rows (with one logit per record only,
 // and none for the second, it was 2.7 records a row).  Fewer columns per record
 // where the vocabulary gives less than 4 records per alternative.
-// Issue slots per logit: 2 for kSub 0, about 9 for kSub 64, beside the 18 that
-// one SM has while its tensor core forms a 128 x 256 x 576 tile: the pass stays
-// bound by the MMAs and the loads of W.
-// kR4: the rank term of ranks up to 4 here, four multiply-adds per logit from
-// staged rows of B (as EpiLse), instead of a tenth K-block in shared memory and in
-// the ring, of which it would use a quarter at most.
-template <int kRing_, int kSub, bool kR4 = false>
+// Bound by the MMAs and their loads of W, as the training step's passes (tensor
+// pipe 54% busy), not by the epilogue: without records or entropy (kSub 0) it is
+// no faster, nor with the two largest of a chunk from a tree of min and max on
+// logits that carry their column in the lowest bits, nor with the rank-4 term in
+// the epilogue instead of a tenth K-block, nor with a fifth ring stage.
+template <int kRing_, int kSub>
 struct EpiScore {
-  static constexpr bool kAug = !kR4;
+  static constexpr bool kAug = true;
   static constexpr bool kDepend = true;
-  static constexpr int kRec = kR4 ? 4 : 0;
+  static constexpr int kRec = 0;
   static constexpr int kRing = kRing_;
-  static constexpr int kRecBufs = kR4 ? 2 : 1;
+  static constexpr int kRecBufs = 1;
   static constexpr int kWarps = 16;
   static constexpr int kCW = 8;
   static constexpr bool kTop = kSub != 0;
@@ -93,11 +92,8 @@ struct EpiScore {
   float S, Slo, E, Elo;  // the same over the row so far, folded every 64 columns (as EpiLse)
   float r1, r2, rest;    // kSub 64: the record so far
   int a1, a2;
-  float2 sU2[kR4 ? 4 : 1];
 
-  __device__ static const float* global_recs(const GemmArgs& g, int b) {
-    return g.Bt + (long long)b * kBN * kRec;
-  }
+  __device__ static const float* global_recs(const GemmArgs& g, int) { return g.Bt; }
   __device__ static int limit(const GemmArgs& g) { return g.V; }
 
   __device__ void begin(const GemmArgs& g, int abs_row) {
@@ -108,13 +104,6 @@ struct EpiScore {
     S = Slo = E = Elo = 0.f;
     r1 = r2 = rest = -INFINITY;
     a1 = a2 = 0;
-    if constexpr (kR4) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float u = g.tok[tidx(valid ? t : 0, j, 4)];
-        sU2[j] = f2(u, u);
-      }
-    }
   }
 
   // Adds the chunk's terms at reference nm = -(reference max) * lg.
@@ -136,19 +125,7 @@ struct EpiScore {
 
   template <bool kTail>
   __device__ __forceinline__ void chunk(const GemmArgs& g, int v0, float (&acc)[kCW],
-                                        const float* recs) {
-    if constexpr (kR4) {
-#pragma unroll
-      for (int p = 0; p < kCW / 2; ++p) {
-        float b[8];
-        ld_vec<8>(recs + p * 8, b);
-        float2 z2 = f2(acc[2 * p], acc[2 * p + 1]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) z2 = __ffma2_rn(sU2[j], f2(b[2 * j], b[2 * j + 1]), z2);
-        acc[2 * p] = z2.x;
-        acc[2 * p + 1] = z2.y;
-      }
-    }
+                                        const float*) {
     if (kTail) {
 #pragma unroll
       for (int i = 0; i < kCW; ++i)
@@ -722,6 +699,7 @@ __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* i
     const int v = ids[min(i, n - 1)];
     const float* su = a.sU + (long long)t * a.R;
     float s = 0.f;
+#pragma unroll 8
     for (int j = lane >> 4; j < a.r; j += 2) s = fmaf(su[j], a.B.at(j, v), s);
     s += __shfl_xor_sync(0xffffffffu, s, 16);
     z += (double)s;
@@ -970,11 +948,15 @@ static __global__ void __launch_bounds__(256, 3) lh_score_few(FewArgs a) {
   if (a.r > 0) {  // thread: one vocab row, every other position
     const int i = tid & (kFewRows - 1), t0 = tid / kFewRows, v = min(v0 + i, a.V - 1);
     float s[4 * NT] = {};
-#pragma unroll 4
-    for (int j = 0; j < a.r; ++j) {
-      const float b = a.B.at(j, v);
+    for (int j = 0; j < a.r; j += 4) {  // R is a multiple of 4, s U of the rest is 0
+      float b[4];
 #pragma unroll
-      for (int n = 0; n < 4 * NT; ++n) s[n] = fmaf(su[(2 * n + t0) * a.R + j], b, s[n]);
+      for (int e = 0; e < 4; ++e) b[e] = j + e < a.r ? a.B.at(j + e, v) : 0.f;
+#pragma unroll
+      for (int n = 0; n < 4 * NT; ++n) {
+        const float4 u = *reinterpret_cast<const float4*>(su + (2 * n + t0) * a.R + j);
+        s[n] = fmaf(u.x, b[0], fmaf(u.y, b[1], fmaf(u.z, b[2], fmaf(u.w, b[3], s[n]))));
+      }
     }
 #pragma unroll
     for (int n = 0; n < 4 * NT; ++n) sz[(2 * n + t0) * kFewLdZ + i] += s[n];
@@ -1437,7 +1419,6 @@ static __global__ void __launch_bounds__(32 * kRowWarps, 3) lh_distill_rows(Dist
   team.red = s_red[no];
   const int t = (int)blockIdx.x * kTeams + no;
   grid_wait();
-  grid_launch();
   if (t >= a.z.T) return;
   const int R = a.z.R;
   const int nslot = a.p.slots(t);
@@ -1594,7 +1575,6 @@ static __global__ void lh_xt(int T, int R, long long ld, const float* __restrict
                              const int* __restrict__ stats,
                              __half* __restrict__ xt) {
   grid_wait();
-  grid_launch();
   const double up = exp2i(scale_exp(stats[kStUMax], 13));
   const long long n = (long long)T * R, stride = (long long)gridDim.x * blockDim.x;
   for (long long k = (long long)blockIdx.x * blockDim.x + threadIdx.x; k < n; k += stride) {
@@ -1623,7 +1603,6 @@ static __global__ void __launch_bounds__(256) lh_dA(int T, int d, const __half* 
   __shared__ __align__(16) float sh[64][64];
   __shared__ __align__(16) float su[64][R];
   grid_wait();
-  grid_launch();
   const int tid = threadIdx.x, tj = tid % TJ, ti = tid / TJ;
   const int c = (int)blockIdx.x, i0 = (int)blockIdx.y * 64;
   const int t_lo = c * kDAChunk, t_hi = min(T, t_lo + kDAChunk);
@@ -1784,6 +1763,14 @@ static __global__ void __launch_bounds__(256) lh_grads(GradArgs a) {
       a.tail[1] = (float)cnt[0];
     }
   }
+}
+
+// A trainer's step between its gradient sums and the optimizer: the passes' error
+// goes to the handle's flag, and a step that counts no position divides by 1.
+static __global__ void lh_tail(const int* stats, float* tail, int* err) {
+  const int e = stats[kStErr];
+  if (e != 0) atomicCAS(err, 0, e);
+  if (tail[1] == 0.f) tail[1] = 1.f;
 }
 
 }  // namespace lce

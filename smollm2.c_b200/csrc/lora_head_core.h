@@ -36,4 +36,11 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
                      const int32_t* ids, const float* teacher, float tau, const float* weight,
                      float* loss, const GradOut& out, void* ws, cudaStream_t st, const char** why);
 
+// After the sums over ranks: lh_tail on a workspace that head_distill_run has used.
+int head_step_tail(const void* ws, float* tail, int* err, cudaStream_t st);
+
+// Smallest and largest sizes (a message, or null).
+const char* head_score_refuses(const HeadCore& hd, int T, int top_k);
+const char* head_distill_refuses(const HeadCore& hd, int T, int K, bool grads, float tau);
+
 }  // namespace lce

@@ -48,7 +48,8 @@ EXPORTS = [
     "lora_ce_merge_weight_device", "lora_ce_merge_last_error", "lora_ce_set_scale",
     "lora_ce_set_weight_q4k", "lora_ce_q4k_dequant", "lora_ce_q4k_dequant_device",
     "lora_ce_q4k_last_error", "lora_ce_apply_grads", "lora_ce_set_copy_timing",
-    "lora_ce_copy_times", "lora_ce_set_comm_timeout",
+    "lora_ce_copy_times", "lora_ce_set_comm_timeout", "lora_ce_score", "lora_ce_score_device",
+    "lora_ce_distill_step", "lora_ce_distill_step_device",
 ]
 
 # Symbols declared in include/lora_body.h.
@@ -180,6 +181,12 @@ def load_library() -> C.CDLL:
     lib.lora_ce_merge_weight_device.restype = C.c_int
     lib.lora_ce_merge_last_error.argtypes = []
     lib.lora_ce_merge_last_error.restype = C.c_char_p
+    lib.lora_ce_score.argtypes = [vp, vp, C.c_int32, C.c_int32, vp, C.c_int32, vp, vp, vp, vp]
+    lib.lora_ce_score_device.argtypes = lib.lora_ce_score.argtypes
+    lib.lora_ce_distill_step.argtypes = [vp, vp, C.c_int32, C.c_int32, C.c_int32, vp, vp, C.c_float,
+                                         vp, C.POINTER(C.c_float)]
+    lib.lora_ce_distill_step_device.argtypes = [vp, vp, C.c_int32, C.c_int32, C.c_int32, vp, vp,
+                                                C.c_float, vp, vp]
     ph = C.POINTER(Head)
     lib.lora_head_score_workspace.argtypes = [ph, C.c_int32, C.c_int32]
     lib.lora_head_score_workspace.restype = C.c_size_t
@@ -456,6 +463,67 @@ class LoraCE:
         n_pred = use_n - 1
         targets = np.ascontiguousarray(np.asarray(tokens, np.int32)[1:use_n])
         return self.step(np.ascontiguousarray(H[:n_pred]), targets)
+
+    @staticmethod
+    def _hidden(H: np.ndarray, dtype: int | None):
+        if dtype is None:
+            dtype = {np.dtype(np.uint16): BF16, np.dtype(np.float16): F16,
+                     np.dtype(np.float32): F32}[H.dtype]
+        return np.ascontiguousarray(H), dtype
+
+    def score(self, H: np.ndarray, tokens: np.ndarray | None = None, top_k: int = 0,
+              dtype: int | None = None) -> dict:
+        """lora_ce_score: entropy [T]; with tokens [T], logprob [T]; with top_k,
+        top_ids and top_logprobs [T][top_k].  H as in step()."""
+        H, dtype = self._hidden(H, dtype)
+        T = H.shape[0]
+        assert H.shape == (T, self.cfg.dim)
+        out = {"entropy": np.empty(T, np.float32)}
+        tok = None
+        if tokens is not None:
+            tok = np.ascontiguousarray(tokens, np.int32)
+            assert tok.shape == (T,)
+            out["logprob"] = np.empty(T, np.float32)
+        if top_k:
+            out["top_ids"] = np.empty((T, max(top_k, 0)), np.int32)
+            out["top_logprobs"] = np.empty((T, max(top_k, 0)), np.float32)
+        p = lambda k: _ptr(out[k]) if k in out else None  # noqa: E731
+        _check(self.lib.lora_ce_score(self.h, _ptr(H), dtype, T, None if tok is None else _ptr(tok),
+                                      top_k, p("logprob"), p("entropy"), p("top_ids"),
+                                      p("top_logprobs")), "lora_ce_score")
+        return out
+
+    def score_device(self, d_H: int, dtype: int, T: int, d_tokens: int, top_k: int, d_logprob: int,
+                     d_entropy: int, d_top_ids: int, d_top_logprobs: int) -> None:
+        """lora_ce_score_device: device addresses, 0 for NULL; on self.stream."""
+        _check(self.lib.lora_ce_score_device(
+            self.h, d_H or None, dtype, T, d_tokens or None, top_k, d_logprob or None,
+            d_entropy or None, d_top_ids or None, d_top_logprobs or None), "lora_ce_score_device")
+
+    def distill_step(self, H: np.ndarray, ids: np.ndarray, teacher: np.ndarray,
+                     temperature: float = 1.0, weight: np.ndarray | None = None,
+                     dtype: int | None = None) -> float:
+        """lora_ce_distill_step on the teacher's lists ids, teacher [T][K]
+        (negative ids: no entry) and optional weights [T]; the mean loss."""
+        H, dtype = self._hidden(H, dtype)
+        i = np.ascontiguousarray(ids, np.int32)
+        z = np.ascontiguousarray(teacher, np.float32)
+        T, K = i.shape
+        assert H.shape == (T, self.cfg.dim) and z.shape == (T, K)
+        w = None if weight is None else np.ascontiguousarray(weight, np.float32)
+        assert w is None or w.shape == (T,)
+        loss = C.c_float()
+        _check(self.lib.lora_ce_distill_step(self.h, _ptr(H), dtype, T, K, _ptr(i), _ptr(z),
+                                             float(temperature), None if w is None else _ptr(w),
+                                             C.byref(loss)), "lora_ce_distill_step")
+        return loss.value
+
+    def distill_step_device(self, d_H: int, dtype: int, T: int, K: int, d_ids: int, d_teacher: int,
+                            temperature: float = 1.0, d_weight: int = 0, d_loss: int = 0) -> None:
+        """lora_ce_distill_step_device: device addresses, 0 for NULL; on self.stream."""
+        _check(self.lib.lora_ce_distill_step_device(
+            self.h, d_H or None, dtype, T, K, d_ids or None, d_teacher or None, float(temperature),
+            d_weight or None, d_loss or None), "lora_ce_distill_step_device")
 
     def sync(self) -> None:
         _check(self.lib.lora_ce_sync(self.h), "lora_ce_sync")
