@@ -585,11 +585,11 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   a.top_k = top_k;
   a.n_pick = std::min(w.n_sub, std::max(top_k, kMinPick));
   a.cap = 2 * score_picks(a.n_pick) + top_k + 65;  // and the given token
-  const size_t team = score_team_smem(a.n_pick, a.cap);
   const bool warps = T >= sms * kRowWarps && w.n_sub <= 32 * 32;
-  void (*rows)(ScoreArgs) = lh_score_rows<kRowWarps, 32>;
-  if (warps) rows = w.n_sub <= 24 * 32 ? lh_score_rows<1, 24> : lh_score_rows<1, 32>;
-  else if (w.n_sub <= 4 * 256) rows = lh_score_rows<kRowWarps, 4>;
+  const int tw = warps ? 1 : w.n_sub <= 8 * 128 ? 4 : 8;  // warps per position
+  void (*rows)(ScoreArgs) = warps ? w.n_sub <= 24 * 32 ? lh_score_rows<1, 24> : lh_score_rows<1, 32>
+                            : tw == 4 ? lh_score_rows<4, 8> : lh_score_rows<8, 32>;
+  const size_t team = score_team_smem(a.n_pick, a.cap, tw);
   const size_t rows_smem =
       warps ? kScoreRows * std::max(team, (size_t)(w.n_sub + 1) * 4) : team;
   if (!allow_smem(reinterpret_cast<const void*>(rows), rows_smem))
@@ -659,7 +659,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   a.top_ids = top_ids;
   a.top_logprobs = top_logprobs;
   const int per = warps ? kScoreRows : 1;
-  const int threads = warps ? 32 * kScoreRows : 32 * kRowWarps;
+  const int threads = 32 * tw * per;
   if (!launch_after(rows, (T + per - 1) / per, threads, rows_smem, st, a) ||
       cudaGetLastError() != cudaSuccess)
     return *why = kNoLaunch, LORA_CE_ECUDA;

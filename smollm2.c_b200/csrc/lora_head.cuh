@@ -28,7 +28,7 @@ namespace lce {
 
 constexpr int kMaxTop = 128;      // largest top_k, largest teacher list
 constexpr int kMinPick = 8;       // logits of a row that are computed again at least
-constexpr int kPickStop = 8;      // the search ends with up to so many records beyond that,
+constexpr int kPickStop = 7;      // the search ends with up to so many records beyond that,
 constexpr int kPickSlack = 24;    // and takes near ties of the last up to so many
 constexpr int kRowWarps = 8;      // warps per block of the per-row kernels
 constexpr int kMaxHead64 = 10;    // hidden size in units of 64
@@ -351,17 +351,21 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
 
 // The same for kTileRows positions per block: all of their hidden states on the
 // way at once (64 elements at a time with the next 64 in flight took 35 us for
-// 2,047 positions, waiting), then a product of tiles, 64 rows of A at a time with
-// the next 64 in flight.
+// 2,047 positions, waiting), then each warp sums its eighth of the hidden size for
+// every position and rank: lanes over neighbouring ranks, A straight from global
+// memory 12 rows at a time, h four elements per load from shared memory, up to 32
+// sums per lane.  (A through shared memory, four sums per thread, a load for each
+// operand of each product and two block barriers per 64 elements: 35 us instead of
+// @@ for 2,047 positions at rank 64.)
 constexpr int kTileRows = 16;
 template <int R>
 __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem) {
-  constexpr int RT = R >= 64 ? 4 : R == 32 ? 2 : 1;      // ranks per thread
-  constexpr int TX = R > 0 ? R / RT : 1;                 // threads over ranks
-  constexpr int NS = R > 0 ? 256 / (TX * kTileRows) : 1; // slices of the 64
+  constexpr int kLanes = R >= 32 ? 32 : R > 0 ? R : 1;  // over ranks
+  constexpr int kPer = R > 32 ? 2 : 1;                  // ranks per lane
+  constexpr int kGroups = 32 / kLanes;                  // positions side by side
+  constexpr int kPos = R > 0 ? kTileRows / kGroups : 1; // and per lane
   const int ldh = a.d + 4;
-  float* hT = smem;                                      // [16][d + 4]
-  float* aT = hT + kTileRows * ldh;                      // [64][R], then [256] sums
+  float* hT = smem;                                     // [16][d + 4], then [8][16][R] sums
   __shared__ float swt[kTileRows];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   if (a.ids) {  // sixteen threads per position, every 16th entry each
@@ -382,18 +386,6 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
     }
     __syncthreads();
   }
-  constexpr int kAPer = R > 0 ? (64 * R + 255) / 256 : 1;
-  float an[kAPer];
-  auto fetch_a = [&](int c) {
-    if constexpr (R > 0) {
-#pragma unroll
-      for (int q = 0; q < kAPer; ++q) {
-        const int k = tid + 256 * q, i = k / R, j = k % R;
-        an[q] = j < a.r ? a.A[(long long)(64 * c + i) * a.lda + j] : 0.f;
-      }
-    }
-  };
-  fetch_a(0);
 #pragma unroll
   for (int p = 0; p < 2; ++p) {  // two rows per warp
     const int row = w + 8 * p, t = t0 + row;
@@ -413,39 +405,47 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
       }
   }
   if constexpr (R > 0) {
-    const int tx = tid % TX, py = tid / TX % kTileRows, sl = tid / (TX * kTileRows);
-    float u[RT];
+    constexpr int kRows = 12;  // of A in flight; d / 8 is a multiple of 8
+    const int j = lane % kLanes, g = lane / kLanes;
+    const int i_lo = a.d / 8 * w, i_hi = i_lo + a.d / 8;
+    float u[kPos][kPer] = {};
+    __syncthreads();
+    for (int i0 = i_lo; i0 < i_hi; i0 += kRows) {
+      float av[kRows][kPer];
 #pragma unroll
-    for (int q = 0; q < RT; ++q) u[q] = 0.f;
-    const int chunks = a.d / 64;
-    for (int c = 0; c < chunks; ++c) {
-      __syncthreads();
+      for (int i = 0; i < kRows; ++i)
 #pragma unroll
-      for (int q = 0; q < kAPer; ++q) aT[tid + 256 * q] = an[q];
-      if (c + 1 < chunks) fetch_a(c + 1);
-      __syncthreads();
-      const float* x = hT + py * ldh + 64 * c;
-#pragma unroll 8
-      for (int i = sl; i < 64; i += NS) {
-        const float h = x[i];
+        for (int q = 0; q < kPer; ++q)
+          av[i][q] = i0 + i < i_hi && j + 32 * q < a.r
+                         ? a.A[(long long)(i0 + i) * a.lda + j + 32 * q] : 0.f;
 #pragma unroll
-        for (int q = 0; q < RT; ++q) u[q] = fmaf(h, aT[i * R + tx * RT + q], u[q]);
+      for (int i = 0; i < kRows; i += 4) {
+        if (i0 + i >= i_hi) break;
+#pragma unroll
+        for (int p = 0; p < kPos; ++p) {
+          const float4 h = *reinterpret_cast<const float4*>(hT + (kGroups * p + g) * ldh + i0 + i);
+#pragma unroll
+          for (int q = 0; q < kPer; ++q)
+            u[p][q] = fmaf(h.w, av[i + 3][q],
+                           fmaf(h.z, av[i + 2][q],
+                                fmaf(h.y, av[i + 1][q], fmaf(h.x, av[i][q], u[p][q]))));
+        }
       }
     }
-    if constexpr (NS > 1) {  // ranks 4 and 8: the slices meet in shared memory
-      __syncthreads();
-      aT[tid] = u[0];
-      __syncthreads();
-      if (sl == 0) {
+    __syncthreads();
 #pragma unroll
-        for (int q = 1; q < NS; ++q) u[0] += aT[tid + q * TX * kTileRows];
-      }
-    }
+    for (int p = 0; p < kPos; ++p)
+#pragma unroll
+      for (int q = 0; q < kPer; ++q)
+        hT[(w * kTileRows + kGroups * p + g) * R + j + 32 * q] = u[p][q];
+    __syncthreads();
     float umax = 0.f;
-    if (sl == 0 && t0 + py < a.T) {
-      const float wt = a.ids ? swt[py] : 0.f;
+    for (int k = tid; k < kTileRows * R; k += 256) {
+      const int p = k / R;
+      float s = hT[k];
 #pragma unroll
-      for (int q = 0; q < RT; ++q) put_u(a, t0 + py, tx * RT + q, u[q], umax, wt);
+      for (int q = 1; q < 8; ++q) s += hT[q * kTileRows * R + k];
+      if (t0 + p < a.T) put_u(a, t0 + p, k % R, s, umax, a.ids ? swt[p] : 0.f);
     }
     if (a.tok)
       for (int q = w; q < kTileRows; q += 8)
@@ -454,7 +454,8 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
   }
 }
 __host__ __device__ inline size_t prep_tile_smem(int R, int d) {
-  return R == 0 ? 0 : (size_t)(kTileRows * (d + 4) + 64 * R) * 4;
+  const size_t h = (size_t)kTileRows * (d + 4), s = (size_t)8 * kTileRows * R;
+  return R == 0 ? 0 : (h > s ? h : s) * 4;
 }
 
 struct PackArgs {
@@ -617,7 +618,7 @@ struct LogitArgs {
 constexpr double kLoss32 = 0.79 * 1.5 / 33554432.0 * 1.4426950408889634;
 template <bool kSum64, class Out>
 __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* ids, int n, int lane,
-                                         Out* out) {
+                                         Out* out, int part = 0, int parts = 1) {
   constexpr int kBatch = 6;
   const int c = lane & 3, g = lane >> 2;
   const long long v0 = ids[min(g, n - 1)], v1 = ids[min(g + 8, n - 1)];
@@ -646,12 +647,13 @@ __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* i
     const __half* w0 = a.W + v0 * a.d + 8 * c;
     const __half* w1 = a.W + v1 * a.d + 8 * c;
     const __half* h = a.h16 + (long long)t * a.d + 8 * c;
-    for (int k0 = 0; k0 < a.d; k0 += 32 * kBatch) {
+    const int steps = a.d / 32, k_hi = steps * (part + 1) / parts * 32;
+    for (int k0 = steps * part / parts * 32; k0 < k_hi; k0 += 32 * kBatch) {
       uint4 p[kBatch], q[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         p[i] = q[i] = zero;
-        if (k0 + 32 * i < a.d) {
+        if (k0 + 32 * i < k_hi) {
           p[i] = *reinterpret_cast<const uint4*>(w0 + k0 + 32 * i);
           q[i] = *reinterpret_cast<const uint4*>(w1 + k0 + 32 * i);
         }
@@ -660,28 +662,34 @@ __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* i
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         uint4 x = zero;
-        if (g == 0 && k0 + 32 * i < a.d) x = *reinterpret_cast<const uint4*>(h + k0 + 32 * i);
+        if (g == 0 && k0 + 32 * i < k_hi) x = *reinterpret_cast<const uint4*>(h + k0 + 32 * i);
         add(p[i], q[i], x);
       }
     }
   }
-  auto step = [&](const __half* w0, const __half* w1, const __half* h, bool in) {
-    add(in ? *reinterpret_cast<const uint4*>(w0) : zero,
-        in ? *reinterpret_cast<const uint4*>(w1) : zero,
-        in && g == 0 ? *reinterpret_cast<const uint4*>(h) : zero);
+  auto row16 = [&](const __half* p, bool in) {
+    return in ? *reinterpret_cast<const uint4*>(p) : zero;
   };
-  if (a.waug) {
+  const bool last = part == parts - 1;  // the rank term's
+  if (a.waug && last) {
     const __half* w0 = a.waug + v0 * a.aug_width + 8 * c;
     const __half* w1 = a.waug + v1 * a.aug_width + 8 * c;
     const __half* h = a.haug + (long long)t * a.aug_width + 8 * c;
     if (a.aug_layout == 1) {
-      for (int k = 0; k < a.aug_width; k += 32)
-        step(w0 + k, w1 + k, h + k, k + 8 * c < a.aug_width);
+#pragma unroll 2
+      for (int k = 0; k < a.aug_width; k += 32) {
+        const bool in = k + 8 * c < a.aug_width;
+        add(row16(w0 + k, in), row16(w1 + k, in), row16(h + k, in && g == 0));
+      }
     } else {  // hi . hi, lo . hi, hi . lo
+#pragma unroll 2
       for (int k = 0; k < a.R; k += 32) {
-        step(w0 + k, w1 + k, h + k, true);
-        step(w0 + a.R + k, w1 + a.R + k, h + k, true);
-        step(w0 + k, w1 + k, h + a.R + k, true);
+        const uint4 hi0 = row16(w0 + k, true), hi1 = row16(w1 + k, true);
+        const uint4 lo0 = row16(w0 + a.R + k, true), lo1 = row16(w1 + a.R + k, true);
+        const uint4 x = row16(h + k, g == 0), y = row16(h + a.R + k, g == 0);
+        add(hi0, hi1, x);
+        add(lo0, lo1, x);
+        add(hi0, hi1, y);
       }
     }
   }
@@ -695,7 +703,7 @@ __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* i
   const int i = lane & 15;
   double z = i < 8 ? a0 : a1;
   if constexpr (kSum64) z = fma(z, kLoss32, z);
-  if (!a.waug && a.r > 0) {  // lane i % 16 takes row i, the halves of the warp every other rank
+  if (!a.waug && a.r > 0 && last) {  // lane i % 16 takes row i, the halves of the warp every other rank
     const int v = ids[min(i, n - 1)];
     const float* su = a.sU + (long long)t * a.R;
     float s = 0.f;
@@ -707,18 +715,20 @@ __device__ __forceinline__ void logits16(const LogitArgs& a, int t, const int* i
   if (lane < 16 && i < n) out[i] = (Out)z;
 }
 
-// How far apart two logits have to be for logits16 to tell their order: several
-// times the largest error seen.
-__device__ __forceinline__ float logit_gap(float z) { return 4e-6f * (1.0f + fabsf(z)); }
-
-// One logit by one warp with 64-bit sums throughout (products of f16 are exact
-// in f32; U is formed again): for those whose order logits16 does not tell.
 __device__ __forceinline__ double warp_sum(double s) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
   return s;
 }
-__device__ __forceinline__ double logit64(const LogitArgs& a, int t, int v, int lane) {
+
+// How far apart two logits have to be for logits16 to tell their order: several
+// times the largest error seen.
+__device__ __forceinline__ float logit_gap(float z) { return 4e-6f * (1.0f + fabsf(z)); }
+
+// One logit by one warp with 64-bit sums throughout (products of f16 are exact in
+// f32): for those whose order logits16 does not tell.  u: scale U[t], from u64.
+__device__ __forceinline__ double logit64(const LogitArgs& a, int t, int v, const double* u,
+                                          int lane) {
   const __half* h = a.h16 + (long long)t * a.d;
   const __half* w = a.W + (long long)v * a.d;
   double z = 0.0;
@@ -729,13 +739,7 @@ __device__ __forceinline__ double logit64(const LogitArgs& a, int t, int v, int 
       const float2 y = __half22float2(*reinterpret_cast<const __half2*>(w + 64 * k + 2 * lane));
       z += (double)(x.x * y.x) + (double)(x.y * y.y);
     }
-  for (int j = 0; j < a.r; ++j) {
-    double u = 0.0;
-#pragma unroll 6
-    for (int i = lane; i < a.d; i += 32)
-      u = fma((double)__half2float(h[i]), (double)a.A[(long long)i * a.lda + j], u);
-    z = fma(u, (double)a.scale * (double)a.B.at(j, v), z);  // the lanes' shares add up below
-  }
+  for (int j = lane; j < a.r; j += 32) z = fma(u[j], (double)a.B.at(j, v), z);
   return warp_sum(z);
 }
 
@@ -746,7 +750,7 @@ template <int TW>
 struct Team {
   static constexpr int kThreads = 32 * TW;
   int tid, lane, w;
-  double* red;  // TW > 1: 2 x TW doubles of shared memory
+  double* red;  // TW > 1: 4 x TW doubles of shared memory
   int parity = 0;
   __device__ __forceinline__ void sync() const {
     if constexpr (TW == 1) __syncwarp();
@@ -757,7 +761,7 @@ struct Team {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, off));
     if constexpr (TW > 1) {
-      T* b = reinterpret_cast<T*>(red + TW * parity);
+      T* b = reinterpret_cast<T*>(red + 2 * TW * parity);
       parity ^= 1;
       if (lane == 0) b[w] = x;
       __syncthreads();
@@ -770,10 +774,30 @@ struct Team {
   __device__ __forceinline__ double sum(double x) {
     return reduce(x, [](double p, double q) { return p + q; });
   }
+  __device__ __forceinline__ double2 sum2(double x, double y) {
+    x = warp_sum(x);
+    y = warp_sum(y);
+    if constexpr (TW > 1) {
+      double* b = red + 2 * TW * parity;
+      parity ^= 1;
+      if (lane == 0) {
+        b[2 * w] = x;
+        b[2 * w + 1] = y;
+      }
+      __syncthreads();
+      x = y = 0.0;
+#pragma unroll
+      for (int i = 0; i < TW; ++i) {
+        x += b[2 * i];
+        y += b[2 * i + 1];
+      }
+    }
+    return make_double2(x, y);
+  }
   __device__ __forceinline__ int count(int x) {
     x = __reduce_add_sync(0xffffffffu, x);
     if constexpr (TW > 1) {
-      int* b = reinterpret_cast<int*>(red + TW * parity);
+      int* b = reinterpret_cast<int*>(red + 2 * TW * parity);
       parity ^= 1;
       if (lane == 0) b[w] = x;
       __syncthreads();
@@ -794,6 +818,28 @@ struct Team {
   }
 };
 
+// u = scale U[t] [r] with 64-bit sums: each warp takes some of the ranks, its lanes
+// neighbouring ones (A is read in whole sectors) and every n-th row of A.  A lane
+// per row instead, each rank of each logit anew, took 100 us for two logits at
+// rank 50.
+template <int TW>
+__device__ __forceinline__ void u64(const LogitArgs& a, int t, const Team<TW>& team, double* u) {
+  const __half* h = a.h16 + (long long)t * a.d;
+  const int per = (a.r + TW - 1) / TW;
+  for (int j0 = per * team.w; j0 < min(a.r, per * (team.w + 1)); j0 += 32) {
+    const int n = min(32, min(a.r, per * (team.w + 1)) - j0);
+    const int span = n == 1 ? 1 : 1 << (32 - __clz(n - 1)), j = team.lane & (span - 1);
+    const float* A = a.A + j0 + min(j, n - 1);
+    double s = 0.0;
+#pragma unroll 16
+    for (int i = team.lane / span; i < a.d; i += 32 / span)
+      s = fma((double)__half2float(h[i]), (double)A[(long long)i * a.lda], s);
+    for (int off = span; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if (team.lane < n) u[j0 + j] = (double)a.scale * s;
+  }
+  team.sync();
+}
+
 // Where the partial sums of a position sit: pass 1 over n_b column tiles,
 // 256-position blocks, tiles split over at most `units` owners.
 struct SlotPlan {
@@ -804,12 +850,12 @@ struct SlotPlan {
   const float* p_ent;
   const float* p_q;
   __device__ __forceinline__ int slots(int t) const {
-    const int ab = t / (2 * kBM);
-    const long long total = (long long)n_a * n_b;
-    const int G = (int)(total < units ? total : units);
-    const int s0 = tile_owner((long long)ab * n_b, total, G);
-    const int s1 = tile_owner((long long)ab * n_b + n_b - 1, total, G);
-    return cparts * (s1 - s0 + 1);
+    // tile_owner in 32 bits: at most 4096 x 2048 tiles, 148 units (few positions:
+    // 4096 of each)
+    const unsigned first = (unsigned)(t / (2 * kBM)) * n_b, total = (unsigned)n_a * n_b;
+    const unsigned G = min(total, (unsigned)units);
+    const unsigned s0 = ((first + 1) * G - 1) / total, s1 = ((first + n_b) * G - 1) / total;
+    return cparts * (int)(s1 - s0 + 1);
   }
 };
 
@@ -818,27 +864,74 @@ struct RowSum {
   double S, E;  // sum of 2^x, sum of 2^x * x, x from M
 };
 
-// A row's slots merged in a fixed order.
+// A row's slots merged in a fixed order.  A thread keeps its first ones in
+// registers from the maximum to the sums: a second read is a second wait.
 template <bool kEnt, int TW>
 __device__ __forceinline__ RowSum merge_row(const SlotPlan& p, int t, int nslot, Team<TW>& team) {
+  constexpr int kKeep = TW == 1 ? 1 : 4;
+  float pm[kKeep], s[kKeep], e[kKeep];
   float M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int k = team.tid + i * team.kThreads;
+    const long long o = (long long)k * p.ld + t;
+    pm[i] = k < nslot ? p.p_max[o] : -INFINITY;
+    s[i] = k < nslot ? p.p_sum[o] : 0.f;
+    e[i] = kEnt && k < nslot ? p.p_ent[o] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) M = fmaxf(M, pm[i]);
 #pragma unroll 2
-  for (int k = team.tid; k < nslot; k += team.kThreads)
+  for (int k = team.tid + kKeep * team.kThreads; k < nslot; k += team.kThreads)
     M = fmaxf(M, p.p_max[(long long)k * p.ld + t]);
   M = team.max_f(M);
   double S = 0.0, E = 0.0;
+  auto add = [&](float m, float sum, float ent) {
+    if (m == -INFINITY && sum == 0.f) return;  // a slice that saw no valid column
+    const float x = m - M, f = exp2f(x);
+    S += (double)(sum * f);
+    if constexpr (kEnt) E += (double)(f * fmaf(x, sum, ent));
+  };
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) add(pm[i], s[i], e[i]);
 #pragma unroll 2
-  for (int k = team.tid; k < nslot; k += team.kThreads) {
+  for (int k = team.tid + kKeep * team.kThreads; k < nslot; k += team.kThreads) {
     const long long o = (long long)k * p.ld + t;
-    const float pm = p.p_max[o], s = p.p_sum[o], e = kEnt ? p.p_ent[o] : 0.f;
-    if (pm == -INFINITY && s == 0.f) continue;  // a slice that saw no valid column
-    const float x = pm - M, f = exp2f(x);
-    S += (double)(s * f);
-    if constexpr (kEnt) E += (double)(f * fmaf(x, s, e));
+    add(p.p_max[o], p.p_sum[o], kEnt ? p.p_ent[o] : 0.f);
   }
-  S = team.sum(S);
-  if constexpr (kEnt) E = team.sum(E);
+  if constexpr (kEnt) {
+    const double2 both = team.sum2(S, E);
+    S = both.x;
+    E = both.y;
+  } else {
+    S = team.sum(S);
+  }
   return RowSum{M, S, E};
+}
+
+// logits16 of n ids to z.  A team of several warps shares a group of 16 where there
+// are few: each warp takes part of the hidden size (zp: 16 TW partial sums).
+template <int TW>
+__device__ __forceinline__ void team_logits(const LogitArgs& a, int t, const int* ids, int n,
+                                            const Team<TW>& team, double* z, double* zp) {
+  const int groups = (n + 15) / 16;
+  if (TW == 1 || 2 * groups > TW) {
+    for (int c = 16 * team.w; c < n; c += 16 * TW)
+      logits16<true>(a, t, ids + c, min(16, n - c), team.lane, z + c);
+    team.sync();
+  } else if (groups > 0) {
+    const int parts = TW / groups, g = team.w / parts;
+    if (g < groups)
+      logits16<true>(a, t, ids + 16 * g, min(16, n - 16 * g), team.lane, zp + 16 * team.w,
+                     team.w - g * parts, parts);
+    team.sync();
+    for (int c = team.tid; c < n; c += team.kThreads) {
+      double s = 0.0;
+      for (int q = 0; q < parts; ++q) s += zp[16 * ((c >> 4) * parts + q) + (c & 15)];
+      z[c] = s;
+    }
+    team.sync();
+  }
 }
 
 // ------------------------------------------------------------- few positions
@@ -1046,8 +1139,8 @@ struct ScoreArgs {
 // record its number, its second and rest, its columns; 64 columns' ids and
 // logits; counters.  A multiple of 16 bytes.
 __host__ __device__ inline int score_picks(int n_pick) { return n_pick + kPickSlack; }
-__host__ __device__ inline size_t score_team_smem(int n_pick, int cap) {
-  return ((size_t)(2 * kRowWarps + cap) * 8 + (size_t)cap * 16 +
+__host__ __device__ inline size_t score_team_smem(int n_pick, int cap, int warps) {
+  return ((size_t)(warps == 1 ? 0 : 20 * warps) * 8 + (size_t)cap * 24 +
           (size_t)score_picks(n_pick) * 16 + 128 * 4 + 16 * 4 + 15) / 16 * 16;
 }
 constexpr int kScoreRows = 4;  // positions per block where each has a warp
@@ -1058,7 +1151,7 @@ constexpr int kScoreRows = 4;  // positions per block where each has a warp
 // less what rounding may have moved, again, with 64-bit sums where two are too
 // close to tell their order; sort, write.  The softmax's sums get the difference.
 template <int TW, int NK>
-static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW == 1 ? 5 : 2)
+static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW == 8 ? 2 : 5)
     lh_score_rows(ScoreArgs a) {
   constexpr int kTeams = TW == 1 ? kScoreRows : 1;
   constexpr int kThreads = 32 * TW;
@@ -1072,10 +1165,11 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   const unsigned below = (1u << lane) - 1u;
   const int no = threadIdx.x / kThreads;
   const int t = (int)blockIdx.x * kTeams + no;
-  const size_t team_bytes = score_team_smem(a.n_pick, a.cap);
+  const size_t team_bytes = score_team_smem(a.n_pick, a.cap, TW);
   const int P = score_picks(a.n_pick);
   team.red = reinterpret_cast<double*>(smem_rows + no * team_bytes);
-  double* z64 = team.red + 2 * kRowWarps;
+  double* zp = team.red + 4 * TW;  // [16 TW]
+  double* z64 = team.red + (TW == 1 ? 0 : 20 * TW);
   int* ids = reinterpret_cast<int*>(z64 + a.cap);
   float* approx = reinterpret_cast<float*>(ids + a.cap);
   float* approx32 = approx + a.cap;  // again, rounded
@@ -1086,7 +1180,7 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   int* pcol = reinterpret_cast<int*>(prest + P);
   int* col_id = pcol + P;
   float* cols = reinterpret_cast<float*>(col_id + 64);
-  int* words = reinterpret_cast<int*>(cols + 64);  // [0..7] picks per warp, [8] picks
+  int* words = reinterpret_cast<int*>(cols + 64);  // [16] counts per warp
 
   grid_wait();
   // this thread's records: (w NK + i) 32 + lane, so that record order is warp order
@@ -1236,19 +1330,39 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
       __syncwarp();
     }
   }
-  for (int c = tid; c < n_p; c += kThreads) {
-    const int k = picked[c];
-    const long long o = sub_idx(t, k, a.n_sub);
-    const int c1 = a.sub > 1 ? a.sub_arg[o] : 0, c2 = a.sub == 64 ? a.sub_arg2[o] : 0;
-    approx[c] = a.sub_max[o];
-    prest[c] = a.sub > 1 ? a.sub_rest[o] : -INFINITY;
-    psecond[c] = a.sub == 64 ? a.sub_second[o] : -INFINITY;
-    ids[c] = k * a.sub + c1;
-    pcol[c] = c1 | c2 << 8;
+  // (the given token comes first, then the candidates)
+  const int c_0 = have_tok ? 1 : 0;
+  {
+    constexpr int kG = TW == 1 ? 3 : 1;  // picks' records in flight per thread
+    for (int c0 = tid; c0 < n_p; c0 += kG * kThreads) {
+      float m[kG], second[kG], rest[kG];
+      int c1[kG], c2[kG];
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+        const int c = min(c0 + i * kThreads, n_p - 1);
+        const long long o = sub_idx(t, picked[c], a.n_sub);
+        m[i] = a.sub_max[o];
+        rest[i] = a.sub > 1 ? a.sub_rest[o] : -INFINITY;
+        second[i] = a.sub == 64 ? a.sub_second[o] : -INFINITY;
+        c1[i] = a.sub > 1 ? a.sub_arg[o] : 0;
+        c2[i] = a.sub == 64 ? a.sub_arg2[o] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+        const int c = c0 + i * kThreads;
+        if (c >= n_p) continue;
+        approx[c_0 + c] = m[i];
+        ids[c_0 + c] = picked[c] * a.sub + c1[i];
+        prest[c] = rest[i];
+        psecond[c] = second[i];
+        pcol[c] = c1[i] | c2[i] << 8;
+      }
+    }
   }
+  if (have_tok && tid == 0) ids[0] = tk;
   team.sync();
   // seconds that reach the bound, then the columns of records whose rest does
-  int n_c = n_p;
+  int n_c = c_0 + n_p;  // (up to a.cap)
   if (a.sub == 64)
     for (int c0 = 0; c0 < n_p; c0 += 32) {  // (every warp finds the same)
       const int c = c0 + lane;
@@ -1263,7 +1377,7 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
     }
   for (int c0 = 0; c0 < n_p && a.sub > 1; c0 += 32) {
     unsigned more = __ballot_sync(kAll, c0 + lane < n_p && prest[min(c0 + lane, n_p - 1)] >= bound);
-    for (; more && n_c < a.cap - 1; more &= more - 1) {
+    for (; more && n_c < a.cap; more &= more - 1) {
       const int c = c0 + __ffs(more) - 1;
       const int v0 = picked[c] * a.sub, c1 = pcol[c] & 255, nv = min(a.sub, a.z.V - v0);
       const int c2 = a.sub == 64 && psecond[c] >= bound ? pcol[c] >> 8 : -1;
@@ -1277,38 +1391,42 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
         const bool take = q < nv && q != c1 && q != c2 && cols[q] >= bound;
         const unsigned bt = __ballot_sync(kAll, take);
         const int at = n_c + __popc(bt & below);
-        if (take && w == 0 && at < a.cap - 1) {
+        if (take && w == 0 && at < a.cap) {
           ids[at] = v0 + q;
           approx[at] = -INFINITY;  // not known: the sums keep it as it is
+          approx32[at] = cols[q];
         }
-        n_c = min(n_c + __popc(bt), a.cap - 1);
+        n_c = min(n_c + __popc(bt), a.cap);
       }
       team.sync();
     }
   }
-  if (have_tok && tid == 0) ids[n_c] = tk;
+  // The pass's logits, made good for their known loss, are off by a few 1e-7 of z:
+  // enough to tell the order of all but those within 1e-5 (1 + |z|) of another.
+  // These, the kMinPick largest (by which the softmax's sums are made good) and
+  // those known only from the columns above are computed again, the others' logits
+  // are the pass's; of 72 candidates of a list of 64 that is about 10, one group of
+  // 16 instead of five.  All, where that is one group anyway.
+  const double ln2 = 0.69314718055994531, log2e = 1.4426950408889634;
+  const double back = (double)a.lg * ln2;
   team.sync();
-  const int n_z = n_c + (have_tok ? 1 : 0);
-  for (int c = 16 * w; c < n_z; c += 16 * TW)
-    logits16<true>(a.z, t, ids + c, min(16, n_z - c), lane, z64 + c);
+  for (int c = c_0 + tid; c < n_c; c += kThreads)
+    if (approx[c] > -INFINITY) approx32[c] = (float)((double)approx[c] * back);
   team.sync();
-  // ranks; all in 64 bits for logits too close to another to tell their order
-  // (the difference of f32 values tells that as well)
-  constexpr int kItems = TW == 1 ? 3 : 1;
-  bool any_close = false;
-  for (int c = lane + 32 * w; c < n_c; c += kThreads) approx32[c] = (float)z64[c];
-  team.sync();
-  for (int c0 = 32 * kItems * w; c0 < n_c && a.top_k > 0; c0 += kItems * kThreads) {
-    float z[kItems], gap[kItems];
-    int rank[kItems], close[kItems];
+  constexpr int kItems = TW == 1 ? 3 : 2;
+  int n_z = n_c;  // [0, n_z) are computed again
+  const bool fits = n_c - c_0 <= kItems * kThreads;
+  for (int b0 = c_0; b0 < n_c && (a.top_k > 0 || n_c > 16); b0 += kItems * kThreads) {
+    float z[kItems], gap[kItems], was[kItems];
+    int rank[kItems], close[kItems], id[kItems];
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const int c = c0 + 32 * i + lane;
+      const int c = b0 + i * kThreads + tid;
       z[i] = c < n_c ? approx32[c] : INFINITY;
-      gap[i] = c < n_c ? logit_gap(z[i]) : -1.f;
+      gap[i] = c < n_c ? 1e-5f * (1.0f + fabsf(z[i])) : -1.f;
       rank[i] = close[i] = 0;
     }
-    for (int q = 0; q < n_c; ++q) {
+    for (int q = c_0; q < n_c; ++q) {
       const float zq = approx32[q];
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
@@ -1316,33 +1434,101 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
         close[i] += fabsf(zq - z[i]) <= gap[i];
       }
     }
+    if (!fits || n_c <= 16) {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int c = b0 + i * kThreads + tid;
+        if (c < n_c) ranks[c] = close[i] > 1 ? -1 : rank[i];  // (it is close to itself)
+      }
+      continue;
+    }
+    // those to be computed again to the front (one round: they all fit)
+    unsigned again[kItems];
+    int n_w = 0;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const int c = c0 + 32 * i + lane;
-      if (c < n_c) {
-        ranks[c] = close[i] > 1 ? -1 : rank[i];  // (it is close to itself)
-        any_close |= close[i] > 1;
+      const int c = min(b0 + i * kThreads + tid, n_c - 1);
+      was[i] = approx[c];
+      id[i] = ids[c];
+      again[i] = __ballot_sync(kAll, gap[i] >= 0.f && (close[i] > 1 || rank[i] < kMinPick ||
+                                                       was[i] == -INFINITY));
+      n_w += __popc(again[i]);
+    }
+    int front = c_0;
+    if constexpr (TW > 1) {
+      if (lane == 0) words[w] = n_w;
+      __syncthreads();
+      n_z = c_0;
+      for (int q = 0; q < TW; ++q) {
+        front += q < w ? words[q] : 0;
+        n_z += words[q];
       }
+    } else {
+      __syncwarp();
+      n_z = c_0 + n_w;
+    }
+    // the others behind: as many of them as stand before a candidate, less those
+    // that have gone to the front
+    int behind = n_z;
+    if constexpr (TW > 1) {
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < kItems; ++i)
+        mine += __popc(__ballot_sync(kAll, gap[i] >= 0.f) & ~again[i]);
+      if (lane == 0) words[8 + w] = mine;
+      __syncthreads();
+      for (int q = 0; q < w; ++q) behind += words[8 + q];
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const unsigned rest = __ballot_sync(kAll, gap[i] >= 0.f) & ~again[i];
+      const bool sel = again[i] >> lane & 1;
+      const int to = sel ? front + __popc(again[i] & below) : behind + __popc(rest & below);
+      if (gap[i] >= 0.f) {
+        ids[to] = id[i];
+        approx[to] = was[i];
+        approx32[to] = z[i];
+        ranks[to] = close[i] > 1 ? -1 : rank[i];
+      }
+      front += __popc(again[i]);
+      behind += __popc(rest);
     }
   }
   team.sync();
-  if (team.count(any_close && a.top_k > 0) > 0) {
-    for (int c0 = 32 * w; c0 < n_c; c0 += kThreads) {
+  team_logits<TW>(a.z, t, ids, n_z, team, z64, zp);
+  for (int c = n_z + tid; c < n_c; c += kThreads) z64[c] = (double)approx[c] * back;
+  team.sync();
+  // in 64 bits throughout those that are too close to another even now
+  bool any_close = false;
+  for (int c = c_0 + tid; c < n_z && a.top_k > 0; c += kThreads) {
+    if (ranks[c] >= 0) continue;
+    const float zc = (float)z64[c], gap = logit_gap(zc);
+    int close = 0;
+    for (int q = c_0; q < n_z; ++q) close += fabsf((float)(z64[q] - z64[c])) <= gap;
+    if (close > 1) {
+      ranks[c] = -2;
+      any_close = true;
+    }
+  }
+  team.sync();
+  if (team.count(any_close) > 0) {
+    double* u = reinterpret_cast<double*>(col_id);  // and cols: [64]
+    u64(a.z, t, team, u);
+    for (int c0 = 32 * w; c0 < n_z; c0 += kThreads) {
       const int c = c0 + lane;
-      unsigned near = __ballot_sync(kAll, c < n_c && ranks[min(c, n_c - 1)] < 0);
+      unsigned near = __ballot_sync(kAll, c >= c_0 && c < n_z && ranks[min(c, n_z - 1)] == -2);
       for (; near; near &= near - 1) {
         const int q = __ffs(near) - 1;
-        const double zq = logit64(a.z, t, ids[c0 + q], lane);
+        const double zq = logit64(a.z, t, ids[c0 + q], u, lane);
         if (lane == q) z64[c] = zq;
       }
     }
   }
   team.sync();
   // the sums with these logits as they are now
-  const double ln2 = 0.69314718055994531, log2e = 1.4426950408889634;
   const double Ml = (double)rs.M;
   double dS = 0.0, dE = 0.0;
-  for (int c = lane; c < n_c; c += 32) {
+  for (int c = c_0 + lane; c < n_z; c += 32) {
     if (!(approx[c] > -INFINITY)) continue;
     const double xe = z64[c] * log2e - Ml, xa = (double)approx[c] * (double)a.lg - Ml;
     // 2^xe - 2^xa = 2^xa (2^(xe - xa) - 1), without the cancellation
@@ -1356,14 +1542,14 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   const double S = rs.S + dS, E = rs.E + dE;
   const double lnS = log(S), lse = Ml * ln2 + lnS;
   if (tid == 0) {
-    if (a.logprob) a.logprob[t] = have_tok ? (float)(z64[n_c] - lse) : nan;
+    if (a.logprob) a.logprob[t] = have_tok ? (float)(z64[0] - lse) : nan;
     if (a.entropy) a.entropy[t] = (float)fmax(0.0, lnS - ln2 * E / S);
   }
-  for (int c = tid; c < n_c && a.top_k > 0; c += kThreads) {
+  for (int c = c_0 + tid; c < n_c && a.top_k > 0; c += kThreads) {
     int rank = ranks[c];
     if (rank < 0) {
       rank = 0;
-      for (int q = 0; q < n_c; ++q)
+      for (int q = c_0; q < n_c; ++q)
         rank += z64[q] > z64[c] || (z64[q] == z64[c] && ids[q] < ids[c]);
     }
     if (rank < a.top_k) {
@@ -1401,10 +1587,11 @@ struct DistillArgs {
 // possible term, summed with integer atomics, so that the order in which
 // positions meet an id does not change the result.
 template <bool kGrads, int TW>
-static __global__ void __launch_bounds__(32 * kRowWarps, 3) lh_distill_rows(DistillArgs a) {
+static __global__ void __launch_bounds__(32 * kRowWarps, TW == 1 ? 3 : 2)
+    lh_distill_rows(DistillArgs a) {
   constexpr int kTeams = kRowWarps / TW, kThreads = 32 * TW;
   constexpr int kPer = (kMaxTop + kThreads - 1) / kThreads;
-  __shared__ double s_red[kTeams][2 * kRowWarps];
+  __shared__ double s_red[kTeams][4 * TW];
   __shared__ int s_n[kTeams];
   __shared__ int s_id[kTeams][kMaxTop];
   __shared__ float s_q[kTeams][kMaxTop];
@@ -1498,9 +1685,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps, 3) lh_distill_rows(Dist
   team.sync();
   const int n = base;
   double loss = 0.0;
-  for (int c = 16 * team.w; c < n; c += 16 * TW)
-    logits16<true>(a.z, t, s_id[no] + c, min(16, n - c), lane, s_z[no] + c);
-  team.sync();
+  team_logits<TW>(a.z, t, s_id[no], n, team, s_z[no], s_Q[no]);
   for (int k = tid; k < n; k += kThreads) {
     const double l = s_lq[no][k];
     loss += exp(l) * (l - s_z[no][k] / (double)a.tau);
@@ -1537,7 +1722,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps, 3) lh_distill_rows(Dist
     const int sl = tid / RL;
     for (int j = tid % RL; j < R; j += RL) {
       double Q = 0.0;
-#pragma unroll 2
+#pragma unroll 4
       for (int k = sl; k < nslot; k += ns) {
         const long long o = (long long)k * a.p.ld + t;
         const float pm = a.p.p_max[o], pq = a.p.p_q[o * R + j];
@@ -1546,12 +1731,30 @@ static __global__ void __launch_bounds__(32 * kRowWarps, 3) lh_distill_rows(Dist
       Q *= xb;
       const double su = (double)a.z.sU[(long long)t * R + j] * (double)wt * fx;
       const bool scatter = j < a.z.r && wt != 0.f && isfinite(su);
-      for (int k = sl; k < n; k += ns) {
-        const int v = s_id[no][k];
-        const float qk = s_q[no][k];
-        const long long o = (long long)v * R + j;
-        Q -= (double)(qk * a.Bt[a.Bt_plain ? o : bidx(v, j, R)]);
-        if (scatter) atomicAdd(&a.corr[o], (unsigned long long)__double2ll_rn(su * (double)qk));
+      // eight entries' rows of B at a time on the way: a load does not pass an
+      // atomic, and one by one each would wait for the L2
+      for (int k0 = sl; k0 < n; k0 += 8 * ns) {
+        float b[8];
+#pragma unroll
+        for (int e8 = 0; e8 < 8; ++e8) {
+          const int k = k0 + e8 * ns;
+          b[e8] = 0.f;
+          if (k < n) {
+            const int v = s_id[no][k];
+            b[e8] = a.Bt[a.Bt_plain ? (long long)v * R + j : bidx(v, j, R)];
+          }
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int e8 = 0; e8 < 8; ++e8) {
+          const int k = k0 + e8 * ns;
+          if (k >= n) continue;
+          const float qk = s_q[no][k];
+          Q -= (double)(qk * b[e8]);
+          if (scatter)
+            atomicAdd(&a.corr[(long long)s_id[no][k] * R + j],
+                      (unsigned long long)__double2ll_rn(su * (double)qk));
+        }
       }
       if constexpr (TW == 1) {
         for (int off = RL; off < 32; off <<= 1) Q += __shfl_xor_sync(0xffffffffu, Q, off);
