@@ -312,6 +312,16 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
     active = wt != 0.f;
     if (tid == 0) a.wt[t] = wt;
   }
+  const int j = R ? tid % R : 0, sl = R ? tid / R : 0, ns = R ? 256 / R : 1;
+  float av[16];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const int i = i0 + q * ns;
+      av[q] = i < a.d && j < a.r ? a.A[(long long)i * a.lda + j] : 0.f;
+    }
+  };
+  fetch(sl);  // on its way beside h
   for (int i = 2 * tid; i < a.d; i += 512) {
     const float2 x = active ? load_pair(a, t, i) : make_float2(0.f, 0.f);
     const __half2 hv = __floats2half2_rn(x.x, x.y);
@@ -319,22 +329,14 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
     *reinterpret_cast<float2*>(sh + i) = __half22float2(hv);
   }
   if (R == 0) return;
-  const int j = tid % R, sl = tid / R, ns = 256 / R;
   float u = 0.f;
   __syncthreads();
-  if (j < a.r) {
-    float av[16];
-    for (int i0 = sl; i0 < a.d; i0 += 16 * ns) {
+  for (int i0 = sl; i0 < a.d; i0 += 16 * ns) {
+    if (i0 != sl) fetch(i0);
 #pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const int i = i0 + q * ns;
-        av[q] = i < a.d ? a.A[(long long)i * a.lda + j] : 0.f;
-      }
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const int i = i0 + q * ns;
-        if (i < a.d) u = fmaf(sh[i], av[q], u);
-      }
+    for (int q = 0; q < 16; ++q) {
+      const int i = i0 + q * ns;
+      if (i < a.d) u = fmaf(sh[i], av[q], u);
     }
   }
   red[tid] = u;
@@ -849,10 +851,11 @@ struct SlotPlan {
   const float* p_sum;
   const float* p_ent;
   const float* p_q;
-  __device__ __forceinline__ int slots(int t) const {
+  __device__ __forceinline__ int slots(int t) const { return slots_of(t / (2 * kBM)); }
+  __device__ __forceinline__ int slots_of(int ab) const {
     // tile_owner in 32 bits: at most 4096 x 2048 tiles, 148 units (few positions:
     // 4096 of each)
-    const unsigned first = (unsigned)(t / (2 * kBM)) * n_b, total = (unsigned)n_a * n_b;
+    const unsigned first = (unsigned)ab * n_b, total = (unsigned)n_a * n_b;
     const unsigned G = min(total, (unsigned)units);
     const unsigned s0 = ((first + 1) * G - 1) / total, s1 = ((first + n_b) * G - 1) / total;
     return cparts * (int)(s1 - s0 + 1);
@@ -1041,14 +1044,20 @@ static __global__ void __launch_bounds__(256, 3) lh_score_few(FewArgs a) {
   if (a.r > 0) {  // thread: one vocab row, every other position
     const int i = tid & (kFewRows - 1), t0 = tid / kFewRows, v = min(v0 + i, a.V - 1);
     float s[4 * NT] = {};
-    for (int j = 0; j < a.r; j += 4) {  // R is a multiple of 4, s U of the rest is 0
-      float b[4];
+    constexpr int kRanks = NT == 4 ? 8 : 16;  // of B in flight
+    for (int j0 = 0; j0 < a.r; j0 += kRanks) {
+      float b[kRanks];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) b[e] = j + e < a.r ? a.B.at(j + e, v) : 0.f;
+      for (int e = 0; e < kRanks; ++e) b[e] = j0 + e < a.r ? a.B.at(j0 + e, v) : 0.f;
+      asm volatile("" ::: "memory");
 #pragma unroll
-      for (int n = 0; n < 4 * NT; ++n) {
-        const float4 u = *reinterpret_cast<const float4*>(su + (2 * n + t0) * a.R + j);
-        s[n] = fmaf(u.x, b[0], fmaf(u.y, b[1], fmaf(u.z, b[2], fmaf(u.w, b[3], s[n]))));
+      for (int e = 0; e < kRanks; e += 4) {  // R is a multiple of 4, s U of the rest is 0
+        if (j0 + e >= a.r) break;
+#pragma unroll
+        for (int n = 0; n < 4 * NT; ++n) {
+          const float4 u = *reinterpret_cast<const float4*>(su + (2 * n + t0) * a.R + j0 + e);
+          s[n] = fmaf(u.x, b[e], fmaf(u.y, b[e + 1], fmaf(u.z, b[e + 2], fmaf(u.w, b[e + 3], s[n]))));
+        }
       }
     }
 #pragma unroll
@@ -1903,15 +1912,20 @@ static __global__ void __launch_bounds__(256) lh_grads(GradArgs a) {
   const long long v0 = (long long)blk * kPackRows, stride = a.Vpad * a.R;
   int slots = 0;
   if (v0 < a.V) {
-    const long long total2 = (long long)((a.V + a.res_rows - 1) / a.res_rows) * a.n_b2;
-    const long long at = v0 / a.res_rows * a.n_b2;
-    slots = a.cparts * (tile_owner(at + a.n_b2 - 1, total2, a.G2) - tile_owner(at, total2, a.G2) + 1);
+    const SlotPlan p{a.cparts, (a.V + a.res_rows - 1) / a.res_rows, a.n_b2, a.G2};
+    slots = p.slots_of((int)v0 / a.res_rows);
   }
   constexpr int ld = kPackRows + 1;
-  const int n = kPackRows * a.R;  // 256 to 4096
+  const int n = kPackRows * a.R, lr = __ffs(a.R) - 1;  // 256 to 4096
   const float* src = a.gBp + v0 * a.R;
   for (int k0 = tid; k0 < n; k0 += 4 * 256) {
     double s[4] = {0.0, 0.0, 0.0, 0.0};
+    long long c[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = k0 + 256 * e, i = 2 * (k >> (lr + 1)) + (k & 1), j = (k & (2 * a.R - 1)) >> 1;
+      c[e] = k < n ? (long long)a.corr[(v0 + i) * a.R + j] : 0;
+    }
 #pragma unroll 4
     for (int q = 0; q < slots; ++q)
 #pragma unroll
@@ -1919,23 +1933,14 @@ static __global__ void __launch_bounds__(256) lh_grads(GradArgs a) {
         if (k0 + 256 * e < n) s[e] += (double)src[q * stride + k0 + 256 * e];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int k = k0 + 256 * e, i = 2 * (k / (2 * a.R)) + (k & 1), j = k % (2 * a.R) / 2;
-      if (k < n) tile[j * ld + i] = v0 + i < a.V ? (float)(s[e] * ex) : 0.f;
-    }
-  }
-  __syncthreads();
-#pragma unroll 4
-  for (int k = tid; k < n; k += 256) {
-    const long long c = (long long)a.corr[v0 * a.R + k];
-    if (c != 0) {
-      float& x = tile[k % a.R * ld + k / a.R];
-      x = (float)((double)x - (double)c * fx);
+      const int k = k0 + 256 * e, i = 2 * (k >> (lr + 1)) + (k & 1), j = (k & (2 * a.R - 1)) >> 1;
+      if (k < n) tile[j * ld + i] = v0 + i < a.V ? (float)(s[e] * ex - (double)c[e] * fx) : 0.f;
     }
   }
   __syncthreads();
   if (a.layout) {
     for (int k = tid; k < n; k += 256)
-      a.gB[v0 * a.R + k] = bad ? nan : tile[k % (2 * a.R) / 2 * ld + 2 * (k / (2 * a.R)) + (k & 1)];
+      a.gB[v0 * a.R + k] = bad ? nan : tile[((k & (2 * a.R - 1)) >> 1) * ld + 2 * (k >> (lr + 1)) + (k & 1)];
   } else {
     for (int k = tid; k < a.r * kPackRows; k += 256) {
       const int j = k / kPackRows, i = k % kPackRows;
