@@ -276,11 +276,44 @@ int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_block
   return 0;
 }
 
-// The pass for few positions, one slot per 128 vocab rows; where records have 64
-// columns and the positions fit.
+// The pass for few positions, one slot per 128 vocab rows.  Its time grows with
+// positions and ranks, that of the tensor-core passes does not.  V = 49152, d = 576,
+// whole calls in us, L2 flushed, at 8 / 16 / 24 / 32 positions: scoring (8
+// alternatives) rank 4 41 / 41 / 45 / 49 against 53 / 51 / 51 / 49, rank 16 43 / 45 /
+// 51 / 55 against 55 / 53 / 53 / 51, rank 64 51 / 57 / 76 / 82 against 70 / 68 / 68 /
+// 66; distillation with gradients, at 8 / 16 / 32, rank 4 51 / 55 / 70 against 82,
+// rank 16 65 / 72 / 92 against 112, rank 64 123 / 139 / 211 against 172 (its own
+// forward and backward passes and no partial gradients, so a higher limit).
+// Scoring: where records have 64 columns.
 constexpr int kFewMax = 32;
-bool few_positions(int T, int sub) { return T <= kFewMax && sub == 64; }
+bool few_score(int T, int R, int sub) { return T <= (R <= 16 ? 24 : 16) && sub == 64; }
+bool few_distill(int T, int R) { return T <= (R <= 16 ? kFewMax : 16); }
 int few_blocks(int V) { return (V + kFewRows - 1) / kFewRows; }
+
+FewArgs few_args(const HeadCore& hd, int R, int T, const __half* h16, const float* sU, float lg) {
+  FewArgs f{};
+  f.W = hd.W;
+  f.h16 = h16;
+  f.sU = sU;
+  f.B = BView{hd.B, hd.V, hd.r, R, hd.layout};
+  f.T = T;
+  f.V = hd.V;
+  f.d = hd.d;
+  f.r = hd.r;
+  f.R = R;
+  f.lg = lg;
+  f.ld = round_up(T, 8);
+  return f;
+}
+
+template <int kMode>
+bool launch_few(const FewArgs& f, int blocks, cudaStream_t st) {
+  const int nt = (f.T + 7) / 8, NT = nt <= 2 ? nt : 4;
+  void (*kern)(FewArgs) = NT == 1 ? lh_few<1, kMode> : NT == 2 ? lh_few<2, kMode> : lh_few<4, kMode>;
+  const size_t smem = few_smem(NT, f.d, f.R);
+  return allow_smem(reinterpret_cast<const void*>(kern), smem) &&
+         launch_after(kern, blocks, 256, smem, st, f);
+}
 
 struct ScoreWs {
   int* stats;
@@ -298,7 +331,7 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
   const long long Vpad = round_up(hd.V, kBN);
   const int n_a = (T + 2 * kBM - 1) / (2 * kBM), n_b = (int)(Vpad / kBN);
   w.sub = record_columns(hd.V, top_k);
-  const size_t part = few_positions(T, w.sub)
+  const size_t part = few_score(T, aug.R, w.sub)
                           ? (size_t)few_blocks(hd.V) * kFewMax
                           : (size_t)4 * most_segments(n_a, n_b) * n_a * 2 * kBM;
   w.n_sub = (hd.V + w.sub - 1) / w.sub;
@@ -323,7 +356,8 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
 struct DistillWs {
   int* stats;
   __half *h16, *haug, *waug, *xv, *xt;
-  float *sU, *wt, *p_max, *p_sum, *p_q, *tok, *Bt, *nml, *xs, *dU, *gAp, *gBp, *Ap;
+  float *sU, *wt, *p_max, *p_sum, *p_q, *tok, *Bt, *nml, *xs, *dU, *gAp, *gBp;
+  float2* ref;
   unsigned long long* corr;
   size_t zero_bytes;  // stats and corr: cleared by every call
   size_t bytes;
@@ -345,6 +379,16 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
   w.h16 = c.take<__half>((size_t)T * hd.d);
   w.sU = c.take<float>((size_t)T * R);
   w.wt = c.take<float>(T);
+  if (few_distill(T, R)) {
+    const size_t slots = (size_t)few_blocks(hd.V) * round_up(T, 8);
+    w.p_max = c.take<float>(slots);
+    w.p_sum = c.take<float>(slots);
+    w.p_q = c.take<float>(grads ? slots * R : 0);
+    w.ref = c.take<float2>(T);
+    w.dU = c.take<float>((size_t)T * R);
+    w.bytes = c.off;
+    return w;
+  }
   // rank 4 keeps the rank term in the epilogues of the gradient passes
   const bool in_mma = !grads || R > 4;
   w.haug = c.take<__half>(in_mma ? (size_t)T * aug.width : 0);
@@ -561,7 +605,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
                    float* top_logprobs, void* ws, cudaStream_t st, const char** why) {
   Aug aug = aug_of(hd.r);
   const ScoreWs w = score_ws(hd, T, top_k, ws);
-  const bool few = few_positions(T, w.sub);
+  const bool few = few_score(T, aug.R, w.sub);
   if (few) aug.layout = aug.width = 0;  // the rank term from B as it is
   const int sms = sm_count();
   GemmArgs g{};
@@ -612,17 +656,20 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
 
   if (few) {
     if (launch_prep(pa, pk, true, 0, false, sms, st)) return *why = kNoFit, LORA_CE_ECUDA;
-    const int nt = (T + 7) / 8, blocks = few_blocks(hd.V);
-    void (*kern)(FewArgs) = nt == 1 ? lh_score_few<1> : nt == 2 ? lh_score_few<2> : lh_score_few<4>;
-    const size_t smem = few_smem(nt <= 2 ? nt : 4, hd.d, aug.R);
-    if (!allow_smem(reinterpret_cast<const void*>(kern), smem))
-      return *why = kNoFit, LORA_CE_ECUDA;
+    const int blocks = few_blocks(hd.V);
     const float lg = (float)((1.0 + kLoss32) / std::log(2.0));
-    const FewArgs f{hd.W, w.h16, w.sU, pk.B, T, hd.V, hd.d, hd.r, aug.R, lg, kFewMax,
-                    w.p_max, w.p_sum, w.p_ent, w.sub_max, w.sub_second, w.sub_rest,
-                    w.sub_arg, w.sub_arg2, w.n_sub};
-    if (!launch_after(kern, blocks, 256, smem, st, f)) return *why = kNoLaunch, LORA_CE_ECUDA;
-    a.p = SlotPlan{1, 1, blocks, blocks, kFewMax, w.p_max, w.p_sum, w.p_ent, nullptr};
+    FewArgs f = few_args(hd, aug.R, T, w.h16, w.sU, lg);
+    f.p_max = w.p_max;
+    f.p_sum = w.p_sum;
+    f.p_ent = w.p_ent;
+    f.sub_max = w.sub_max;
+    f.sub_second = w.sub_second;
+    f.sub_rest = w.sub_rest;
+    f.sub_arg = w.sub_arg;
+    f.sub_arg2 = w.sub_arg2;
+    f.n_sub = w.n_sub;
+    if (!launch_few<kFewScore>(f, blocks, st)) return *why = kNoLaunch, LORA_CE_ECUDA;
+    a.p = SlotPlan{1, 1, blocks, blocks, f.ld, w.p_max, w.p_sum, w.p_ent, nullptr};
     a.lg = lg;
   } else {
     const PassPlan p = score_plan(g.kblocks, w.sub);
@@ -674,11 +721,11 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   Aug aug = aug_of(hd.r);
   const int R = aug.R;
   const DistillWs w = distill_ws(hd, T, grads, ws);
-  const bool tc = grads && R >= 16;
-  if (grads && R == 4) aug.layout = aug.width = 0;  // the rank term in the epilogues
+  const bool few = few_distill(T, R), tc = grads && R >= 16 && !few;
+  if ((grads && R == 4) || few) aug.layout = aug.width = 0;  // no packed rank term
   Step s{hd, w, aug, T, sm_count(), tau, st, GemmArgs{}, SlotPlan{}};
   fill_pass1(s.g, hd, aug, T, tau);
-  s.Bt = hd.layout ? hd.B : w.Bt;
+  s.Bt = few ? nullptr : hd.layout ? hd.B : w.Bt;
   s.g.err = w.stats + kStErr;
   s.g.p_max = w.p_max;
   s.g.p_sum = w.p_sum;
@@ -700,7 +747,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pa.K = K;
   pa.tau = tau;
   pa.wt = w.wt;
-  if (grads && !tc) {
+  if (grads && !tc && !few) {
     pa.tok = w.tok;
     pa.Tpad = (int)round_up(T, kBN);
   }
@@ -710,7 +757,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pk.r = hd.r;
   pk.R = R;
   pk.Vpad = s.g.Vpad;
-  pk.Bt = grads && !hd.layout ? w.Bt : nullptr;
+  pk.Bt = grads && !few && !hd.layout ? w.Bt : nullptr;
   pk.Bt_plain = tc;  // the rank sums' passes have xv instead
   pk.waug = aug.width ? w.waug : nullptr;
   pk.aug_layout = aug.layout;
@@ -724,7 +771,17 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
     return *why = kNoFit, LORA_CE_ECUDA;
 
   int rc = 0;
-  if (grads) {
+  const float few_lg = (float)((1.0 + kLoss32) / (std::log(2.0) * (double)tau));
+  FewArgs f = few_args(hd, R, T, w.h16, w.sU, few_lg);
+  const int v_blocks = few_blocks(hd.V);
+  if (few) {
+    f.p_max = w.p_max;
+    f.p_sum = w.p_sum;
+    f.p_q = w.p_q;
+    if (!(grads ? launch_few<kFewForward>(f, v_blocks, st) : launch_few<kFewLoss>(f, v_blocks, st)))
+      return *why = kNoLaunch, LORA_CE_ECUDA;
+    s.slots = SlotPlan{1, 1, v_blocks, v_blocks, f.ld, w.p_max, w.p_sum, nullptr, w.p_q};
+  } else if (grads) {
     rc = grad_pass<1>(s, R, why);
   } else {
     const PassPlan p = score_plan(s.g.kblocks, 0);
@@ -752,7 +809,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   a.z.R = R;
   a.z.B.R = R;
   a.p = s.slots;
-  a.lg = s.g.lg;
+  a.lg = few ? few_lg : s.g.lg;
   a.tau = tau;
   a.scale = hd.scale;
   a.K = K;
@@ -763,7 +820,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   a.Bt_plain = pk.Bt && tc;
   a.stats = w.stats;
   a.loss = loss;
-  a.tok = grads && !tc ? w.tok : nullptr;
+  a.tok = grads && !tc && !few ? w.tok : nullptr;
+  a.ref = grads && few ? w.ref : nullptr;
   a.nml = tc ? w.nml : nullptr;
   a.xs = w.xs;
   a.dU = w.dU;
@@ -775,6 +833,24 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
     return *why = kNoLaunch, LORA_CE_ECUDA;
   if (!grads) {
     if (cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
+    return 0;
+  }
+  const int a_blocks = ((out.layout ? R : hd.r) * hd.d + 255) / 256;
+  if (few) {
+    f.ref = w.ref;
+    f.corr = w.corr;
+    f.dU = w.dU;
+    f.stats = w.stats;
+    f.gA = out.gA;
+    f.gB = out.gB;
+    f.layout = out.layout;
+    f.Vpad = s.g.Vpad;
+    f.v_blocks = out.layout ? (int)(s.g.Vpad / kFewRows) : v_blocks;
+    f.loss = loss;
+    f.wt = w.wt;
+    f.tail = out.tail;
+    if (!launch_few<kFewBackward>(f, f.v_blocks + a_blocks, st) ||
+        cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
     return 0;
   }
   if (tc) {
@@ -813,7 +889,6 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   ga.loss = loss;
   ga.wt = w.wt;
   ga.tail = out.tail;
-  const int a_blocks = ((out.layout ? R : hd.r) * hd.d + 255) / 256;
   if (!launch_after(lh_grads, (int)(s.g.Vpad / kPackRows) + a_blocks, 256, 0, st, ga) ||
       cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
   return 0;

@@ -358,7 +358,7 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
 // memory 12 rows at a time, h four elements per load from shared memory, up to 32
 // sums per lane.  (A through shared memory, four sums per thread, a load for each
 // operand of each product and two block barriers per 64 elements: 35 us instead of
-// @@ for 2,047 positions at rank 64.)
+// 21 for 2,047 positions at rank 64, B packed beside them.)
 constexpr int kTileRows = 16;
 template <int R>
 __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem) {
@@ -614,7 +614,7 @@ struct LogitArgs {
 // operands have it), so W is read 16 bytes at a time.
 // kSum64: each 32 products are added up in a fresh accumulator, whose known loss
 // (kLoss32, as acc_short) is small and made good, and go to a 64-bit sum: off by
-// 4.3e-7 (1 + |z|) at most over 524,288 logits at hidden sizes 576 and 64, ranks
+// 5e-7 (1 + |z|) at most over 524,288 logits at hidden sizes 576 and 64, ranks
 // 0, 4 and 64.  About 250 instructions for 16 logits; with every product in 64
 // bits it is 1,600.  Else one f32 accumulator: to compare with a bound.
 constexpr double kLoss32 = 0.79 * 1.5 / 33554432.0 * 1.4426950408889634;
@@ -938,6 +938,7 @@ __device__ __forceinline__ void team_logits(const LogitArgs& a, int t, const int
 }
 
 // ------------------------------------------------------------- few positions
+enum FewMode { kFewScore, kFewLoss, kFewForward, kFewBackward };
 struct FewArgs {
   const __half* W;
   const __half* h16;
@@ -945,23 +946,69 @@ struct FewArgs {
   BView B;
   int T, V, d, r, R;
   float lg;
+  // forward: one slot per block
   long long ld;  // row stride of the partials
   float* p_max;
   float* p_sum;
   float* p_ent;
+  float* p_q;
+  // score: records of 64 columns
   float* sub_max;
   float* sub_second;
   float* sub_rest;
   uint8_t* sub_arg;
   uint8_t* sub_arg2;
   int n_sub;
+  // backward
+  const float2* ref;               // [T] reference max (log2), weight * tau / sum
+  const unsigned long long* corr;  // [Vpad][R], row by row
+  const float* dU;                 // [T][R]
+  const int* stats;
+  int v_blocks;  // the blocks behind them form gA
+  float* gA;
+  float* gB;
+  int layout;
+  long long Vpad;
+  const float* loss;
+  const float* wt;
+  float* tail;
 };
 constexpr int kFewRows = 128;           // vocab rows per block, 16 per warp
 constexpr int kFewLdZ = kFewRows + 4;   // floats per position of the logit tile
 __host__ __device__ constexpr int few_ldh(int d) { return d + 32; }  // f16 per position
-__host__ __device__ inline size_t few_smem(int NT, int d, int R) {
+__host__ __device__ inline size_t few_front(int NT, int d) {
   const size_t h = (size_t)8 * NT * few_ldh(d) * 2, z = (size_t)8 * NT * kFewLdZ * 4;
-  return (h > z ? h : z) + (size_t)8 * NT * R * 4;
+  return h > z ? h : z;
+}
+__host__ __device__ inline size_t few_smem(int NT, int d, int R) {
+  return few_front(NT, d) + (size_t)(8 * NT + kFewLdZ) * R * 4;
+}
+
+// Sum of losses and number of counted positions, by one block of 256.
+__device__ __forceinline__ void put_tail(const float* loss, const float* wt, int T, float* tail) {
+  __shared__ double red[256];
+  __shared__ int cnt[256];
+  const int tid = threadIdx.x;
+  double s = 0.0;
+  int c = 0;
+  for (int t = tid; t < T; t += 256) {
+    s += (double)loss[t];
+    c += wt[t] != 0.f;
+  }
+  red[tid] = s;
+  cnt[tid] = c;
+  __syncthreads();
+  for (int w = 128; w > 0; w >>= 1) {
+    if (tid < w) {
+      red[tid] += red[tid + w];
+      cnt[tid] += cnt[tid + w];
+    }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    tail[0] = (float)red[0];
+    tail[1] = (float)cnt[0];
+  }
 }
 
 // The pass over z for up to 8 NT positions, bound by reading W once: a warp takes
@@ -969,17 +1016,41 @@ __host__ __device__ inline size_t few_smem(int NT, int d, int R) {
 // and the positions as B, from shared memory; every 32 products have their own
 // accumulator (kLoss32).  The rank term from B as it is, so that nothing of the
 // vocabulary's side is packed.  Then the block's logits, in shared memory, give
-// the same partial sums and records as EpiScore<64>, one slot per block.
-template <int NT>
-static __global__ void __launch_bounds__(256, 3) lh_score_few(FewArgs a) {
+//   score: the same partial sums and records as EpiScore<64>, one slot per block;
+//   distill forward: partial sums, and with gradients those of p B^T;
+//   distill backward: gB of the block's rows, whole: all positions are here, so
+//   there are no partial gradients to write and join.  More blocks form gA.
+// The tensor-core passes take 26 and 20 us for 1 to 256 positions (V = 49152, rank
+// 4: three tiles per SM, each with an epilogue over 256 rows), and 10 more to pack
+// B and to join the partial gradients.  This one: 13 us for up to 8 positions, 20 to
+// 25 for 32, by when the mma and their operands' reads from shared memory, once per
+// 16 vocab rows, take as long as W.
+template <int NT, int kMode>
+static __global__ void __launch_bounds__(256, 3) lh_few(FewArgs a) {
   constexpr int kUnroll = 6;
   constexpr unsigned kAll = 0xffffffffu;
   extern __shared__ __align__(16) uint8_t smem_few[];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, c = lane & 3, g = lane >> 2;
   const int ldh = few_ldh(a.d);
+  if (kMode == kFewBackward && (int)blockIdx.x >= a.v_blocks) {
+    grid_wait();
+    const int blk = (int)blockIdx.x - a.v_blocks, ra = a.layout ? a.R : a.r;
+    const int k = blk * 256 + tid;
+    if (k < a.d * ra) {
+      const int i = k / ra, j = k - i * ra;
+      float s = 0.f;
+#pragma unroll 8
+      for (int t = 0; t < a.T; ++t)
+        s = fmaf(__half2float(a.h16[(long long)t * a.d + i]), a.dU[(long long)t * a.R + j], s);
+      a.gA[k] = s;
+    }
+    if (a.tail && blk == 0) put_tail(a.loss, a.wt, a.T, a.tail);
+    return;
+  }
   __half* sh = reinterpret_cast<__half*>(smem_few);
   float* sz = reinterpret_cast<float*>(smem_few);  // over h once that is used up
-  float* su = reinterpret_cast<float*>(smem_few + few_smem(NT, a.d, 0));
+  float* su = reinterpret_cast<float*>(smem_few + few_front(NT, a.d));
+  float* sb = su + 8 * NT * a.R;                   // [R][kFewLdZ]
   const int v0 = (int)blockIdx.x * kFewRows;
   const __half* w0 = a.W + (long long)min(v0 + 16 * w + g, a.V - 1) * a.d + 8 * c;
   const __half* w1 = a.W + (long long)min(v0 + 16 * w + g + 8, a.V - 1) * a.d + 8 * c;
@@ -995,16 +1066,29 @@ static __global__ void __launch_bounds__(256, 3) lh_score_few(FewArgs a) {
       }
     }
   };
-  fetch(0);  // W is the caller's: its reads need not wait for the kernel ahead
+  fetch(0);  // W and B are the caller's: their reads need not wait for the kernel ahead
+  {
+    const int i = tid & (kFewRows - 1);
+    for (int j = tid / kFewRows; j < a.R; j += 2) {
+      const bool in = j < a.r && v0 + i < a.V;
+      const float* src = in ? a.B.p + (a.B.layout ? bidx(v0 + i, j, a.R) : (long long)j * a.V + v0 + i)
+                            : a.B.p;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                       (unsigned)__cvta_generic_to_shared(sb + j * kFewLdZ + i)),
+                   "l"(src), "r"(in ? 4 : 0) : "memory");
+    }
+  }
   grid_wait();
-  grid_launch();
-  for (int k = tid; k < 8 * NT * (a.d / 8); k += 256) {
-    const int t = k / (a.d / 8), i = k % (a.d / 8) * 8;
-    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-    if (t < a.T) x = *reinterpret_cast<const uint4*>(a.h16 + (long long)t * a.d + i);
-    *reinterpret_cast<uint4*>(sh + t * ldh + i) = x;
+  if (kMode != kFewBackward) grid_launch();
+  for (int t = w; t < 8 * NT; t += 8) {
+    for (int i = 8 * lane; i < a.d; i += 256) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (t < a.T) x = *reinterpret_cast<const uint4*>(a.h16 + (long long)t * a.d + i);
+      *reinterpret_cast<uint4*>(sh + t * ldh + i) = x;
+    }
   }
   for (int k = tid; k < 8 * NT * a.R; k += 256) su[k] = k < a.T * a.R ? a.sU[k] : 0.f;
+  asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
   float z[NT][4] = {};
   for (int k0 = 0; k0 < a.d; k0 += 32 * kUnroll) {
@@ -1015,17 +1099,17 @@ static __global__ void __launch_bounds__(256, 3) lh_score_few(FewArgs a) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const uint4 x = *reinterpret_cast<const uint4*>(sh + (8 * n + g) * ldh + k + 8 * c);
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          auto mma = [&](unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
-                         unsigned b1) {
-            asm volatile(
-                "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
-                "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-          };
-          mma(p[i].x, q[i].x, p[i].y, q[i].y, x.x, x.y);
-          mma(p[i].z, q[i].z, p[i].w, q[i].w, x.z, x.w);
+          float d[4];
+          asm volatile(
+              "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+              "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+              : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+              : "r"(p[i].x), "r"(q[i].x), "r"(p[i].y), "r"(q[i].y), "r"(x.x), "r"(x.y), "f"(0.f));
+          asm volatile(
+              "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+              "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+              : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+              : "r"(p[i].z), "r"(q[i].z), "r"(p[i].w), "r"(q[i].w), "r"(x.z), "r"(x.w));
 #pragma unroll
           for (int e = 0; e < 4; ++e) z[n][e] += d[e];
         }
@@ -1041,82 +1125,138 @@ static __global__ void __launch_bounds__(256, 3) lh_score_few(FewArgs a) {
     for (int e = 0; e < 4; ++e)
       sz[(8 * n + 2 * c + (e & 1)) * kFewLdZ + 16 * w + g + 8 * (e >> 1)] = z[n][e];
   __syncthreads();
+  const int vi = tid & (kFewRows - 1), t0 = tid / kFewRows;
   if (a.r > 0) {  // thread: one vocab row, every other position
-    const int i = tid & (kFewRows - 1), t0 = tid / kFewRows, v = min(v0 + i, a.V - 1);
     float s[4 * NT] = {};
-    constexpr int kRanks = NT == 4 ? 8 : 16;  // of B in flight
-    for (int j0 = 0; j0 < a.r; j0 += kRanks) {
-      float b[kRanks];
+    for (int j = 0; j < a.r; j += 4) {  // R is a multiple of 4, the rest is 0
+      float b[4];
 #pragma unroll
-      for (int e = 0; e < kRanks; ++e) b[e] = j0 + e < a.r ? a.B.at(j0 + e, v) : 0.f;
-      asm volatile("" ::: "memory");
+      for (int e = 0; e < 4; ++e) b[e] = sb[(j + e) * kFewLdZ + vi];
 #pragma unroll
-      for (int e = 0; e < kRanks; e += 4) {  // R is a multiple of 4, s U of the rest is 0
-        if (j0 + e >= a.r) break;
+      for (int n = 0; n < 4 * NT; ++n) {
+        const float4 u = *reinterpret_cast<const float4*>(su + (2 * n + t0) * a.R + j);
+        s[n] = fmaf(u.x, b[0], fmaf(u.y, b[1], fmaf(u.z, b[2], fmaf(u.w, b[3], s[n]))));
+      }
+    }
 #pragma unroll
-        for (int n = 0; n < 4 * NT; ++n) {
-          const float4 u = *reinterpret_cast<const float4*>(su + (2 * n + t0) * a.R + j0 + e);
-          s[n] = fmaf(u.x, b[e], fmaf(u.y, b[e + 1], fmaf(u.z, b[e + 2], fmaf(u.w, b[e + 3], s[n]))));
+    for (int n = 0; n < 4 * NT; ++n) sz[(2 * n + t0) * kFewLdZ + vi] += s[n];
+    __syncthreads();
+  }
+  if constexpr (kMode == kFewBackward) {
+    // dz = p weight tau, then gB = dz^T (scale U) over all positions, less the
+    // entries' part
+    for (int t = w; t < 8 * NT; t += 8) {
+      const float2 ref = t < a.T ? a.ref[t] : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float& x = sz[t * kFewLdZ + lane + 32 * i];
+        x = ref.y == 0.f ? 0.f : ex2f(fmaxf(fmaf(x, a.lg, -ref.x), -1e30f)) * ref.y;
+      }
+    }
+    __syncthreads();
+    const double fx = exp2i(-scale_exp(a.stats[kStUMax], 37));
+    const int v = v0 + vi, T = a.T;
+    for (int j = 4 * t0; j < a.R; j += 8) {
+      float s[4] = {};
+      unsigned long long sparse[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sparse[e] = v < a.V ? a.corr[(long long)v * a.R + j + e] : 0ull;
+#pragma unroll 4
+      for (int t = 0; t < T; ++t) {
+        const float x = sz[t * kFewLdZ + vi];
+        const float4 u = *reinterpret_cast<const float4*>(su + t * a.R + j);
+        s[0] = fmaf(x, u.x, s[0]);
+        s[1] = fmaf(x, u.y, s[1]);
+        s[2] = fmaf(x, u.z, s[2]);
+        s[3] = fmaf(x, u.w, s[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = (float)((double)s[e] - (double)(long long)sparse[e] * fx);
+        if (a.layout) {
+          if (v < a.Vpad) a.gB[bidx(v, j + e, a.R)] = v < a.V ? x : 0.f;
+        } else if (j + e < a.r && v < a.V) {
+          a.gB[(long long)(j + e) * a.V + v] = x;
         }
       }
     }
-#pragma unroll
-    for (int n = 0; n < 4 * NT; ++n) sz[(2 * n + t0) * kFewLdZ + i] += s[n];
-    __syncthreads();
-  }
-  // a warp per position: partial sums of the block's rows, two records
-  for (int t = w; t < a.T; t += 8) {
-    float x[4];
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = v0 + lane + 32 * i < a.V ? sz[t * kFewLdZ + lane + 32 * i] : -INFINITY;
-      m = fmaxf(m, x[i]);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, off));
-    const float mL = m * a.lg;
-    float S = 0.f, E = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float y = fmaxf(fmaf(x[i], a.lg, -mL), -1e30f), e = ex2f(y);
-      S += e;
-      E = fmaf(e, y, E);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      S += __shfl_xor_sync(kAll, S, off);
-      E += __shfl_xor_sync(kAll, E, off);
-    }
-    if (lane == 0) {
-      const long long o = (long long)blockIdx.x * a.ld + t;
-      a.p_max[o] = mL;
-      a.p_sum[o] = S;
-      a.p_ent[o] = E;
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int rec = v0 / 64 + half;
-      if (rec >= a.n_sub) break;
-      // the three largest, equal ones by column: columns lane and lane + 32
-      unsigned k0 = order_key(x[2 * half]), k1 = order_key(x[2 * half + 1]);
-      unsigned top[3];
-      int at[3];
-#pragma unroll
-      for (int q3 = 0; q3 < 3; ++q3) {
-        top[q3] = __reduce_max_sync(kAll, max(k0, k1));
-        at[q3] = (int)__reduce_min_sync(kAll, k0 == top[q3]   ? (unsigned)lane
-                                              : k1 == top[q3] ? (unsigned)lane + 32u : 64u);
-        if (at[q3] == lane) k0 = 0u;
-        if (at[q3] == lane + 32) k1 = 0u;
+  } else {
+    // a warp per position: partial sums of the block's rows; score: two records
+    for (int t = w; t < a.T; t += 8) {
+      float x[4];
+      float m = -INFINITY;
+  #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = v0 + lane + 32 * i < a.V ? sz[t * kFewLdZ + lane + 32 * i] : -INFINITY;
+        m = fmaxf(m, x[i]);
+      }
+  #pragma unroll
+      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, off));
+      const float mL = m * a.lg;
+      float S = 0.f, E = 0.f;
+  #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = fmaxf(fmaf(x[i], a.lg, -mL), -1e30f), e = ex2f(y);
+        S += e;
+        if (kMode == kFewScore) E = fmaf(e, y, E);
+        if (kMode == kFewForward) sz[t * kFewLdZ + lane + 32 * i] = e;
+      }
+  #pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        S += __shfl_xor_sync(kAll, S, off);
+        if (kMode == kFewScore) E += __shfl_xor_sync(kAll, E, off);
       }
       if (lane == 0) {
-        const long long o = sub_idx(t, rec, a.n_sub);
-        a.sub_max[o] = key_float(top[0]);
-        a.sub_second[o] = key_float(top[1]);
-        a.sub_rest[o] = key_float(top[2]);
-        a.sub_arg[o] = (uint8_t)at[0];
-        a.sub_arg2[o] = (uint8_t)at[1];
+        const long long o = (long long)blockIdx.x * a.ld + t;
+        a.p_max[o] = mL;
+        a.p_sum[o] = S;
+        if (kMode == kFewScore) a.p_ent[o] = E;
+      }
+      if constexpr (kMode == kFewScore) {
+  #pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int rec = v0 / 64 + half;
+          if (rec >= a.n_sub) break;
+          // the three largest, equal ones by column: columns lane and lane + 32
+          unsigned k0 = order_key(x[2 * half]), k1 = order_key(x[2 * half + 1]);
+          unsigned top[3];
+          int at[3];
+  #pragma unroll
+          for (int q3 = 0; q3 < 3; ++q3) {
+            top[q3] = __reduce_max_sync(kAll, max(k0, k1));
+            at[q3] = (int)__reduce_min_sync(kAll, k0 == top[q3]   ? (unsigned)lane
+                                                  : k1 == top[q3] ? (unsigned)lane + 32u : 64u);
+            if (at[q3] == lane) k0 = 0u;
+            if (at[q3] == lane + 32) k1 = 0u;
+          }
+          if (lane == 0) {
+            const long long o = sub_idx(t, rec, a.n_sub);
+            a.sub_max[o] = key_float(top[0]);
+            a.sub_second[o] = key_float(top[1]);
+            a.sub_rest[o] = key_float(top[2]);
+            a.sub_arg[o] = (uint8_t)at[0];
+            a.sub_arg2[o] = (uint8_t)at[1];
+          }
+        }
+      }
+    }
+    if constexpr (kMode == kFewForward) {  // sum of e B[j] for each position and rank
+      __syncthreads();
+      for (int k = tid; k < a.T * a.R; k += 256) {
+        const int t = k / a.R, j = k & (a.R - 1);
+        const float4* x = reinterpret_cast<const float4*>(sz + t * kFewLdZ);
+        const float4* b = reinterpret_cast<const float4*>(sb + j * kFewLdZ);
+        float s[4] = {};
+  #pragma unroll 8
+        for (int i = 0; i < kFewRows / 4; ++i) {
+          const float4 e = x[i], y = b[i];
+          s[0] = fmaf(e.x, y.x, s[0]);
+          s[1] = fmaf(e.y, y.y, s[1]);
+          s[2] = fmaf(e.z, y.z, s[2]);
+          s[3] = fmaf(e.w, y.w, s[3]);
+        }
+        a.p_q[((long long)blockIdx.x * a.ld + t) * a.R + j] = (s[0] + s[1]) + (s[2] + s[3]);
       }
     }
   }
@@ -1577,12 +1717,13 @@ struct DistillArgs {
   const int32_t* ids;
   const float* teacher;
   float* wt;      // in: weight * tau of rows with entries; out: 0 where none counts
-  const float* Bt;  // [Vpad][R] (gradients): bidx layout, or row by row
+  const float* Bt;  // [Vpad][R] (gradients): bidx layout, or row by row; null: z.B
   int Bt_plain;
   const int* stats;
   float* loss;
   // gradients
   float* tok;     // records of ranks 4, 8
+  float2* ref;    // few positions
   float* nml;     // tensor-core rank sums: exponent offsets, factors of the rank operand
   float* xs;
   float* dU;      // [T][R]
@@ -1712,6 +1853,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps, TW == 1 ? 3 : 2)
         a.tok[tidx(t, R, R)] = -rs.M;
         a.tok[tidx(t, R + 1, R)] = wt == 0.f ? 0.f : wt * inv;
       }
+      if (a.ref) a.ref[t] = make_float2(rs.M, wt == 0.f ? 0.f : wt * inv);
       if (a.nml) {
         // p = 2^(z lg + nml - 14) xs: the exponent's share of 1 / S is a whole
         // power of two and what rounding takes from nml goes into xs, so that a
@@ -1740,6 +1882,10 @@ static __global__ void __launch_bounds__(32 * kRowWarps, TW == 1 ? 3 : 2)
       Q *= xb;
       const double su = (double)a.z.sU[(long long)t * R + j] * (double)wt * fx;
       const bool scatter = j < a.z.r && wt != 0.f && isfinite(su);
+      const bool pairs = a.Bt ? !a.Bt_plain : a.z.B.layout != 0;
+      const long long bs = a.Bt ? R : 1;
+      const float* bp = a.Bt ? a.Bt + (pairs ? 0 : j) : a.z.B.p + (pairs ? 0 : (long long)j * a.z.V);
+      if (!a.Bt && j >= a.z.r) bp = nullptr;
       // eight entries' rows of B at a time on the way: a load does not pass an
       // atomic, and one by one each would wait for the L2
       for (int k0 = sl; k0 < n; k0 += 8 * ns) {
@@ -1748,9 +1894,9 @@ static __global__ void __launch_bounds__(32 * kRowWarps, TW == 1 ? 3 : 2)
         for (int e8 = 0; e8 < 8; ++e8) {
           const int k = k0 + e8 * ns;
           b[e8] = 0.f;
-          if (k < n) {
+          if (k < n && bp) {
             const int v = s_id[no][k];
-            b[e8] = a.Bt[a.Bt_plain ? (long long)v * R + j : bidx(v, j, R)];
+            b[e8] = bp[pairs ? bidx(v, j, R) : (long long)v * bs];
           }
         }
         asm volatile("" ::: "memory");
@@ -1802,7 +1948,7 @@ static __global__ void lh_xt(int T, int R, long long ld, const float* __restrict
 // gAp[c][i][j] = sum over the kDAChunk positions of chunk c of h16[t][i] dU[t][j]:
 // blocks of 64 hidden elements by all R ranks, 64 positions at a time through
 // shared memory with the next 64 in flight.  (lce_dA_partial takes 16 ranks per
-// launch: 50 us at rank 64 and 8,000 positions, this DA_US.)
+// launch: 50 us at rank 64 and 8,000 positions, this 21.)
 template <int R>
 static __global__ void __launch_bounds__(256) lh_dA(int T, int d, const __half* __restrict__ h16,
                                                     const float* __restrict__ dU,
@@ -1947,30 +2093,7 @@ static __global__ void __launch_bounds__(256) lh_grads(GradArgs a) {
       if (v0 + i < a.V) a.gB[(long long)j * a.V + v0 + i] = bad ? nan : tile[j * ld + i];
     }
   }
-  if (a.tail && blk == 0) {
-    __shared__ double red[256];
-    __shared__ int cnt[256];
-    double s = 0.0;
-    int c = 0;
-    for (int t = tid; t < a.T; t += 256) {
-      s += (double)a.loss[t];
-      c += a.wt[t] != 0.f;
-    }
-    red[tid] = s;
-    cnt[tid] = c;
-    __syncthreads();
-    for (int w = 128; w > 0; w >>= 1) {
-      if (tid < w) {
-        red[tid] += red[tid + w];
-        cnt[tid] += cnt[tid + w];
-      }
-      __syncthreads();
-    }
-    if (tid == 0) {
-      a.tail[0] = (float)red[0];
-      a.tail[1] = (float)cnt[0];
-    }
-  }
+  if (a.tail && blk == 0) put_tail(a.loss, a.wt, a.T, a.tail);
 }
 
 // A trainer's step between its gradient sums and the optimizer: the passes' error

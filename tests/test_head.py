@@ -452,6 +452,28 @@ def test_distill_loss_alone(T, V, d, r, K, tau, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("T,V,d,r,K,tau,dtype", [
+    (1, 4099, 128, 64, 20, 1.0, "f16"),
+    (8, 129, 64, 4, 8, 2.0, "bf16"),       # a block of vocabulary rows and one more
+    (9, 20001, 576, 16, 64, 1.0, "bf16"),
+    (16, 1000, 640, 33, 8, 1.0, "f32"),
+    (17, 127, 320, 7, 4, 0.5, "bf16"),
+    (32, 49152, 576, 8, 20, 1.5, "f16"),
+    (40, 3000, 640, 64, 128, 2.0, "bf16"),
+    (47, 2047, 192, 1, 8, 1.0, "f32"),
+    (48, 100000, 64, 16, 8, 1.0, "bf16"),
+    (49, 4099, 128, 16, 8, 1.0, "bf16"),   # the first of the tensor-core passes
+])
+@pytest.mark.parametrize("grads", [True, False])
+def test_distill_of_few_positions(T, V, d, r, K, tau, dtype, grads):
+    p = Problem(T, V, d, r, dtype, seed=2)
+    p.lists(K)
+    if T % 2 == 0:
+        p.weight = p.u(T) * (p.u(T) < 0.7)
+    check_distill(p, tau, grads)
+
+
+@gpu
 @pytest.mark.parametrize("r", [4, 8, 16, 64])
 def test_gradient_is_the_slope_of_the_loss(r):
     """Central differences of the 64-bit loss along a random direction: the
