@@ -155,7 +155,19 @@ struct GemmArgs {
   uint8_t* sub_arg;
   uint8_t* sub_arg2;
   int n_sub;
+  // kDepend, kTemp: positions that count, in front of the others, if only the
+  // device knows how many; null: T.  by_b: they are the streamed operand.
+  const int* active;
+  int by_b;
 };
+
+// Tiles of `tile` positions to run where `active` count, of `all`: not less than
+// give each of G owners one, with `other` tiles of the other operand, nor than a
+// quarter (the fewer they are, the more owners share a row and the more partials a
+// row has).
+__device__ __forceinline__ int active_tiles(int active, int tile, int all, int other, int G) {
+  return max(max((active + tile - 1) / tile, (all + 3) / 4), (G + other - 1) / other);
+}
 
 // Dynamic shared memory: [resident K-blocks | streamed ring (ring bytes) | staged
 // column records (2 x kBN x rec floats, optional) | barriers].
@@ -568,11 +580,9 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
   const int lane = threadIdx.x & 31;
   const uint32_t rank = kPair == 2 ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
-  const long long total = (long long)g.n_a * g.n_b;
+  int n_a = g.n_a, n_b = g.n_b;
   const int G = gridDim.x / kPair;              // tile-range owners (CTAs or pairs)
   const int unit = blockIdx.x / kPair;
-  const long long x_begin = tile_start(unit, total, G);
-  const long long x_end = tile_start(unit + 1, total, G);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSt; ++i) {
@@ -614,7 +624,14 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
   const uint32_t tmem_base = *tmem_slot;
   if constexpr (Epi::kDepend) {  // set up beside the end of the kernel ahead
     grid_wait();
+    if (g.active) {
+      if (g.by_b) n_b = active_tiles(*g.active, kBN, n_b, n_a, G);
+      else n_a = active_tiles(*g.active, kResRows, n_a, n_b, G);
+    }
   }
+  const long long total = (long long)n_a * n_b;
+  const long long x_begin = tile_start(unit, total, G);
+  const long long x_end = tile_start(unit + 1, total, G);
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)
@@ -627,8 +644,8 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
       for (int i = 0; i < kMaxStages; ++i) issued_parity[i] = -1;
       bool ok = true;
       for (long long x = x_begin; x < x_end && ok; ++x) {
-        const int a = (int)(x / g.n_b);
-        const int b = (int)(x % g.n_b);
+        const int a = (int)(x / n_b);
+        const int b = (int)(x % n_b);
         if (a != cur_a) {
           if (a_uses > 0 &&
               !mbar_wait(&bars[kBarAEmpty], (a_uses - 1) & 1, g.err, kErrWaitProducer)) {
@@ -693,7 +710,7 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
       long long li = 0;
       bool ok = true;
       for (long long x = x_begin; x < x_end && ok; ++x, ++li) {
-        const int a = (int)(x / g.n_b);
+        const int a = (int)(x / n_b);
         if (a != cur_a) {
           if (!mbar_wait(&bars[kBarAFull], a_uses & 1, g.err, kErrWaitMma)) break;
           ++a_uses;
@@ -761,7 +778,7 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
           for (int i = 0; i < n_str_aug; ++i) release(aug_stage[i]);
         }
         if (!ok) break;
-        const bool last_of_a = x + 1 == x_end || (int)((x + 1) / g.n_b) != a;
+        const bool last_of_a = x + 1 == x_end || (int)((x + 1) / n_b) != a;
         if constexpr (kPair == 2) {
           umma_commit_pair(&bars[kBarAccFull + buf], 0x3);
           if (last_of_a) umma_commit_pair(&bars[kBarAEmpty], 0x3);
@@ -792,11 +809,11 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
     long long li = 0;
     bool failed = false;
     for (long long x = x_begin; x < x_end; ++x, ++li) {
-      const int a = (int)(x / g.n_b);
-      const int b = (int)(x % g.n_b);
+      const int a = (int)(x / n_b);
+      const int b = (int)(x % n_b);
       if (a != cur_a) {
         if (cur_a >= 0 && !failed)
-          epi.flush(g, kColParts * (unit - tile_owner((long long)cur_a * g.n_b, total, G)) + half);
+          epi.flush(g, kColParts * (unit - tile_owner((long long)cur_a * n_b, total, G)) + half);
         epi.begin(g, (g.a0 + a) * kResRows + (int)rank * kBM + row);
         cur_a = a;
       }
@@ -861,7 +878,7 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
       }
     }
     if (cur_a >= 0 && !failed)
-      epi.flush(g, kColParts * (unit - tile_owner((long long)cur_a * g.n_b, total, G)) + half);
+      epi.flush(g, kColParts * (unit - tile_owner((long long)cur_a * n_b, total, G)) + half);
   } else if (warp == kRecWarp) {
     // ------------------------------------------------ record loader (both CTAs)
     // The records of tile li (256 columns, one contiguous block in global)
@@ -871,7 +888,7 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
       long long li = 0;
       int issued = 0;
       for (long long x = x_begin; x < x_end; ++x, ++li) {
-        const int b = (int)(x % g.n_b);
+        const int b = (int)(x % n_b);
         const int buf = (int)(li % kRB);
         const uint32_t use = (uint32_t)(li / kRB);
         if (use > 0 &&

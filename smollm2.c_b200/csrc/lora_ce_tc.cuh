@@ -215,11 +215,9 @@ __global__ void __launch_bounds__(kThreadsT, 1)
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  const long long total = (long long)g.n_a * g.n_b;
+  int n_a = g.n_a, n_b = g.n_b;
   const int G = gridDim.x / 2;
   const int unit = blockIdx.x / 2;
-  const long long x_begin = tile_start(unit, total, G);
-  const long long x_end = tile_start(unit + 1, total, G);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSt; ++i) {
@@ -260,7 +258,14 @@ __global__ void __launch_bounds__(kThreadsT, 1)
   const uint32_t tmem_base = *tmem_slot;
   if constexpr (kTemp) {  // launched to depend on the kernel ahead
     grid_wait();
+    if (g.active) {
+      if (kPass == 2) n_b = active_tiles(*g.active, kBNT, n_b, n_a, G);
+      else n_a = active_tiles(*g.active, kResRows, n_a, n_b, G);
+    }
   }
+  const long long total = (long long)n_a * n_b;
+  const long long x_begin = tile_start(unit, total, G);
+  const long long x_end = tile_start(unit + 1, total, G);
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)
@@ -273,8 +278,8 @@ __global__ void __launch_bounds__(kThreadsT, 1)
       for (int i = 0; i < kMaxStT; ++i) issued_parity[i] = -1;
       bool ok = true;
       for (long long x = x_begin; x < x_end && ok; ++x) {
-        const int a = (int)(x / g.n_b);
-        const int b = tc_tile_b(x, a, g.n_b, total, G);
+        const int a = (int)(x / n_b);
+        const int b = tc_tile_b(x, a, n_b, total, G);
         if (a != cur_a) {
           if (a_uses > 0 &&
               !mbar_wait(&bars[kTAEmpty], (a_uses - 1) & 1, g.err, kErrWaitProducer)) {
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
         return true;
       };
       for (long long x = x_begin; x < x_end && ok; ++x, ++li) {
-        const int a = (int)(x / g.n_b);
+        const int a = (int)(x / n_b);
         bool first = a != cur_a;  // of an accumulation: a block's, or a period's
         if (first) {
           if (!mbar_wait(&bars[kTAFull], a_uses & 1, g.err, kErrWaitMma)) break;
@@ -433,7 +438,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
           }
           for (int i = 0; i < n_str_aug; ++i) umma_commit_pair(&bars[kTEmpty + aug_stage[i]], 0x3);
         }
-        const bool last_of_a = x + 1 == x_end || (int)((x + 1) / g.n_b) != a;
+        const bool last_of_a = x + 1 == x_end || (int)((x + 1) / n_b) != a;
         umma_commit_pair(&bars[kTZFull + buf], 0x3);
         if (last_of_a) umma_commit_pair(&bars[kTAEmpty], 0x3);
         if (have_prev && !rank_mmas()) {
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
     // The rank accumulator of the finished block: pass 1 q (this half's
     // ranks, zeros for the other half's), pass 2 dB (this half's ranks).
     auto flush_block = [&](int a_done, int blk_done) {
-      const int seg = unit - tile_owner((long long)a_done * g.n_b, total, G);
+      const int seg = unit - tile_owner((long long)a_done * n_b, total, G);
       if constexpr (kTemp) {
         drain(pending);
         pending = -1;
@@ -580,8 +585,8 @@ __global__ void __launch_bounds__(kThreadsT, 1)
     };
 
     for (long long x = x_begin; x < x_end; ++x, ++li) {
-      const int a = (int)(x / g.n_b);
-      const int b = tc_tile_b(x, a, g.n_b, total, G);
+      const int a = (int)(x / n_b);
+      const int b = tc_tile_b(x, a, n_b, total, G);
       if (a != cur_a) {
         if (cur_a >= 0) flush_block(cur_a, blk);
         rr = (g.a0 + a) * kResRows + (int)rank * kBM + row;
@@ -808,7 +813,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
           drain(pending);
           pending = -1;
         }
-        const bool last_of_a = x + 1 == x_end || (int)((x + 1) / g.n_b) != a;
+        const bool last_of_a = x + 1 == x_end || (int)((x + 1) / n_b) != a;
         if (in_blk % kDrain == kDrain - 1 || last_of_a) pending = blk;
         ++in_blk;
       }
@@ -822,7 +827,7 @@ __global__ void __launch_bounds__(kThreadsT, 1)
     if (lane == 0) {
       long long li = 0;
       for (long long x = x_begin; x < x_end; ++x, ++li) {
-        const int b = tc_tile_b(x, (int)(x / g.n_b), g.n_b, total, G);
+        const int b = tc_tile_b(x, (int)(x / n_b), n_b, total, G);
         const int xb = (int)(li % kXN);
         const long long use = li / kXN;
         if (use >= 1 && !mbar_wait(&bars[kTXEmpty + xb], (uint32_t)((use - 1) & 1), g.err,

@@ -135,6 +135,15 @@ int most_segments(int n_a, int n_b) {
   return (int)std::min<long long>(G, n_b / run + 2);
 }
 
+// Most where, of n_a (or n_b) tiles of positions, as few as a quarter may run
+// (active_tiles).
+int most_segments_by_a(int n_a, int n_b) {
+  return std::max(most_segments(n_a, n_b), most_segments((n_a + 3) / 4, n_b));
+}
+int most_segments_by_b(int n_a, int n_b) {
+  return std::max(most_segments(n_a, n_b), most_segments(n_a, (n_b + 3) / 4));
+}
+
 struct Carve {
   uint8_t* base;
   size_t off = 0;
@@ -358,6 +367,8 @@ struct DistillWs {
   __half *h16, *haug, *waug, *xv, *xt;
   float *sU, *wt, *p_max, *p_sum, *p_q, *tok, *Bt, *nml, *xs, *dU, *gAp, *gBp;
   float2* ref;
+  int* order;
+  unsigned* masks;
   unsigned long long* corr;
   size_t zero_bytes;  // stats and corr: cleared by every call
   size_t bytes;
@@ -372,7 +383,7 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
   const long long Vpad = round_up(hd.V, kBN), Tpad = round_up(T, kBN);
   const int bn = grads && tc ? tc_bn(R) : kBN;
   const int n_a = (T + 2 * kBM - 1) / (2 * kBM), n_b = (hd.V + bn - 1) / bn;
-  const size_t part = (size_t)(grads && tc ? 2 : 4) * most_segments(n_a, n_b) * n_a * 2 * kBM;
+  const size_t part = (size_t)(grads && tc ? 2 : 4) * most_segments_by_a(n_a, n_b) * n_a * 2 * kBM;
   w.stats = c.take<int>(kStatWords);
   if (grads) w.corr = c.take<unsigned long long>((size_t)Vpad * R);
   w.zero_bytes = c.off;
@@ -389,6 +400,8 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
     w.bytes = c.off;
     return w;
   }
+  w.order = c.take<int>(T);
+  w.masks = c.take<unsigned>((T + 31) / 32);
   // rank 4 keeps the rank term in the epilogues of the gradient passes
   const bool in_mma = !grads || R > 4;
   w.haug = c.take<__half>(in_mma ? (size_t)T * aug.width : 0);
@@ -398,7 +411,7 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
   if (grads) {
     // chunks of four or eight epilogue columns a row: up to 4 slots per owner
     const int n_a2 = (hd.V + 2 * kBM - 1) / (2 * kBM), n_b2 = (T + bn - 1) / bn;
-    const size_t segs = (size_t)(tc ? 1 : 4) * most_segments(n_a2, n_b2);
+    const size_t segs = (size_t)(tc ? 1 : 4) * most_segments_by_b(n_a2, n_b2);
     w.p_q = c.take<float>(part * R);
     w.tok = c.take<float>(tc ? 0 : (size_t)Tpad * tok_stride(R));
     w.Bt = c.take<float>(hd.layout ? 0 : (size_t)Vpad * R);
@@ -462,7 +475,7 @@ struct Step {
   cudaStream_t st;
   GemmArgs g;      // pass 1's, filled
   SlotPlan slots;  // out: pass 1's partials
-  int cparts2 = 0, n_b2 = 0, G2 = 0;
+  int cparts2 = 0, n_b2 = 0, bn2 = 0, G2 = 0;
   const float* Bt = nullptr;
 };
 
@@ -511,6 +524,8 @@ int sums_pass2(Step& s, const char** why) {
   if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
   s.g.n_a = (s.hd.V + 2 * kBM - 1) / (2 * kBM);
   s.g.n_b = s.n_b2 = (s.T + kBN - 1) / kBN;
+  s.g.by_b = 1;
+  s.bn2 = kBN;
   s.G2 = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
   s.cparts2 = col_parts(Epi::kWarps);
   if (!launch_pairs(p.kern, s.G2, p.threads, p.smem, s.st, mw, mh, mwa, mha, s.g))
@@ -552,6 +567,7 @@ int tc_pass(Step& s, const char** why) {
                        s.w.p_q};
   } else {
     s.n_b2 = s.g.n_b;
+    s.bn2 = tc_bn(R);
     s.G2 = G;
     s.cparts2 = 1;
   }
@@ -737,7 +753,12 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
 
   if (cudaMemsetAsync(w.stats, 0, w.zero_bytes, st) != cudaSuccess)
     return *why = "cudaMemsetAsync failed", LORA_CE_ECUDA;
+  // weights may leave whole tiles of positions without one that counts
+  const bool order = weight && !few && T > 2 * kBM;
+  if (order) lh_order<<<1, 1024, 0, st>>>(T, K, weight, ids, w.masks, w.order, w.stats);
+  s.g.active = order ? w.stats + kStActive : nullptr;
   PrepArgs pa = prep_args(hd, aug, H, dtype, T);
+  pa.order = order ? w.order : nullptr;
   pa.h16 = w.h16;
   pa.sU = w.sU;
   pa.haug = aug.width ? w.haug : nullptr;
@@ -815,6 +836,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   a.K = K;
   a.ids = ids;
   a.teacher = teacher;
+  a.order = pa.order;
+  a.active = s.g.active;
   a.wt = w.wt;
   a.Bt = s.Bt;
   a.Bt_plain = pk.Bt && tc;
@@ -876,6 +899,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   ga.cparts = s.cparts2;
   ga.res_rows = 2 * kBM;
   ga.n_b2 = s.n_b2;
+  ga.bn2 = s.bn2;
+  ga.active = s.g.active;
   ga.G2 = s.G2;
   ga.Vpad = s.g.Vpad;
   ga.gAp = w.gAp;

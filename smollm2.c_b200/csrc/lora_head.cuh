@@ -34,7 +34,7 @@ constexpr int kRowWarps = 8;      // warps per block of the per-row kernels
 constexpr int kMaxHead64 = 10;    // hidden size in units of 64
 
 // Device words at the start of a workspace.
-enum : int { kStErr = 0, kStBMax = 1, kStUMax = 2, kStatWords = 64 };
+enum : int { kStErr = 0, kStBMax = 1, kStUMax = 2, kStActive = 3, kStatWords = 64 };
 
 // B of the head: [r][V] (layout 0), or the pair-interleaved layout of a
 // trainer's handle at kernel rank R (layout 1, bidx).
@@ -241,9 +241,78 @@ struct PrepArgs {
   int K;
   float tau;
   float* wt;
+  const int* order;  // position in row t of what is prepared, or null: t
   int* stats;
+  __device__ __forceinline__ int source(int t) const { return order ? order[t] : t; }
 };
 
+// order: the positions that count (a weight other than 0 and an entry), then the
+// others, each in ascending order; their number to stats[kStActive].  The passes run
+// over the tiles that hold one that counts, a quarter of all at least: at 8,000
+// positions of which 30% are a masked prompt, rank 64, the call takes 1,680 us
+// instead of 2,300.
+// One block: each warp takes a run of positions, 32 side by side at a time (a
+// thread for a run of its own, its loads and stores a line each, took 13 us instead of 11).
+static __global__ void __launch_bounds__(1024) lh_order(int T, int K,
+                                                        const float* __restrict__ weight,
+                                                        const int32_t* __restrict__ ids,
+                                                        unsigned* __restrict__ masks,  // [T / 32]
+                                                        int* __restrict__ order,
+                                                        int* __restrict__ stats) {
+  constexpr int kStep = 8;  // groups of 32 in flight
+  constexpr unsigned kAll = 0xffffffffu;
+  __shared__ int s_n[32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int groups = (T + 31) / 32, per = (groups + 31) / 32;
+  const int g_lo = min(groups, w * per), g_hi = min(groups, g_lo + per);
+  int n = 0;
+  for (int g0 = g_lo; g0 < g_hi; g0 += kStep) {
+    float wt[kStep];
+    int id[kStep];
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      const int t = 32 * (g0 + i) + lane;
+      const bool in = g0 + i < g_hi && t < T;
+      wt[i] = in ? weight[t] : 0.f;
+      id[i] = in ? ids[(long long)t * K] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      if (g0 + i >= g_hi) break;
+      bool any = wt[i] != 0.f && id[i] >= 0;
+      unsigned look = __ballot_sync(kAll, wt[i] != 0.f && id[i] < 0);
+      for (; look; look &= look - 1) {  // the first entry is absent: seldom
+        const int q = __ffs(look) - 1;
+        bool some = false;
+        for (int k = lane; k < K; k += 32)
+          some |= ids[(long long)(32 * (g0 + i) + q) * K + k] >= 0;
+        some = __any_sync(kAll, some);
+        if (lane == q) any = some;
+      }
+      const unsigned m = __ballot_sync(kAll, any);
+      if (lane == 0) masks[g0 + i] = m;
+      n += __popc(m);
+    }
+  }
+  if (lane == 0) s_n[w] = n;
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int q = 0; q < 32; ++q) {
+    before += q < w ? s_n[q] : 0;
+    total += s_n[q];
+  }
+  int front = before, back = total + 32 * g_lo - before;
+  for (int g0 = g_lo; g0 < g_hi; ++g0) {
+    const unsigned m = masks[g0], below = (1u << lane) - 1u;
+    const int t = 32 * g0 + lane;
+    if (t < T) order[m >> lane & 1u ? front + __popc(m & below) : back + __popc(~m & below)] = t;
+    front += __popc(m);
+    back += 32 - __popc(m);
+  }
+  if (threadIdx.x == 0) stats[kStActive] = total;
+}
+
+// Elements i, i + 1 of position t.
 __device__ __forceinline__ float2 load_pair(const PrepArgs& a, int t, int i) {
   const long long o = (long long)t * a.d + i;
   if (a.dtype == 0) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(
@@ -251,6 +320,23 @@ __device__ __forceinline__ float2 load_pair(const PrepArgs& a, int t, int i) {
   if (a.dtype == 1) return __half22float2(*reinterpret_cast<const __half2*>(
                         reinterpret_cast<const __half*>(a.H) + o));
   return *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(a.H) + o);
+}
+
+// Elements 64 k + 2 lane, + 1 of position t for every k: all on their way at once.
+__device__ __forceinline__ void load_row(const PrepArgs& a, int t, int lane,
+                                         float2 (&x)[kMaxHead64]) {
+  const long long o = ((long long)t * a.d >> 1) + lane;
+  auto all = [&](auto* row, auto widen) {
+#pragma unroll
+    for (int k = 0; k < kMaxHead64; ++k)
+      if (64 * k < a.d) x[k] = widen(row[o + 32 * k]);
+  };
+  if (a.dtype == 0)
+    all(reinterpret_cast<const __nv_bfloat162*>(a.H), [](__nv_bfloat162 p) { return __bfloat1622float2(p); });
+  else if (a.dtype == 1)
+    all(reinterpret_cast<const __half2*>(a.H), [](__half2 p) { return __half22float2(p); });
+  else
+    all(reinterpret_cast<const float2*>(a.H), [](float2 p) { return p; });
 }
 
 // weight * tau of a position that counts, else 0
@@ -306,9 +392,10 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
   }
   float wt = 0.f;
   bool active = true;
+  const int from = a.source(t);
   if (a.ids) {
-    const bool mine = tid < a.K && a.ids[(long long)t * a.K + tid] >= 0;
-    wt = row_weight(a, t, __syncthreads_or(mine));
+    const bool mine = tid < a.K && a.ids[(long long)from * a.K + tid] >= 0;
+    wt = row_weight(a, from, __syncthreads_or(mine));
     active = wt != 0.f;
     if (tid == 0) a.wt[t] = wt;
   }
@@ -323,7 +410,7 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
   };
   fetch(sl);  // on its way beside h
   for (int i = 2 * tid; i < a.d; i += 512) {
-    const float2 x = active ? load_pair(a, t, i) : make_float2(0.f, 0.f);
+    const float2 x = active ? load_pair(a, from, i) : make_float2(0.f, 0.f);
     const __half2 hv = __floats2half2_rn(x.x, x.y);
     *reinterpret_cast<__half2*>(a.h16 + (long long)t * a.d + i) = hv;
     *reinterpret_cast<float2*>(sh + i) = __half22float2(hv);
@@ -369,21 +456,23 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
   const int ldh = a.d + 4;
   float* hT = smem;                                     // [16][d + 4], then [8][16][R] sums
   __shared__ float swt[kTileRows];
+  __shared__ int sfrom[kTileRows];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   if (a.ids) {  // sixteen threads per position, every 16th entry each
-    const int t = t0 + (tid >> 4);
+    const int t = t0 + (tid >> 4), from = t < a.T ? a.source(t) : 0;
     bool any = false;
     if (t < a.T) {
 #pragma unroll
       for (int q = 0; q < kMaxTop / 16; ++q) {
         const int k = (tid & 15) + 16 * q;
-        any |= k < a.K && a.ids[(long long)t * a.K + k] >= 0;
+        any |= k < a.K && a.ids[(long long)from * a.K + k] >= 0;
       }
     }
     const unsigned b = __ballot_sync(0xffffffffu, any) >> (lane & 16) & 0xffffu;
     if ((tid & 15) == 0) {
-      const float wt = t < a.T ? row_weight(a, t, b != 0) : 0.f;
+      const float wt = t < a.T ? row_weight(a, from, b != 0) : 0.f;
       swt[tid >> 4] = wt;
+      sfrom[tid >> 4] = from;
       if (t < a.T) a.wt[t] = wt;
     }
     __syncthreads();
@@ -392,10 +481,12 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
   for (int p = 0; p < 2; ++p) {  // two rows per warp
     const int row = w + 8 * p, t = t0 + row;
     const bool in = t < a.T && (!a.ids || swt[row] != 0.f);
+    const int from = !in ? 0 : a.ids ? sfrom[row] : t;
     float2 x[kMaxHead64];
 #pragma unroll
     for (int k = 0; k < kMaxHead64; ++k)
-      x[k] = in && 64 * k < a.d ? load_pair(a, t, 64 * k + 2 * lane) : make_float2(0.f, 0.f);
+      x[k] = make_float2(0.f, 0.f);
+    if (in) load_row(a, from, lane, x);
 #pragma unroll
     for (int k = 0; k < kMaxHead64; ++k)
       if (64 * k < a.d) {
@@ -1720,6 +1811,8 @@ struct DistillArgs {
   const float* Bt;  // [Vpad][R] (gradients): bidx layout, or row by row; null: z.B
   int Bt_plain;
   const int* stats;
+  const int* order;   // as PrepArgs, and the number of positions that count
+  const int* active;
   float* loss;
   // gradients
   float* tok;     // records of ranks 4, 8
@@ -1758,7 +1851,15 @@ static __global__ void __launch_bounds__(32 * kRowWarps, TW == 1 ? 3 : 2)
   grid_wait();
   if (t >= a.z.T) return;
   const int R = a.z.R;
-  const int nslot = a.p.slots(t);
+  const int at = a.order ? a.order[t] : t;
+  int nslot = 0;  // behind those that count the passes need not have been
+  if (!a.active) {
+    nslot = a.p.slots(t);
+  } else if (t < *a.active) {
+    SlotPlan p = a.p;
+    p.n_a = active_tiles(*a.active, 2 * kBM, p.n_a, p.n_b, min(p.units, p.n_a * p.n_b));
+    nslot = p.slots(t);
+  }
   const float nan = __int_as_float(0x7fc00000);
   float wt = a.wt[t];
   // the teacher's distribution
@@ -1772,8 +1873,8 @@ static __global__ void __launch_bounds__(32 * kRowWarps, TW == 1 ? 3 : 2)
     id[i] = -1;
     lq[i] = 0.0;
     if (wt != 0.f && k < a.K) {
-      const int v = a.ids[(long long)t * a.K + k];
-      const float x = a.teacher[(long long)t * a.K + k];
+      const int v = a.ids[(long long)at * a.K + k];
+      const float x = a.teacher[(long long)at * a.K + k];
       if (v >= a.z.V || (v >= 0 && !(x < INFINITY))) wrong = 1;
       else if (v >= 0 && x > -INFINITY) {
         id[i] = v;
@@ -1783,7 +1884,8 @@ static __global__ void __launch_bounds__(32 * kRowWarps, TW == 1 ? 3 : 2)
     }
   }
   if (tid == 0) s_n[no] = 0;
-  const RowSum rs = merge_row<false>(a.p, t, nslot, team);
+  RowSum rs = merge_row<false>(a.p, t, nslot, team);
+  if (nslot == 0) rs = RowSum{0.f, 1.0, 0.0};
   wrong = team.count(wrong);
   top = team.reduce(top, [](double p, double q) { return fmax(p, q); });
   if (top == -INFINITY && !wrong) wt = 0.f;  // no entry left
@@ -1843,7 +1945,7 @@ static __global__ void __launch_bounds__(32 * kRowWarps, TW == 1 ? 3 : 2)
   loss = team.sum(loss);
   const bool gave_up = *reinterpret_cast<const volatile int*>(a.stats + kStErr) != 0;
   if (tid == 0)
-    a.loss[t] = wrong || gave_up ? nan
+    a.loss[at] = wrong || gave_up ? nan
                 : counts         ? (float)((double)wt * (double)a.tau * (loss + lse)) : 0.f;
   if constexpr (kGrads) {
     const float inv = (float)(1.0 / rs.S);
@@ -2017,6 +2119,8 @@ static __global__ void __launch_bounds__(256) lh_dA(int T, int d, const __half* 
 
 struct GradArgs {
   int T, d, V, r, R, n_chunks, cparts, res_rows, n_b2, G2;
+  const int* active;  // as DistillArgs; bn2 positions per tile
+  int bn2;
   long long Vpad;
   const float* gAp;                // [chunk][d][R]
   const float* gBp;                // [seg][Vpad][R] bidx
@@ -2058,7 +2162,8 @@ static __global__ void __launch_bounds__(256) lh_grads(GradArgs a) {
   const long long v0 = (long long)blk * kPackRows, stride = a.Vpad * a.R;
   int slots = 0;
   if (v0 < a.V) {
-    const SlotPlan p{a.cparts, (a.V + a.res_rows - 1) / a.res_rows, a.n_b2, a.G2};
+    SlotPlan p{a.cparts, (a.V + a.res_rows - 1) / a.res_rows, a.n_b2, a.G2};
+    if (a.active) p.n_b = active_tiles(*a.active, a.bn2, p.n_b, p.n_a, a.G2);
     slots = p.slots_of((int)v0 / a.res_rows);
   }
   constexpr int ld = kPackRows + 1;

@@ -475,6 +475,42 @@ def test_distill_of_few_positions(T, V, d, r, K, tau, dtype, grads):
 
 @gpu
 @pytest.mark.parametrize("r", [4, 8, 16, 64])
+@pytest.mark.parametrize("T,V,d,share", [
+    (257, 1000, 64, 0.5), (290, 4099, 128, 0.0), (700, 2048, 576, 0.3), (1500, 300, 64, 0.05),
+    (3000, 4099, 64, 0.001), (2048, 777, 128, 1.0), (5000, 200, 64, 0.4),
+])
+def test_masked_positions_anywhere(r, T, V, d, share):
+    """Weights of 0 in whole stretches and one by one, over more than one tile of
+    positions: the passes leave their tiles out, and what lies there does not
+    matter.  None, few, and all of them count; the loss is that of the weights."""
+    p = Problem(T, V, d, r, seed=4)
+    p.lists(9, ragged=share < 1.0)
+    torch = p.torch
+    w = 0.5 + 0.5 * p.u(T)
+    w = torch.where(p.u(T) < share, w, torch.zeros_like(w))
+    if 0.0 < share < 1.0:
+        w[: T // 5] = 0.0
+        w[T // 2: T // 2 + 3] = 1.0
+        tol = p.tol()
+        p.tol = lambda: tol  # of the rows as they were
+        p.H[w == 0] = math.nan
+        p.teacher[w == 0] = math.inf
+    p.weight = w
+    out, (loss, *_) = check_distill(p, 1.5)
+    assert bool((out["loss"][w == 0] == 0).all())
+    alone = p.distill(1.5, grads=False)["loss"]
+    tol = 1.5**2 * 2 * (p.tol() / 1.5 + 2.0**-20)
+    assert float((alone.double() - loss).abs().max()) <= tol + 2.0**-24 * float(loss.abs().max())
+    if share == 1.0:  # nothing to leave out: the order is the positions' own
+        p.weight = torch.ones_like(w)
+        a = p.distill(1.5)
+        p.weight = None
+        b = p.distill(1.5)
+        assert all(torch.equal(a[k], b[k]) for k in a)
+
+
+@gpu
+@pytest.mark.parametrize("r", [4, 8, 16, 64])
 def test_gradient_is_the_slope_of_the_loss(r):
     """Central differences of the 64-bit loss along a random direction: the
     truncation error of a step e is e^2 / 6 times a third derivative of order
