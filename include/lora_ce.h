@@ -169,8 +169,9 @@ int lora_ce_score_device(lora_ce_handle* h, const void* d_H, int32_t h_dtype, in
  * sums over all ranks, divided by the number of counted positions (weight not 0 and
  * at least one entry) over all ranks, then the clip and Adam as lora_ce_step.
  * *loss_out: the sum of losses over that number.  A step that counts no position
- * anywhere has loss 0 and applies a gradient of zero.  lora_ce_get_grads and
- * lora_ce_get_token_loss read the step's gradients and losses.  The host variant
+ * anywhere has loss 0 and applies a gradient of zero.  lora_ce_get_grads (n_pred:
+ * counted positions, 1 where there are none) and lora_ce_get_token_loss read the
+ * step's gradients and losses.  The host variant
  * refuses weights that are not finite and, in rows with a weight, ids >= vocab and
  * logits of NaN or +inf; in device buffers those make loss and gradients NaN. */
 int lora_ce_distill_step(lora_ce_handle* h, const void* H, int32_t h_dtype, int32_t T, int32_t K,
