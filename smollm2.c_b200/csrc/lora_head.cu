@@ -28,6 +28,20 @@ int hfail(int code, const char* msg) {
   return code;
 }
 
+// A C entry's body: no exception leaves it, and a failed call leaves no CUDA error
+// behind for the caller's next check.
+template <class F>
+int entry(F&& body) {
+  int rc = LORA_CE_ENOMEM;
+  try {
+    rc = body();
+  } catch (...) {
+    g_head_error.clear();
+  }
+  if (rc) cudaGetLastError();
+  return rc;
+}
+
 // How the rank term joins the MMA: one K-block up to rank 16, 2R columns above.
 // Its operands are only as wide as they are used (a multiple of 16 bytes); the
 // loads fill the rest of a 64-column block with zeros.
@@ -98,9 +112,10 @@ int resident_pairs(const void* kern, int threads, int smem) {
   return n;
 }
 
-// Same for kernels without clusters: only the shared-memory attribute.
+// Same for kernels without clusters: only the shared-memory attribute.  48 KB need
+// none, which a kernel's static arrays (up to 8 KB here) share.
 bool allow_smem(const void* kern, size_t smem) {
-  if (smem <= 48 * 1024) return true;
+  if (smem <= 40 * 1024) return true;
   static std::mutex mu;
   static std::map<std::pair<int, const void*>, size_t> known;
   int dev = 0;
@@ -176,7 +191,19 @@ bool launch_pairs(K kern, int pairs, int threads, int smem, cudaStream_t st, con
   return cudaLaunchKernelEx(&lc, kern, args...) == cudaSuccess;
 }
 
-// The same for any other kernel that waits.
+// A kernel that waits for all that is ahead of it in the stream.
+template <class K, class... Args>
+bool launch_plain(K kern, int blocks, int threads, size_t smem, cudaStream_t st,
+                  const Args&... args) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)blocks);
+  lc.blockDim = dim3((unsigned)threads);
+  lc.dynamicSmemBytes = smem;
+  lc.stream = st;
+  return cudaLaunchKernelEx(&lc, kern, args...) == cudaSuccess;
+}
+
+// One that waits by itself (grid_wait).
 template <class K, class... Args>
 bool launch_after(K kern, int blocks, int threads, size_t smem, cudaStream_t st,
                   const Args&... args) {
@@ -281,8 +308,8 @@ int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_block
       std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R, pa.d) : (size_t)(pa.d + 256) * 4,
                pack ? (size_t)pk.R * (kPackRows + 1) * 4 : 0);
   if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return LORA_CE_ECUDA;
-  kern<<<prep_blocks + max_blocks + pack_blocks, 256, smem, st>>>(pa, pk, prep_blocks, max_blocks);
-  return 0;
+  return launch_plain(kern, prep_blocks + max_blocks + pack_blocks, 256, smem, st, pa, pk,
+                      prep_blocks, max_blocks) ? 0 : LORA_CE_ECUDA;
 }
 
 // The pass for few positions, one slot per 128 vocab rows.  Its time grows with
@@ -723,8 +750,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   a.top_logprobs = top_logprobs;
   const int per = warps ? kScoreRows : 1;
   const int threads = 32 * tw * per;
-  if (!launch_after(rows, (T + per - 1) / per, threads, rows_smem, st, a) ||
-      cudaGetLastError() != cudaSuccess)
+  if (!launch_after(rows, (T + per - 1) / per, threads, rows_smem, st, a))
     return *why = kNoLaunch, LORA_CE_ECUDA;
   return 0;
 }
@@ -755,7 +781,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
     return *why = "cudaMemsetAsync failed", LORA_CE_ECUDA;
   // weights may leave whole tiles of positions without one that counts
   const bool order = weight && !few && T > 2 * kBM;
-  if (order) lh_order<<<1, 1024, 0, st>>>(T, K, weight, ids, w.masks, w.order, w.stats);
+  if (order && !launch_plain(lh_order, 1, 1024, 0, st, T, K, weight, ids, w.masks, w.order, w.stats))
+    return *why = kNoLaunch, LORA_CE_ECUDA;
   s.g.active = order ? w.stats + kStActive : nullptr;
   PrepArgs pa = prep_args(hd, aug, H, dtype, T);
   pa.order = order ? w.order : nullptr;
@@ -854,10 +881,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
                     : (warps ? lh_distill_rows<false, 1> : lh_distill_rows<false, kRowWarps>);
   if (!launch_after(rows, warps ? (T + kRowWarps - 1) / kRowWarps : T, 32 * kRowWarps, 0, st, a))
     return *why = kNoLaunch, LORA_CE_ECUDA;
-  if (!grads) {
-    if (cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
-    return 0;
-  }
+  if (!grads) return 0;
   const int a_blocks = ((out.layout ? R : hd.r) * hd.d + 255) / 256;
   if (few) {
     f.ref = w.ref;
@@ -872,8 +896,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
     f.loss = loss;
     f.wt = w.wt;
     f.tail = out.tail;
-    if (!launch_few<kFewBackward>(f, f.v_blocks + a_blocks, st) ||
-        cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
+    if (!launch_few<kFewBackward>(f, f.v_blocks + a_blocks, st))
+      return *why = kNoLaunch, LORA_CE_ECUDA;
     return 0;
   }
   if (tc) {
@@ -914,14 +938,14 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   ga.loss = loss;
   ga.wt = w.wt;
   ga.tail = out.tail;
-  if (!launch_after(lh_grads, (int)(s.g.Vpad / kPackRows) + a_blocks, 256, 0, st, ga) ||
-      cudaGetLastError() != cudaSuccess) return *why = kNoLaunch, LORA_CE_ECUDA;
+  if (!launch_after(lh_grads, (int)(s.g.Vpad / kPackRows) + a_blocks, 256, 0, st, ga))
+    return *why = kNoLaunch, LORA_CE_ECUDA;
   return 0;
 }
 
 int head_step_tail(const void* ws, float* tail, int* err, cudaStream_t st) {
-  lh_tail<<<1, 1, 0, st>>>(static_cast<const int*>(ws), tail, err);
-  return cudaGetLastError() == cudaSuccess ? 0 : LORA_CE_ECUDA;
+  return launch_plain(lh_tail, 1, 1, 0, st, static_cast<const int*>(ws), tail, err) ? 0
+                                                                                    : LORA_CE_ECUDA;
 }
 
 namespace {
@@ -1033,94 +1057,109 @@ extern "C" {
 const char* lora_head_last_error(void) { return g_head_error.c_str(); }
 
 size_t lora_head_score_workspace(const lora_head* h, int32_t T, int32_t top_k) {
-  return check_score(h, T, top_k) ? 0 : head_score_bytes(core_of(h), T, top_k);
+  size_t bytes = 0;
+  entry([&] {
+    const int rc = check_score(h, T, top_k);
+    if (!rc) bytes = head_score_bytes(core_of(h), T, top_k);
+    return rc;
+  });
+  return bytes;
 }
 
 size_t lora_head_distill_workspace(const lora_head* h, int32_t T, int32_t K, int32_t grads) {
-  if (check_distill(h, T, K, grads != 0, 1.0f)) return 0;
-  return head_distill_bytes(core_of(h), T, K, grads != 0);
+  size_t bytes = 0;
+  entry([&] {
+    const int rc = check_distill(h, T, K, grads != 0, 1.0f);
+    if (!rc) bytes = head_distill_bytes(core_of(h), T, K, grads != 0);
+    return rc;
+  });
+  return bytes;
 }
 
 int lora_head_score(const lora_head* h, const void* H, int32_t h_dtype, int32_t T,
                     const int32_t* tokens, int32_t top_k, float* logprob, float* entropy,
                     int32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes,
                     void* stream) {
-  if (int rc = check_score(h, T, top_k)) return rc;
-  if (h_dtype < LORA_CE_BF16 || h_dtype > LORA_CE_F32)
-    return hfail(LORA_CE_EINVAL, "bad hidden-state dtype");
-  if ((tokens == nullptr) != (logprob == nullptr))
-    return hfail(LORA_CE_EINVAL, "tokens and logprob go together");
-  if (!logprob && !entropy && top_k == 0) return hfail(LORA_CE_EINVAL, "nothing is asked for");
-  Buffers b;
-  struct {
-    const void* p;
-    uintptr_t align;
-    const char* name;
-    bool used;
-  } all[] = {{h->W, 16, "W", true},
-             {h->A, 4, "A", h->rank > 0},
-             {h->B, 4, "B", h->rank > 0},
-             {H, 16, "H", true},
-             {tokens, 4, "tokens", tokens != nullptr},
-             {logprob, 4, "logprob", logprob != nullptr},
-             {entropy, 4, "entropy", entropy != nullptr},
-             {top_ids, 4, "top_ids", top_k > 0},
-             {top_logprobs, 4, "top_logprobs", top_k > 0},
-             {ws, 256, "workspace", true}};
-  for (const auto& x : all)
-    if (x.used) b.need(x.p, x.align, x.name);
-  if (!b.rc && ws_bytes < head_score_bytes(core_of(h), T, top_k))
-    return hfail(LORA_CE_EINVAL, "workspace too small");
-  for (const auto& x : all)
-    if (x.used) b.here(x.p, x.name);
-  if (b.rc) return b.rc;
-  if (int rc = check_arch()) return rc;
-  const char* why = "";
-  const int rc = head_score_run(core_of(h), H, h_dtype, T, tokens, top_k, logprob, entropy,
-                                top_ids, top_logprobs, ws, static_cast<cudaStream_t>(stream), &why);
-  return rc ? hfail(rc, why) : 0;
+  return entry([&]() -> int {
+    if (int rc = check_score(h, T, top_k)) return rc;
+    if (h_dtype < LORA_CE_BF16 || h_dtype > LORA_CE_F32)
+      return hfail(LORA_CE_EINVAL, "bad hidden-state dtype");
+    if ((tokens == nullptr) != (logprob == nullptr))
+      return hfail(LORA_CE_EINVAL, "tokens and logprob go together");
+    if (!logprob && !entropy && top_k == 0) return hfail(LORA_CE_EINVAL, "nothing is asked for");
+    Buffers b;
+    struct {
+      const void* p;
+      uintptr_t align;
+      const char* name;
+      bool used;
+    } all[] = {{h->W, 16, "W", true},
+               {h->A, 4, "A", h->rank > 0},
+               {h->B, 4, "B", h->rank > 0},
+               {H, 16, "H", true},
+               {tokens, 4, "tokens", tokens != nullptr},
+               {logprob, 4, "logprob", logprob != nullptr},
+               {entropy, 4, "entropy", entropy != nullptr},
+               {top_ids, 4, "top_ids", top_k > 0},
+               {top_logprobs, 4, "top_logprobs", top_k > 0},
+               {ws, 256, "workspace", true}};
+    for (const auto& x : all)
+      if (x.used) b.need(x.p, x.align, x.name);
+    if (!b.rc && ws_bytes < head_score_bytes(core_of(h), T, top_k))
+      return hfail(LORA_CE_EINVAL, "workspace too small");
+    for (const auto& x : all)
+      if (x.used) b.here(x.p, x.name);
+    if (b.rc) return b.rc;
+    if (int rc = check_arch()) return rc;
+    const char* why = "";
+    const int rc = head_score_run(core_of(h), H, h_dtype, T, tokens, top_k, logprob, entropy,
+                                  top_ids, top_logprobs, ws, static_cast<cudaStream_t>(stream), &why);
+    return rc ? hfail(rc, why) : 0;
+  });
 }
 
 int lora_head_distill(const lora_head* h, const void* H, int32_t h_dtype, int32_t T, int32_t K,
                       const int32_t* ids, const float* teacher, float temperature,
                       const float* weight, float* loss, float* gA, float* gB, void* ws,
                       size_t ws_bytes, void* stream) {
-  if ((gA == nullptr) != (gB == nullptr))
-    return hfail(LORA_CE_EINVAL, "gA and gB go together");
-  const bool grads = gA != nullptr;
-  if (int rc = check_distill(h, T, K, grads, temperature)) return rc;
-  if (h_dtype < LORA_CE_BF16 || h_dtype > LORA_CE_F32)
-    return hfail(LORA_CE_EINVAL, "bad hidden-state dtype");
-  Buffers b;
-  struct {
-    const void* p;
-    uintptr_t align;
-    const char* name;
-    bool used;
-  } all[] = {{h->W, 16, "W", true},
-             {h->A, 4, "A", h->rank > 0},
-             {h->B, 4, "B", h->rank > 0},
-             {H, 16, "H", true},
-             {ids, 4, "ids", true},
-             {teacher, 4, "teacher", true},
-             {weight, 4, "weight", weight != nullptr},
-             {loss, 4, "loss", true},
-             {gA, 4, "gA", grads},
-             {gB, 4, "gB", grads},
-             {ws, 256, "workspace", true}};
-  for (const auto& x : all)
-    if (x.used) b.need(x.p, x.align, x.name);
-  if (!b.rc && ws_bytes < head_distill_bytes(core_of(h), T, K, grads))
-    return hfail(LORA_CE_EINVAL, "workspace too small");
-  for (const auto& x : all)
-    if (x.used) b.here(x.p, x.name);
-  if (b.rc) return b.rc;
-  if (int rc = check_arch()) return rc;
-  const char* why = "";
-  const int rc = head_distill_run(core_of(h), H, h_dtype, T, K, ids, teacher, temperature, weight,
-                                  loss, GradOut{gA, gB, 0, nullptr}, ws,
-                                  static_cast<cudaStream_t>(stream), &why);
-  return rc ? hfail(rc, why) : 0;
+  return entry([&]() -> int {
+    if ((gA == nullptr) != (gB == nullptr))
+      return hfail(LORA_CE_EINVAL, "gA and gB go together");
+    const bool grads = gA != nullptr;
+    if (int rc = check_distill(h, T, K, grads, temperature)) return rc;
+    if (h_dtype < LORA_CE_BF16 || h_dtype > LORA_CE_F32)
+      return hfail(LORA_CE_EINVAL, "bad hidden-state dtype");
+    Buffers b;
+    struct {
+      const void* p;
+      uintptr_t align;
+      const char* name;
+      bool used;
+    } all[] = {{h->W, 16, "W", true},
+               {h->A, 4, "A", h->rank > 0},
+               {h->B, 4, "B", h->rank > 0},
+               {H, 16, "H", true},
+               {ids, 4, "ids", true},
+               {teacher, 4, "teacher", true},
+               {weight, 4, "weight", weight != nullptr},
+               {loss, 4, "loss", true},
+               {gA, 4, "gA", grads},
+               {gB, 4, "gB", grads},
+               {ws, 256, "workspace", true}};
+    for (const auto& x : all)
+      if (x.used) b.need(x.p, x.align, x.name);
+    if (!b.rc && ws_bytes < head_distill_bytes(core_of(h), T, K, grads))
+      return hfail(LORA_CE_EINVAL, "workspace too small");
+    for (const auto& x : all)
+      if (x.used) b.here(x.p, x.name);
+    if (b.rc) return b.rc;
+    if (int rc = check_arch()) return rc;
+    const char* why = "";
+    const int rc = head_distill_run(core_of(h), H, h_dtype, T, K, ids, teacher, temperature, weight,
+                                    loss, GradOut{gA, gB, 0, nullptr}, ws,
+                                    static_cast<cudaStream_t>(stream), &why);
+    return rc ? hfail(rc, why) : 0;
+  });
 }
 
 }  // extern "C"

@@ -106,16 +106,17 @@ struct EpiScore {
     a1 = a2 = 0;
   }
 
-  // Adds the chunk's terms at reference nm = -(reference max) * lg.
+  // Adds the chunk's terms at reference nm = -(reference max) * lg; the first `n_in`
+  // columns are the vocabulary's.
   template <bool kTail>
-  __device__ __forceinline__ void sum(const float (&z)[kCW], float2 L2, float nm) {
+  __device__ __forceinline__ void sum(const float (&z)[kCW], float2 L2, float nm, int n_in) {
     const float2 nm2 = f2(nm, nm);
 #pragma unroll
     for (int p = 0; p < kCW / 2; ++p) {
       float2 x2 = __ffma2_rn(f2(z[2 * p], z[2 * p + 1]), L2, nm2);
-      if (kTail && kTop) {  // masked columns: e = 0 and e * x = 0, not 0 * inf
-        x2.x = fmaxf(x2.x, -1e30f);
-        x2.y = fmaxf(x2.y, -1e30f);
+      if (kTail && kTop) {  // columns past the vocabulary: e = 0 and e * x = 0, not 0 * inf
+        if (2 * p >= n_in) x2.x = -1e30f;
+        if (2 * p + 1 >= n_in) x2.y = -1e30f;
       }
       const float2 e2 = f2(ex2f(x2.x), ex2f(x2.y));
       s2 = __fadd2_rn(s2, e2);
@@ -202,7 +203,7 @@ struct EpiScore {
       mL = to;
     }
     __syncwarp();  // rejoin before the next warp-wide TMEM load
-    sum<kTail>(acc, L2, -mL);
+    sum<kTail>(acc, L2, -mL, g.V - v0);
     if (((v0 + kCW) & 63) == 0) fold();
   }
 
@@ -1241,7 +1242,7 @@ static __global__ void __launch_bounds__(256, 3) lh_few(FewArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float& x = sz[t * kFewLdZ + lane + 32 * i];
-        x = ref.y == 0.f ? 0.f : ex2f(fmaxf(fmaf(x, a.lg, -ref.x), -1e30f)) * ref.y;
+        x = ref.y == 0.f ? 0.f : ex2f(fmaf(x, a.lg, -ref.x)) * ref.y;
       }
     }
     __syncthreads();
@@ -1288,7 +1289,8 @@ static __global__ void __launch_bounds__(256, 3) lh_few(FewArgs a) {
       float S = 0.f, E = 0.f;
   #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float y = fmaxf(fmaf(x[i], a.lg, -mL), -1e30f), e = ex2f(y);
+        // past the vocabulary e = 0 and e * y = 0, not 0 * inf
+        const float y = v0 + lane + 32 * i < a.V ? fmaf(x[i], a.lg, -mL) : -1e30f, e = ex2f(y);
         S += e;
         if (kMode == kFewScore) E = fmaf(e, y, E);
         if (kMode == kFewForward) sz[t * kFewLdZ + lane + 32 * i] = e;
@@ -1453,8 +1455,8 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   const bool have_tok = tk >= 0 && tk < a.z.V;
   const RowSum rs = merge_row<true>(a.p, t, a.p.slots(t), team);
   const float nan = __int_as_float(0x7fc00000);
-  // NaN or infinite logits, or a pass that gave up
-  if (!isfinite(rs.M) || !isfinite(rs.S) ||
+  // NaN or infinite logits (-inf: 0 * inf in E), or a pass that gave up
+  if (!isfinite(rs.M) || !isfinite(rs.S) || !isfinite(rs.E) ||
       *reinterpret_cast<const volatile int*>(a.stats + kStErr) != 0) {
     if (tid == 0) {
       if (a.logprob) a.logprob[t] = nan;

@@ -348,7 +348,7 @@ def test_near_ties_are_ordered_by_the_exact_logits():
 
 
 @gpu
-@pytest.mark.parametrize("T", [40, 1200])
+@pytest.mark.parametrize("T", [20, 40, 1200])
 def test_not_a_number_stays_in_its_row(T):
     torch = pytest.importorskip("torch")
     p = Problem(T, 1000, 64, 4, "f32")
@@ -369,6 +369,95 @@ def test_not_a_number_stays_in_its_row(T):
     rest[[7, 9, 11, 13, 14]] = False
     for key in good:
         assert torch.equal(out[key][rest], good[key][rest])
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 24, 40, 1200])
+@pytest.mark.parametrize("v", [0, 500, 4098])
+@pytest.mark.parametrize("value", [math.nan, -math.inf])
+def test_a_weight_that_is_not_finite_shows(T, v, value):
+    """One logit of a row NaN or infinite, in a full tile or the last: the row's
+    results are NaN and ids -1, of every row here."""
+    p = Problem(T, 4099, 64, 4, "f32")
+    p.H[:, 3] = 1.0
+    p.W[v, 3] = value
+    out = p.score(5)
+    assert bool(out["logprob"].isnan().all()) and bool(out["entropy"].isnan().all())
+    assert bool((out["ids"] == -1).all()) and bool(out["lps"].isnan().all())
+    if math.isnan(value):
+        p.lists(6, ragged=False)
+        d = p.distill(1.0)
+        assert bool(d["loss"].isnan().all()) and bool(d["gA"].isnan().all())
+
+
+@gpu
+@pytest.mark.parametrize("r", [4, 16, 33])
+@pytest.mark.parametrize("what", ["id", "nan logit", "nan hidden", "nan weight", "no entries"])
+def test_bad_rows_among_few_positions(r, what):
+    torch = pytest.importorskip("torch")
+    T, V, d, K = 15, 500, 64, 4
+    p = Problem(T, V, d, r, "f32")
+    p.lists(K, ragged=False)
+    p.weight = torch.ones(T, device="cuda")
+    good = p.distill(1.0)
+    if what == "id":
+        p.ids[7, 2] = V
+    elif what == "nan logit":
+        p.teacher[7, 1] = math.nan
+    elif what == "nan hidden":
+        p.H[7, 5] = math.nan
+    elif what == "nan weight":
+        p.weight[7] = math.nan
+    else:
+        p.ids[7] = -1
+        p.H[7] = math.nan
+    out = p.distill(1.0)
+    rest = torch.arange(T, device="cuda") != 7
+    assert torch.equal(out["loss"][rest], good["loss"][rest])
+    if what == "no entries":
+        assert float(out["loss"][7]) == 0 and bool(out["gB"].isfinite().all())
+        p.weight[7] = 0
+        p.ids[7] = V + 9
+        again = p.distill(1.0)
+        assert all(torch.equal(out[k], again[k]) for k in out)
+    else:
+        assert math.isnan(float(out["loss"][7]))
+        assert bool(out["gA"].isnan().all()) and bool(out["gB"].isnan().all())
+
+
+@gpu
+def test_the_first_call_of_a_process_can_be_captured():
+    """Kernels load, limits are asked for and set inside a capture as well."""
+    import subprocess
+    import sys
+
+    code = """
+import sys; sys.path[:0] = [%r, %r]
+import torch, test_head
+out = {}
+for T in (5, 300):
+    p = test_head.Problem(T, 1000, 64, 16)
+    p.lists(6)
+    p.weight = p.u(T)
+    s = dict(logprob=torch.zeros(T, device="cuda"), entropy=torch.zeros(T, device="cuda"),
+             ids=torch.zeros(T, 4, device="cuda", dtype=torch.int32), lps=torch.zeros(T, 4, device="cuda"))
+    d = dict(loss=torch.zeros(T, device="cuda"), gA=torch.zeros(64, 16, device="cuda"),
+             gB=torch.zeros(16, 1000, device="cuda"))
+    w = torch.empty(1 << 26, dtype=torch.uint8, device="cuda")
+    st = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        p.score(4, stream=st, ws=w, out=s)
+        p.distill(1.5, stream=st, ws=w, out=d)
+    g.replay()
+    torch.cuda.synchronize()
+    a, b = p.score(4), p.distill(1.5)
+    assert all(torch.equal(a[k], s[k]) for k in a), T
+    assert all(torch.equal(b[k], d[k]) for k in b), T
+print("captured")
+""" % (os.path.dirname(os.path.abspath(lora_ce.__file__)), os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 @gpu
