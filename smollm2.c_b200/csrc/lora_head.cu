@@ -664,15 +664,18 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   g.sub_arg = w.sub_arg;
   g.sub_arg2 = w.sub_arg2;
   g.n_sub = w.n_sub;
-  // per-row kernel: a warp per position, or the whole block where positions
-  // are too few to fill the SMs that way
+  // per-row kernel: a warp per position, or four where that many positions do not
+  // fill the SMs (eight where there are more than 1,024 records).  V = 49152, whole
+  // calls in us, four warps against one: 8 alternatives at 600 / 1,184 / 2,047 / 3,000
+  // positions 90 / 127 / 176 / 246 against 106 / 127 / 176 / 231; 64 alternatives 102 /
+  // 143 / 209 / 293 against 133 / 166 / 242 / 276
   ScoreArgs a{};
   a.n_sub = w.n_sub;
   a.sub = w.sub;
   a.top_k = top_k;
   a.n_pick = std::min(w.n_sub, std::max(top_k, kMinPick));
   a.cap = 2 * score_picks(a.n_pick) + top_k + 65;  // and the given token
-  const bool warps = T >= sms * kRowWarps && w.n_sub <= 32 * 32;
+  const bool warps = T >= sms * (top_k > 16 ? 16 : 8) && w.n_sub <= 32 * 32;
   const int tw = warps ? 1 : w.n_sub <= 8 * 128 ? 4 : 8;  // warps per position
   void (*rows)(ScoreArgs) = warps ? w.n_sub <= 24 * 32 ? lh_score_rows<1, 24> : lh_score_rows<1, 32>
                             : tw == 4 ? lh_score_rows<4, 8> : lh_score_rows<8, 32>;
@@ -876,7 +879,11 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   a.xs = w.xs;
   a.dU = w.dU;
   a.corr = w.corr;
-  const bool warps = T >= s.sms * kRowWarps;
+  // a warp per position, or a block of eight; V = 49152, whole calls in us, eight
+  // against one: rank 4, 8 entries at 450 / 600 / 1,184 positions 125 / 152 / 207
+  // against 129 / 143 / 186; rank 64, 64 entries at 900 / 1,184 / 1,600 453 / 524 / 661
+  // against 479 / 541 / 649
+  const bool warps = T >= s.sms * (K > 16 ? 10 : 4);
   auto rows = grads ? (warps ? lh_distill_rows<true, 1> : lh_distill_rows<true, kRowWarps>)
                     : (warps ? lh_distill_rows<false, 1> : lh_distill_rows<false, kRowWarps>);
   if (!launch_after(rows, warps ? (T + kRowWarps - 1) / kRowWarps : T, 32 * kRowWarps, 0, st, a))

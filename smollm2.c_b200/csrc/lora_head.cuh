@@ -30,7 +30,7 @@ constexpr int kMaxTop = 128;      // largest top_k, largest teacher list
 constexpr int kMinPick = 8;       // logits of a row that are computed again at least
 constexpr int kPickStop = 7;      // the search ends with up to so many records beyond that,
 constexpr int kPickSlack = 24;    // and takes near ties of the last up to so many
-constexpr int kRowWarps = 8;      // warps per block of the per-row kernels
+constexpr int kRowWarps = 8;      // warps per block of lh_distill_rows
 constexpr int kMaxHead64 = 10;    // hidden size in units of 64
 
 // Device words at the start of a workspace.
@@ -900,12 +900,6 @@ struct Team {
       for (int i = 0; i < TW; ++i) x += b[i];
     }
     return x;
-  }
-  __device__ __forceinline__ unsigned max_u(unsigned x) {
-    return reduce(x, [](unsigned p, unsigned q) { return p > q ? p : q; });
-  }
-  __device__ __forceinline__ unsigned min_u(unsigned x) {
-    return reduce(x, [](unsigned p, unsigned q) { return p < q ? p : q; });
   }
   __device__ __forceinline__ float max_f(float x) {
     return reduce(x, [](float p, float q) { return fmaxf(p, q); });
