@@ -758,6 +758,12 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   return 0;
 }
 
+template <bool kGrads>
+void (*distill_rows(int tw))(DistillArgs) {
+  return tw == 1   ? lh_distill_rows<kGrads, 1>
+         : tw == 4 ? lh_distill_rows<kGrads, 4> : lh_distill_rows<kGrads, 8>;
+}
+
 int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
                      const int32_t* ids, const float* teacher, float tau, const float* weight,
                      float* loss, const GradOut& out, void* ws, cudaStream_t st,
@@ -879,14 +885,15 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   a.xs = w.xs;
   a.dU = w.dU;
   a.corr = w.corr;
-  // a warp per position, or a block of eight; V = 49152, whole calls in us, eight
-  // against one: rank 4, 8 entries at 450 / 600 / 1,184 positions 125 / 152 / 207
-  // against 129 / 143 / 186; rank 64, 64 entries at 900 / 1,184 / 1,600 453 / 524 / 661
-  // against 479 / 541 / 649
-  const bool warps = T >= s.sms * (K > 16 ? 10 : 4);
-  auto rows = grads ? (warps ? lh_distill_rows<true, 1> : lh_distill_rows<true, kRowWarps>)
-                    : (warps ? lh_distill_rows<false, 1> : lh_distill_rows<false, kRowWarps>);
-  if (!launch_after(rows, warps ? (T + kRowWarps - 1) / kRowWarps : T, 32 * kRowWarps, 0, st, a))
+  // warps per position: eight while blocks of eight fit beside each other, one where
+  // that many positions fill the SMs.  V = 49152, whole calls in us.  Eight / four, rank
+  // 64, 64 entries, 150 and 300 positions: 217 / 238, 279 / 272; rank 4, 8 entries, 450:
+  // 125 / 115.  Four / one, rank 4, 1,184 and 2,047 positions: 188 / 184, 276 / 254;
+  // rank 64: 508 / 541, 741 / 727.
+  const int tw = T <= 2 * s.sms ? 8 : T < 10 * s.sms ? 4 : 1;
+  const int per = tw == 1 ? kRowWarps : 1;
+  if (!launch_after(grads ? distill_rows<true>(tw) : distill_rows<false>(tw), (T + per - 1) / per,
+                    32 * tw * per, 0, st, a))
     return *why = kNoLaunch, LORA_CE_ECUDA;
   if (!grads) return 0;
   const int a_blocks = ((out.layout ? R : hd.r) * hd.d + 255) / 256;

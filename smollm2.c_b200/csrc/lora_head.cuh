@@ -30,7 +30,7 @@ constexpr int kMaxTop = 128;      // largest top_k, largest teacher list
 constexpr int kMinPick = 8;       // logits of a row that are computed again at least
 constexpr int kPickStop = 7;      // the search ends with up to so many records beyond that,
 constexpr int kPickSlack = 24;    // and takes near ties of the last up to so many
-constexpr int kRowWarps = 8;      // warps per block of lh_distill_rows
+constexpr int kRowWarps = 8;      // lh_distill_rows: positions per block where each has a warp
 constexpr int kMaxHead64 = 10;    // hidden size in units of 64
 
 // Device words at the start of a workspace.
@@ -839,7 +839,7 @@ __device__ __forceinline__ double logit64(const LogitArgs& a, int t, int v, cons
 
 // ------------------------------------------------------------- teams
 // The per-row kernels give a position to one warp, or, where positions are too
-// few to fill the SMs with warps, to a block of eight.
+// few to fill the SMs with warps, to a block of four or eight.
 template <int TW>
 struct Team {
   static constexpr int kThreads = 32 * TW;
@@ -1370,10 +1370,10 @@ struct ScoreArgs {
   float* top_logprobs;
 };
 
-// Shared memory of one team: reductions; logits computed again [cap, the given
-// token's last]; ids, logits as the pass had them, and ranks [cap]; per picked
-// record its number, its second and rest, its columns; 64 columns' ids and
-// logits; counters.  A multiple of 16 bytes.
+// Shared memory of one team: reductions and shares of logits (several warps); per
+// candidate, the given token first [cap]: its logit, id, the pass's logit, that one
+// made good, its rank; per picked record its number, its second and rest, its
+// columns; 64 columns' ids and logits; counters.  A multiple of 16 bytes.
 __host__ __device__ inline int score_picks(int n_pick) { return n_pick + kPickSlack; }
 __host__ __device__ inline size_t score_team_smem(int n_pick, int cap, int warps) {
   return ((size_t)(warps == 1 ? 0 : 20 * warps) * 8 + (size_t)cap * 24 +
@@ -1382,10 +1382,12 @@ __host__ __device__ inline size_t score_team_smem(int n_pick, int cap, int warps
 constexpr int kScoreRows = 4;  // positions per block where each has a warp
 
 // One team per position, NK records per thread.  Merge the sums; bisect for a
-// threshold that n_pick to n_pick + kPickStop records reach: it is a lower
-// bound of the n_pick-th largest logit; compute every logit that reaches it,
-// less what rounding may have moved, again, with 64-bit sums where two are too
-// close to tell their order; sort, write.  The softmax's sums get the difference.
+// threshold that n_pick to n_pick + kPickStop records reach: it is a lower bound of
+// the n_pick-th largest logit; the candidates are the logits that reach it, less what
+// rounding may have moved; compute again those whose order the pass's logits do not
+// tell, sort, write.  The softmax's sums get the difference.
+// 4,096 positions, 64 alternatives: 115 us, 140 with every candidate computed again,
+// which was five groups of 16 rows of W a position, read from L2.
 template <int TW, int NK>
 static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW == 8 ? 2 : 5)
     lh_score_rows(ScoreArgs a) {
@@ -1826,9 +1828,10 @@ struct DistillArgs {
 // possible term, summed with integer atomics, so that the order in which
 // positions meet an id does not change the result.
 template <bool kGrads, int TW>
-static __global__ void __launch_bounds__(32 * kRowWarps, TW == 1 ? 3 : 2)
+static __global__ void
+    __launch_bounds__(32 * (TW == 1 ? kRowWarps : TW), TW == 1 ? 3 : TW == 4 ? 4 : 2)
     lh_distill_rows(DistillArgs a) {
-  constexpr int kTeams = kRowWarps / TW, kThreads = 32 * TW;
+  constexpr int kTeams = TW == 1 ? kRowWarps : 1, kThreads = 32 * TW;
   constexpr int kPer = (kMaxTop + kThreads - 1) / kThreads;
   __shared__ double s_red[kTeams][4 * TW];
   __shared__ int s_n[kTeams];
