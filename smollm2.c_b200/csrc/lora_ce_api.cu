@@ -1740,7 +1740,7 @@ int lora_ce_distill_step_device(lora_ce_handle* h, const void* dH, int32_t dtype
   LCE_CUDA(cudaSetDevice(h->cfg.device));
   rc = run_distill_step(h, dH, dtype, T, K, d_ids, d_teacher, temperature, d_weight,
                         d_loss ? d_loss : h->d_loss);
-  if (rc) h->poisoned = true;
+  if (rc && rc != LORA_CE_ENOMEM) h->poisoned = true;  // (no workspace: nothing was done)
   return rc;
 }
 
@@ -1774,7 +1774,7 @@ int lora_ce_distill_step(lora_ce_handle* h, const void* H, int32_t dtype, int32_
   rc = run_distill_step(h, h->in_H, dtype, T, K, d_ids, d_teacher, temperature,
                         weight ? d_weight : nullptr, h->d_loss);
   if (rc) {
-    h->poisoned = true;
+    if (rc != LORA_CE_ENOMEM) h->poisoned = true;
     return rc;
   }
   LCE_CUDA(cudaMemcpyAsync(h->res_host, h->d_loss, 4, cudaMemcpyDeviceToHost, h->stream));
