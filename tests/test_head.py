@@ -751,13 +751,15 @@ def test_one_entry_is_the_cross_entropy_of_the_step(r, T):
 
 @gpu
 @pytest.mark.parametrize("r", [4, 16])
-def test_streams_graphs_and_repeats(r):
+@pytest.mark.parametrize("T", [12, 300, 700])  # few positions; most; masked ones among them
+def test_streams_graphs_and_repeats(T, r):
     """The same bits from another stream, from a captured and replayed graph with
     new inputs in its buffers, and from two calls at once."""
     torch = pytest.importorskip("torch")
-    p, o = Problem(300, 4099, 128, r), Problem(300, 4099, 128, r, seed=1)
+    p, o = Problem(T, 4099, 128, r), Problem(T, 4099, 128, r, seed=1)
     for x in (p, o):
         x.lists(8)
+        x.weight = x.u(T) * (x.u(T) < 0.5) if T == 700 else torch.ones(T, device="cuda")
     first = dict(p.score(8), **p.distill(2.0))
     other = dict(o.score(8), **o.distill(2.0))
     torch.cuda.synchronize()
@@ -781,7 +783,7 @@ def test_streams_graphs_and_repeats(r):
         p.score(8, out=so, ws=ws1, stream=torch.cuda.current_stream())
         p.distill(2.0, out=do, ws=ws2, stream=torch.cuda.current_stream())
     for q, want in ((o, other), (p, first), (o, other)):
-        keep = {k: getattr(q, k).clone() for k in ("H", "A", "B", "W", "ids", "teacher", "tokens")}
+        keep = {k: getattr(q, k).clone() for k in ("H", "A", "B", "W", "ids", "teacher", "tokens", "weight")}
         for k, v in keep.items():
             getattr(p, k).copy_(v)
         graph.replay()
@@ -791,8 +793,9 @@ def test_streams_graphs_and_repeats(r):
         if q is p:
             continue
         # p's own inputs come back for the next round
-        fresh = Problem(300, 4099, 128, r)
+        fresh = Problem(T, 4099, 128, r)
         fresh.lists(8)
+        fresh.weight = fresh.u(T) * (fresh.u(T) < 0.5) if T == 700 else torch.ones(T, device="cuda")
         for k in keep:
             getattr(p, k).copy_(getattr(fresh, k))
 
