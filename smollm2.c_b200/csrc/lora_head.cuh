@@ -1389,10 +1389,12 @@ constexpr int kScoreRows = 4;  // positions per block where each has a warp
 // the n_pick-th largest logit; the candidates are the logits that reach it, less what
 // rounding may have moved; compute again those whose order the pass's logits do not
 // tell, sort, write.  The softmax's sums get the difference.
-// 4,096 positions, 64 alternatives: 115 us, 140 with every candidate computed again,
-// which was five groups of 16 rows of W a position, read from L2.
+// 4,096 positions, 64 alternatives: 103 us (with every candidate computed again, five
+// groups of 16 rows of W a position, 25 more).  Waits for L2 and for instructions; 16
+// warps an SM, with the registers that leaves, do better than 20 (115), 24 (142) or 12
+// (112).
 template <int TW, int NK>
-static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW == 8 ? 2 : 5)
+static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW == 8 ? 2 : TW == 1 ? 4 : 5)
     lh_score_rows(ScoreArgs a) {
   constexpr int kTeams = TW == 1 ? kScoreRows : 1;
   constexpr int kThreads = 32 * TW;
@@ -1835,7 +1837,7 @@ struct DistillArgs {
 // and of B per position, 100 KB, from L2.
 template <bool kGrads, int TW>
 static __global__ void
-    __launch_bounds__(32 * (TW == 1 ? kRowWarps : TW), TW == 1 ? 3 : TW == 4 ? 4 : 2)
+    __launch_bounds__(32 * (TW == 1 ? kRowWarps : TW), TW == 8 ? 2 : TW == 4 ? 4 : kGrads ? 3 : 2)
     lh_distill_rows(DistillArgs a) {
   constexpr int kTeams = TW == 1 ? kRowWarps : 1, kThreads = 32 * TW;
   constexpr int kPer = (kMaxTop + kThreads - 1) / kThreads;
