@@ -1384,6 +1384,67 @@ __host__ __device__ inline size_t score_team_smem(int n_pick, int cap, int warps
 }
 constexpr int kScoreRows = 4;  // positions per block where each has a warp
 
+// Cuts a position's list of candidates [c_0, n_c) to `keep` (at least C) of them: the
+// threshold rises to the C-th largest of the list, what lies below it goes, and of its
+// near ties the highest ids.  For lists that overflow: a record of many large logits,
+// or many such records.
+struct Cut {
+  int n_c;  // the new end
+  float bound, above;
+};
+template <int TW>
+__device__ __noinline__ Cut tidy_candidates(Team<TW> team, int C, int keep, int c_0, int n_c,
+                                            float eps, float bound, float above, int* ids,
+                                            float* approx, float* approx32, int* ranks, float* kth,
+                                            int* words) {
+  team.sync();
+  for (int c = c_0 + team.tid; c < n_c; c += team.kThreads)
+    if (approx[c] > -INFINITY) approx32[c] = approx[c];
+  team.sync();
+  for (int c = c_0 + team.tid; c < n_c; c += team.kThreads) {
+    int rank = 0;
+    for (int q = c_0; q < n_c; ++q)
+      rank += approx32[q] > approx32[c] || (approx32[q] == approx32[c] && q < c);
+    if (rank == C - 1) *kth = approx32[c];
+  }
+  team.sync();
+  bound = fmaxf(bound, *kth - eps);
+  above = fmaxf(above, *kth + eps);
+  int n_above = 0;
+  for (int c = c_0; c < n_c; ++c) n_above += approx32[c] > above;
+  for (int c = c_0 + team.tid; c < n_c; c += team.kThreads) {
+    bool stays = approx32[c] > above;
+    if (!stays && approx32[c] >= bound) {
+      int before = n_above;
+      for (int q = c_0; q < n_c; ++q)
+        before += approx32[q] >= bound && !(approx32[q] > above) && ids[q] < ids[c];
+      stays = before < keep;
+    }
+    ranks[c] = stays;
+  }
+  team.sync();
+  if (team.w == 0) {
+    int n = c_0;
+    for (int c0 = c_0; c0 < n_c; c0 += 32) {
+      const int c = c0 + team.lane, at = min(c, n_c - 1);
+      const int id = ids[at];
+      const float x = approx[at], y = approx32[at];
+      const unsigned b = __ballot_sync(0xffffffffu, c < n_c && ranks[at] != 0);
+      if (b >> team.lane & 1u) {
+        const int to = n + __popc(b & ((1u << team.lane) - 1u));
+        ids[to] = id;
+        approx[to] = x;
+        approx32[to] = y;
+      }
+      n += __popc(b);
+      __syncwarp();
+    }
+    if (team.lane == 0) words[15] = n;
+  }
+  team.sync();
+  return Cut{words[15], bound, above};
+}
+
 // One team per position, NK records per thread.  Merge the sums; bisect for a
 // threshold that n_pick to n_pick + kPickStop records reach: it is a lower bound of
 // the n_pick-th largest logit; the candidates are the logits that reach it, less what
@@ -1517,7 +1578,8 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   // P (equal or nearly equal maxima, as of a padding row), those surely above it
   // and of the others the lowest
   const float eps = 1e-5f * (1.0f + fmaxf(fabsf(lo), fabsf(rs.M)));
-  const float bound = lo - eps, above = lo + eps;
+  float bound = lo - eps, above = lo + eps;
+  const float first = bound;  // what a record's second had to reach
   int room = P;
   bool crowded;
   {
@@ -1618,30 +1680,49 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
       }
       n_c += __popc(b);
     }
-  for (int c0 = 0; c0 < n_p && a.sub > 1; c0 += 32) {
-    unsigned more = __ballot_sync(kAll, c0 + lane < n_p && prest[min(c0 + lane, n_p - 1)] >= bound);
-    for (; more && n_c < a.cap; more &= more - 1) {
-      const int c = c0 + __ffs(more) - 1;
-      const int v0 = picked[c] * a.sub, c1 = pcol[c] & 255, nv = min(a.sub, a.z.V - v0);
-      const int c2 = a.sub == 64 && psecond[c] >= bound ? pcol[c] >> 8 : -1;
-      for (int q = tid; q < nv; q += kThreads) col_id[q] = v0 + q;
-      team.sync();
-      for (int q = 16 * w; q < nv; q += 16 * TW)
-        logits16<false>(a.z, t, col_id + q, min(16, nv - q), lane, cols + q);
-      team.sync();
-      for (int q0 = 0; q0 < nv; q0 += 32) {  // (every warp finds the same)
-        const int q = q0 + lane;
-        const bool take = q < nv && q != c1 && q != c2 && cols[q] >= bound;
-        const unsigned bt = __ballot_sync(kAll, take);
-        const int at = n_c + __popc(bt & below);
-        if (take && w == 0 && at < a.cap) {
-          ids[at] = v0 + q;
-          approx[at] = -INFINITY;  // not known: the sums keep it as it is
-          approx32[at] = cols[q];
+  // First the records whose rest lies above the threshold: their columns may come
+  // before all that is known, however many ties the threshold has.  Then those whose
+  // rest is a near tie of it, lowest ids first, as far as there is room.
+  for (int ph = 0; ph < 2 && a.sub > 1; ++ph) {
+    auto tidy = [&] {
+      const Cut cut = tidy_candidates(team, C, 2 * P, c_0, n_c, eps, bound, above, ids, approx,
+                                      approx32, ranks, cols, words);
+      n_c = cut.n_c;
+      bound = cut.bound;
+      above = cut.above;
+    };
+    if (ph == 1 && n_c - c_0 > 2 * P) tidy();
+    for (int c0 = 0; c0 < n_p; c0 += 32) {
+      const float rest = c0 + lane < n_p ? prest[c0 + lane] : -INFINITY;
+      unsigned more = __ballot_sync(kAll, rest >= bound && (ph == 1 || rest > above));
+      for (; more && n_c < a.cap; more &= more - 1) {
+        const int c = c0 + __ffs(more) - 1;
+        if (ph == 0) {
+          if (n_c - c_0 > 2 * P) tidy();
+          if (!(prest[c] > above)) continue;  // the threshold has risen
         }
-        n_c = min(n_c + __popc(bt), a.cap);
+        const int v0 = picked[c] * a.sub, c1 = pcol[c] & 255, nv = min(a.sub, a.z.V - v0);
+        const int c2 = a.sub == 64 && psecond[c] >= first ? pcol[c] >> 8 : -1;
+        for (int q = tid; q < nv; q += kThreads) col_id[q] = v0 + q;
+        team.sync();
+        if (ph == 0 && tid == 0) prest[c] = -INFINITY;  // done with
+        for (int q = 16 * w; q < nv; q += 16 * TW)
+          logits16<false>(a.z, t, col_id + q, min(16, nv - q), lane, cols + q);
+        team.sync();
+        for (int q0 = 0; q0 < nv; q0 += 32) {  // (every warp finds the same)
+          const int q = q0 + lane;
+          const bool take = q < nv && q != c1 && q != c2 && cols[q] >= bound;
+          const unsigned bt = __ballot_sync(kAll, take);
+          const int at = n_c + __popc(bt & below);
+          if (take && w == 0 && at < a.cap) {
+            ids[at] = v0 + q;
+            approx[at] = -INFINITY;  // not known: the sums keep it as it is
+            approx32[at] = cols[q];
+          }
+          n_c = min(n_c + __popc(bt), a.cap);
+        }
+        team.sync();
       }
-      team.sync();
     }
   }
   // The pass's logits, made good for their known loss, are off by a few 1e-7 of z:
