@@ -75,8 +75,8 @@ int lora_head_score(const lora_head* head, const void* H, int32_t h_dtype, int32
 
 /* Distillation.  ids, teacher [T][K] (K 1..128): the teacher's top logits (or
  * log probabilities; a constant per row cancels) and their token ids.  An entry
- * with a negative id is absent and its logit not looked at; a logit of -inf
- * weighs nothing; entries of one row with the same id add up.  With
+ * with a negative id is absent and its logit not looked at; so is one of an id
+ * below vocab with a logit of -inf; entries of one row with the same id add up.  With
  *   q = softmax(teacher[t] / temperature) over the row's entries,
  *   p = softmax(z[t] / temperature) over the vocabulary,
  *   loss[t] = weight[t] temperature^2 sum_k q_k (log q_k - log p[ids_k]).

@@ -790,7 +790,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
     return *why = "cudaMemsetAsync failed", LORA_CE_ECUDA;
   // weights may leave whole tiles of positions without one that counts
   const bool order = weight && !few && T > 2 * kBM;
-  if (order && !launch_plain(lh_order, 1, 1024, 0, st, T, K, weight, ids, w.masks, w.order, w.stats))
+  if (order && !launch_plain(lh_order, 1, 1024, 0, st, T, K, hd.V, weight, ids,
+                             teacher, w.masks, w.order, w.stats))
     return *why = kNoLaunch, LORA_CE_ECUDA;
   s.g.active = order ? w.stats + kStActive : nullptr;
   PrepArgs pa = prep_args(hd, aug, H, dtype, T);
@@ -800,6 +801,8 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pa.haug = aug.width ? w.haug : nullptr;
   pa.stats = w.stats;
   pa.ids = ids;
+  pa.teacher = teacher;
+  pa.V = hd.V;
   pa.weight = weight;
   pa.K = K;
   pa.tau = tau;

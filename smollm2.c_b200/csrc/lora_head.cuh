@@ -241,6 +241,8 @@ struct PrepArgs {
   // position that has at least one entry, else 0 (and its hidden state is read
   // as zeros, whatever it holds)
   const int32_t* ids;
+  const float* teacher;
+  int V;
   const float* weight;
   int K;
   float tau;
@@ -250,6 +252,12 @@ struct PrepArgs {
   __device__ __forceinline__ int source(int t) const { return order ? order[t] : t; }
 };
 
+// A teacher's entry that is there: a logit of -inf weighs nothing, as no entry does.
+// (Ids past the vocabulary, NaN and +inf are: lh_distill_rows reports them.)
+__device__ __forceinline__ bool is_entry(int id, float logit, int V) {
+  return id >= 0 && (id >= V || logit != -INFINITY);
+}
+
 // order: the positions that count (a weight other than 0 and an entry), then the
 // others, each in ascending order; their number to stats[kStActive].  The passes run
 // over the tiles that hold one that counts, a quarter of all at least: at 8,000
@@ -257,9 +265,10 @@ struct PrepArgs {
 // instead of 2,300.
 // One block: each warp takes a run of positions, 32 side by side at a time (a
 // thread for a run of its own, its loads and stores a line each, took 13 us instead of 11).
-static __global__ void __launch_bounds__(1024) lh_order(int T, int K,
+static __global__ void __launch_bounds__(1024) lh_order(int T, int K, int V,
                                                         const float* __restrict__ weight,
                                                         const int32_t* __restrict__ ids,
+                                                        const float* __restrict__ teacher,
                                                         unsigned* __restrict__ masks,  // [T / 32]
                                                         int* __restrict__ order,
                                                         int* __restrict__ stats) {
@@ -272,24 +281,24 @@ static __global__ void __launch_bounds__(1024) lh_order(int T, int K,
   int n = 0;
   for (int g0 = g_lo; g0 < g_hi; g0 += kStep) {
     float wt[kStep];
-    int id[kStep];
+    bool first[kStep];
 #pragma unroll
     for (int i = 0; i < kStep; ++i) {
       const int t = 32 * (g0 + i) + lane;
       const bool in = g0 + i < g_hi && t < T;
       wt[i] = in ? weight[t] : 0.f;
-      id[i] = in ? ids[(long long)t * K] : 0;
+      first[i] = in && is_entry(ids[(long long)t * K], teacher[(long long)t * K], V);
     }
 #pragma unroll
     for (int i = 0; i < kStep; ++i) {
       if (g0 + i >= g_hi) break;
-      bool any = wt[i] != 0.f && id[i] >= 0;
-      unsigned look = __ballot_sync(kAll, wt[i] != 0.f && id[i] < 0);
+      bool any = wt[i] != 0.f && first[i];
+      unsigned look = __ballot_sync(kAll, wt[i] != 0.f && !first[i]);
       for (; look; look &= look - 1) {  // the first entry is absent: seldom
         const int q = __ffs(look) - 1;
+        const long long o = (long long)(32 * (g0 + i) + q) * K;
         bool some = false;
-        for (int k = lane; k < K; k += 32)
-          some |= ids[(long long)(32 * (g0 + i) + q) * K + k] >= 0;
+        for (int k = lane; k < K; k += 32) some |= is_entry(ids[o + k], teacher[o + k], V);
         some = __any_sync(kAll, some);
         if (lane == q) any = some;
       }
@@ -398,7 +407,8 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
   bool active = true;
   const int from = a.source(t);
   if (a.ids) {
-    const bool mine = tid < a.K && a.ids[(long long)from * a.K + tid] >= 0;
+    const long long o = (long long)from * a.K + tid;
+    const bool mine = tid < a.K && is_entry(a.ids[o], a.teacher[o], a.V);
     wt = row_weight(a, from, __syncthreads_or(mine));
     active = wt != 0.f;
     if (tid == 0) a.wt[t] = wt;
@@ -469,7 +479,8 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
 #pragma unroll
       for (int q = 0; q < kMaxTop / 16; ++q) {
         const int k = (tid & 15) + 16 * q;
-        any |= k < a.K && a.ids[(long long)from * a.K + k] >= 0;
+        const long long o = (long long)from * a.K + k;
+        any |= k < a.K && is_entry(a.ids[o], a.teacher[o], a.V);
       }
     }
     const unsigned b = __ballot_sync(0xffffffffu, any) >> (lane & 16) & 0xffffu;
@@ -1976,7 +1987,6 @@ static __global__ void
   if (nslot == 0) rs = RowSum{0.f, 1.0, 0.0};
   wrong = team.count(wrong);
   top = team.reduce(top, [](double p, double q) { return fmax(p, q); });
-  if (top == -INFINITY && !wrong) wt = 0.f;  // no entry left
   double total = 0.0;
   double e[kPer];
 #pragma unroll

@@ -6,7 +6,7 @@ import math
 
 import pytest
 
-from test_head import Problem, check_score
+from test_head import Problem, check_distill, check_score
 
 gpu = pytest.mark.gpu
 
@@ -59,3 +59,68 @@ def test_larger_logits_are_not_lost_among_ties(T, V, k, what):
     wherever they lie and however many ties there are."""
     p = Given(T, _crowds(V, what))
     check_score(p, k, p.score(k))
+
+
+@gpu
+@pytest.mark.parametrize("r", [3, 8, 16, 64])
+@pytest.mark.parametrize("T", [7, 31, 100, 300, 1500])
+@pytest.mark.parametrize("weights", [False, True])
+def test_rows_whose_entries_are_all_minus_infinity_hold_anything(T, r, weights):
+    """Such a row has no entry: loss 0 and no part in the gradients, the same bits
+    as with no ids, with NaN and infinities in its hidden state."""
+    import torch
+    V, K = 1000, 6
+    p = Problem(T, V, 64, r, "f32")
+    p.lists(K, ragged=False)
+    p.weight = torch.where(torch.arange(T, device="cuda") % 3 == 0, 0.0, 1.0) if weights else None
+    off = torch.arange(T, device="cuda") % 5 == 2
+    p.teacher[off] = -math.inf
+    p.teacher[::2, 0] = -math.inf  # and some first entries alone
+    ids = p.ids.clone()
+    p.ids[off] = -1
+    clean = p.distill(1.5), p.distill(1.5, grads=False)["loss"]
+    p.ids = ids
+    check_distill(p, 1.5)
+    p.H[off, 1] = math.nan
+    p.H[2] = math.inf
+    got = p.distill(1.5), p.distill(1.5, grads=False)["loss"]
+    for key in clean[0]:
+        assert bool(torch.isfinite(clean[0][key]).all()), key
+        assert torch.equal(got[0][key], clean[0][key]), key
+    assert torch.equal(got[1], clean[1]) and bool((got[1][off] == 0).all())
+    # an id past the vocabulary is reported whatever its logit
+    p.ids[2, 3] = V
+    if weights:
+        p.weight[2] = 1
+    assert math.isnan(float(p.distill(1.5)["loss"][2]))
+
+
+@gpu
+def test_a_step_counts_no_row_of_minus_infinity():
+    """The trainer's mean is over rows with an entry."""
+    import numpy as np
+
+    import lora_ce
+    T, V, d, r, K = 40, 500, 64, 4, 3
+    rng = np.random.default_rng(5)
+    W = (rng.standard_normal((V, d)) / 8).astype(np.float16)
+    H = rng.standard_normal((T, d)).astype(np.float32)
+    ids = rng.integers(0, V, (T, K)).astype(np.int32)
+    z = rng.standard_normal((T, K)).astype(np.float32)
+    losses = []
+    for absent in (True, False):
+        m = lora_ce.LoraCE(lora_ce.default_config(d, V, r, T))
+        m.set_weight(W.view(np.uint16))
+        m.set_adapter(np.full((d, r), 0.1, np.float32),
+                      np.full((r, V), 0.01, np.float32), 0)
+        i, t, h = ids.copy(), z.copy(), H.copy()
+        if absent:
+            i[5:20] = -1
+        else:
+            t[5:20] = -np.inf
+            h[5:20, 3] = np.nan
+        losses.append(m.distill_step(h, i, t, 1.0))
+        losses.append(m.get_adapter()[1].copy())
+        m.close()
+    assert losses[0] == losses[2] and np.isfinite(losses[0])
+    assert np.isfinite(losses[1]).all() and np.array_equal(losses[1], losses[3])
