@@ -53,7 +53,9 @@ typedef struct lora_ce_config {
     int32_t rank;       /* r: 1..256, LORA_MAX_RANK (src/train.c:20).  Run
                            at 4, 8, 16, 32, 64, 128 or 256 with zero
                            padding, which leaves every result unchanged;
-                           ranks above 64 take a slower path that keeps the
+                           ranks 5 to 64 have scale.(h.A) and B as pairs of
+                           f16 (a magnitude of 65,520 or more counts as an
+                           infinity); ranks above 64 take a slower path that keeps the
                            logit rows of a block of positions in HBM */
     float scale;        /* alpha / r (train_create: src/train.c:62-63) */
     float lr;           /* learning rate */

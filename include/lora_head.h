@@ -9,7 +9,9 @@
  *
  *   z[t] = h[t].W^T + scale.(h[t].A).B      h = f16(H), as lora_ce_step reads it
  *
- * and never write the T x V logits to memory.  They keep no state: every
+ * and never write the T x V logits to memory.  As in the step, ranks above 4 have
+ * scale.(h.A) and B as pairs of f16: a magnitude of 65,520 or more counts as an
+ * infinity (calls of few positions take it as it is).  They keep no state: every
  * buffer is the caller's and lies on the current device (a pointer to other
  * memory is refused), the work is enqueued on `stream` (a cudaStream_t; NULL =
  * legacy default stream) and the call returns without waiting.  The workspace

@@ -147,6 +147,7 @@ struct GemmArgs {
   // times the accumulator correction), and the lazy-max thresholds in units of z
   float lg, lazy, redo;
   float drain_gain;   // 1 + the relative loss of one accumulation of rank sums (lce_gemm_tc)
+  const float* sU4;   // EpiScore of ranks up to 4: [T][4] s * U
   // EpiScore (lora_head.cuh): entropy sums, and the records of a row's logits
   float* p_ent;       // [seg][Tcap]
   float* sub_max;     // [T / 8][n_sub][8]: eight rows' records side by side

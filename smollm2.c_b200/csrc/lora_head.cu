@@ -42,7 +42,8 @@ int entry(F&& body) {
   return rc;
 }
 
-// How the rank term joins the MMA: one K-block up to rank 16, 2R columns above.
+// How the rank term joins the MMA: one K-block up to rank 16, 2R columns above; not
+// at all up to rank 4, where the epilogues add it in f32.
 // Its operands are only as wide as they are used (a multiple of 16 bytes); the
 // loads fill the rest of a 64-column block with zeros.
 struct Aug {
@@ -52,6 +53,7 @@ Aug aug_of(int r) {
   Aug a;
   if (r == 0) return a;
   a.R = kernel_rank(r);
+  if (a.R == 4) return a;
   a.layout = a.R <= 16 ? 1 : 2;
   a.width = a.R <= 16 ? (3 * a.R + 7) / 8 * 8 : 2 * a.R;
   return a;
@@ -62,9 +64,7 @@ void aug_schedule(GemmArgs& g, const Aug& a) {
     case 16: RankPlan<16>::schedule(g); break;
     case 32: RankPlan<32>::schedule(g); break;
     case 64: RankPlan<64>::schedule(g); break;
-    default:
-      g.n_aug = a.R ? 1 : 0;  // rank 4: 12 of 64 columns, one K-step
-      g.aug_a[0] = g.aug_b[0] = 0;
+    default: g.n_aug = 0;
   }
 }
 
@@ -228,22 +228,27 @@ struct PassPlan {
   int threads = 0, smem = 0;
 };
 
-// EpiScore with the largest ring that fits beside the resident K-blocks.
+// EpiScore with the largest ring that fits beside the resident K-blocks (and, up to
+// rank 4, two tiles of staged rows of B).
 template <class Epi>
 PassPlan plan_of(int kblocks) {
-  return PassPlan{lce_gemm_kernel<Epi, false, 2>, block_threads(Epi::kWarps),
-                  SmemLayout::bytes(kblocks, 0, Epi::kRing)};
+  constexpr bool kStaged = Epi::kRec != 0;
+  return PassPlan{lce_gemm_kernel<Epi, kStaged, 2>, block_threads(Epi::kWarps),
+                  SmemLayout::bytes(kblocks, Epi::kRec * Epi::kRecBufs, Epi::kRing)};
 }
 template <int kSub>
-PassPlan score_plan(int kblocks) {
-  return kblocks <= 10   ? plan_of<EpiScore<65536, kSub>>(kblocks)
-         : kblocks == 11 ? plan_of<EpiScore<49152, kSub>>(kblocks)
-                         : plan_of<EpiScore<32768, kSub>>(kblocks);
+PassPlan score_plan(int kblocks, bool r4) {
+  if (r4)
+    return kblocks <= 9 ? plan_of<EpiScore<65536, kSub, true>>(kblocks)
+                        : plan_of<EpiScore<49152, kSub, true>>(kblocks);
+  return kblocks <= 10   ? plan_of<EpiScore<65536, kSub, false>>(kblocks)
+         : kblocks == 11 ? plan_of<EpiScore<49152, kSub, false>>(kblocks)
+                         : plan_of<EpiScore<32768, kSub, false>>(kblocks);
 }
-PassPlan score_plan(int kblocks, int sub) {
-  return sub == 64  ? score_plan<64>(kblocks)
-         : sub == 8 ? score_plan<8>(kblocks)
-         : sub == 1 ? score_plan<1>(kblocks) : score_plan<0>(kblocks);
+PassPlan score_plan(int kblocks, int sub, bool r4) {
+  return sub == 64  ? score_plan<64>(kblocks, r4)
+         : sub == 8 ? score_plan<8>(kblocks, r4)
+         : sub == 1 ? score_plan<1>(kblocks, r4) : score_plan<0>(kblocks, r4);
 }
 
 // Columns per record: the widest that leaves four records per alternative.
@@ -354,7 +359,7 @@ bool launch_few(const FewArgs& f, int blocks, cudaStream_t st) {
 struct ScoreWs {
   int* stats;
   __half *h16, *haug, *waug;
-  float *sU, *p_max, *p_sum, *p_ent, *sub_max, *sub_second, *sub_rest;
+  float *sU, *Bt, *p_max, *p_sum, *p_ent, *sub_max, *sub_second, *sub_rest;
   uint8_t *sub_arg, *sub_arg2;
   int sub, n_sub;
   size_t bytes;
@@ -367,8 +372,8 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
   const long long Vpad = round_up(hd.V, kBN);
   const int n_a = (T + 2 * kBM - 1) / (2 * kBM), n_b = (int)(Vpad / kBN);
   w.sub = record_columns(hd.V, top_k);
-  const size_t part = few_score(T, aug.R, w.sub)
-                          ? (size_t)few_blocks(hd.V) * kFewMax
+  const bool few = few_score(T, aug.R, w.sub);
+  const size_t part = few ? (size_t)few_blocks(hd.V) * kFewMax
                           : (size_t)4 * most_segments(n_a, n_b) * n_a * 2 * kBM;
   w.n_sub = (hd.V + w.sub - 1) / w.sub;
   w.stats = c.take<int>(kStatWords);
@@ -376,6 +381,7 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
   w.sU = c.take<float>((size_t)T * aug.R);
   w.haug = c.take<__half>((size_t)T * aug.width);
   w.waug = c.take<__half>((size_t)Vpad * aug.width);
+  w.Bt = c.take<float>(aug.R == 4 && !few && !hd.layout ? (size_t)Vpad * 4 : 0);
   w.p_max = c.take<float>(part);
   w.p_sum = c.take<float>(part);
   w.p_ent = c.take<float>(part);
@@ -429,19 +435,17 @@ DistillWs distill_ws(const HeadCore& hd, int T, bool grads, void* ws) {
   }
   w.order = c.take<int>(T);
   w.masks = c.take<unsigned>((T + 31) / 32);
-  // rank 4 keeps the rank term in the epilogues of the gradient passes
-  const bool in_mma = !grads || R > 4;
-  w.haug = c.take<__half>(in_mma ? (size_t)T * aug.width : 0);
-  w.waug = c.take<__half>(in_mma ? (size_t)Vpad * aug.width : 0);
+  w.haug = c.take<__half>((size_t)T * aug.width);
+  w.waug = c.take<__half>((size_t)Vpad * aug.width);
   w.p_max = c.take<float>(part);
   w.p_sum = c.take<float>(part);
+  if (grads || R == 4) w.Bt = c.take<float>(hd.layout ? 0 : (size_t)Vpad * R);
   if (grads) {
     // chunks of four or eight epilogue columns a row: up to 4 slots per owner
     const int n_a2 = (hd.V + 2 * kBM - 1) / (2 * kBM), n_b2 = (T + bn - 1) / bn;
     const size_t segs = (size_t)(tc ? 1 : 4) * most_segments_by_b(n_a2, n_b2);
     w.p_q = c.take<float>(part * R);
     w.tok = c.take<float>(tc ? 0 : (size_t)Tpad * tok_stride(R));
-    w.Bt = c.take<float>(hd.layout ? 0 : (size_t)Vpad * R);
     w.xv = c.take<__half>(tc ? (size_t)2 * R * Vpad : 0);
     w.xt = c.take<__half>(tc ? (size_t)2 * R * Tpad : 0);
     w.nml = c.take<float>(tc ? (size_t)Tpad + kMaxBNT : 0);
@@ -648,9 +652,10 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
                    float* top_logprobs, void* ws, cudaStream_t st, const char** why) {
   Aug aug = aug_of(hd.r);
   const ScoreWs w = score_ws(hd, T, top_k, ws);
-  const bool few = few_score(T, aug.R, w.sub);
+  const bool few = few_score(T, aug.R, w.sub), r4 = aug.R == 4 && !few;
   if (few) aug.layout = aug.width = 0;  // the rank term from B as it is
   const int sms = sm_count();
+  const float* const Bt = !r4 ? nullptr : hd.layout ? hd.B : w.Bt;
   GemmArgs g{};
   fill_pass1(g, hd, aug, T, 1.0f);
   g.n_b = (int)(g.Vpad / kBN);
@@ -664,6 +669,8 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   g.sub_arg = w.sub_arg;
   g.sub_arg2 = w.sub_arg2;
   g.n_sub = w.n_sub;
+  g.sU4 = w.sU;
+  g.Bt = Bt;
   // per-row kernel: a warp per position, or four where that many positions do not
   // fill the SMs (eight where there are more than 1,024 records).  V = 49152, whole
   // calls in us, four warps against one: 8 alternatives at 600 / 1,184 / 2,047 / 3,000
@@ -696,6 +703,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   pk.r = hd.r;
   pk.R = aug.R;
   pk.Vpad = g.Vpad;
+  pk.Bt = r4 && !hd.layout ? w.Bt : nullptr;
   pk.waug = aug.width ? w.waug : nullptr;
   pk.aug_layout = aug.layout;
   pk.aug_width = aug.width;
@@ -718,7 +726,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
     a.p = SlotPlan{1, 1, blocks, blocks, f.ld, w.p_max, w.p_sum, w.p_ent, nullptr};
     a.lg = lg;
   } else {
-    const PassPlan p = score_plan(g.kblocks, w.sub);
+    const PassPlan p = score_plan(g.kblocks, w.sub, r4);
     const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
                                                          p.threads, p.smem));
     if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
@@ -730,16 +738,17 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
     if (aug.width && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
                       !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
       return *why = kNoMap, LORA_CE_ECUDA;
-    if (launch_prep(pa, pk, true, 0, pk.waug != nullptr, sms, st))
+    if (launch_prep(pa, pk, true, 0, pk.Bt || pk.waug, sms, st))
       return *why = kNoFit, LORA_CE_ECUDA;
     const int G = (int)std::min<long long>(units, (long long)g.n_a * g.n_b);
     if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, g))
       return *why = kNoLaunch, LORA_CE_ECUDA;
-    a.p = SlotPlan{col_parts(EpiScore<65536, 64>::kWarps), g.n_a, g.n_b, units, g.Tcap,
+    a.p = SlotPlan{col_parts(EpiScore<65536, 64, false>::kWarps), g.n_a, g.n_b, units, g.Tcap,
                    w.p_max, w.p_sum, w.p_ent, nullptr};
     a.lg = g.lg;
   }
   a.z = logit_args(hd, aug, T, w.h16, w.sU, w.haug, w.waug);
+  if (Bt) a.z.B = BView{Bt, hd.V, hd.r, aug.R, 1};  // a row's ranks side by side
   a.sub_max = w.sub_max;
   a.sub_second = w.sub_second;
   a.sub_rest = w.sub_rest;
@@ -773,15 +782,16 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   const int R = aug.R;
   const DistillWs w = distill_ws(hd, T, grads, ws);
   const bool few = few_distill(T, R), tc = grads && R >= 16 && !few;
-  if ((grads && R == 4) || few) aug.layout = aug.width = 0;  // no packed rank term
+  if (few) aug.layout = aug.width = 0;  // the rank term from B as it is
   Step s{hd, w, aug, T, sm_count(), tau, st, GemmArgs{}, SlotPlan{}};
   fill_pass1(s.g, hd, aug, T, tau);
-  s.Bt = few ? nullptr : hd.layout ? hd.B : w.Bt;
+  s.Bt = few || !(grads || R == 4) ? nullptr : hd.layout ? hd.B : w.Bt;
   s.g.err = w.stats + kStErr;
   s.g.p_max = w.p_max;
   s.g.p_sum = w.p_sum;
   s.g.p_q = w.p_q;
   s.g.tok = w.tok;
+  s.g.sU4 = w.sU;
   s.g.Bt = s.Bt;
   s.g.gBp = w.gBp;
   s.g.nml = w.nml;
@@ -817,7 +827,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pk.r = hd.r;
   pk.R = R;
   pk.Vpad = s.g.Vpad;
-  pk.Bt = grads && !few && !hd.layout ? w.Bt : nullptr;
+  pk.Bt = s.Bt && !hd.layout ? w.Bt : nullptr;
   pk.Bt_plain = tc;  // the rank sums' passes have xv instead
   pk.waug = aug.width ? w.waug : nullptr;
   pk.aug_layout = aug.layout;
@@ -844,7 +854,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   } else if (grads) {
     rc = grad_pass<1>(s, R, why);
   } else {
-    const PassPlan p = score_plan(s.g.kblocks, 0);
+    const PassPlan p = score_plan(s.g.kblocks, 0, R == 4);
     const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
                                                          p.threads, p.smem));
     if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
@@ -860,7 +870,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
     const int G = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
     if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, s.g))
       rc = (*why = kNoLaunch, LORA_CE_ECUDA);
-    s.slots = SlotPlan{col_parts(EpiScore<65536, 0>::kWarps), s.g.n_a, s.g.n_b, units,
+    s.slots = SlotPlan{col_parts(EpiScore<65536, 0, false>::kWarps), s.g.n_a, s.g.n_b, units,
                        s.g.Tcap, w.p_max, w.p_sum, nullptr, nullptr};
   }
   if (rc) return rc;
@@ -868,6 +878,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   a.z = logit_args(hd, aug, T, w.h16, w.sU, w.haug, w.waug);
   a.z.R = R;
   a.z.B.R = R;
+  if (s.Bt && R == 4) a.z.B = BView{s.Bt, hd.V, hd.r, R, 1};  // a row's ranks side by side
   a.p = s.slots;
   a.lg = few ? few_lg : s.g.lg;
   a.tau = tau;

@@ -73,17 +73,17 @@ __device__ __forceinline__ long long sub_idx(int t, int k, int n_sub) {
 // Bound by the MMAs and their loads of W, as the training step's passes (tensor
 // pipe 54% busy), not by the epilogue: without records or entropy (kSub 0) it is
 // no faster, nor with the two largest of a chunk from a tree of min and max on
-// logits that carry their column in the lowest bits, nor with the rank-4 term in
-// the epilogue instead of a tenth K-block, nor with a fifth ring stage.
-// 8,192 positions, V = 49152, d = 576, rank 4: 415 us, 1.24 PFLOP/s with the rank
-// term's K-block counted.
-template <int kRing_, int kSub>
+// logits that carry their column in the lowest bits, nor with a fifth ring stage.
+// kR4: the rank term of ranks up to 4 here, in f32 from staged rows of B (as EpiLse),
+// so that those ranks have f32's range, as in the training step.  As f16 pairs in a
+// K-block of its own a call of 8,192 positions took 581 us instead of 592.
+template <int kRing_, int kSub, bool kR4>
 struct EpiScore {
-  static constexpr bool kAug = true;
+  static constexpr bool kAug = !kR4;
   static constexpr bool kDepend = true;
-  static constexpr int kRec = 0;
+  static constexpr int kRec = kR4 ? 4 : 0;
   static constexpr int kRing = kRing_;
-  static constexpr int kRecBufs = 1;
+  static constexpr int kRecBufs = kR4 ? 2 : 1;
   static constexpr int kWarps = 16;
   static constexpr int kCW = 8;
   static constexpr bool kTop = kSub != 0;
@@ -95,8 +95,11 @@ struct EpiScore {
   float S, Slo, E, Elo;  // the same over the row so far, folded every 64 columns (as EpiLse)
   float r1, r2, rest;    // kSub 64: the record so far
   int a1, a2;
+  float2 sU2[kR4 ? 4 : 1];
 
-  __device__ static const float* global_recs(const GemmArgs& g, int) { return g.Bt; }
+  __device__ static const float* global_recs(const GemmArgs& g, int b) {
+    return g.Bt + (long long)b * kBN * kRec;
+  }
   __device__ static int limit(const GemmArgs& g) { return g.V; }
 
   __device__ void begin(const GemmArgs& g, int abs_row) {
@@ -107,6 +110,12 @@ struct EpiScore {
     S = Slo = E = Elo = 0.f;
     r1 = r2 = rest = -INFINITY;
     a1 = a2 = 0;
+    if constexpr (kR4) {
+      float u[4];
+      ld_vec<4>(g.sU4 + 4ll * (valid ? t : 0), u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sU2[j] = f2(u[j], u[j]);
+    }
   }
 
   // Adds the chunk's terms at reference nm = -(reference max) * lg; the first `n_in`
@@ -129,7 +138,19 @@ struct EpiScore {
 
   template <bool kTail>
   __device__ __forceinline__ void chunk(const GemmArgs& g, int v0, float (&acc)[kCW],
-                                        const float*) {
+                                        const float* recs) {
+    if constexpr (kR4) {
+#pragma unroll
+      for (int p = 0; p < kCW / 2; ++p) {
+        float b[8];
+        ld_vec<8>(recs + p * 8, b);
+        float2 z2 = f2(acc[2 * p], acc[2 * p + 1]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z2 = __ffma2_rn(sU2[j], f2(b[2 * j], b[2 * j + 1]), z2);
+        acc[2 * p] = z2.x;
+        acc[2 * p + 1] = z2.y;
+      }
+    }
     if (kTail) {
 #pragma unroll
       for (int i = 0; i < kCW; ++i)

@@ -124,3 +124,65 @@ def test_a_step_counts_no_row_of_minus_infinity():
         m.close()
     assert losses[0] == losses[2] and np.isfinite(losses[0])
     assert np.isfinite(losses[1]).all() and np.array_equal(losses[1], losses[3])
+
+
+def _same_bits(a, b):
+    import torch
+    return all(torch.equal(a[key], b[key]) for key in a)
+
+
+@gpu
+@pytest.mark.parametrize("e", [-24, -18, 18, 24])
+@pytest.mark.parametrize("T,V,d,r,k", [(9, 49152, 64, 4, 8), (25, 49152, 64, 4, 8), (300, 4099, 640, 3, 8),
+                                       (40, 3000, 576, 1, 60), (1300, 1000, 64, 2, 0)])
+def test_low_ranks_have_the_range_of_f32(T, V, d, r, k, e):
+    """A power of two moved from B to A changes no bit of what ranks up to 4 compute,
+    far past f16's range, in any path: the products are the same f32 products."""
+    p = Problem(T, V, d, r)
+    p.lists(8)
+    score, full, loss = p.score(k), p.distill(1.5), p.distill(1.5, grads=False)
+    p.A *= 2.0**e
+    p.B *= 2.0**-e
+    assert _same_bits(p.score(k), score)
+    assert p.torch.equal(p.distill(1.5, grads=False)["loss"], loss["loss"])
+    got = p.distill(1.5)
+    got["gA"] *= 2.0**e
+    got["gB"] *= 2.0**-e
+    assert _same_bits(got, full)
+    check_score(p, k, p.score(k))
+    check_distill(p, 1.5)
+
+
+class Pairs(Problem):
+    """The rank term of f16 pairs: hi + lo is off by at most 2^-25 (the spacing of
+    subnormal f16 is 2^-24) or 2^-23 of the value, lo . lo is left out, 2^-22 of a
+    product at most.  So each of r products is off by 2^-25 (|s U| + |B|) + 2^-21 |s U| |B|."""
+
+    def tol(self):
+        u = float((self.scale * (self.H.half().float() @ self.A)).abs().max())
+        b = float(self.B.abs().max())
+        return super().tol() + self.r * (2.0**-25 * (u + b) + 2.0**-21 * u * b)
+
+
+@gpu
+@pytest.mark.parametrize("r", [8, 16, 33])
+@pytest.mark.parametrize("T", [40, 300])
+def test_operands_past_f16_are_infinite_at_higher_ranks(T, r):
+    """From rank 5 on the rank term's operands are pairs of f16: up to 65,504 they are
+    read, past it a position's s U makes its own results NaN."""
+    import torch
+    p = Pairs(T, 1000, 64, r, "f32")
+    p.B /= 32.0
+    p.A *= 32.0
+    p.H[7] *= 4096.0  # s U of about 2^18
+    p.lists(8)
+    out, d = p.score(5), p.distill(1.0, grads=False)["loss"]
+    assert math.isnan(float(out["logprob"][7])) and bool((out["ids"][7] == -1).all())
+    assert math.isnan(float(d[7])) and bool(p.distill(1.0)["gB"].isnan().all())
+    rest = torch.arange(T, device="cuda") != 7
+    p.H[7] = p.H[6]
+    want = p.score(5)
+    for key in out:
+        assert torch.equal(out[key][rest], want[key][rest]), key
+    check_score(p, 5, want)
+    check_distill(p, 1.0)
