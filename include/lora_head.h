@@ -67,9 +67,16 @@ size_t lora_head_distill_workspace(const lora_head* head, int32_t T, int32_t K, 
  *                       logits in descending order, equal ones by ascending id
  *                       (ordered by logits computed with 64-bit sums); not
  *                       read with top_k 0.  Where more than 24 further tokens
- *                       come within 1e-5 (1 + |z|) of the last one, those of
- *                       them with the lowest ids are ordered.
- * A position whose logits hold a NaN or an infinity gets NaN, and ids -1. */
+ *                       come within 2^-18 G of the last one, those of them
+ *                       with the lowest ids are ordered.
+ * A position whose logits hold a NaN or an infinity gets NaN, and ids -1.
+ *
+ * Accuracy.  A logit's f32 sum is off by up to n 2^-23 G[t], n <= dim / 16 + 12,
+ *   G[t] = |h| max |W[v]| + |scale h.A| max |B[:, v]| + |scale| |h| max |A[:, j]| max |B[:, v]|
+ * (the norms of W and B in the bound above: of 1,024 rows spread over the vocabulary), as
+ * G bounds its partial sums; log sum e^z, and with it logprob, entropy and the losses
+ * below, by as much at worst.  That is where channels of h cancel; where the partial
+ * sums grow evenly towards the logit it is about 2e-7 |z|. */
 int lora_head_score(const lora_head* head, const void* H, int32_t h_dtype, int32_t T,
                     const int32_t* tokens, int32_t top_k, float* logprob, float* entropy,
                     int32_t* top_ids, float* top_logprobs, void* workspace,

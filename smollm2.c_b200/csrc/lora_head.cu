@@ -293,10 +293,10 @@ void fill_pass1(GemmArgs& g, const HeadCore& hd, const Aug& aug, int T, float ta
 
 // lh_prep over positions and vocab rows: a block per position up to two an SM,
 // else kTileRows positions per block.
-int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_blocks, bool pack,
-                int sms, cudaStream_t st) {
+int launch_prep(const PrepArgs& pa, const PackArgs& pk, const NormArgs& na, bool rows,
+                int max_blocks, bool pack, int sms, cudaStream_t st) {
   const bool tiles = pa.Tpad > 2 * sms;
-  void (*kern)(PrepArgs, PackArgs, int, int) = lh_prep<-1>;
+  void (*kern)(PrepArgs, PackArgs, NormArgs, int, int, int) = lh_prep<-1>;
   if (tiles) {
     switch (pa.R) {
       case 0: kern = lh_prep<0>; break;
@@ -310,11 +310,12 @@ int launch_prep(const PrepArgs& pa, const PackArgs& pk, bool rows, int max_block
   const int prep_blocks = !rows ? 0 : tiles ? (pa.Tpad + kTileRows - 1) / kTileRows : pa.Tpad;
   const int pack_blocks = pack ? (int)(pk.Vpad / kPackRows) : 0;
   const size_t smem =
-      std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R, pa.d) : (size_t)(pa.d + 256) * 4,
+      std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R, pa.d) : (size_t)(pa.d + 264) * 4,
                pack ? (size_t)pk.R * (kPackRows + 1) * 4 : 0);
   if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return LORA_CE_ECUDA;
-  return launch_plain(kern, prep_blocks + max_blocks + pack_blocks, 256, smem, st, pa, pk,
-                      prep_blocks, max_blocks) ? 0 : LORA_CE_ECUDA;
+  const int norm_blocks = na.out ? kNormBlocks + (na.r ? 1 : 0) : 0;
+  return launch_plain(kern, norm_blocks + prep_blocks + max_blocks + pack_blocks, 256, smem, st,
+                      pa, pk, na, norm_blocks, prep_blocks, max_blocks) ? 0 : LORA_CE_ECUDA;
 }
 
 // The pass for few positions, one slot per 128 vocab rows.  Its time grows with
@@ -359,7 +360,7 @@ bool launch_few(const FewArgs& f, int blocks, cudaStream_t st) {
 struct ScoreWs {
   int* stats;
   __half *h16, *haug, *waug;
-  float *sU, *Bt, *p_max, *p_sum, *p_ent, *sub_max, *sub_second, *sub_rest;
+  float *sU, *Bt, *norms, *hn, *p_max, *p_sum, *p_ent, *sub_max, *sub_second, *sub_rest;
   uint8_t *sub_arg, *sub_arg2;
   int sub, n_sub;
   size_t bytes;
@@ -382,6 +383,8 @@ ScoreWs score_ws(const HeadCore& hd, int T, int top_k, void* ws) {
   w.haug = c.take<__half>((size_t)T * aug.width);
   w.waug = c.take<__half>((size_t)Vpad * aug.width);
   w.Bt = c.take<float>(aug.R == 4 && !few && !hd.layout ? (size_t)Vpad * 4 : 0);
+  w.norms = c.take<float>(2 * kNormBlocks + 1);
+  w.hn = c.take<float>(T);
   w.p_max = c.take<float>(part);
   w.p_sum = c.take<float>(part);
   w.p_ent = c.take<float>(part);
@@ -696,6 +699,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   pa.h16 = w.h16;
   pa.sU = w.sU;
   pa.haug = aug.width ? w.haug : nullptr;
+  pa.hn = top_k > 0 ? w.hn : nullptr;
   pa.stats = w.stats;
   PackArgs pk{};
   pk.B = BView{hd.B, hd.V, hd.r, aug.R, hd.layout};
@@ -708,8 +712,18 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   pk.aug_layout = aug.layout;
   pk.aug_width = aug.width;
 
+  NormArgs na{};
+  na.W = hd.W;
+  na.V = hd.V;
+  na.d = hd.d;
+  na.B = pk.B;
+  na.A = hd.A;
+  na.lda = hd.lda;
+  na.r = hd.r;
+  na.out = top_k > 0 ? w.norms : nullptr;
+
   if (few) {
-    if (launch_prep(pa, pk, true, 0, false, sms, st)) return *why = kNoFit, LORA_CE_ECUDA;
+    if (launch_prep(pa, pk, na, true, 0, false, sms, st)) return *why = kNoFit, LORA_CE_ECUDA;
     const int blocks = few_blocks(hd.V);
     const float lg = (float)((1.0 + kLoss32) / std::log(2.0));
     FewArgs f = few_args(hd, aug.R, T, w.h16, w.sU, lg);
@@ -738,7 +752,7 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
     if (aug.width && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
                       !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
       return *why = kNoMap, LORA_CE_ECUDA;
-    if (launch_prep(pa, pk, true, 0, pk.Bt || pk.waug, sms, st))
+    if (launch_prep(pa, pk, na, true, 0, pk.Bt || pk.waug, sms, st))
       return *why = kNoFit, LORA_CE_ECUDA;
     const int G = (int)std::min<long long>(units, (long long)g.n_a * g.n_b);
     if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, g))
@@ -748,6 +762,9 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
     a.lg = g.lg;
   }
   a.z = logit_args(hd, aug, T, w.h16, w.sU, w.haug, w.waug);
+  a.norms = w.norms;
+  a.hn = w.hn;
+  a.steps = 4 * g.kmain + (g.kblocks > g.kmain ? g.n_aug : 0);
   if (Bt) a.z.B = BView{Bt, hd.V, hd.r, aug.R, 1};  // a row's ranks side by side
   a.sub_max = w.sub_max;
   a.sub_second = w.sub_second;
@@ -836,8 +853,9 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pk.stats = w.stats;
   const bool pack = pk.Bt || pk.waug || pk.xv;
   // the scale of xv needs the largest |B| first
-  if (launch_prep(pa, pk, true, tc ? 2 * s.sms : 0, pack && !tc, s.sms, st) ||
-      (tc && launch_prep(pa, pk, false, 0, true, s.sms, st)))
+  const NormArgs no{};
+  if (launch_prep(pa, pk, no, true, tc ? 2 * s.sms : 0, pack && !tc, s.sms, st) ||
+      (tc && launch_prep(pa, pk, no, false, 0, true, s.sms, st)))
     return *why = kNoFit, LORA_CE_ECUDA;
 
   int rc = 0;

@@ -254,6 +254,7 @@ struct PrepArgs {
   int lda, r, R;   // R: r rounded up to a kernel rank; 0 without an adapter
   float scale;
   __half* h16;     // [T][d]
+  float* hn;       // [T] |h16|, or null
   float* sU;       // [T][R] s * U
   float* tok;      // records (tidx layout) or null
   __half* haug;    // [T][aug_width] or null
@@ -418,7 +419,7 @@ __device__ __forceinline__ void put_max(const PrepArgs& a, float umax) {
 // (one warp per position, 4 loads at a time, took 40 us at rank 4 and 140 us at
 // rank 16; this 6 and 9 us).
 __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
-  float* red = sh + a.d;  // [256] behind h's [d]
+  float* red = sh + a.d;  // [256 + 8] behind h's [d]
   const int tid = threadIdx.x, R = a.R;
   if (t >= a.T) {
     if (a.tok) put_fields(a, t, 0, tid, 256);
@@ -444,15 +445,27 @@ __device__ __forceinline__ void prep_row(const PrepArgs& a, int t, float* sh) {
     }
   };
   fetch(sl);  // on its way beside h
+  float hh = 0.f;
   for (int i = 2 * tid; i < a.d; i += 512) {
     const float2 x = active ? load_pair(a, from, i) : make_float2(0.f, 0.f);
     const __half2 hv = __floats2half2_rn(x.x, x.y);
     *reinterpret_cast<__half2*>(a.h16 + (long long)t * a.d + i) = hv;
-    *reinterpret_cast<float2*>(sh + i) = __half22float2(hv);
+    const float2 hf = __half22float2(hv);
+    *reinterpret_cast<float2*>(sh + i) = hf;
+    hh = fmaf(hf.x, hf.x, fmaf(hf.y, hf.y, hh));
+  }
+  if (a.hn) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) hh += __shfl_xor_sync(0xffffffffu, hh, off);
+    if ((tid & 31) == 0) red[256 + (tid >> 5)] = hh;
+  }
+  __syncthreads();
+  if (a.hn && tid == 0) {
+    for (int q = 1; q < 8; ++q) hh += red[256 + q];
+    a.hn[t] = sqrtf(hh);
   }
   if (R == 0) return;
   float u = 0.f;
-  __syncthreads();
   for (int i0 = sl; i0 < a.d; i0 += 16 * ns) {
     if (i0 != sl) fetch(i0);
 #pragma unroll
@@ -523,15 +536,22 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
     for (int k = 0; k < kMaxHead64; ++k)
       x[k] = make_float2(0.f, 0.f);
     if (in) load_row(a, from, lane, x);
+    float hh = 0.f;
 #pragma unroll
     for (int k = 0; k < kMaxHead64; ++k)
       if (64 * k < a.d) {
         const __half2 hv = __floats2half2_rn(x[k].x, x[k].y);
+        const float2 hf = __half22float2(hv);
         if (t < a.T)
           *reinterpret_cast<__half2*>(a.h16 + (long long)t * a.d + 64 * k + 2 * lane) = hv;
-        if constexpr (R > 0)
-          *reinterpret_cast<float2*>(hT + row * ldh + 64 * k + 2 * lane) = __half22float2(hv);
+        if constexpr (R > 0) *reinterpret_cast<float2*>(hT + row * ldh + 64 * k + 2 * lane) = hf;
+        hh = fmaf(hf.x, hf.x, fmaf(hf.y, hf.y, hh));
       }
+    if (a.hn) {
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) hh += __shfl_xor_sync(0xffffffffu, hh, off);
+      if (lane == 0 && t < a.T) a.hn[t] = sqrtf(hh);
+    }
   }
   if constexpr (R > 0) {
     constexpr int kRows = 12;  // of A in flight; d / 8 is a multiple of 8
@@ -678,25 +698,108 @@ __device__ __forceinline__ void pack_tile(const PackArgs& a, long long v0, float
   }
 }
 
-// Blocks [0, prep_blocks) take positions (kRank < 0: one each; else kTileRows at
-// kernel rank kRank), the next max_blocks look for the largest finite |B| (the
-// scale of a later launch's xv), the others pack vocab rows.
+// What the errors of logits are measured by (logit_gaps): the largest |W[v]| and
+// |B[:, v]| of kNormBlocks runs of up to kNormRows vocab rows, spread over the vocabulary
+// (all of up to 1,024), and the largest |A[:, j]|.  All of W, 57 MB, would take longer
+// than the rest of a short call's preparation (one token 29 -> 42 us).
+constexpr int kNormBlocks = 32, kNormRows = 32;
+struct NormArgs {
+  const __half* W;
+  int V, d;
+  BView B;
+  const float* A;
+  int lda, r;
+  float* out;  // [kNormBlocks] W, [kNormBlocks] B, A; or null: not wanted
+};
+__device__ __forceinline__ void norm_block(const NormArgs& a, int blk) {
+  __shared__ double red[256];
+  __shared__ float redW[8];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  int n;  // columns (of A, of B): their squares are split over threads tid % n
+  double s = 0.0;
+  if (blk >= kNormBlocks) {
+    n = a.r > 32 ? 64 : a.r > 16 ? 32 : 16;
+    const int j = tid % n;
+    if (j < a.r)
+#pragma unroll 16
+      for (int i = tid / n; i < a.d; i += 256 / n) {
+        const double x = (double)a.A[(long long)i * a.lda + j];
+        s = fma(x, x, s);
+      }
+  } else {
+    n = kNormRows;
+    const int v_lo = (int)((long long)a.V * blk / kNormBlocks);
+    const int v_hi = min((int)((long long)a.V * (blk + 1) / kNormBlocks), v_lo + kNormRows);
+    // eight lanes per row of W, whole sectors, all of it and of B at once
+    const int vw = v_lo + (tid >> 3), vb = v_lo + tid % n;
+    uint4 x[kMaxHead64];
+#pragma unroll
+    for (int k = 0; k < kMaxHead64; ++k)
+      x[k] = 64 * k < a.d && vw < v_hi
+                 ? reinterpret_cast<const uint4*>(a.W + (long long)vw * a.d)[(tid & 7) + 8 * k]
+                 : make_uint4(0u, 0u, 0u, 0u);
+    if (vb < v_hi)
+#pragma unroll 8
+      for (int j = tid / n; j < a.r; j += 256 / n) {
+        const double y = (double)a.B.at(j, vb);
+        s = fma(y, y, s);
+      }
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMaxHead64; ++k) {
+      const __half2* h = reinterpret_cast<const __half2*>(&x[k]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 y = __half22float2(h[e]);
+        q = fmaf(y.x, y.x, fmaf(y.y, y.y, q));
+      }
+    }
+    for (int off = 1; off < 8; off <<= 1) q += __shfl_xor_sync(0xffffffffu, q, off);
+    q = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(q)));
+    if (lane == 0) redW[w] = q;
+  }
+  red[tid] = s;
+  __syncthreads();
+  if (w != 0) return;
+  double top = 0.0;
+  for (int c = lane; c < n; c += 32) {
+    double x = 0.0;
+    for (int k = c; k < 256; k += n) x += red[k];
+    top = fmax(top, x);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, off));
+  if (lane != 0) return;
+  a.out[kNormBlocks + blk] = (float)sqrt(top);
+  if (blk < kNormBlocks) {
+    float q = redW[0];
+    for (int k = 1; k < 8; ++k) q = fmaxf(q, redW[k]);
+    a.out[blk] = sqrtf(q);
+  }
+}
+
+// Blocks [0, norm_blocks) take norms, the next prep_blocks positions (kRank < 0: one
+// each; else kTileRows at kernel rank kRank), the next max_blocks look for the largest
+// finite |B| (the scale of a later launch's xv), the others pack vocab rows.
 template <int kRank>
-static __global__ void __launch_bounds__(256) lh_prep(PrepArgs a, PackArgs b, int prep_blocks,
+static __global__ void __launch_bounds__(256) lh_prep(PrepArgs a, PackArgs b, NormArgs n,
+                                                      int norm_blocks, int prep_blocks,
                                                       int max_blocks) {
   extern __shared__ __align__(16) float smem_prep[];
-  const int blk = (int)blockIdx.x;
+  const int blk = (int)blockIdx.x - norm_blocks;
   grid_launch();  // (a kernel launched to depend waits for this one's end)
-  if (blk < prep_blocks) {
+  if (blk < 0) {
+    norm_block(n, blk + norm_blocks);
+  } else if (blk < prep_blocks) {
     if (blk == 0 && threadIdx.x == 0 && !a.ids) a.stats[kStErr] = 0;
     if constexpr (kRank < 0) prep_row(a, blk, smem_prep);
     else prep_tile<kRank>(a, blk * kTileRows, smem_prep);
   } else if (blk < prep_blocks + max_blocks) {
     float m = 0.f;
-    const long long n = b.B.layout ? b.Vpad * b.R : (long long)b.r * b.V;  // (padding is 0)
+    const long long size = b.B.layout ? b.Vpad * b.R : (long long)b.r * b.V;  // (padding is 0)
     const long long step = (long long)max_blocks * 256;
 #pragma unroll 8
-    for (long long k = (long long)(blk - prep_blocks) * 256 + threadIdx.x; k < n; k += step) {
+    for (long long k = (long long)(blk - prep_blocks) * 256 + threadIdx.x; k < size; k += step) {
       const float x = fabsf(b.B.p[k]);
       m = isfinite(x) ? fmaxf(m, x) : m;
     }
@@ -849,10 +952,6 @@ __device__ __forceinline__ double warp_sum(double s) {
   for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
   return s;
 }
-
-// How far apart two logits have to be for logits16 to tell their order: several
-// times the largest error seen.
-__device__ __forceinline__ float logit_gap(float z) { return 4e-6f * (1.0f + fabsf(z)); }
 
 // One logit by one warp with 64-bit sums throughout (products of f16 are exact in
 // f32): for those whose order logits16 does not tell.  u: scale U[t], from u64.
@@ -1387,6 +1486,9 @@ static __global__ void __launch_bounds__(256, 3) lh_few(FewArgs a) {
 // ------------------------------------------------------------- score, per row
 struct ScoreArgs {
   LogitArgs z;
+  const float* norms;  // NormArgs::out, PrepArgs::hn (with alternatives)
+  const float* hn;
+  int steps;           // the MMA steps of a logit of the pass
   SlotPlan p;
   float lg;
   int n_sub, sub, top_k;  // records, columns per record
@@ -1415,6 +1517,50 @@ __host__ __device__ inline size_t score_team_smem(int n_pick, int cap, int warps
           (size_t)score_picks(n_pick) * 16 + 128 * 4 + 16 * 4 + 15) / 16 * 16;
 }
 constexpr int kScoreRows = 4;  // positions per block where each has a warp
+
+// How far apart two logits of position t have to be for their order to be told, by a
+// warp.  A sum's rounding follows its partial sums, not the logit, and these are at
+// most g = |h| max |W[v]| + |s U| max |B[:, v]|, as channels that cancel show: hidden
+// states whose partial sums were 50 times their logits had alternatives out of order
+// when this went by the logit.
+//   pass: each of its n MMA steps cuts off less than a unit in the last place of a
+//         partial sum, half of one on average and that 2^-24 of the sum at most, always
+//         towards zero: sums of g all along would lose n 2^-24 g more than sums near 0
+//   again: logits16's sums of 32 products, at most two such losses each, come to
+//         2 2^-23 g by Cauchy and Schwarz; the largest error measured is 1.8 2^-23 g
+// Both have s U rounded to f32: sums of up to 80 terms with a standard deviation of
+// about 2^-23 |h| |A[:, j]|, for which 8 2^-23 |h| |A[:, j]| max |B[:, v]| is taken; and
+// where the rank term is of f16 pairs, what these leave out: 2^-25 of each s U[j] and
+// B[j][v] and 2^-21 of their product.
+struct Gaps {
+  float pass, again;
+};
+// What a lane reads for them, and the gaps: apart, so that the reads are on their way
+// beside others.
+struct GapReads {
+  float h, w, b, A, u;
+};
+__device__ __forceinline__ GapReads read_gaps(const LogitArgs& z, const float* norms,
+                                              const float* hn, int t, int lane) {
+  const float* su = z.sU + (long long)t * z.R;
+  const float u1 = lane < z.r ? fabsf(su[lane]) : 0.f;
+  const float u2 = lane + 32 < z.r ? fabsf(su[lane + 32]) : 0.f;
+  return GapReads{hn[t], norms[lane], norms[kNormBlocks + lane],
+                  z.r > 0 ? norms[2 * kNormBlocks] : 0.f, fmaxf(u1, u2)};
+}
+__device__ __forceinline__ Gaps logit_gaps(const LogitArgs& z, const GapReads& x, int steps) {
+  auto most = [&](float y) {  // y >= 0
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(y)));
+  };
+  float g = x.h * most(x.w), e = 0.f;
+  if (z.r > 0) {
+    const float root = sqrtf((float)z.r), b = most(x.b), u = root * most(x.u);  // >= |s U|
+    g = fmaf(u, b, g);
+    e = 8.f * (x.h * x.A * fabsf(z.scale)) * b;
+    if (z.waug) e += 0.5f * root * (u + b) + 4.f * u * b;
+  }
+  return Gaps{0x1p-23f * fmaf(0.5f * (float)steps, g, e), 0x1p-23f * fmaf(4.f, g, e)};
+}
 
 // Cuts a position's list of candidates [c_0, n_c) to `keep` (at least C) of them: the
 // threshold rises to the C-th largest of the list, what lies below it goes, and of its
@@ -1546,6 +1692,8 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
     }
   }
   const int tk = a.tokens ? a.tokens[t] : -1;
+  GapReads gr = {};
+  if (a.top_k > 0) gr = read_gaps(a.z, a.norms, a.hn, t, lane);
   const bool have_tok = tk >= 0 && tk < a.z.V;
   const RowSum rs = merge_row<true>(a.p, t, a.p.slots(t), team);
   const float nan = __int_as_float(0x7fc00000);
@@ -1563,6 +1711,7 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
     return;
   }
 
+  const Gaps gaps = a.top_k > 0 ? logit_gaps(a.z, gr, a.steps) : Gaps{0.f, 0.f};
   // threshold `lo`: at least C records reach it, n_lo of them where that is known
   // to be few enough
   const int C = a.n_pick;
@@ -1609,7 +1758,7 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   // records that reach the threshold but for rounding; where they are more than
   // P (equal or nearly equal maxima, as of a padding row), those surely above it
   // and of the others the lowest
-  const float eps = 1e-5f * (1.0f + fmaxf(fabsf(lo), fabsf(rs.M)));
+  const float eps = gaps.pass;
   float bound = lo - eps, above = lo + eps;
   const float first = bound;  // what a record's second had to reach
   int room = P;
@@ -1757,9 +1906,8 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
       }
     }
   }
-  // The pass's logits, made good for their known loss, are off by a few 1e-7 of z:
-  // enough to tell the order of all but those within 1e-5 (1 + |z|) of another.
-  // These, the kMinPick largest (by which the softmax's sums are made good) and
+  // The pass's logits, made good for their known loss, tell the order of all but those
+  // within gaps.pass of another.  These, the kMinPick largest (by which the softmax's sums are made good) and
   // those known only from the columns above are computed again, the others' logits
   // are the pass's; of 72 candidates of a list of 64 that is about 10, one group of
   // 16 instead of five.  All, where that is one group anyway.
@@ -1779,7 +1927,7 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
     for (int i = 0; i < kItems; ++i) {
       const int c = b0 + i * kThreads + tid;
       z[i] = c < n_c ? approx32[c] : INFINITY;
-      gap[i] = c < n_c ? 1e-5f * (1.0f + fabsf(z[i])) : -1.f;
+      gap[i] = c < n_c ? gaps.pass : -1.f;
       rank[i] = close[i] = 0;
     }
     for (int q = c_0; q < n_c; ++q) {
@@ -1858,9 +2006,8 @@ static __global__ void __launch_bounds__(TW == 1 ? 32 * kScoreRows : 32 * TW, TW
   bool any_close = false;
   for (int c = c_0 + tid; c < n_z && a.top_k > 0; c += kThreads) {
     if (ranks[c] >= 0) continue;
-    const float zc = (float)z64[c], gap = logit_gap(zc);
     int close = 0;
-    for (int q = c_0; q < n_z; ++q) close += fabsf((float)(z64[q] - z64[c])) <= gap;
+    for (int q = c_0; q < n_z; ++q) close += fabsf((float)(z64[q] - z64[c])) <= gaps.again;
     if (close > 1) {
       ranks[c] = -2;
       any_close = true;

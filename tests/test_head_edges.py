@@ -186,3 +186,34 @@ def test_operands_past_f16_are_infinite_at_higher_ranks(T, r):
         assert torch.equal(out[key][rest], want[key][rest]), key
     check_score(p, 5, want)
     check_distill(p, 1.0)
+
+
+class Cancelling(Problem):
+    """Two channels of the hidden state far above the others whose parts of every
+    logit cancel, the first and the last of the sum (or, in the adapter, of h . A):
+    partial sums up to 100 times the logits."""
+
+    def __init__(self, T, V, d, r, adapter=False, by=512.0):
+        super().__init__(T, V, d, r)
+        torch = self.torch
+        a = (0.5 + self.u(V)).half()
+        self.W[:, 0] = self.W[:, d - 1] = 0 if adapter else a
+        if r:
+            b = 0.5 + self.u(r)
+            self.A[0] = self.A[d - 1] = b if adapter else 0
+        K = by * 2.0 ** torch.arange(T, device="cuda").remainder(3).neg()
+        self.H[:, 0], self.H[:, d - 1] = K.to(self.H.dtype), -K.to(self.H.dtype)
+
+
+@gpu
+@pytest.mark.parametrize("T,V,d,r,k,adapter", [
+    (9, 49152, 576, 0, 64, False), (24, 49152, 576, 16, 64, True),
+    (100, 49152, 576, 0, 64, False), (300, 49152, 576, 4, 64, False), (300, 49152, 576, 64, 64, True),
+    (2500, 49152, 576, 0, 64, False), (200, 4099, 640, 8, 20, True), (60, 140000, 128, 33, 100, False),
+    (500, 1000, 320, 3, 100, True),
+])
+def test_order_of_logits_whose_sums_cancel(T, V, d, r, k, adapter):
+    """Ids are those of the 64-bit logits where an f32 sum's rounding, which follows
+    its partial sums, is far above what the logits' own size suggests."""
+    p = Cancelling(T, V, d, r, adapter)
+    check_score(p, k, p.score(k))
