@@ -683,11 +683,12 @@ __device__ __forceinline__ void pack_tile(const PackArgs& a, long long v0, float
     }
   }
   if (a.xv) {
-    const float up = (float)exp2i(scale_exp(a.stats[kStBMax], 13));
+    const double up = exp2i(scale_exp(a.stats[kStBMax], 13));  // past f32 for a tiny B
 #pragma unroll 2
     for (int k = tid; k < R * (kPackRows / 2); k += 256) {
       const int j = k / (kPackRows / 2), i = 2 * (k % (kPackRows / 2));
-      const float x = tile[j * ld + i] * up, y = tile[j * ld + i + 1] * up;
+      const float x = (float)((double)tile[j * ld + i] * up);
+      const float y = (float)((double)tile[j * ld + i + 1] * up);
       const __half2 hi = __floats2half2_rn(x, y);
       const float2 hf = __half22float2(hi);
       const long long o = (long long)j * a.Vpad + v0 + i;

@@ -217,3 +217,15 @@ def test_order_of_logits_whose_sums_cancel(T, V, d, r, k, adapter):
     its partial sums, is far above what the logits' own size suggests."""
     p = Cancelling(T, V, d, r, adapter)
     check_score(p, k, p.score(k))
+
+
+@gpu
+@pytest.mark.parametrize("r", [4, 8, 16, 64])
+@pytest.mark.parametrize("T", [12, 100, 300])
+@pytest.mark.parametrize("e", [-118, -60, 0])
+def test_gradients_of_a_tiny_adapter(T, r, e):
+    """The scale that brings B into f16's range is itself past f32's where B is tiny."""
+    p = Problem(T, 1000, 64, r)
+    p.lists(8)
+    p.B *= 2.0**e
+    check_distill(p, 1.0)
