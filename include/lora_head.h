@@ -22,7 +22,9 @@
  *
  * Conventions as lora_ce.h: 0 or a negative LORA_CE_E* code, nothing aborts;
  * lora_head_last_error() describes the last failure on the calling thread.
- * Host-side errors enqueue nothing.  A device-side error (a bounded wait that
+ * An error found on the host enqueues nothing, but for a launch that fails
+ * ("kernel launch failed"): those ahead of it have been enqueued, so wait for the
+ * stream before freeing the call's buffers.  A device-side error (a bounded wait that
  * expired) turns every output into NaN, and ids into -1.
  */
 #ifndef LORA_HEAD_H

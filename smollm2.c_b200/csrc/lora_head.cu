@@ -170,14 +170,22 @@ struct Carve {
   }
 };
 
-// Launch of a GEMM pass on CTA pairs, with a programmatic dependency on the kernel
-// ahead (whose end the kernel waits for by itself, grid_wait).
-template <class K, class... Args>
-bool launch_pairs(K kern, int pairs, int threads, int smem, cudaStream_t st, const Args&... args) {
+// A GEMM pass on CTA pairs, all but launched.
+struct Pass {
+  const void* kern = nullptr;
+  int threads = 0, smem = 0, G = 0;
+  int n_maps = 0;
+  CUtensorMap maps[5];
+  GemmArgs g{};
+};
+
+// Launch with a programmatic dependency on the kernel ahead (whose end the kernel
+// waits for by itself, grid_wait).
+bool launch_pass(Pass& p, cudaStream_t st) {
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3((unsigned)(2 * pairs));
-  lc.blockDim = dim3((unsigned)threads);
-  lc.dynamicSmemBytes = (size_t)smem;
+  lc.gridDim = dim3((unsigned)(2 * p.G));
+  lc.blockDim = dim3((unsigned)p.threads);
+  lc.dynamicSmemBytes = (size_t)p.smem;
   lc.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -188,7 +196,10 @@ bool launch_pairs(K kern, int pairs, int threads, int smem, cudaStream_t st, con
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   lc.attrs = attr;
   lc.numAttrs = 2;
-  return cudaLaunchKernelEx(&lc, kern, args...) == cudaSuccess;
+  void* args[6];
+  for (int i = 0; i < p.n_maps; ++i) args[i] = &p.maps[i];
+  args[p.n_maps] = &p.g;
+  return cudaLaunchKernelExC(&lc, p.kern, args) == cudaSuccess;
 }
 
 // A kernel that waits for all that is ahead of it in the stream.
@@ -293,29 +304,40 @@ void fill_pass1(GemmArgs& g, const HeadCore& hd, const Aug& aug, int T, float ta
 
 // lh_prep over positions and vocab rows: a block per position up to two an SM,
 // else kTileRows positions per block.
-int launch_prep(const PrepArgs& pa, const PackArgs& pk, const NormArgs& na, bool rows,
-                int max_blocks, bool pack, int sms, cudaStream_t st) {
+struct PrepPlan {
+  void (*kern)(PrepArgs, PackArgs, NormArgs, int, int, int) = nullptr;
+  int norm_blocks = 0, prep_blocks = 0, max_blocks = 0, pack_blocks = 0;
+  size_t smem = 0;
+  bool ok = false;
+};
+PrepPlan plan_prep(const PrepArgs& pa, const PackArgs& pk, const NormArgs& na, bool rows,
+                   int max_blocks, bool pack, int sms) {
+  PrepPlan p;
   const bool tiles = pa.Tpad > 2 * sms;
-  void (*kern)(PrepArgs, PackArgs, NormArgs, int, int, int) = lh_prep<-1>;
+  p.kern = lh_prep<-1>;
   if (tiles) {
     switch (pa.R) {
-      case 0: kern = lh_prep<0>; break;
-      case 4: kern = lh_prep<4>; break;
-      case 8: kern = lh_prep<8>; break;
-      case 16: kern = lh_prep<16>; break;
-      case 32: kern = lh_prep<32>; break;
-      default: kern = lh_prep<64>; break;
+      case 0: p.kern = lh_prep<0>; break;
+      case 4: p.kern = lh_prep<4>; break;
+      case 8: p.kern = lh_prep<8>; break;
+      case 16: p.kern = lh_prep<16>; break;
+      case 32: p.kern = lh_prep<32>; break;
+      default: p.kern = lh_prep<64>; break;
     }
   }
-  const int prep_blocks = !rows ? 0 : tiles ? (pa.Tpad + kTileRows - 1) / kTileRows : pa.Tpad;
-  const int pack_blocks = pack ? (int)(pk.Vpad / kPackRows) : 0;
-  const size_t smem =
-      std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R, pa.d) : (size_t)(pa.d + 264) * 4,
-               pack ? (size_t)pk.R * (kPackRows + 1) * 4 : 0);
-  if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return LORA_CE_ECUDA;
-  const int norm_blocks = na.out ? kNormBlocks + (na.r ? 1 : 0) : 0;
-  return launch_plain(kern, norm_blocks + prep_blocks + max_blocks + pack_blocks, 256, smem, st,
-                      pa, pk, na, norm_blocks, prep_blocks, max_blocks) ? 0 : LORA_CE_ECUDA;
+  p.norm_blocks = na.out ? kNormBlocks + (na.r ? 1 : 0) : 0;
+  p.prep_blocks = !rows ? 0 : tiles ? (pa.Tpad + kTileRows - 1) / kTileRows : pa.Tpad;
+  p.max_blocks = max_blocks;
+  p.pack_blocks = pack ? (int)(pk.Vpad / kPackRows) : 0;
+  p.smem = std::max(!rows ? 0 : tiles ? prep_tile_smem(pa.R, pa.d) : (size_t)(pa.d + 264) * 4,
+                    pack ? (size_t)pk.R * (kPackRows + 1) * 4 : 0);
+  p.ok = allow_smem(reinterpret_cast<const void*>(p.kern), p.smem);
+  return p;
+}
+bool launch_prep(const PrepPlan& p, const PrepArgs& pa, const PackArgs& pk, const NormArgs& na,
+                 cudaStream_t st) {
+  return launch_plain(p.kern, p.norm_blocks + p.prep_blocks + p.max_blocks + p.pack_blocks, 256,
+                      p.smem, st, pa, pk, na, p.norm_blocks, p.prep_blocks, p.max_blocks);
 }
 
 // The pass for few positions, one slot per 128 vocab rows.  Its time grows with
@@ -348,13 +370,22 @@ FewArgs few_args(const HeadCore& hd, int R, int T, const __half* h16, const floa
   return f;
 }
 
+struct FewPlan {
+  void (*kern)(FewArgs) = nullptr;
+  size_t smem = 0;
+  bool ok = true;
+};
 template <int kMode>
-bool launch_few(const FewArgs& f, int blocks, cudaStream_t st) {
+FewPlan plan_few(const FewArgs& f) {
   const int nt = (f.T + 7) / 8, NT = nt <= 2 ? nt : 4;
-  void (*kern)(FewArgs) = NT == 1 ? lh_few<1, kMode> : NT == 2 ? lh_few<2, kMode> : lh_few<4, kMode>;
-  const size_t smem = few_smem(NT, f.d, f.R);
-  return allow_smem(reinterpret_cast<const void*>(kern), smem) &&
-         launch_after(kern, blocks, 256, smem, st, f);
+  FewPlan p;
+  p.kern = NT == 1 ? lh_few<1, kMode> : NT == 2 ? lh_few<2, kMode> : lh_few<4, kMode>;
+  p.smem = few_smem(NT, f.d, f.R);
+  p.ok = allow_smem(reinterpret_cast<const void*>(p.kern), p.smem);
+  return p;
+}
+bool launch_few(const FewPlan& p, const FewArgs& f, int blocks, cudaStream_t st) {
+  return launch_after(p.kern, blocks, 256, p.smem, st, f);
 }
 
 struct ScoreWs {
@@ -499,136 +530,148 @@ PrepArgs prep_args(const HeadCore& hd, const Aug& aug, const void* H, int dtype,
   return p;
 }
 
-// The gradient passes of kernel rank R.
+// The passes of one call.
 struct Step {
   const HeadCore& hd;
-  const DistillWs& w;
+  const __half *h16, *haug, *waug;
   Aug aug;
   int T, sms;
-  float tau;
-  cudaStream_t st;
   GemmArgs g;      // pass 1's, filled
+  const DistillWs* w;
+  Pass one, two;   // out
   SlotPlan slots;  // out: pass 1's partials
   int cparts2 = 0, n_b2 = 0, bn2 = 0, G2 = 0;
-  const float* Bt = nullptr;
 };
 
 constexpr const char* kNoMap = "cuTensorMapEncodeTiled failed";
 constexpr const char* kNoFit = "a GEMM pass cannot be made resident on this device";
 constexpr const char* kNoLaunch = "kernel launch failed";
 
-template <class Epi>
-int sums_pass1(Step& s, const char** why) {
-  const int d = s.hd.d;
-  CUtensorMap mh, mw, mha, mwa;
-  if (!make_map(&mh, s.w.h16, s.T, d, kBM) || !make_map(&mw, s.hd.W, s.hd.V, d, kBM))
-    return *why = kNoMap, LORA_CE_ECUDA;
-  mha = mh;
-  mwa = mw;
-  if (Epi::kAug && (!make_map(&mha, s.w.haug, s.T, s.aug.width, kBM) ||
-                    !make_map(&mwa, s.w.waug, s.hd.V, s.aug.width, kBM)))
-    return *why = kNoMap, LORA_CE_ECUDA;
-  const PassPlan p = sums_plan<Epi>(s.g.kblocks);
-  const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
-                                                       p.threads, p.smem));
+int pair_units(const Pass& p) {
+  return std::min(kMaxPairs, resident_pairs(p.kern, p.threads, p.smem));
+}
+
+// Positions as rows of both operands' maps [h, W] or [W, h], and the rank term's.
+int operand_maps(const Step& s, bool aug, bool w_first, int box_a, int box_b, Pass& p,
+                 const char** why) {
+  const int d = s.hd.d, aw = s.aug.width, V = s.hd.V, T = s.T;
+  CUtensorMap* m = p.maps;
+  const int h = w_first ? 1 : 0, w = 1 - h;
+  const int box_h = w_first ? box_b : box_a, box_w = w_first ? box_a : box_b;
+  bool ok = make_map(&m[h], s.h16, T, d, box_h) && make_map(&m[w], s.hd.W, V, d, box_w);
+  if (ok && aug)
+    ok = make_map(&m[2 + h], s.haug, T, aw, box_h) && make_map(&m[2 + w], s.waug, V, aw, box_w);
+  if (!ok) return *why = kNoMap, LORA_CE_ECUDA;
+  if (!aug) {
+    m[2] = m[0];
+    m[3] = m[1];
+  }
+  p.n_maps = 4;
+  return 0;
+}
+
+// Pass 1 of a kernel that lce_gemm_kernel makes of an epilogue.
+int rows_pass(Step& s, const PassPlan& plan, bool aug, int cparts, float* p_ent, float* p_q,
+              const char** why) {
+  Pass& p = s.one;
+  p.kern = reinterpret_cast<const void*>(plan.kern);
+  p.threads = plan.threads;
+  p.smem = plan.smem;
+  if (int rc = operand_maps(s, aug, false, kBM, kBM, p, why)) return rc;
+  const int units = pair_units(p);
   if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
   s.g.n_b = (int)(s.g.Vpad / kBN);
-  const int G = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
-  if (!launch_pairs(p.kern, G, p.threads, p.smem, s.st, mh, mw, mha, mwa, s.g))
-    return *why = kNoLaunch, LORA_CE_ECUDA;
-  s.slots = SlotPlan{col_parts(Epi::kWarps), s.g.n_a, s.g.n_b, units, s.g.Tcap,
-                     s.w.p_max, s.w.p_sum, nullptr, s.w.p_q};
+  p.G = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
+  p.g = s.g;
+  s.slots = SlotPlan{cparts, s.g.n_a, s.g.n_b, units, s.g.Tcap, s.g.p_max, s.g.p_sum, p_ent, p_q};
   return 0;
 }
 
 template <class Epi>
 int sums_pass2(Step& s, const char** why) {
-  const int d = s.hd.d;
-  CUtensorMap mh, mw, mha, mwa;
-  if (!make_map(&mh, s.w.h16, s.T, d, kBM) || !make_map(&mw, s.hd.W, s.hd.V, d, kBM))
-    return *why = kNoMap, LORA_CE_ECUDA;
-  mha = mh;
-  mwa = mw;
-  if (Epi::kAug && (!make_map(&mha, s.w.haug, s.T, s.aug.width, kBM) ||
-                    !make_map(&mwa, s.w.waug, s.hd.V, s.aug.width, kBM)))
-    return *why = kNoMap, LORA_CE_ECUDA;
-  const PassPlan p = sums_plan<Epi>(s.g.kblocks);
-  const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
-                                                       p.threads, p.smem));
+  const PassPlan plan = sums_plan<Epi>(s.g.kblocks);
+  Pass& p = s.two;
+  p.kern = reinterpret_cast<const void*>(plan.kern);
+  p.threads = plan.threads;
+  p.smem = plan.smem;
+  if (int rc = operand_maps(s, Epi::kAug, true, kBM, kBM, p, why)) return rc;
+  const int units = pair_units(p);
   if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
-  s.g.n_a = (s.hd.V + 2 * kBM - 1) / (2 * kBM);
-  s.g.n_b = s.n_b2 = (s.T + kBN - 1) / kBN;
-  s.g.by_b = 1;
+  p.g = s.g;
+  p.g.n_a = (s.hd.V + 2 * kBM - 1) / (2 * kBM);
+  p.g.n_b = s.n_b2 = (s.T + kBN - 1) / kBN;
+  p.g.by_b = 1;
   s.bn2 = kBN;
-  s.G2 = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
+  p.G = s.G2 = (int)std::min<long long>(units, (long long)p.g.n_a * p.g.n_b);
   s.cparts2 = col_parts(Epi::kWarps);
-  if (!launch_pairs(p.kern, s.G2, p.threads, p.smem, s.st, mw, mh, mwa, mha, s.g))
-    return *why = kNoLaunch, LORA_CE_ECUDA;
   return 0;
 }
 
 template <int kPass, int R>
 int tc_pass(Step& s, const char** why) {
-  const int d = s.hd.d, V = s.hd.V, T = s.T, aw = s.aug.width;
-  const long long Tpad = round_up(T, kBN);
-  const int half = tc_bn(R) / 2;
-  CUtensorMap mres, mstr, mra, msa, mx;
-  const bool ok =
-      kPass == 1 ? make_map(&mres, s.w.h16, T, d, kBM) && make_map(&mstr, s.hd.W, V, d, half) &&
-                       make_map(&mra, s.w.haug, T, aw, kBM) &&
-                       make_map(&msa, s.w.waug, V, aw, half) &&
-                       make_map_ld(&mx, s.w.xv, 2 * R, V, s.g.Vpad, R)
-                 : make_map(&mres, s.hd.W, V, d, kBM) && make_map(&mstr, s.w.h16, T, d, half) &&
-                       make_map(&mra, s.w.waug, V, aw, kBM) &&
-                       make_map(&msa, s.w.haug, T, aw, half) &&
-                       make_map_ld(&mx, s.w.xt, 2 * R, T, Tpad, R);
-  if (!ok) return *why = kNoMap, LORA_CE_ECUDA;
-  s.g.stages = TcLayout::stages(s.g.kblocks, R);
-  s.g.drain_gain = (float)(1.0 + acc_short(2 * tc_drain(R) * tc_bn(R) / 16, 0));
-  const int smem = TcLayout::bytes(s.g.kblocks, s.g.stages, R);
-  auto kern = lce_gemm_tc<kPass, R, true>;
-  if (s.g.stages < 2 || smem > kMaxDynSmem) return *why = kNoFit, LORA_CE_ECUDA;
-  const int units =
-      std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(kern), kThreadsT, smem));
+  const int V = s.hd.V, T = s.T, half = tc_bn(R) / 2;
+  Pass& p = kPass == 1 ? s.one : s.two;
+  if (int rc = operand_maps(s, true, kPass == 2, kBM, half, p, why)) return rc;
+  if (!(kPass == 1 ? make_map_ld(&p.maps[4], s.w->xv, 2 * R, V, s.g.Vpad, R)
+                   : make_map_ld(&p.maps[4], s.w->xt, 2 * R, T, round_up(T, kBN), R)))
+    return *why = kNoMap, LORA_CE_ECUDA;
+  p.n_maps = 5;
+  p.g = s.g;
+  p.g.stages = TcLayout::stages(s.g.kblocks, R);
+  p.g.drain_gain = (float)(1.0 + acc_short(2 * tc_drain(R) * tc_bn(R) / 16, 0));
+  p.kern = reinterpret_cast<const void*>(lce_gemm_tc<kPass, R, true>);
+  p.threads = kThreadsT;
+  p.smem = TcLayout::bytes(s.g.kblocks, p.g.stages, R);
+  if (p.g.stages < 2 || p.smem > kMaxDynSmem) return *why = kNoFit, LORA_CE_ECUDA;
+  const int units = pair_units(p);
   if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
-  s.g.n_a = ((kPass == 1 ? T : V) + 2 * kBM - 1) / (2 * kBM);
-  s.g.n_b = ((kPass == 1 ? V : T) + tc_bn(R) - 1) / tc_bn(R);
-  const int G = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
-  if (!launch_pairs(kern, G, kThreadsT, smem, s.st, mres, mstr, mra, msa, mx, s.g))
-    return *why = kNoLaunch, LORA_CE_ECUDA;
+  p.g.n_a = ((kPass == 1 ? T : V) + 2 * kBM - 1) / (2 * kBM);
+  p.g.n_b = ((kPass == 1 ? V : T) + tc_bn(R) - 1) / tc_bn(R);
+  p.G = (int)std::min<long long>(units, (long long)p.g.n_a * p.g.n_b);
   if (kPass == 1) {
-    s.slots = SlotPlan{2, s.g.n_a, s.g.n_b, units, s.g.Tcap, s.w.p_max, s.w.p_sum, nullptr,
-                       s.w.p_q};
+    s.slots = SlotPlan{2, p.g.n_a, p.g.n_b, units, s.g.Tcap, s.g.p_max, s.g.p_sum, nullptr,
+                       s.g.p_q};
   } else {
-    s.n_b2 = s.g.n_b;
+    s.n_b2 = p.g.n_b;
     s.bn2 = tc_bn(R);
-    s.G2 = G;
+    s.G2 = p.G;
     s.cparts2 = 1;
   }
   return 0;
 }
 
-template <int kPass>
-int grad_pass(Step& s, int R, const char** why) {
+template <class EL, class EG>
+int sums_passes(Step& s, const char** why) {
+  if (int rc = rows_pass(s, sums_plan<EL>(s.g.kblocks), EL::kAug, col_parts(EL::kWarps), nullptr,
+                         s.g.p_q, why))
+    return rc;
+  return sums_pass2<EG>(s, why);
+}
+template <int R>
+int tc_passes(Step& s, const char** why) {
+  const int rc = tc_pass<1, R>(s, why);
+  return rc ? rc : tc_pass<2, R>(s, why);
+}
+
+// Both gradient passes of kernel rank R.
+int grad_passes(Step& s, int R, const char** why) {
   switch (R) {
     case 4:
-      if constexpr (kPass == 1) return sums_pass1<EpiLse<4, false, false, true>>(s, why);
-      else return sums_pass2<EpiGrad<4, false, false, true>>(s, why);
+      return sums_passes<EpiLse<4, false, false, true>, EpiGrad<4, false, false, true>>(s, why);
     case 8:
-      if constexpr (kPass == 1) return sums_pass1<EpiLse<8, true, false, true>>(s, why);
-      else return sums_pass2<EpiGrad<8, true, false, true>>(s, why);
-    case 16: return tc_pass<kPass, 16>(s, why);
-    case 32: return tc_pass<kPass, 32>(s, why);
-    default: return tc_pass<kPass, 64>(s, why);
+      return sums_passes<EpiLse<8, true, false, true>, EpiGrad<8, true, false, true>>(s, why);
+    case 16: return tc_passes<16>(s, why);
+    case 32: return tc_passes<32>(s, why);
+    default: return tc_passes<64>(s, why);
   }
 }
 
 template <int R>
-bool launch_dA(const Step& s, const DistillWs& w) {
+bool launch_dA(const Step& s, const DistillWs& w, cudaStream_t st) {
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3((unsigned)((s.T + kDAChunk - 1) / kDAChunk), (unsigned)(s.hd.d / 64));
   lc.blockDim = dim3(256);
-  lc.stream = s.st;
+  lc.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -661,7 +704,6 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   const float* const Bt = !r4 ? nullptr : hd.layout ? hd.B : w.Bt;
   GemmArgs g{};
   fill_pass1(g, hd, aug, T, 1.0f);
-  g.n_b = (int)(g.Vpad / kBN);
   g.err = w.stats + kStErr;
   g.p_max = w.p_max;
   g.p_sum = w.p_sum;
@@ -722,8 +764,10 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
   na.r = hd.r;
   na.out = top_k > 0 ? w.norms : nullptr;
 
+  // all that can be refused comes before the first launch
+  const PrepPlan prep = plan_prep(pa, pk, na, true, 0, !few && (pk.Bt || pk.waug), sms);
+  if (!prep.ok) return *why = kNoFit, LORA_CE_ECUDA;
   if (few) {
-    if (launch_prep(pa, pk, na, true, 0, false, sms, st)) return *why = kNoFit, LORA_CE_ECUDA;
     const int blocks = few_blocks(hd.V);
     const float lg = (float)((1.0 + kLoss32) / std::log(2.0));
     FewArgs f = few_args(hd, aug.R, T, w.h16, w.sU, lg);
@@ -736,29 +780,20 @@ int head_score_run(const HeadCore& hd, const void* H, int dtype, int T, const in
     f.sub_arg = w.sub_arg;
     f.sub_arg2 = w.sub_arg2;
     f.n_sub = w.n_sub;
-    if (!launch_few<kFewScore>(f, blocks, st)) return *why = kNoLaunch, LORA_CE_ECUDA;
+    const FewPlan pass = plan_few<kFewScore>(f);
+    if (!pass.ok) return *why = kNoFit, LORA_CE_ECUDA;
+    if (!launch_prep(prep, pa, pk, na, st) || !launch_few(pass, f, blocks, st))
+      return *why = kNoLaunch, LORA_CE_ECUDA;
     a.p = SlotPlan{1, 1, blocks, blocks, f.ld, w.p_max, w.p_sum, w.p_ent, nullptr};
     a.lg = lg;
   } else {
-    const PassPlan p = score_plan(g.kblocks, w.sub, r4);
-    const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
-                                                         p.threads, p.smem));
-    if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
-    CUtensorMap mh, mw, mha, mwa;
-    if (!make_map(&mh, w.h16, T, hd.d, kBM) || !make_map(&mw, hd.W, hd.V, hd.d, kBM))
-      return *why = kNoMap, LORA_CE_ECUDA;
-    mha = mh;
-    mwa = mw;
-    if (aug.width && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
-                      !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
-      return *why = kNoMap, LORA_CE_ECUDA;
-    if (launch_prep(pa, pk, na, true, 0, pk.Bt || pk.waug, sms, st))
-      return *why = kNoFit, LORA_CE_ECUDA;
-    const int G = (int)std::min<long long>(units, (long long)g.n_a * g.n_b);
-    if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, g))
+    Step s{hd, w.h16, w.haug, w.waug, aug, T, sms, g, nullptr};
+    if (int rc = rows_pass(s, score_plan(g.kblocks, w.sub, r4), aug.width != 0,
+                           col_parts(EpiScore<65536, 64, false>::kWarps), w.p_ent, nullptr, why))
+      return rc;
+    if (!launch_prep(prep, pa, pk, na, st) || !launch_pass(s.one, st))
       return *why = kNoLaunch, LORA_CE_ECUDA;
-    a.p = SlotPlan{col_parts(EpiScore<65536, 64, false>::kWarps), g.n_a, g.n_b, units, g.Tcap,
-                   w.p_max, w.p_sum, w.p_ent, nullptr};
+    a.p = s.slots;
     a.lg = g.lg;
   }
   a.z = logit_args(hd, aug, T, w.h16, w.sU, w.haug, w.waug);
@@ -800,26 +835,21 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   const DistillWs w = distill_ws(hd, T, grads, ws);
   const bool few = few_distill(T, R), tc = grads && R >= 16 && !few;
   if (few) aug.layout = aug.width = 0;  // the rank term from B as it is
-  Step s{hd, w, aug, T, sm_count(), tau, st, GemmArgs{}, SlotPlan{}};
+  Step s{hd, w.h16, w.haug, w.waug, aug, T, sm_count(), GemmArgs{}, &w};
   fill_pass1(s.g, hd, aug, T, tau);
-  s.Bt = few || !(grads || R == 4) ? nullptr : hd.layout ? hd.B : w.Bt;
+  const float* const Bt = few || !(grads || R == 4) ? nullptr : hd.layout ? hd.B : w.Bt;
   s.g.err = w.stats + kStErr;
   s.g.p_max = w.p_max;
   s.g.p_sum = w.p_sum;
   s.g.p_q = w.p_q;
   s.g.tok = w.tok;
   s.g.sU4 = w.sU;
-  s.g.Bt = s.Bt;
+  s.g.Bt = Bt;
   s.g.gBp = w.gBp;
   s.g.nml = w.nml;
 
-  if (cudaMemsetAsync(w.stats, 0, w.zero_bytes, st) != cudaSuccess)
-    return *why = "cudaMemsetAsync failed", LORA_CE_ECUDA;
   // weights may leave whole tiles of positions without one that counts
   const bool order = weight && !few && T > 2 * kBM;
-  if (order && !launch_plain(lh_order, 1, 1024, 0, st, T, K, hd.V, weight, ids,
-                             teacher, w.masks, w.order, w.stats))
-    return *why = kNoLaunch, LORA_CE_ECUDA;
   s.g.active = order ? w.stats + kStActive : nullptr;
   PrepArgs pa = prep_args(hd, aug, H, dtype, T);
   pa.order = order ? w.order : nullptr;
@@ -844,7 +874,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pk.r = hd.r;
   pk.R = R;
   pk.Vpad = s.g.Vpad;
-  pk.Bt = s.Bt && !hd.layout ? w.Bt : nullptr;
+  pk.Bt = Bt && !hd.layout ? w.Bt : nullptr;
   pk.Bt_plain = tc;  // the rank sums' passes have xv instead
   pk.waug = aug.width ? w.waug : nullptr;
   pk.aug_layout = aug.layout;
@@ -852,51 +882,43 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   pk.xv = tc ? w.xv : nullptr;
   pk.stats = w.stats;
   const bool pack = pk.Bt || pk.waug || pk.xv;
-  // the scale of xv needs the largest |B| first
   const NormArgs no{};
-  if (launch_prep(pa, pk, no, true, tc ? 2 * s.sms : 0, pack && !tc, s.sms, st) ||
-      (tc && launch_prep(pa, pk, no, false, 0, true, s.sms, st)))
-    return *why = kNoFit, LORA_CE_ECUDA;
-
-  int rc = 0;
+  // all that can be refused comes before the first launch; the scale of xv needs the
+  // largest |B| first
+  const PrepPlan prep = plan_prep(pa, pk, no, true, tc ? 2 * s.sms : 0, pack && !tc, s.sms);
+  const PrepPlan prep2 = tc ? plan_prep(pa, pk, no, false, 0, true, s.sms) : PrepPlan{};
+  if (!prep.ok || (tc && !prep2.ok)) return *why = kNoFit, LORA_CE_ECUDA;
   const float few_lg = (float)((1.0 + kLoss32) / (std::log(2.0) * (double)tau));
   FewArgs f = few_args(hd, R, T, w.h16, w.sU, few_lg);
   const int v_blocks = few_blocks(hd.V);
+  FewPlan forward, backward;
   if (few) {
     f.p_max = w.p_max;
     f.p_sum = w.p_sum;
     f.p_q = w.p_q;
-    if (!(grads ? launch_few<kFewForward>(f, v_blocks, st) : launch_few<kFewLoss>(f, v_blocks, st)))
-      return *why = kNoLaunch, LORA_CE_ECUDA;
+    forward = grads ? plan_few<kFewForward>(f) : plan_few<kFewLoss>(f);
+    if (grads) backward = plan_few<kFewBackward>(f);
+    if (!forward.ok || !backward.ok) return *why = kNoFit, LORA_CE_ECUDA;
     s.slots = SlotPlan{1, 1, v_blocks, v_blocks, f.ld, w.p_max, w.p_sum, nullptr, w.p_q};
-  } else if (grads) {
-    rc = grad_pass<1>(s, R, why);
   } else {
-    const PassPlan p = score_plan(s.g.kblocks, 0, R == 4);
-    const int units = std::min(kMaxPairs, resident_pairs(reinterpret_cast<const void*>(p.kern),
-                                                         p.threads, p.smem));
-    if (units < 1) return *why = kNoFit, LORA_CE_ECUDA;
-    CUtensorMap mh, mw, mha, mwa;
-    if (!make_map(&mh, w.h16, T, hd.d, kBM) || !make_map(&mw, hd.W, hd.V, hd.d, kBM))
-      return *why = kNoMap, LORA_CE_ECUDA;
-    mha = mh;
-    mwa = mw;
-    if (aug.width && (!make_map(&mha, w.haug, T, aug.width, kBM) ||
-                      !make_map(&mwa, w.waug, hd.V, aug.width, kBM)))
-      return *why = kNoMap, LORA_CE_ECUDA;
-    s.g.n_b = (int)(s.g.Vpad / kBN);
-    const int G = (int)std::min<long long>(units, (long long)s.g.n_a * s.g.n_b);
-    if (!launch_pairs(p.kern, G, p.threads, p.smem, st, mh, mw, mha, mwa, s.g))
-      rc = (*why = kNoLaunch, LORA_CE_ECUDA);
-    s.slots = SlotPlan{col_parts(EpiScore<65536, 0, false>::kWarps), s.g.n_a, s.g.n_b, units,
-                       s.g.Tcap, w.p_max, w.p_sum, nullptr, nullptr};
+    const int rc = grads ? grad_passes(s, R, why)
+                         : rows_pass(s, score_plan(s.g.kblocks, 0, R == 4), aug.width != 0,
+                                     col_parts(EpiScore<65536, 0, false>::kWarps), nullptr, nullptr,
+                                     why);
+    if (rc) return rc;
   }
-  if (rc) return rc;
+  if (cudaMemsetAsync(w.stats, 0, w.zero_bytes, st) != cudaSuccess)
+    return *why = "cudaMemsetAsync failed", LORA_CE_ECUDA;
+  if ((order && !launch_plain(lh_order, 1, 1024, 0, st, T, K, hd.V, weight, ids, teacher, w.masks,
+                              w.order, w.stats)) ||
+      !launch_prep(prep, pa, pk, no, st) || (tc && !launch_prep(prep2, pa, pk, no, st)) ||
+      !(few ? launch_few(forward, f, v_blocks, st) : launch_pass(s.one, st)))
+    return *why = kNoLaunch, LORA_CE_ECUDA;
   DistillArgs a{};
   a.z = logit_args(hd, aug, T, w.h16, w.sU, w.haug, w.waug);
   a.z.R = R;
   a.z.B.R = R;
-  if (s.Bt && R == 4) a.z.B = BView{s.Bt, hd.V, hd.r, R, 1};  // a row's ranks side by side
+  if (Bt && R == 4) a.z.B = BView{Bt, hd.V, hd.r, R, 1};  // a row's ranks side by side
   a.p = s.slots;
   a.lg = few ? few_lg : s.g.lg;
   a.tau = tau;
@@ -907,7 +929,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
   a.order = pa.order;
   a.active = s.g.active;
   a.wt = w.wt;
-  a.Bt = s.Bt;
+  a.Bt = Bt;
   a.Bt_plain = pk.Bt && tc;
   a.stats = w.stats;
   a.loss = loss;
@@ -942,7 +964,7 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
     f.loss = loss;
     f.wt = w.wt;
     f.tail = out.tail;
-    if (!launch_few<kFewBackward>(f, f.v_blocks + a_blocks, st))
+    if (!launch_few(backward, f, f.v_blocks + a_blocks, st))
       return *why = kNoLaunch, LORA_CE_ECUDA;
     return 0;
   }
@@ -953,11 +975,11 @@ int head_distill_run(const HeadCore& hd, const void* H, int dtype, int T, int K,
                       (const float*)w.xs, (const int*)w.stats, w.xt))
       return *why = kNoLaunch, LORA_CE_ECUDA;
   }
-  if ((rc = grad_pass<2>(s, R, why))) return rc;
-  const bool dA_ok = R == 4    ? launch_dA<4>(s, w)
-                     : R == 8  ? launch_dA<8>(s, w)
-                     : R == 16 ? launch_dA<16>(s, w)
-                     : R == 32 ? launch_dA<32>(s, w) : launch_dA<64>(s, w);
+  if (!launch_pass(s.two, st)) return *why = kNoLaunch, LORA_CE_ECUDA;
+  const bool dA_ok = R == 4    ? launch_dA<4>(s, w, st)
+                     : R == 8  ? launch_dA<8>(s, w, st)
+                     : R == 16 ? launch_dA<16>(s, w, st)
+                     : R == 32 ? launch_dA<32>(s, w, st) : launch_dA<64>(s, w, st);
   if (!dA_ok) return *why = kNoLaunch, LORA_CE_ECUDA;
   GradArgs ga{};
   ga.T = T;
