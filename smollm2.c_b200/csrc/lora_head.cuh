@@ -2103,7 +2103,6 @@ static __global__ void
   constexpr int kTeams = TW == 1 ? kRowWarps : 1, kThreads = 32 * TW;
   constexpr int kPer = (kMaxTop + kThreads - 1) / kThreads;
   __shared__ double s_red[kTeams][4 * TW];
-  __shared__ int s_n[kTeams];
   __shared__ int s_id[kTeams][kMaxTop];
   __shared__ float s_q[kTeams][kMaxTop];
   __shared__ double s_lq[kTeams][kMaxTop];
@@ -2151,7 +2150,6 @@ static __global__ void
       }
     }
   }
-  if (tid == 0) s_n[no] = 0;
   RowSum rs = merge_row<false>(a.p, t, nslot, team);
   if (nslot == 0) rs = RowSum{0.f, 1.0, 0.0};
   wrong = team.count(wrong);
