@@ -229,3 +229,103 @@ def test_gradients_of_a_tiny_adapter(T, r, e):
     p.lists(8)
     p.B *= 2.0**e
     check_distill(p, 1.0)
+
+
+@gpu
+@pytest.mark.parametrize("T,r", [(16, 0), (17, 4), (23, 16), (24, 0), (24, 4), (24, 9), (25, 0), (25, 4),
+                                 (25, 16), (8, 33), (16, 33), (17, 33), (16, 64), (17, 64)])
+@pytest.mark.parametrize("V,d,k", [(20001, 128, 8), (49152, 576, 20), (2048, 640, 5)])
+def test_score_on_both_sides_of_few_positions(T, r, V, d, k):
+    """Up to 24 positions (16 above rank 16) have a pass of their own where records
+    have 64 columns, as they do here."""
+    p = Problem(T, V, d, r)
+    check_score(p, k, p.score(k))
+
+
+@gpu
+@pytest.mark.parametrize("T,r", [(16, 4), (17, 4), (31, 8), (32, 1), (32, 16), (33, 4), (33, 8), (33, 16),
+                                 (16, 33), (17, 33), (16, 64), (17, 64)])
+@pytest.mark.parametrize("V,d,K", [(4099, 128, 8), (20001, 576, 33)])
+@pytest.mark.parametrize("grads", [True, False])
+def test_distill_on_both_sides_of_few_positions(T, r, V, d, K, grads):
+    """The same limit is 32 positions, 16 above rank 16."""
+    p = Problem(T, V, d, r)
+    p.lists(K)
+    check_distill(p, 1.5, grads)
+
+
+def check_elements(p, tau):
+    """Every element of gA and gB by itself, against the sum of its absolute terms N.
+      * a probability, and with it a term, is off by tol of itself (test_head.py)
+      * the sums of the terms: 64 accumulations in f32 at a time, 2^-17 of N, and the
+        f16 pairs of their operands, 2^-21; 2^-16 for both
+      * s U in f32, a sum in eight parts of d / 8: d / 8 + 8 roundings of the sum of its
+        absolute terms, which stands for |U| in gB's N
+      * gB's sparse part is in units of 2^-38 of the largest |w s U| tau at least, and
+        its operand is a pair of f16 in units of 2^-39 of it: 2^-37 per position"""
+    import torch
+    out = p.distill(tau)
+    _, gA, gB, _, _ = p.distill64(tau)
+    w = torch.ones(p.T, dtype=torch.float64, device="cuda") if p.weight is None else p.weight.double()
+    ids = p.ids.long()
+    t = torch.where(ids >= 0, p.teacher.double() / tau, -math.inf)
+    counted = (t > -math.inf).any(1) & (w != 0)
+    q = torch.softmax(torch.where(counted[:, None], t, 0.0), 1) * ((ids >= 0) & counted[:, None])
+    H = p.H.half().double()
+    A, B, s = p.A.double(), p.B.double(), abs(p.scale)
+    dz = torch.softmax((H @ p.W.double().T + p.scale * (H @ A) @ B) / tau, 1)
+    dz = dz.scatter_add_(1, ids.clamp(min=0), q) * (w.abs() * counted * tau)[:, None]
+    U, U_abs = (H @ A).abs(), H.abs() @ A.abs()
+    rel = p.tol() / tau + 2.0**-20 + 2.0**-16
+    NA = s * (H.abs().T @ (dz @ B.abs().T))
+    bound = rel * s * (U.T @ dz) + (p.d / 8 + 8) * 2.0**-24 * s * (U_abs.T @ dz)
+    bound = bound + p.T * 2.0**-37 * s * float((U * (w.abs() * tau)[:, None]).max())
+    assert bool(((out["gA"].double() - gA).abs() <= rel * NA + 1e-44).all())
+    assert bool(((out["gB"].double() - gB).abs() <= bound).all())
+
+
+@gpu
+@pytest.mark.parametrize("T,V,d,r,K,tau,dtype", [
+    (5, 20001, 576, 4, 8, 1.0, "bf16"), (32, 1000, 64, 16, 20, 2.0, "f16"), (16, 4099, 128, 64, 64, 1.0, "bf16"),
+    (100, 4099, 576, 3, 33, 1.0, "f32"), (255, 4099, 128, 8, 20, 2.0, "bf16"),
+    (300, 4099, 128, 16, 33, 1.0, "bf16"), (700, 3000, 192, 64, 10, 1.5, "bf16"),
+    (2000, 1000, 64, 32, 8, 0.5, "f16"), (129, 49152, 576, 33, 64, 1.0, "bf16"),
+    (4000, 777, 64, 4, 128, 4.0, "bf16"),
+])
+@pytest.mark.parametrize("weights", [None, "uniform", "masked"])
+def test_every_element_of_the_gradients(T, V, d, r, K, tau, dtype, weights):
+    p = Problem(T, V, d, r, dtype)
+    p.lists(K)
+    if weights:
+        p.weight = p.u(T) * (p.u(T) < (0.4 if weights == "masked" else 2.0))
+    check_elements(p, tau)
+
+
+@gpu
+@pytest.mark.parametrize("r", [4, 16])
+def test_a_distillation_step_through_a_communicator(r):
+    """A communicator of one rank: the sums go through its all-reduce and come back the
+    same bits."""
+    import numpy as np
+
+    import lora_ce
+    T, V, d, K = 60, 700, 128, 4
+    rng = np.random.default_rng(r)
+    W = (rng.standard_normal((V, d)) / 8).astype(np.float16)
+    A, B = rng.standard_normal((d, r)).astype(np.float32) / 8, rng.standard_normal((r, V)).astype(np.float32) / 20
+    H = rng.standard_normal((T, d)).astype(np.float32)
+    ids, z = rng.integers(-1, V, (T, K)).astype(np.int32), rng.standard_normal((T, K)).astype(np.float32)
+    weight = (rng.random(T) < 0.7).astype(np.float32)
+    got = []
+    for comm in (False, True):
+        m = lora_ce.LoraCE(lora_ce.default_config(d, V, r, T, clip_norm=0.5))
+        m.set_weight(W.view(np.uint16))
+        m.set_adapter(A, B, 0)
+        if comm:
+            m.comm_init(1, 0, lora_ce.LoraCE.nccl_unique_id())
+        got.append([m.distill_step(H, ids, z, 2.0, weight) for _ in range(2)] + list(m.get_adapter()) +
+                   list(m.get_grads()))
+        m.close()
+    for a, b in zip(*got):
+        assert np.array_equal(a, b)
+    assert got[0][4] == 2
