@@ -329,6 +329,12 @@ def run_reference_arm(args):
     world = env_int("WORLD_SIZE", 1)
     if rank != 0:
         return
+    import oracle as orc
+    if not orc.ref_available():
+        # the restatement in oracle/ is this repository's own code, not the reference
+        print(json.dumps({"impl": "reference", "unavailable":
+                          "oracle/_ref (the reference's train.c) is not built here"}), flush=True)
+        return
     ref = CpuReference()
     per_step = max(2.0, min(8.0, 150.0 / max(1, args.steps + args.warmup)))
     for _ in range(args.warmup):
