@@ -584,6 +584,15 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
   int n_a = g.n_a, n_b = g.n_b;
   const int G = gridDim.x / kPair;              // tile-range owners (CTAs or pairs)
   const int unit = blockIdx.x / kPair;
+  long long total, x_begin, x_end;
+  auto split = [&] {
+    total = (long long)n_a * n_b;
+    x_begin = tile_start(unit, total, G);
+    x_end = tile_start(unit + 1, total, G);
+  };
+  // (below the barriers it cost EpiLse<16> a spill, above them it costs EpiLse<4> with
+  // kTemp one)
+  if constexpr (!Epi::kDepend) split();
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSt; ++i) {
@@ -629,10 +638,8 @@ __global__ void __launch_bounds__(block_threads(Epi::kWarps), 1)
       if (g.by_b) n_b = active_tiles(*g.active, kBN, n_b, n_a, G);
       else n_a = active_tiles(*g.active, kResRows, n_a, n_b, G);
     }
+    split();
   }
-  const long long total = (long long)n_a * n_b;
-  const long long x_begin = tile_start(unit, total, G);
-  const long long x_end = tile_start(unit + 1, total, G);
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)
