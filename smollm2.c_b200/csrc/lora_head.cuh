@@ -277,7 +277,7 @@ struct PrepArgs {
 // A teacher's entry that is there: a logit of -inf weighs nothing, as no entry does.
 // (Ids past the vocabulary, NaN and +inf are: lh_distill_rows reports them.)
 __device__ __forceinline__ bool is_entry(int id, float logit, int V) {
-  return id >= 0 && (id >= V || logit != -INFINITY);
+  return (id >= 0) & ((id >= V) | (logit != -INFINITY));  // (both are read at once)
 }
 
 // order: the positions that count (a weight other than 0 and an entry), then the
@@ -285,8 +285,9 @@ __device__ __forceinline__ bool is_entry(int id, float logit, int V) {
 // over the tiles that hold one that counts, a quarter of all at least: at 8,000
 // positions of which 30% are a masked prompt, rank 64, the call takes 1,680 us
 // instead of 2,300.
-// One block: each warp takes a run of positions, 32 side by side at a time (a
-// thread for a run of its own, its loads and stores a line each, took 13 us instead of 11).
+// One block: each warp takes a run of positions, 32 side by side at a time: 14 us at
+// 8,000 positions (11 without the teacher's logits, which a list of -inf alone needs; 13
+// then with a run of its own for each thread, its loads and stores a line each).
 static __global__ void __launch_bounds__(1024) lh_order(int T, int K, int V,
                                                         const float* __restrict__ weight,
                                                         const int32_t* __restrict__ ids,
@@ -303,19 +304,22 @@ static __global__ void __launch_bounds__(1024) lh_order(int T, int K, int V,
   int n = 0;
   for (int g0 = g_lo; g0 < g_hi; g0 += kStep) {
     float wt[kStep];
-    bool first[kStep];
+    int id[kStep];
+    float x[kStep];
 #pragma unroll
     for (int i = 0; i < kStep; ++i) {
       const int t = 32 * (g0 + i) + lane;
       const bool in = g0 + i < g_hi && t < T;
       wt[i] = in ? weight[t] : 0.f;
-      first[i] = in && is_entry(ids[(long long)t * K], teacher[(long long)t * K], V);
+      id[i] = in ? ids[(long long)t * K] : -1;
+      x[i] = in ? teacher[(long long)t * K] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < kStep; ++i) {
       if (g0 + i >= g_hi) break;
-      bool any = wt[i] != 0.f && first[i];
-      unsigned look = __ballot_sync(kAll, wt[i] != 0.f && !first[i]);
+      const bool first = is_entry(id[i], x[i], V);
+      bool any = wt[i] != 0.f && first;
+      unsigned look = __ballot_sync(kAll, wt[i] != 0.f && !first);
       for (; look; look &= look - 1) {  // the first entry is absent: seldom
         const int q = __ffs(look) - 1;
         const long long o = (long long)(32 * (g0 + i) + q) * K;
@@ -510,12 +514,17 @@ __device__ __forceinline__ void prep_tile(const PrepArgs& a, int t0, float* smem
     const int t = t0 + (tid >> 4), from = t < a.T ? a.source(t) : 0;
     bool any = false;
     if (t < a.T) {
+      int id[kMaxTop / 16];
+      float x[kMaxTop / 16];
 #pragma unroll
       for (int q = 0; q < kMaxTop / 16; ++q) {
         const int k = (tid & 15) + 16 * q;
         const long long o = (long long)from * a.K + k;
-        any |= k < a.K && is_entry(a.ids[o], a.teacher[o], a.V);
+        id[q] = k < a.K ? a.ids[o] : -1;
+        x[q] = k < a.K ? a.teacher[o] : 0.f;
       }
+#pragma unroll
+      for (int q = 0; q < kMaxTop / 16; ++q) any |= is_entry(id[q], x[q], a.V);
     }
     const unsigned b = __ballot_sync(0xffffffffu, any) >> (lane & 16) & 0xffffu;
     if ((tid & 15) == 0) {
