@@ -68,8 +68,8 @@ void aug_schedule(GemmArgs& g, const Aug& a) {
   }
 }
 
-// The share by which the accumulator of a large logit falls short
-// (lora_head.cuh): partial sums at 1/n, 2/n .. 1 of it over the n K-steps of
+// The share by which the accumulator of a large logit falls short where its partial
+// sums grow evenly (lora_head.cuh): partial sums at 1/n, 2/n .. 1 of it over the n K-steps of
 // h . W, then at all of it over the rank term's.
 double acc_short(int n, int n_aug) {
   return 0.79 * (0.5 * (n + 1) + n_aug) * std::ldexp(1.0, -25) / std::log(2.0);

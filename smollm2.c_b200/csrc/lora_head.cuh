@@ -15,7 +15,12 @@
 // and 576 alike (6.2e-7 z at 576, with a spread of 1.6e-7 z; an f32 product of
 // a library has no shortfall and a spread of 3e-7 z).  acc_short() gives the
 // measured share and the softmax's exponent factor makes it good
-// (GemmArgs::lg).  Sums of many terms go in two levels (EpiLse, lce_gemm_tc).
+// (GemmArgs::lg).  That is for partial sums that grow evenly towards the logit.  Where
+// channels of h cancel, the shortfall follows the partial sums, up to n 2^-24 of them,
+// and no factor of z makes it good: two channels whose parts of every logit are 32 to 48
+// and cancel leave log probabilities of 300 positions 2e-5 off on average and 4.5e-5 at
+// most, parts of 128 to 192 9e-5 and 2e-4 (an f32 product of a library: 1e-6 and 7e-5,
+// 1e-6 and 3e-4).  The order of alternatives takes them into account (logit_gaps).  Sums of many terms go in two levels (EpiLse, lce_gemm_tc).
 // Gradients of 8192 positions against 64 bits, where a bias adds up and
 // rounding does not: rank 4 9e-6 with neither, 6e-6 with the factor, 4e-7 with
 // both; rank 64 2e-5, 1.5e-5, 4e-7 (a library's f32 products: 2e-6 to 3e-6).
@@ -76,7 +81,8 @@ __device__ __forceinline__ long long sub_idx(int t, int k, int n_sub) {
 // logits that carry their column in the lowest bits, nor with a fifth ring stage.
 // kR4: the rank term of ranks up to 4 here, in f32 from staged rows of B (as EpiLse),
 // so that those ranks have f32's range, as in the training step.  As f16 pairs in a
-// K-block of its own a call of 8,192 positions took 581 us instead of 592.
+// K-block of its own, which it filled by a quarter, the pass took as long (8,192
+// positions, V = 49152, d = 576: 417 us, as pairs 420).
 template <int kRing_, int kSub, bool kR4>
 struct EpiScore {
   static constexpr bool kAug = !kR4;
@@ -1637,8 +1643,10 @@ __device__ __noinline__ Cut tidy_candidates(Team<TW> team, int C, int keep, int 
 // threshold that n_pick to n_pick + kPickStop records reach: it is a lower bound of
 // the n_pick-th largest logit; the candidates are the logits that reach it, less what
 // rounding may have moved; compute again those whose order the pass's logits do not
-// tell, sort, write.  The softmax's sums get the difference.
-// 4,096 positions, 64 alternatives: 103 us (with every candidate computed again, five
+// tell, sort, write.  The softmax's sums get the difference.  What keeps a list whole
+// that overflows (tidy_candidates) costs 4 of the 106 us without being called: two turns
+// over the records, and a call's registers.
+// 4,096 positions, 64 alternatives: 106 us (with every candidate computed again, five
 // groups of 16 rows of W a position, 25 more).  Waits for L2 and for instructions; 16
 // warps an SM, with the registers that leaves, do better than 20 (115), 24 (142) or 12
 // (112).
